@@ -560,6 +560,107 @@ UCB_API int ucb_compact_rows(const void* src_dev, int64_t row_bytes, const uint8
                      const int64_t* types_dev, void* dst_dev, int64_t* types_out_dev,
                      int64_t* prefix_dev, int64_t* kept_host, void* stream);
 
+/* ------------------------------------------------------------------ head norm + rotation
+ * No counterpart in the reference's physical engine (its model code runs the
+ * per-head norms and the rotary embedding as separate framework calls).
+ * Query rows [tokens, q_heads, head_dim] and key rows [tokens, k_heads,
+ * head_dim] (k_heads may be 0; dtype UCB_BF16, UCB_F16 or UCB_F32; strides in
+ * elements, channels contiguous): y = x * rsqrt(mean(x^2) + eps) * weight
+ * (weights [head_dim] of the same dtype, NULL = ones), then the rotation by
+ * row positions[t] of the tables cos_dev, sin_dev (fp32 [table_rows,
+ * rotary_dim / 2]): channels (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * `interleaved`; channels from rotary_dim on are only normalised.  fp32
+ * arithmetic, one rounding.  The outputs may be the inputs.  rotary_dim 0: no
+ * rotation.  2 <= head_dim <= 256.  positions: int32, or int64 when
+ * positions_64.  A position outside the tables sets device error bit 2 and
+ * its rows become NaN. */
+UCB_API int ucb_head_norm_rope(const void* query_dev, int64_t q_stride_token, int64_t q_stride_head, int q_heads,
+                               const void* key_dev, int64_t k_stride_token, int64_t k_stride_head, int k_heads,
+                               const void* q_weight_dev, const void* k_weight_dev, const float* cos_dev,
+                               const float* sin_dev, const void* positions_dev, int positions_64,
+                               int64_t table_rows, int64_t tokens, int head_dim, int rotary_dim, int interleaved,
+                               int dtype, float eps, void* q_out_dev, int64_t qo_stride_token,
+                               int64_t qo_stride_head, void* k_out_dev, int64_t ko_stride_token,
+                               int64_t ko_stride_head, void* stream);
+
+/* ------------------------------------------------------------------ 8-bit block cache
+ * No counterpart in the reference (its quantized segments are frozen and
+ * grouped along tokens or channels).  Keys and values of num_seqs sequences
+ * in 8 bits, in blocks of block_tokens tokens, one fp32 scale for each block
+ * and KV head: value = code * scale, scale = max(amax / 127, 2^-120) over the
+ * block's tokens so far, code = clamp(rint(x * (1 / scale)), -127, 127) (a NaN
+ * or infinite input makes its block's scale NaN or infinite, its codes 0).
+ * key_low / key_high hold the smallest and largest key code of each channel
+ * over the block's tokens.  Token t of sequence s lies in row t % block_tokens
+ * of block block_table[s][t / block_tokens].  pending_key / pending_value keep
+ * the unquantised rows of each sequence's incomplete block, so a block that
+ * grows row by row is always the quantisation of all its rows.  lengths are
+ * read on the device: a write expects them already advanced by its rows.
+ * head_dim 64 or 128; block_tokens 16, 32, 64 or 128; num_seqs <= 4096; all
+ * tensors contiguous; codes, bounds and pending rows 16-byte aligned. */
+typedef struct ucb_block8_cache {
+  int8_t* key_code;            /* [num_blocks, kv_heads, block_tokens, head_dim] */
+  int8_t* value_code;          /* same */
+  float* key_scale;            /* [num_blocks, kv_heads] */
+  float* value_scale;          /* same */
+  int8_t* key_low;             /* [num_blocks, kv_heads, head_dim] */
+  int8_t* key_high;            /* same */
+  void* pending_key;           /* [num_seqs, kv_heads, block_tokens, head_dim], dtype */
+  void* pending_value;         /* same */
+  const int32_t* block_table;  /* [num_seqs, max_blocks] */
+  const int32_t* lengths;      /* [num_seqs] */
+  int64_t num_blocks;
+  int32_t num_seqs;
+  int32_t max_blocks;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t block_tokens;
+  int32_t dtype;               /* UCB_BF16 or UCB_F16: rows written, read and queries */
+} ucb_block8_cache;
+
+/* Append key/value rows [rows, kv_heads, head_dim] (channels contiguous):
+ * rows [starts[s], starts[s+1]) are the last tokens of sequence s, that is
+ * tokens [lengths[s] - n, lengths[s]); starts_dev int32 [num_seqs + 1], or
+ * NULL for one row each.  Every touched block is requantised from all its rows when its
+ * scale grows.  Lengths beyond the table, blocks outside the pool and row
+ * ranges outside [0, rows) set device error bit 2 and write nothing. */
+UCB_API int ucb_block8_write(const ucb_block8_cache* cache, const void* key_dev, int64_t key_stride_token,
+                             int64_t key_stride_head, const void* value_dev, int64_t value_stride_token,
+                             int64_t value_stride_head, int64_t rows, const int32_t* starts_dev, void* stream);
+
+/* The restored last rows of every sequence (as above) in dtype, contiguous
+ * [rows, kv_heads, head_dim]. */
+UCB_API int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, const int32_t* starts_dev, void* key_out_dev,
+                            void* value_out_dev, void* stream);
+
+/* The `count` blocks of each sequence and KV head that a query [num_seqs,
+ * q_heads, head_dim] may need most, int32 [num_seqs, kv_heads, count],
+ * ascending, -1 past the end: the first `first` and the last `recent` blocks,
+ * then those of largest score (ties to the lower block).  score_j =
+ * key_scale_j * max over the KV head's query heads of qscale * sum_d
+ * max(qcode_d low_jd, qcode_d high_jd), qcode the query head in 8 bits by the
+ * cache's rule: an upper bound of the block's logits up to the query's
+ * rounding.  first + recent <= count <= 4096.  workspace_dev:
+ * ucb_block8_select_workspace_bytes bytes, 16-byte aligned. */
+UCB_API int64_t ucb_block8_select_workspace_bytes(const ucb_block8_cache* cache);
+UCB_API int ucb_block8_select(const ucb_block8_cache* cache, const void* query_dev, int64_t q_stride_seq,
+                              int64_t q_stride_head, int q_heads, int count, int first, int recent,
+                              int32_t* blocks_dev, void* workspace_dev, void* stream);
+
+/* Attention of query [num_seqs, queries, q_heads, head_dim] (channels
+ * contiguous, 1 <= queries <= 16) over the cache: query i of a sequence is its
+ * token lengths[s] - queries + i and sees the tokens up to itself (none: output
+ * 0, LSE -inf).  blocks_dev int32 [num_seqs, kv_heads, num_selected] limits it
+ * to the tokens of these blocks (negative entries are skipped, no block may
+ * be named twice); NULL = all.  out [num_seqs, queries, q_heads, head_dim] in
+ * dtype, lse fp32 [num_seqs, queries, q_heads] natural log (or NULL).
+ * workspace_dev: ucb_block8_attention_workspace_bytes bytes, 16-byte aligned. */
+UCB_API int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads);
+UCB_API int ucb_block8_attention(const ucb_block8_cache* cache, const void* query_dev, int64_t q_stride_seq,
+                                 int64_t q_stride_query, int64_t q_stride_head, int queries, int q_heads,
+                                 const int32_t* blocks_dev, int num_selected, float softmax_scale, void* out_dev,
+                                 float* lse_dev, void* workspace_dev, void* stream);
+
 /* ------------------------------------------------------------------ self test
  * Checks on the current device that mma.sync f16 consumes fp16 subnormal
  * operands exactly (the decode kernel feeds small integer codes as subnormals).

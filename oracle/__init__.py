@@ -17,6 +17,9 @@ implementation (Superone77/UniCache) and cites the file:line it follows:
                        accumulation, trim and budget requests
 * ``oracle.compact``   dense-cache keep-mask compaction
 
+``oracle.block8`` (head norm with rotation, 8-bit block cache) has no counterpart
+in the reference: it follows the definitions in ``include/unicache_b200.h``.
+
 Parity pin: the oracle is checked bit-for-bit against golden vectors written
 by ``tests/golden/make_golden.py``, which imports the reference's own Python
 implementation (``unicache.storage.physical`` and friends) and records its

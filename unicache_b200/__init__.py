@@ -12,10 +12,13 @@ from .adapters import (
     batched_long_query_attention,
     fused_h2o_decode,
     fused_mixed_decode,
+    int8_block_decode,
     long_query_attention_summary,
     merge_attention_summaries,
+    sparse_int8_block_decode,
 )
 from .core import PhysicalCacheRequest
+from .kernels import head_norm_rope, rope_table
 from .operators import (
     H2OPhysicalGQAOperator,
     KIVIPackedQuantizationOperator,
@@ -27,6 +30,7 @@ from .storage import (
     CacheMutationResult,
     GQAH2OCache,
     HostPackedKIVI,
+    Int8BlockCache,
     PackedKIVICache,
     PhysicalLayerCache,
     PhysicalSegment,

@@ -84,6 +84,28 @@ class UcbDecodePair(ctypes.Structure):
     ]
 
 
+class UcbBlock8Cache(ctypes.Structure):
+    _fields_ = [
+        ("key_code", c_void_p),
+        ("value_code", c_void_p),
+        ("key_scale", c_void_p),
+        ("value_scale", c_void_p),
+        ("key_low", c_void_p),
+        ("key_high", c_void_p),
+        ("pending_key", c_void_p),
+        ("pending_value", c_void_p),
+        ("block_table", c_void_p),
+        ("lengths", c_void_p),
+        ("num_blocks", c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_tokens", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); the exact set declared in include/unicache_b200.h.
 SIGNATURES = {
     "ucb_last_error": (ctypes.c_char_p, []),
@@ -159,6 +181,19 @@ SIGNATURES = {
                                c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p]),
     "ucb_compact_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                  ctypes.POINTER(c_int64), c_void_p]),
+    "ucb_head_norm_rope": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int,
+                                   c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                   c_void_p]),
+    "ucb_block8_write": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                 c_void_p]),
+    "ucb_block8_read": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ucb_block8_select_workspace_bytes": (c_int64, [c_void_p]),
+    "ucb_block8_select": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+                                  c_void_p, c_void_p]),
+    "ucb_block8_attention_workspace_bytes": (c_int64, [c_void_p, c_int, c_int]),
+    "ucb_block8_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_int,
+                                     c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ucb_selftest_mma_subnormal": (c_int, [ctypes.POINTER(c_float), c_void_p]),
     "ucb_host_device_pointer": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "ucb_copy_ranges": (c_int, [c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64),

@@ -6,8 +6,10 @@ from .attention import (
     batched_long_query_attention,
     fused_h2o_decode,
     fused_mixed_decode,
+    int8_block_decode,
     long_query_attention_summary,
     merge_attention_summaries,
+    sparse_int8_block_decode,
 )
 
 __all__ = [
@@ -16,6 +18,8 @@ __all__ = [
     "batched_long_query_attention",
     "fused_h2o_decode",
     "fused_mixed_decode",
+    "int8_block_decode",
     "long_query_attention_summary",
     "merge_attention_summaries",
+    "sparse_int8_block_decode",
 ]

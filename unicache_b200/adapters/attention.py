@@ -17,6 +17,12 @@ unicache/adapters/bagel.py):
                                   segments (bagel.py:1598-1858 with q_len > 1)
 * ``batched_long_query_attention`` several samples' query blocks in one
                                   launch (bagel.py:773-980, varlen)
+
+and, over the growing 8-bit cache, which the reference has not:
+
+* ``int8_block_decode``           one to a few query tokens of every sequence
+* ``sparse_int8_block_decode``    one query token over the blocks that its
+                                  bounds choose
 """
 
 from __future__ import annotations
@@ -26,6 +32,7 @@ import math
 import torch
 
 from .. import kernels
+from ..storage.int8_block import Int8BlockCache
 from ..storage.physical import GQAH2OCache, PackedKIVICache
 
 
@@ -258,3 +265,19 @@ def long_query_attention_summary(query: torch.Tensor, segments: list, *, dense_k
     tables = kernels.long_query_tables([segs], hkv, [0], [lq * (hq // hkv)], query.device, include_residual)
     out, lse = kernels.long_query_attention(q, tables, num_kv_heads=hkv, staged=staged)
     return out.to(query.dtype), lse
+
+
+def int8_block_decode(query: torch.Tensor, cache: Int8BlockCache, *, softmax_scale: float | None = None):
+    """Causal attention of every sequence's last tokens, query [num_seqs, q_heads, head_dim] or
+    [num_seqs, queries, q_heads, head_dim], over the whole cache: (out, lse)."""
+
+    return kernels.block8_attention(query, cache, softmax_scale=softmax_scale)
+
+
+def sparse_int8_block_decode(query: torch.Tensor, cache: Int8BlockCache, *, count: int, first: int = 1,
+                             recent: int = 2, softmax_scale: float | None = None):
+    """Attention of query [num_seqs, q_heads, head_dim] over ``count`` blocks of each sequence and KV
+    head (``Int8BlockCache.select``): (blocks, out, lse)."""
+
+    blocks = kernels.block8_select(query, cache, count=count, first=first, recent=recent)
+    return (blocks, *kernels.block8_attention(query, cache, blocks=blocks, softmax_scale=softmax_scale))

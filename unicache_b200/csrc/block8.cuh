@@ -1,0 +1,48 @@
+// Shared pieces of the 8-bit block cache kernels (ucb_block8_*).
+#pragma once
+
+#include "common.cuh"
+
+namespace ucb {
+namespace block8 {
+
+constexpr float LEAST_SCALE = 7.52316384526264e-37f;  // 2^-120: 1 / scale stays finite, blocks of zeros have codes 0
+
+// A block's scale from the largest magnitude of its values.  NaN stays NaN.
+__device__ __forceinline__ float scale_of(float amax) {
+  const float s = __fdiv_rn(amax, 127.f);
+  return s < LEAST_SCALE ? LEAST_SCALE : s;
+}
+
+// clamp(rint(x * inverse)): the products that are not numbers (a NaN or infinite
+// input, whose scale is NaN or infinite) become 0, as __float2int_rn gives.
+__device__ __forceinline__ int code_of(float x, float inverse) {
+  const int c = __float2int_rn(__fmul_rn(x, inverse));
+  return max(-127, min(127, c));
+}
+
+// Pool block of a sequence's j-th block, -1 (and the error bit) when the table
+// names none.
+__device__ __forceinline__ int64_t pool_block(const ucb_block8_cache& c, int s, int j, unsigned int* err) {
+  const int b = c.block_table[(int64_t)s * c.max_blocks + j];
+  if (b < 0 || b >= c.num_blocks) {
+    atomicOr(err, DEVERR_BAD_DESCRIPTOR);
+    return -1;
+  }
+  return b;
+}
+
+// Tokens of a sequence, limited to what its table row can hold.
+__device__ __forceinline__ int held_tokens(const ucb_block8_cache& c, int s, unsigned int* err) {
+  const int n = c.lengths[s];
+  const int64_t most = (int64_t)c.max_blocks * c.block_tokens;
+  if (n >= 0 && n <= most) return n;
+  atomicOr(err, DEVERR_BAD_DESCRIPTOR);
+  return n < 0 ? 0 : (int)most;
+}
+
+// Checks that every entry point makes before it touches the GPU.
+int check_cache(const ucb_block8_cache* c, const char* what);
+
+}  // namespace block8
+}  // namespace ucb

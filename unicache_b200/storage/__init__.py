@@ -1,6 +1,7 @@
 """Physical storage layouts and their B200 kernels (counterpart of unicache/storage)."""
 
 from .hierarchy import HostPackedKIVI, QuantizedHostArchive, QuantizedWorkingSetTransition, to_host
+from .int8_block import Int8BlockCache
 from .kivi_b200 import (
     dequantize_kivi_chunk,
     packed_kivi_attention_parts,
@@ -22,6 +23,7 @@ __all__ = [
     "CacheMutationResult",
     "GQAH2OCache",
     "HostPackedKIVI",
+    "Int8BlockCache",
     "QuantizedHostArchive",
     "QuantizedWorkingSetTransition",
     "PackedKIVICache",
