@@ -412,6 +412,27 @@ def test_poisoned_blocks_show_and_stale_rows_do_not():
     assert out[0].isfinite().all()  # unused rows, blocks and scales are garbage (make_cache)
 
 
+def test_poison_of_later_tokens_stays_out_of_earlier_rows():
+    """Four tokens written at once, the last alone in its block with a NaN and an infinity: the rows
+    before it do not see that block."""
+
+    need_gpu()
+    for block in (16, 64):
+        lengths = [block * 3 + 1]
+        cache, gen = make_cache(lengths, block=block)
+        key, value = (make_rows(gen, lengths, 4, 128, torch.bfloat16) for _ in range(2))
+        key[-1, 0, 3], value[-1, 1, 2], value[-1, 2, 9] = float("nan"), float("nan"), float("inf")
+        cache.advance(lengths[0])
+        cache.write(key, value, starts=starts_of(lengths))
+        query = make_query(gen, (1, 4, 28, 128), torch.bfloat16)
+        out, lse = cache.attention(query)
+        clean, _, _, _ = filled([block * 3], block=block)
+        clean.write(key[:-1], value[:-1], starts=starts_of([block * 3]))
+        expect, expect_lse = clean.attention(query[:, :3])
+        assert torch.allclose(out[:, :3].float(), expect.float(), atol=2e-2) and torch.allclose(lse[:, :3], expect_lse)
+        assert out[0, 3, :21].isnan().any(-1).all() and out[0, 3, 21:].isfinite().all()
+
+
 def test_code_offsets_past_32_bits():
     need_gpu()
     heads, dim, block = 8, 128, 128

@@ -198,14 +198,16 @@ class Int8BlockCache:
 
         return kernels.block8_attention(query, self, blocks=blocks, softmax_scale=softmax_scale)
 
-    def attention_workspace(self, queries: int, q_heads: int) -> torch.Tensor | None:
+    def attention_workspace(self, queries: int, q_heads: int) -> torch.Tensor:
         """Scratch of one attention launch, on the current stream."""
 
         size = self._workspace_bytes.get((queries, q_heads))
         if size is None:
             size = int(_capi.load().ucb_block8_attention_workspace_bytes(self.descriptor, queries, q_heads))
+            if size < 0:
+                raise RuntimeError("the device of the block cache is unavailable")
             self._workspace_bytes[(queries, q_heads)] = size
-        return torch.empty(size, device=self.device, dtype=torch.uint8) if size else None
+        return torch.empty(size, device=self.device, dtype=torch.uint8)
 
     # ---------------------------------------------------------------- accounting
     @property
