@@ -26,9 +26,12 @@
 // Arithmetic: codes become fp16 exactly (bytes placed under 1024's exponent, minus
 // 1152); a query row is scaled by a power of two to at most 2^14 and held in
 // fp16 (bf16 and fp16 rows exactly, but for elements 2^-28 of the row's largest);
-// logits, sums and outputs in fp32.  Weights are rounded to fp16 for
-// the value product only, at 2^6 to 2^14 times their softmax value relative to the
-// running reference, so that weights down to 2^-20 keep 11 bits.
+// logits, sums and outputs in fp32.  A weight is rounded to fp16 for the value
+// product only, after its block's value scale has been added to its exponent, and
+// relative to the largest such product so far (at 2^6, up to 2^14 before the
+// reference moves): every contribution to the output above 2^-20 of the largest
+// keeps 11 bits, whatever the blocks' scales are.  The sum of weights is kept
+// in fp32 against a reference of its own.
 #include <algorithm>
 
 #include "block8.cuh"
@@ -44,29 +47,33 @@ struct AttnParams {
   int queries, q_heads, group, rows, row_tiles;  // rows = group * queries of a KV head
   const int32_t* blocks;
   int selected;
-  int tile_shift;    // log2(tiles of 16 tokens in a block)
+  int q_aligned;     // query rows can be read 8 bytes at a time
+  int step_shift;    // log2(steps in a block)
   float scale_log2;  // softmax scale * log2(e)
   void* out;
   float* lse;
   float* partials;  // [2 * grid] states of pairs that cross CTAs
+  float* spill;     // [grid * warps] states of segments that are not a warp's last
   int* links;       // [grid][4]: last CTA of the pair that starts in this CTA and goes on (-1: none), s, h, row tile
   unsigned int* err;
 };
 
-constexpr int TILE = 16;
-constexpr int MIN_TILES = 2;  // a warp's least share, where there is more than that
-constexpr float LIFT = 6.f;   // log2 of a weight at the reference maximum
-constexpr float LAZY = 14.f;  // a weight may reach 2^LAZY before the reference moves
+constexpr int TILE = 16;     // tokens of one matrix product
+constexpr int MIN_STEPS = 1;  // a warp's least share, where there is more than that
+constexpr float LIFT = 6.f;   // log2 of the largest weight when its reference is set
+constexpr float LAZY = 14.f;  // a weight may reach 2^LAZY before its reference moves
+constexpr float LAZY_SUM = 100.f;
 
-template <int D, int NT> struct Shape {
+// U tiles of 16 tokens a step: two, or one where a block is a single tile.
+template <int D, int NT, int U> struct Shape {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int WARPS = NT == 1 ? 12 : 8;
-  static constexpr int STAGES = D == 64 ? 6 : NT == 1 ? 3 : 4;
-  static constexpr int STAGE_BYTES = 2 * TILE * D;
-  static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, reference, sum, padding
-  static constexpr int STATE_BYTES = ROWS * ROW_FLOATS * 4;
-  static constexpr int RING_BYTES = STAGES * STAGE_BYTES > STATE_BYTES ? STAGES * STAGE_BYTES : STATE_BYTES;
-  static constexpr int WARP_BYTES = RING_BYTES + STATE_BYTES;
+  static constexpr int WARPS = D == 128 && NT == 2 ? 8 : 12;
+  static constexpr int TILE_BYTES = 2 * TILE * D;
+  static constexpr int STAGES = D == 64 || U == 1 ? 4 : 2;
+  static constexpr int STAGE_BYTES = U * TILE_BYTES;
+  static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its reference, the sum's reference, the sum
+  static constexpr int STATE_FLOATS = ROWS * ROW_FLOATS;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES > STATE_FLOATS * 4 ? STAGES * STAGE_BYTES : STATE_FLOATS * 4;
 };
 
 __device__ __forceinline__ void cp_async16_some(uint32_t dst, const void* src, int bytes) {
@@ -86,76 +93,90 @@ __device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t select) {
   return y;
 }
 
-// A (sequence, KV head, row tile) triple and where a share of its tiles begins.
+// A (sequence, KV head, row tile) triple and where its steps begin in the flat order.
 struct Pair {
-  int s, h, rt, tiles;
-  int64_t base;  // flat index of its first tile
+  int s, h, rt, steps;
+  int64_t base;
 };
 
-// Segment of one warp in shared memory, for the merge of its CTA.
+// Segment of one warp, for the merge of its CTA.
 struct Segment {
-  int used, ends;  // ends: holds the pair's last tile
+  int used, ends;  // ends: holds the pair's last step
   int s, h, rt;
+  const float* state;
 };
 
-template <typename T, int D>
-__device__ __forceinline__ void write_row(const AttnParams& p, int s, int h, int row, int d0, const float* o, int n,
-                                          float inverse) {
-  const int l = row / p.group, head = h * p.group + row % p.group;
-  T* out = static_cast<T*>(p.out) + (((int64_t)s * p.queries + l) * p.q_heads + head) * D + d0;
-  for (int i = 0; i < n; ++i) out[i] = Dtype<T>::from_f(o[i] * inverse);
+__device__ __forceinline__ float load_element(const AttnParams& p, const void* q, int64_t at) {
+  return p.c.dtype == UCB_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(q)[at])
+                               : __half2float(static_cast<const __half*>(q)[at]);
 }
 
-__device__ __forceinline__ void write_lse(const AttnParams& p, int s, int h, int row, float ref, float sum) {
-  const int l = row / p.group, head = h * p.group + row % p.group;
-  if (p.lse)
-    p.lse[((int64_t)s * p.queries + l) * p.q_heads + head] =
-        sum == 0.f ? -INFINITY : (ref == -INFINITY ? sum : (ref + log2f(sum)) * 0.693147180559945309f);
+__device__ __forceinline__ uint32_t pack_out(const AttnParams& p, float lo, float hi) {
+  return p.c.dtype == UCB_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
 
-// A row's states merged: reference, sum and one channel.  A state without a token has
-// reference -inf and sum 0; products, not branches, so that a NaN comes through.
+__device__ __forceinline__ int64_t out_row(const AttnParams& p, int s, int h, int row) {
+  return ((int64_t)s * p.queries + row / p.group) * p.q_heads + h * p.group + row % p.group;
+}
+
+__device__ __forceinline__ void write_lse(const AttnParams& p, int64_t row, float ref, float sum) {
+  if (p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (ref == -INFINITY ? sum : (ref + log2f(sum)) * 0.693147180559945309f);
+}
+
+// 2^(ref - sum_ref) / sum, the factor of an unnormalised row; 0 where no token was seen.
+__device__ __forceinline__ float normaliser(float ref, float sum_ref, float sum) {
+  return sum == 0.f || (ref == -INFINITY && sum == sum) ? 0.f : exp2f(ref - sum_ref) / sum;
+}
+
+// States of one row and channel merged.  A state without a token has references -inf and sum 0; products, not
+// branches, so that a NaN comes through.
 struct Merged {
-  float ref, sum, value;
+  float value, ref, sum_ref, sum;
 };
 template <typename Get> __device__ __forceinline__ Merged merge_states(int n, Get get) {
-  Merged m{-INFINITY, 0.f, 0.f};
-  for (int i = 0; i < n; ++i) m.ref = fmaxf(m.ref, get(i).ref);
+  Merged m{0.f, -INFINITY, -INFINITY, 0.f};
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
     const Merged x = get(i);
-    const float f = x.ref == -INFINITY ? 0.f : fast_exp2(x.ref - m.ref);
-    m.sum = fmaf(f, x.sum, m.sum);
-    m.value = fmaf(f, x.value, m.value);
+    m.ref = fmaxf(m.ref, x.ref);
+    m.sum_ref = fmaxf(m.sum_ref, x.sum_ref);
+  }
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const Merged x = get(i);
+    m.value = fmaf(x.ref == -INFINITY ? 0.f : fast_exp2(x.ref - m.ref), x.value, m.value);
+    m.sum = fmaf(x.sum_ref == -INFINITY ? 0.f : fast_exp2(x.sum_ref - m.sum_ref), x.sum, m.sum);
   }
   return m;
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(const AttnParams p) {
-  using S = Shape<D, NT>;
-  constexpr int MT = D / 16;        // value products of 16 channels
-  constexpr int KS = D / 16;        // key products of 16 channels
-  constexpr int VB = D / 8;         // bytes of a value row that a lane holds
+template <int D, int NT, int U>
+__global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kernel(const AttnParams p) {
+  using S = Shape<D, NT, U>;
+  constexpr int MT = D / 16;          // value products of 16 channels
+  constexpr int KS = D / 16;          // key products of 16 channels
+  constexpr int VB = D / 8;           // bytes of a value row that a lane holds
+  constexpr int STEP = U * TILE;      // tokens of a step
   const ucb_block8_cache& c = p.c;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Segment segments[S::WARPS][2];
   __shared__ int warp_sums[S::WARPS];
-  int* prefix = reinterpret_cast<int*>(smem + S::WARPS * S::WARP_BYTES);  // [num_seqs + 1], dense only
+  int* prefix = reinterpret_cast<int*>(smem + S::WARPS * S::RING_BYTES);  // [num_seqs + 1], dense only
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cq = lane & 3;
   const int bt = c.block_tokens, heads_rows = c.kv_heads * p.row_tiles;
-  const int tiles_in_block = 1 << p.tile_shift;
+  const int step_mask = (1 << p.step_shift) - 1;
 
-  // ---- the flat order: tiles of every sequence (at least one, so that every row is written)
+  // ---- the flat order: steps of every sequence (at least one, so that every row is written)
   int64_t total;
-  const int listed_tiles = p.selected << p.tile_shift;
+  const int listed_steps = p.selected << p.step_shift;
   if (p.blocks) {
-    total = (int64_t)c.num_seqs * listed_tiles * heads_rows;
+    total = (int64_t)c.num_seqs * listed_steps * heads_rows;
   } else {
     int carry = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int base = 0; base < c.num_seqs; base += S::WARPS * 32) {
       const int i = base + threadIdx.x;
-      int v = i < c.num_seqs ? max(1, (held_tokens(c, i, p.err) + TILE - 1) / TILE) : 0;
+      int v = i < c.num_seqs ? max(1, (int)(((int64_t)held_tokens(c, i, p.err) + STEP - 1) / STEP)) : 0;
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
@@ -172,46 +193,45 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
     }
     total = (int64_t)carry * heads_rows;
   }
-  const int64_t all_workers = (int64_t)gridDim.x * S::WARPS;
-  const int64_t workers = max((int64_t)1, min(all_workers, total / MIN_TILES));
+  const int64_t workers = max((int64_t)1, min((int64_t)gridDim.x * S::WARPS, total / MIN_STEPS));
   const int64_t worker = (int64_t)blockIdx.x * S::WARPS + warp;
   if (lane == 0) segments[warp][0].used = segments[warp][1].used = 0;
   auto share = [&](int64_t w) { return w >= workers ? total : total * w / workers; };
   auto locate = [&](int64_t t) {
     Pair a;
     if (p.blocks) {
-      const int64_t pair = t / listed_tiles;
+      const int64_t pair = t / listed_steps;
       a.s = (int)(pair / heads_rows);
-      a.tiles = listed_tiles;
+      a.steps = listed_steps;
       const int u = (int)(pair % heads_rows);
       a.h = u / p.row_tiles;
       a.rt = u % p.row_tiles;
-      a.base = pair * listed_tiles;
+      a.base = pair * listed_steps;
     } else {
       const int unit = (int)(t / heads_rows);
-      int lo = 0, hi = c.num_seqs - 1;  // the last sequence whose first tile is not after t
+      int lo = 0, hi = c.num_seqs - 1;  // the last sequence whose first step is not after t
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (prefix[mid] <= unit) lo = mid; else hi = mid - 1;
       }
       a.s = lo;
-      a.tiles = prefix[lo + 1] - prefix[lo];
+      a.steps = prefix[lo + 1] - prefix[lo];
       const int64_t first = (int64_t)prefix[lo] * heads_rows;
-      const int u = (int)((t - first) / a.tiles);
+      const int u = (int)((t - first) / a.steps);
       a.h = u / p.row_tiles;
       a.rt = u % p.row_tiles;
-      a.base = first + (int64_t)u * a.tiles;
+      a.base = first + (int64_t)u * a.steps;
     }
     return a;
   };
 
-  unsigned char* ring = smem + warp * S::WARP_BYTES;
+  unsigned char* ring = smem + warp * S::RING_BYTES;
   const uint32_t ring_at = smem_u32(ring);
   int64_t t = share(worker);
   const int64_t t_end = share(worker + 1);
   if (worker < workers) while (t < t_end) {
     const Pair a = locate(t);
-    const int begin = (int)(t - a.base), end = (int)min((int64_t)a.tiles, t_end - a.base);
+    const int begin = (int)(t - a.base), end = (int)min((int64_t)a.steps, t_end - a.base);
     t = a.base + end;
     const int len = held_tokens(c, a.s, p.err);
     const int32_t* list = p.blocks ? p.blocks + ((int64_t)a.s * c.kv_heads + a.h) * p.selected : nullptr;
@@ -221,7 +241,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
     // ---- block descriptors: lane i holds entry window + i, `next` the 32 entries after
     struct Entry {
       int block, token;
-      float ks, vs;
+      float ks, lv;  // key scale, log2 of the value scale
     };
     auto fetch = [&](int k) {
       Entry e{-1, 0, 0.f, 0.f};
@@ -240,11 +260,45 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
       if (e.block >= 0) {
         const int64_t at = (int64_t)e.block * c.kv_heads + a.h;
         e.ks = c.key_scale[at];
-        e.vs = c.value_scale[at];
+        e.lv = log2f(c.value_scale[at]);
       }
     };
-    int window = begin >> p.tile_shift;
+    int window = begin >> p.step_shift;
     Entry now = fetch(window + lane), next = fetch(window + 32 + lane);
+
+    auto issue = [&](int i) {
+      if (i < end) {
+        const int rel = (i >> p.step_shift) - window;
+        const int block = __shfl_sync(0xffffffffu, rel < 32 ? now.block : next.block, rel & 31);
+        const int token = __shfl_sync(0xffffffffu, rel < 32 ? now.token : next.token, rel & 31);
+        const int row0 = (i & step_mask) * STEP, n = len - token - row0;
+        if (block >= 0 && n > 0) {
+          const int64_t at = (((int64_t)block * c.kv_heads + a.h) * bt + row0) * D;
+          const int8_t* k = c.key_code + at + r * D + 16 * cq;
+          const int8_t* v = c.value_code + at + 2 * cq * D + VB * r;
+          const uint32_t to = ring_at + ((i - begin) % S::STAGES) * S::STAGE_BYTES;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {  // (token r or r + 8, low or high half of the channels)
+              const int tok = u * TILE + (x & 1) * 8, ch = (x >> 1) * 64;
+              cp_async16_some(to + u * S::TILE_BYTES + x * 512 + lane * 16, k + tok * D + ch, r + tok < n ? 16 : 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int tok = u * TILE + (x & 1) + (x & 2) * 4;
+              const int bytes = 2 * cq + tok < n ? VB : 0;
+              const uint32_t at_slot = to + u * S::TILE_BYTES + TILE * D + (x * 32 + lane) * VB;
+              if (D == 128) cp_async16_some(at_slot, v + tok * D, bytes);
+              else cp_async8_some(at_slot, v + tok * D, bytes);
+            }
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int x = 0; x < S::STAGES - 1; ++x) issue(begin + x);
     fetch_scales(now);
     bool next_scaled = false;
 
@@ -255,17 +309,30 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
     for (int nt = 0; nt < NT; ++nt) {
       const int row = a.rt * S::ROWS + nt * 8 + r;
       const bool real = row < p.rows;
-      const T* q = static_cast<const T*>(p.q) + a.s * p.q_ss + (real ? row / p.group : 0) * p.q_sl +
-                   (a.h * p.group + (real ? row % p.group : 0)) * p.q_sh;
+      const int64_t q0 = a.s * p.q_ss + (real ? row / p.group : 0) * p.q_sl +
+                         (a.h * p.group + (real ? row % p.group : 0)) * p.q_sh;
       float x[KS][4];
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
+      for (int i = 0; i < KS; ++i) {
+        const int64_t at = q0 + 64 * (i / 4) + 16 * cq + 4 * (i % 4);
+        if (p.q_aligned) {
+          const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at);
+          const bool bf = c.dtype == UCB_BF16;
+          x[i][0] = bf ? Dtype<__nv_bfloat16>::lo(w.x) : Dtype<__half>::lo(w.x);
+          x[i][1] = bf ? Dtype<__nv_bfloat16>::hi(w.x) : Dtype<__half>::hi(w.x);
+          x[i][2] = bf ? Dtype<__nv_bfloat16>::lo(w.y) : Dtype<__half>::lo(w.y);
+          x[i][3] = bf ? Dtype<__nv_bfloat16>::hi(w.y) : Dtype<__half>::hi(w.y);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[i][k] = load_element(p, p.q, at + k);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          x[i][k] = real ? Dtype<T>::to_f(q[64 * (i / 4) + 16 * cq + 4 * (i % 4) + k]) : 0.f;
+          if (!real) x[i][k] = 0.f;
           top = fmaxf(top, fabsf(x[i][k]));
         }
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // power of two that brings the largest element to [2^13, 2^14); both factors are normal numbers
@@ -290,73 +357,20 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
       }
     const int sure = len - p.queries + 1;  // tokens that every row sees
 
-    float o[NT][MT][4], acc[NT][MT][4], ref[NT][2], sum[NT][2];
+    // Unnormalised output and its reference (of s + log2 value scale), sum of weights and its own (of s).
+    float o[NT][MT][4], ref[NT][2], sum[NT][2], sum_ref[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      ref[nt][0] = ref[nt][1] = -INFINITY;
+      ref[nt][0] = ref[nt][1] = sum_ref[nt][0] = sum_ref[nt][1] = -INFINITY;
       sum[nt][0] = sum[nt][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[nt][j][k] = acc[nt][j][k] = 0.f;
+        for (int k = 0; k < 4; ++k) o[nt][j][k] = 0.f;
     }
-    float open_scale = 0.f;
-    int open_entry = -1, open_token = 0;
-    // the open block's products, times its scale, into the output; a row that sees none of the block takes
-    // nothing of it, a scale that is not a number included
-    auto flush = [&]() {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float scale[2] = {open_token < col_limit[nt][0] ? open_scale : 0.f,
-                                open_token < col_limit[nt][1] ? open_scale : 0.f};
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            o[nt][j][k] = fmaf(acc[nt][j][k], scale[k & 1], o[nt][j][k]);
-            acc[nt][j][k] = 0.f;
-          }
-      }
-    };
 
-    auto issue = [&](int i) {
-      if (i < end) {
-        const int rel = (i >> p.tile_shift) - window;
-        const int block = __shfl_sync(0xffffffffu, rel < 32 ? now.block : next.block, rel & 31);
-        const int token = __shfl_sync(0xffffffffu, rel < 32 ? now.token : next.token, rel & 31);
-        const int row0 = (i & (tiles_in_block - 1)) * TILE, n = len - token - row0;
-        if (block >= 0 && n > 0) {
-          const int64_t at = (((int64_t)block * c.kv_heads + a.h) * bt + row0) * D;
-          const int8_t* k = c.key_code + at + r * D + 16 * cq;
-          const int8_t* v = c.value_code + at + 2 * cq * D + VB * r;
-          const uint32_t to = ring_at + ((i - begin) % S::STAGES) * S::STAGE_BYTES;
-          const int k0 = r < n ? 16 : 0, k1 = r + 8 < n ? 16 : 0;
-          cp_async16_some(to + lane * 16, k, k0);
-          cp_async16_some(to + 512 + lane * 16, k + 8 * D, k1);
-          if (D == 128) {
-            cp_async16_some(to + 1024 + lane * 16, k + 64, k0);
-            cp_async16_some(to + 1536 + lane * 16, k + 8 * D + 64, k1);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int tok = 2 * cq + (x & 1) + (x & 2) * 4;
-              cp_async16_some(to + 2048 + x * 512 + lane * 16, v + ((x & 1) + (x & 2) * 4) * D, tok < n ? 16 : 0);
-            }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int tok = 2 * cq + (x & 1) + (x & 2) * 4;
-              cp_async8_some(to + 1024 + x * 256 + lane * 8, v + ((x & 1) + (x & 2) * 4) * D, tok < n ? 8 : 0);
-            }
-          }
-        }
-      }
-      cp_async_commit();
-    };
-
-#pragma unroll
-    for (int x = 0; x < S::STAGES - 1; ++x) issue(begin + x);
     for (int i = begin; i < end; ++i) {
-      int entry = i >> p.tile_shift;
+      const int entry = i >> p.step_shift;
       if (entry - window >= 32) {
         if (!next_scaled) fetch_scales(next);
         now = next;
@@ -368,70 +382,79 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
         next_scaled = true;
       }
       cp_async_wait<S::STAGES - 2>();
-      issue(i + S::STAGES - 1);  // into the slot of the tile before, whose values were used
+      issue(i + S::STAGES - 1);  // into the slot of the step before, whose values were used
       const int rel = entry - window;
       const int block = __shfl_sync(0xffffffffu, now.block, rel);
-      const int first_token = __shfl_sync(0xffffffffu, now.token, rel) + (i & (tiles_in_block - 1)) * TILE;
+      const int first_token = __shfl_sync(0xffffffffu, now.token, rel) + (i & step_mask) * STEP;
       if (block < 0 || first_token >= len) continue;
       const float ks = __shfl_sync(0xffffffffu, now.ks, rel);
-      if (entry != open_entry) {
-        if (open_entry >= 0) flush();
-        open_entry = entry;
-        open_scale = __shfl_sync(0xffffffffu, now.vs, rel);
-        open_token = __shfl_sync(0xffffffffu, now.token, rel);
-      }
+      const float lv = __shfl_sync(0xffffffffu, now.lv, rel);
       const unsigned char* slot = ring + ((i - begin) % S::STAGES) * S::STAGE_BYTES;
 
       // ---- logits of 16 tokens (rows) and 8 query rows (columns)
-      float s[NT][4];
+      float s[U][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int u = 0; u < U; ++u) {
+        float part[KS / 4][NT][4];
 #pragma unroll
-      for (int half = 0; half < KS / 4; ++half) {
-        const uint4 ka = *reinterpret_cast<const uint4*>(slot + half * 1024 + lane * 16);
-        const uint4 kb = *reinterpret_cast<const uint4*>(slot + half * 1024 + 512 + lane * 16);
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        for (int half = 0; half < KS / 4; ++half) {
+          const unsigned char* at = slot + u * S::TILE_BYTES + half * 1024 + lane * 16;
+          const uint4 ka = *reinterpret_cast<const uint4*>(at);
+          const uint4 kb = *reinterpret_cast<const uint4*>(at + 512);
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
-          const uint32_t f[4] = {halves(xa, 0x4140), halves(xb, 0x4140), halves(xa, 0x4342), halves(xb, 0x4342)};
+          for (int nt = 0; nt < NT; ++nt) part[half][nt][0] = part[half][nt][1] = part[half][nt][2] = part[half][nt][3] = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], f, qb[nt][half * 4 + w][0], qb[nt][half * 4 + w][1]);
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
+            const uint32_t f[4] = {halves(xa, 0x4140), halves(xb, 0x4140), halves(xa, 0x4342), halves(xb, 0x4342)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(part[half][nt], f, qb[nt][half * 4 + w][0], qb[nt][half * 4 + w][1]);
+          }
         }
-      }
-
-      // ---- weights 2^(s - ref)
-      bool move = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[nt][k] *= col_scale[nt][k & 1] * ks;
-      if (first_token + TILE > sure) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (first_token + r + (k & 2) * 4 >= col_limit[nt][k & 1]) s[nt][k] = -INFINITY;
+            s[u][nt][k] = (KS == 8 ? part[0][nt][k] + part[KS / 4 - 1][nt][k] : part[0][nt][k]) * (col_scale[nt][k & 1] * ks);
       }
+      const bool masked = first_token + STEP > sure;
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (first_token + u * TILE + r + (k & 2) * 4 >= col_limit[nt][k & 1]) s[u][nt][k] = -INFINITY;
+      }
+
+      // ---- references
+      float top[NT][2];
+      bool move = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) move |= fmaxf(s[nt][k], s[nt][k + 2]) > ref[nt][k] + LAZY;
+        for (int k = 0; k < 2; ++k) {
+          top[nt][k] = fmaxf(s[0][nt][k], s[0][nt][k + 2]);
+          if (U == 2) top[nt][k] = fmaxf(top[nt][k], fmaxf(s[U - 1][nt][k], s[U - 1][nt][k + 2]));
+          move |= top[nt][k] > fminf(ref[nt][k] - lv + LAZY, sum_ref[nt][k] + LAZY_SUM);
+        }
       if (__any_sync(0xffffffffu, move)) {
-        flush();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float top = fmaxf(s[nt][k], s[nt][k + 2]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float to = fmaxf(ref[nt][k], top - LIFT);
-            const float f = ref[nt][k] == -INFINITY ? 0.f : fast_exp2(ref[nt][k] - to);
+            float m = top[nt][k];
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            const float to = fmaxf(ref[nt][k], m + lv - LIFT), sum_to = fmaxf(sum_ref[nt][k], m);
             // a NaN that the sums already hold stays: 0 * NaN
-            sum[nt][k] *= f;
+            const float f = ref[nt][k] == -INFINITY ? 0.f : fast_exp2(ref[nt][k] - to);
+            sum[nt][k] *= sum_ref[nt][k] == -INFINITY ? 0.f : fast_exp2(sum_ref[nt][k] - sum_to);
             ref[nt][k] = to;
+            sum_ref[nt][k] = sum_to;
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               o[nt][j][k] *= f;
@@ -439,53 +462,67 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
             }
           }
       }
-      uint32_t pb[NT][2];
+
+      // ---- weights, times the value scale for the output
+      uint32_t pb[U][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
+        float base[2], sum_base[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float base = ref[nt][k & 1];
-          w[k] = fast_exp2(s[nt][k] - (base == -INFINITY ? 0.f : base));
+        for (int k = 0; k < 2; ++k) {
+          base[k] = ref[nt][k] == -INFINITY ? (lv == lv ? INFINITY : lv) : ref[nt][k] - lv;
+          sum_base[k] = sum_ref[nt][k] == -INFINITY ? 0.f : sum_ref[nt][k];
         }
-        sum[nt][0] += w[0] + w[2];
-        sum[nt][1] += w[1] + w[3];
-        pb[nt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
-        pb[nt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            w[k] = fast_exp2(s[u][nt][k] - base[k & 1]);
+            if (masked && s[u][nt][k] == -INFINITY) w[k] = 0.f;  // whatever the block's scale is
+            sum[nt][k & 1] += fast_exp2(s[u][nt][k] - sum_base[k & 1]);
+          }
+          pb[u][nt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
+          pb[u][nt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
+        }
       }
 
       // ---- output: channels (rows) of 16 tokens times the weights
-      uint32_t vw[4][D / 32];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4*>(slot + 2048 + x * 512 + lane * 16);
-          vw[x][0] = v.x, vw[x][1] = v.y, vw[x][D / 32 - 2] = v.z, vw[x][D / 32 - 1] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(slot + 1024 + x * 256 + lane * 8);
-          vw[x][0] = v.x, vw[x][1] = v.y;
+      for (int u = 0; u < U; ++u) {
+        uint32_t vw[4][D / 32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const unsigned char* at = slot + u * S::TILE_BYTES + TILE * D + (x * 32 + lane) * VB;
+          if (D == 128) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            vw[x][0] = v.x, vw[x][1] = v.y, vw[x][D / 32 - 2] = v.z, vw[x][D / 32 - 1] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            vw[x][0] = v.x, vw[x][1] = v.y;
+          }
         }
-      }
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        const uint32_t w0 = vw[0][w] ^ 0x80808080u, w1 = vw[1][w] ^ 0x80808080u;
-        const uint32_t w2 = vw[2][w] ^ 0x80808080u, w3 = vw[3][w] ^ 0x80808080u;
+        for (int w = 0; w < D / 32; ++w) {
+          const uint32_t w0 = vw[0][w] ^ 0x80808080u, w1 = vw[1][w] ^ 0x80808080u;
+          const uint32_t w2 = vw[2][w] ^ 0x80808080u, w3 = vw[3][w] ^ 0x80808080u;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {  // channel pairs (4w, 4w + 1) and (4w + 2, 4w + 3) of the lane's run
-          const uint32_t x01 = prmt(w0, w1, y ? 0x7362 : 0x5140), x23 = prmt(w2, w3, y ? 0x7362 : 0x5140);
-          const uint32_t f[4] = {halves(x01, 0x4140), halves(x01, 0x4342), halves(x23, 0x4140), halves(x23, 0x4342)};
+          for (int y = 0; y < 2; ++y) {  // channel pairs (4w, 4w + 1) and (4w + 2, 4w + 3) of the lane's run
+            const uint32_t x01 = prmt(w0, w1, y ? 0x7362 : 0x5140), x23 = prmt(w2, w3, y ? 0x7362 : 0x5140);
+            const uint32_t f[4] = {halves(x01, 0x4140), halves(x01, 0x4342), halves(x23, 0x4140), halves(x23, 0x4342)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][2 * w + y], f, pb[nt][0], pb[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + y], f, pb[u][nt][0], pb[u][nt][1]);
+          }
         }
       }
     }
     cp_async_wait<0>();
-    if (open_entry >= 0) flush();
 
-    // ---- the segment's result: lane (r, cq) holds channels VB * r .. of rows 2 cq and 2 cq + 1
-    const bool whole = begin == 0 && end == a.tiles;
+    // ---- the segment's result: lane (r, cq) holds channels VB * r .. of rows 2 cq and 2 cq + 1.  A warp's last
+    // segment stays in its ring, an earlier one that a warp before began goes through global memory.
+    const bool whole = begin == 0 && end == a.steps;
     const int which = begin == 0 ? 1 : 0;
-    float* state = reinterpret_cast<float*>(which ? ring : ring + S::RING_BYTES);
+    float* state = t >= t_end ? reinterpret_cast<float*>(ring) : p.spill + worker * S::STATE_FLOATS;
     __syncwarp();  // every lane is done with the ring before states overwrite it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -496,55 +533,65 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int in_tile = nt * 8 + 2 * cq + k, row = a.rt * S::ROWS + in_tile;
-        float run[2 * MT];
+        const float f = whole ? normaliser(ref[nt][k], sum_ref[nt][k], l) : 1.f;
+        float run[VB];
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          run[2 * j] = o[nt][j][k];
-          run[2 * j + 1] = o[nt][j][k + 2];
+          run[2 * j] = o[nt][j][k] * f;
+          run[2 * j + 1] = o[nt][j][k + 2] * f;
         }
         if (whole) {
           if (row < p.rows) {
-            write_row<T, D>(p, a.s, a.h, row, VB * r, run, VB, l == 0.f ? 0.f : __fdividef(1.f, l));
-            if (r == 0) write_lse(p, a.s, a.h, row, ref[nt][k], l);
+            const int64_t to = out_row(p, a.s, a.h, row);
+            uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D + VB * r);
+#pragma unroll
+            for (int i = 0; i < VB / 8; ++i)
+              out[i] = make_uint4(pack_out(p, run[8 * i], run[8 * i + 1]), pack_out(p, run[8 * i + 2], run[8 * i + 3]),
+                                  pack_out(p, run[8 * i + 4], run[8 * i + 5]), pack_out(p, run[8 * i + 6], run[8 * i + 7]));
+            if (r == 0) write_lse(p, to, sum_ref[nt][k], l);
           }
         } else {
           float* at = state + in_tile * S::ROW_FLOATS;
 #pragma unroll
           for (int i = 0; i < VB; i += 4)
             *reinterpret_cast<float4*>(at + VB * r + i) = make_float4(run[i], run[i + 1], run[i + 2], run[i + 3]);
-          if (r == 0) at[D] = ref[nt][k], at[D + 1] = l;
+          if (r == 0) at[D] = ref[nt][k], at[D + 1] = sum_ref[nt][k], at[D + 2] = l;
         }
       }
-    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == a.tiles, a.s, a.h, a.rt};
+    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == a.steps, a.s, a.h, a.rt, state};
   }
   __syncthreads();
 
   // ---- chains of segments of one pair: complete ones are written, the CTA's first and last may go on
   // in other CTAs.  A warp's slot 0 continues the pair that was open before it, slot 1 opens one.
-  auto state_of = [&](int w, int which) {
-    return reinterpret_cast<const float*>(smem + w * S::WARP_BYTES + (which ? 0 : S::RING_BYTES));
-  };
   if (threadIdx.x == 0) p.links[blockIdx.x * 4] = -1;
   int open_w = 0, open_which = 0, open_n = 0;  // the open chain: first segment and count
   bool from_before = false;
   auto emit = [&](const Segment& seg, bool ended) {
-    const int n = open_n, w0 = open_w, which0 = open_which;
     const bool complete = ended && !from_before;
-    float* to = p.partials + ((int64_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * (S::ROWS * S::ROW_FLOATS);
-    for (int item = threadIdx.x; item < S::ROWS * D; item += S::WARPS * 32) {
-      const int in_tile = item / D, d = item % D, row = seg.rt * S::ROWS + in_tile;
+    float* to = p.partials + ((int64_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * S::STATE_FLOATS;
+    for (int item = threadIdx.x; item < S::ROWS * D / 2; item += S::WARPS * 32) {
+      const int in_tile = item / (D / 2), d = item % (D / 2) * 2, row = seg.rt * S::ROWS + in_tile;
       if (row >= p.rows) break;
-      const Merged m = merge_states(n, [&](int i) {
-        const float* at = state_of(w0 + i, i ? 0 : which0) + in_tile * S::ROW_FLOATS;
-        return Merged{at[D], at[D + 1], at[d]};
+      float second = 0.f;
+      auto state = [&](int i) { return segments[open_w + i][i ? 0 : open_which].state + in_tile * S::ROW_FLOATS; };
+      const Merged m = merge_states(open_n, [&](int i) {
+        const float* at = state(i);
+        return Merged{at[d], at[D], at[D + 1], at[D + 2]};
       });
+      for (int i = 0; i < open_n; ++i) {
+        const float* at = state(i);
+        second = fmaf(at[D] == -INFINITY ? 0.f : fast_exp2(at[D] - m.ref), at[d + 1], second);
+      }
       if (complete) {
-        const float value = m.sum == 0.f ? 0.f : m.value / m.sum;
-        write_row<T, D>(p, seg.s, seg.h, row, d, &value, 1, 1.f);
-        if (d == 0) write_lse(p, seg.s, seg.h, row, m.ref, m.sum);
+        const float f = normaliser(m.ref, m.sum_ref, m.sum);
+        const int64_t out = out_row(p, seg.s, seg.h, row);
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + out * D + d) = pack_out(p, m.value * f, second * f);
+        if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
       } else {
-        to[in_tile * S::ROW_FLOATS + d] = m.value;
-        if (d == 0) to[in_tile * S::ROW_FLOATS + D] = m.ref, to[in_tile * S::ROW_FLOATS + D + 1] = m.sum;
+        float* at = to + in_tile * S::ROW_FLOATS;
+        *reinterpret_cast<float2*>(at + d) = make_float2(m.value, second);
+        if (d == 0) at[D] = m.ref, at[D + 1] = m.sum_ref, at[D + 2] = m.sum;
       }
     }
   };
@@ -569,22 +616,19 @@ __global__ void __launch_bounds__(Shape<D, NT>::WARPS * 32, 1) attention_kernel(
   if (open_n) {
     emit(last, false);
     if (!from_before && threadIdx.x == 0) {  // the pair that starts here ends in a later CTA
-      const int64_t mine = share(min(workers, ((int64_t)blockIdx.x + 1) * S::WARPS)) - 1;
-      const Pair a = locate(mine);
-      const int64_t tile = a.base + a.tiles - 1;
-      int64_t w = min(workers - 1, ((tile + 1) * workers - 1) / total);
+      const Pair a = locate(share(min(workers, ((int64_t)blockIdx.x + 1) * S::WARPS)) - 1);
+      const int64_t step = a.base + a.steps - 1;
       int* link = p.links + blockIdx.x * 4;
       link[1] = a.s, link[2] = a.h, link[3] = a.rt;
-      link[0] = (int)(w / S::WARPS);
+      link[0] = (int)(min(workers - 1, ((step + 1) * workers - 1) / total) / S::WARPS);
     }
   }
 }
 
 // Pairs that cross CTAs: block (c, row) merges row `row` of the pair that
 // starts in CTA c: its state there and those that the CTAs up to its last one continue it by.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(D) attention_merge_kernel(const AttnParams p) {
-  using S = Shape<D, NT>;
+template <int D, int NT, int U> __global__ void __launch_bounds__(D) attention_merge_kernel(const AttnParams p) {
+  using S = Shape<D, NT, U>;
   const int* link = p.links + blockIdx.x * 4;
   const int end = link[0];
   if (end < 0) return;
@@ -593,11 +637,13 @@ __global__ void __launch_bounds__(D) attention_merge_kernel(const AttnParams p) 
   const Merged m = merge_states(end - (int)blockIdx.x + 1, [&](int i) {
     const int64_t slot = (int64_t)(blockIdx.x + i) * 2 + (i == 0);
     const float* at = p.partials + (slot * S::ROWS + blockIdx.y) * S::ROW_FLOATS;
-    return Merged{at[D], at[D + 1], at[d]};
+    return Merged{at[d], at[D], at[D + 1], at[D + 2]};
   });
-  const float value = m.sum == 0.f ? 0.f : m.value / m.sum;
-  write_row<T, D>(p, link[1], link[2], row, d, &value, 1, 1.f);
-  if (d == 0) write_lse(p, link[1], link[2], row, m.ref, m.sum);
+  const float value = m.value * normaliser(m.ref, m.sum_ref, m.sum);
+  const int64_t out = out_row(p, link[1], link[2], row);
+  if (p.c.dtype == UCB_BF16) static_cast<__nv_bfloat16*>(p.out)[out * D + d] = __float2bfloat16_rn(value);
+  else static_cast<__half*>(p.out)[out * D + d] = __float2half_rn(value);
+  if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
 }
 
 int multiprocessors() {
@@ -608,24 +654,34 @@ int multiprocessors() {
   return counts[dev];
 }
 
-template <typename T, int D, int NT> int launch(const AttnParams& p, int sms, cudaStream_t stream) {
-  using S = Shape<D, NT>;
-  const int smem = S::WARPS * S::WARP_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
-  const cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "ucb_block8_attention: %s", cudaGetErrorString(e));
+constexpr int MOST_SEQS = 4096;
+
+template <int D, int NT, int U> int launch(AttnParams& p, int sms, cudaStream_t stream) {
+  using S = Shape<D, NT, U>;
+  static bool ready[64] = {false};  // the attribute is a device's; setting it twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!ready[dev & 63]) {
+    const cudaError_t e = cudaFuncSetAttribute(attention_kernel<D, NT, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               S::WARPS * S::RING_BYTES + (MOST_SEQS + 1) * 4);
+    if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "ucb_block8_attention: %s", cudaGetErrorString(e));
+    ready[dev & 63] = true;
+  }
+  const int smem = S::WARPS * S::RING_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
+  p.step_shift = U == 1 ? 0 : p.c.block_tokens == 32 ? 0 : p.c.block_tokens == 64 ? 1 : 2;
   const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
-  const int64_t tiles = (entries << p.tile_shift) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
-  const int64_t wanted = (tiles + S::WARPS * MIN_TILES - 1) / (S::WARPS * MIN_TILES);
+  const int64_t steps = (entries << p.step_shift) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
+  const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(sms, wanted));
-  attention_kernel<T, D, NT><<<grid, S::WARPS * 32, smem, stream>>>(p);
-  attention_merge_kernel<T, D, NT><<<dim3(grid, S::ROWS), D, 0, stream>>>(p);
+  p.spill = p.partials + (int64_t)sms * 2 * S::STATE_FLOATS;
+  p.links = reinterpret_cast<int*>(p.spill + (int64_t)sms * S::WARPS * S::STATE_FLOATS);
+  attention_kernel<D, NT, U><<<grid, S::WARPS * 32, smem, stream>>>(p);
+  attention_merge_kernel<D, NT, U><<<dim3(grid, S::ROWS), D, 0, stream>>>(p);
   return ucb_host::check_launch("block8 attention_kernel");
 }
 
-template <typename T> int launch_shape(const AttnParams& p, int sms, cudaStream_t stream) {
-  const bool wide = p.rows > 8;
-  if (p.c.head_dim == 128) return wide ? launch<T, 128, 2>(p, sms, stream) : launch<T, 128, 1>(p, sms, stream);
-  return wide ? launch<T, 64, 2>(p, sms, stream) : launch<T, 64, 1>(p, sms, stream);
+template <int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
+  return p.c.block_tokens == TILE ? launch<D, NT, 1>(p, sms, stream) : launch<D, NT, 2>(p, sms, stream);
 }
 
 }  // namespace
@@ -635,12 +691,12 @@ template <typename T> int launch_shape(const AttnParams& p, int sms, cudaStream_
 using ucb_host::set_error;
 namespace b8 = ucb::block8;
 
-// States of two pairs and one link for each CTA, up to 16 rows.
+// For each CTA (one on every multiprocessor): states of two pairs that cross CTAs, one state for each warp, one link.
 extern "C" int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads) {
   if (b8::check_cache(cache, "ucb_block8_attention_workspace_bytes") || queries < 1 || q_heads < 1) return -1;
   const int64_t sms = b8::multiprocessors();
-  const int rows = (int64_t)q_heads / cache->kv_heads * queries > 8 ? 16 : 8;
-  return sms > 0 ? sms * (2 * rows * (cache->head_dim + 4) * 4 + 16) : -1;
+  const int64_t rows = (int64_t)q_heads / cache->kv_heads * queries > 8 ? 16 : 8;
+  return sms > 0 ? sms * ((2 + b8::Shape<128, 1, 1>::WARPS) * rows * (cache->head_dim + 4) * 4 + 16) : -1;
 }
 
 extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const void* query, int64_t q_ss, int64_t q_sl,
@@ -653,8 +709,8 @@ extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const void* q
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: query heads must be divisible by KV heads");
   if (blocks && (num_selected < 1 || num_selected > 1 << 20))
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: a selection needs 1 to 2^20 entries");
-  if (reinterpret_cast<uintptr_t>(workspace) & 15)
-    return set_error(UCB_ERR_INVALID, "ucb_block8_attention: workspace must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(out)) & 15)
+    return set_error(UCB_ERR_INVALID, "ucb_block8_attention: out and workspace must be 16-byte aligned");
   unsigned int* err = ucb_host::device_error_word();
   const int sms = b8::multiprocessors();
   if (!err || sms < 1) return set_error(UCB_ERR_CUDA, "ucb_block8_attention: no device");
@@ -662,18 +718,18 @@ extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const void* q
   p.c = *cache;
   p.q = query;
   p.q_ss = q_ss, p.q_sl = q_sl, p.q_sh = q_sh;
+  p.q_aligned = reinterpret_cast<uintptr_t>(query) % 8 == 0 && (q_ss | q_sl | q_sh) % 4 == 0;
   p.queries = queries, p.q_heads = q_heads;
   p.group = q_heads / cache->kv_heads;
   p.rows = p.group * queries;
   const int tile_rows = p.rows > 8 ? 16 : 8;
   p.row_tiles = (p.rows + tile_rows - 1) / tile_rows;
   p.blocks = blocks, p.selected = num_selected;
-  p.tile_shift = cache->block_tokens == 16 ? 0 : cache->block_tokens == 32 ? 1 : cache->block_tokens == 64 ? 2 : 3;
   p.scale_log2 = softmax_scale * 1.44269504088896341f;
   p.out = out, p.lse = lse;
   p.partials = static_cast<float*>(workspace);
-  p.links = reinterpret_cast<int*>(p.partials + (int64_t)sms * 2 * tile_rows * (cache->head_dim + 4));
   p.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return cache->dtype == UCB_BF16 ? b8::launch_shape<__nv_bfloat16>(p, sms, s) : b8::launch_shape<__half>(p, sms, s);
+  if (cache->head_dim == 128) return tile_rows == 16 ? b8::launch_block<128, 2>(p, sms, s) : b8::launch_block<128, 1>(p, sms, s);
+  return tile_rows == 16 ? b8::launch_block<64, 2>(p, sms, s) : b8::launch_block<64, 1>(p, sms, s);
 }
