@@ -525,6 +525,18 @@ def test_selection_among_many_blocks(blocks, count):
         check_select(cache, make_query(gen, (2, 8, 64), torch.bfloat16), lengths, count=count)
 
 
+def test_selection_of_more_blocks_than_shared_memory_holds():
+    need_gpu()
+    blocks = 60000
+    cache, gen = make_cache([16 * blocks], heads=1, dim=64, block=16, seed=1)
+    cache.lengths.fill_(16 * blocks - 3)
+    shape = cache.key_low.shape
+    cache.key_high.copy_(torch.randint(0, 128, shape, generator=gen, device="cuda"))
+    cache.key_low.copy_(-torch.randint(0, 128, shape, generator=gen, device="cuda"))
+    cache.key_scale.copy_(torch.rand(shape[:2], generator=gen, device="cuda"))
+    check_select(cache, make_query(gen, (1, 20, 64), torch.bfloat16), [16 * blocks - 3], count=300)
+
+
 def test_selection_with_zeros_negatives_and_poison():
     need_gpu()
     lengths = [64 * 20] * 4

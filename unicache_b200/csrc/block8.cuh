@@ -41,6 +41,27 @@ __device__ __forceinline__ int held_tokens(const ucb_block8_cache& c, int s, uns
   return n < 0 ? 0 : (int)most;
 }
 
+// Programmatic dependent launch: a kernel launched by launch_dependent may become resident once every CTA of the kernel
+// before it has called launch_dependents (or ended), and reads nothing of it before wait_for_primary returns.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename P>
+int launch_dependent(void (*kernel)(const P), dim3 grid, dim3 block, cudaStream_t stream, const P& params, const char* what) {
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.stream = stream;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, params);
+  if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  return UCB_OK;
+}
+
 // Checks that every entry point makes before it touches the GPU.
 int check_cache(const ucb_block8_cache* c, const char* what);
 

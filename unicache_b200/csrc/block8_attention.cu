@@ -15,13 +15,14 @@
 // unnormalised rows) are merged in shared memory within a CTA, and across CTAs by
 // a second small kernel.
 //
-// Loads: each lane copies by cp.async exactly the bytes that its own matrix
-// fragments need, into slots that no other lane reads: a deep private queue
-// without barriers, and conflict-free.  The order of channels within a
-// product of 16 (and of tokens) is free as long as both operands have it, so
-// the fragments are 16-byte runs of the pool's rows: key lane (r, c) holds
-// channels 16c.. of tokens r and r + 8, value lane (r, c) channels 16r.. of
-// tokens 2c, 2c + 1, 2c + 8, 2c + 9.
+// Loads: every warp copies its own steps by cp.async, whole 128-byte lines an instruction,
+// into a private ring of shared memory: a deep queue without barriers.  The
+// order of channels within a product of 16 (and of tokens) is free as long as both
+// operands have it, so the fragments are 16-byte units of the pool's rows:
+// key lane (r, c) reads units c and c + 4 of tokens r and r + 8, value lane
+// (r, c) unit r (8 bytes of it at D = 64) of tokens 2c, 2c + 1, 2c + 8, 2c + 9.
+// A unit lies at its place within 128 bytes XOR (t & 6) ^ (t & 1) << 2 of its
+// token t, which makes both reads and the copies free of bank conflicts.
 //
 // Arithmetic: codes become fp16 exactly (bytes placed under 1024's exponent, minus
 // 1152); a query row is scaled by a power of two to at most 2^14 and held in
@@ -49,6 +50,8 @@ struct AttnParams {
   int selected;
   int q_aligned;     // query rows can be read 8 bytes at a time
   int step_shift;    // log2(steps in a block)
+  int front_ctas;    // CTAs that are resident at once; those after them have smaller shares
+  float tail_share;  // of all steps, for the latter
   float scale_log2;  // softmax scale * log2(e)
   void* out;
   float* lse;
@@ -60,27 +63,27 @@ struct AttnParams {
 
 constexpr int TILE = 16;     // tokens of one matrix product
 constexpr int MIN_STEPS = 1;  // a warp's least share, where there is more than that
+constexpr int CTAS_PER_SM = 4;  // at most, in one launch
+constexpr float TAIL_SHARE = 0.06f;
+constexpr int TAIL_FROM = 1000;
 constexpr float LIFT = 6.f;   // log2 of the largest weight when its reference is set
 constexpr float LAZY = 14.f;  // a weight may reach 2^LAZY before its reference moves
 constexpr float LAZY_SUM = 100.f;
 
-// U tiles of 16 tokens a step: two, or one where a block is a single tile.
+// U tiles of 16 tokens a step, two CTAs a multiprocessor.
 template <int D, int NT, int U> struct Shape {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int WARPS = D == 128 && NT == 2 ? 8 : 12;
-  static constexpr int TILE_BYTES = 2 * TILE * D;
-  static constexpr int STAGES = D == 64 || U == 1 ? 4 : 2;
-  static constexpr int STAGE_BYTES = U * TILE_BYTES;
+  static constexpr int WARPS = NT == 1 ? 8 : D == 64 ? 6 : 4;
+  static constexpr int STEP_BYTES = U * 2 * TILE * D;
+  static constexpr int STAGES = 98304 / (WARPS * STEP_BYTES);
   static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its reference, the sum's reference, the sum
   static constexpr int STATE_FLOATS = ROWS * ROW_FLOATS;
-  static constexpr int RING_BYTES = STAGES * STAGE_BYTES > STATE_FLOATS * 4 ? STAGES * STAGE_BYTES : STATE_FLOATS * 4;
+  static constexpr int RING_BYTES = STAGES * STEP_BYTES;
+  static_assert(RING_BYTES >= STATE_FLOATS * 4, "a state fits a ring");
 };
 
 __device__ __forceinline__ void cp_async16_some(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async8_some(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -95,21 +98,15 @@ __device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t select) {
 
 // A (sequence, KV head, row tile) triple and where its steps begin in the flat order.
 struct Pair {
-  int s, h, rt, steps;
-  int64_t base;
+  int s, h, rt, steps, base;
 };
 
 // Segment of one warp, for the merge of its CTA.
 struct Segment {
   int used, ends;  // ends: holds the pair's last step
   int s, h, rt;
-  const float* state;
+  const float* spilled;  // null: in the warp's ring
 };
-
-__device__ __forceinline__ float load_element(const AttnParams& p, const void* q, int64_t at) {
-  return p.c.dtype == UCB_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(q)[at])
-                               : __half2float(static_cast<const __half*>(q)[at]);
-}
 
 __device__ __forceinline__ uint32_t pack_out(const AttnParams& p, float lo, float hi) {
   return p.c.dtype == UCB_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
@@ -128,30 +125,57 @@ __device__ __forceinline__ float normaliser(float ref, float sum_ref, float sum)
   return sum == 0.f || (ref == -INFINITY && sum == sum) ? 0.f : exp2f(ref - sum_ref) / sum;
 }
 
-// States of one row and channel merged.  A state without a token has references -inf and sum 0; products, not
-// branches, so that a NaN comes through.
+// States of one row merged, four channels of it.  A state without a token has references -inf and sum 0; products, not
+// branches, so that a NaN comes through.  `get(i)` points to state i's row: D channels, then reference, sum reference, sum.
 struct Merged {
-  float value, ref, sum_ref, sum;
+  float4 value;
+  float ref, sum_ref, sum;
 };
-template <typename Get> __device__ __forceinline__ Merged merge_states(int n, Get get) {
-  Merged m{0.f, -INFINITY, -INFINITY, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const Merged x = get(i);
-    m.ref = fmaxf(m.ref, x.ref);
-    m.sum_ref = fmaxf(m.sum_ref, x.sum_ref);
-  }
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const Merged x = get(i);
-    m.value = fmaf(x.ref == -INFINITY ? 0.f : fast_exp2(x.ref - m.ref), x.value, m.value);
-    m.sum = fmaf(x.sum_ref == -INFINITY ? 0.f : fast_exp2(x.sum_ref - m.sum_ref), x.sum, m.sum);
+template <int D, typename Get> __device__ __forceinline__ Merged merge_states(int first, int n, int stride, int d, Get get) {
+  Merged m{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f};
+  for (int i = first; i < n; i += 4 * stride) {  // four at a time, their loads together
+    float4 x[4], y[4];
+    float ref = m.ref, sum_ref = m.sum_ref;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * stride < n) {
+        const float* at = get(i + k * stride);
+        x[k] = *reinterpret_cast<const float4*>(at + D);
+        y[k] = *reinterpret_cast<const float4*>(at + d);
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * stride < n) {
+        ref = fmaxf(ref, x[k].x);
+        sum_ref = fmaxf(sum_ref, x[k].y);
+      }
+    float f = m.ref == -INFINITY ? 0.f : fast_exp2(m.ref - ref);
+    m.value = make_float4(m.value.x * f, m.value.y * f, m.value.z * f, m.value.w * f);
+    m.sum *= m.sum_ref == -INFINITY ? 0.f : fast_exp2(m.sum_ref - sum_ref);
+    m.ref = ref;
+    m.sum_ref = sum_ref;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * stride < n) {
+        f = x[k].x == -INFINITY ? 0.f : fast_exp2(x[k].x - ref);
+        m.value.x = fmaf(f, y[k].x, m.value.x);
+        m.value.y = fmaf(f, y[k].y, m.value.y);
+        m.value.z = fmaf(f, y[k].z, m.value.z);
+        m.value.w = fmaf(f, y[k].w, m.value.w);
+        m.sum = fmaf(x[k].y == -INFINITY ? 0.f : fast_exp2(x[k].y - sum_ref), x[k].z, m.sum);
+      }
   }
   return m;
 }
 
+__device__ __forceinline__ void write_four(const AttnParams& p, int64_t at, const Merged& m) {
+  const float f = normaliser(m.ref, m.sum_ref, m.sum);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+      make_uint2(pack_out(p, m.value.x * f, m.value.y * f), pack_out(p, m.value.z * f, m.value.w * f));
+}
+
 template <int D, int NT, int U>
-__global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kernel(const AttnParams p) {
   using S = Shape<D, NT, U>;
   constexpr int MT = D / 16;          // value products of 16 channels
   constexpr int KS = D / 16;          // key products of 16 channels
@@ -167,16 +191,16 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
   const int step_mask = (1 << p.step_shift) - 1;
 
   // ---- the flat order: steps of every sequence (at least one, so that every row is written)
-  int64_t total;
+  int total;
   const int listed_steps = p.selected << p.step_shift;
   if (p.blocks) {
-    total = (int64_t)c.num_seqs * listed_steps * heads_rows;
+    total = c.num_seqs * listed_steps * heads_rows;
   } else {
     int carry = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int base = 0; base < c.num_seqs; base += S::WARPS * 32) {
       const int i = base + threadIdx.x;
-      int v = i < c.num_seqs ? max(1, (int)(((int64_t)held_tokens(c, i, p.err) + STEP - 1) / STEP)) : 0;
+      int v = i < c.num_seqs ? max(1, (held_tokens(c, i, p.err) + STEP - 1) / STEP) : 0;
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
@@ -191,24 +215,36 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
       if (i < c.num_seqs) prefix[i + 1] = before + v;
       __syncthreads();
     }
-    total = (int64_t)carry * heads_rows;
+    total = carry * heads_rows;
   }
-  const int64_t workers = max((int64_t)1, min((int64_t)gridDim.x * S::WARPS, total / MIN_STEPS));
-  const int64_t worker = (int64_t)blockIdx.x * S::WARPS + warp;
+  const int worker = blockIdx.x * S::WARPS + warp;
   if (lane == 0) segments[warp][0].used = segments[warp][1].used = 0;
-  auto share = [&](int64_t w) { return w >= workers ? total : total * w / workers; };
-  auto locate = [&](int64_t t) {
+  // shares: `front` workers have an equal part of all but the last `tail` steps, the others `piece` steps each
+  const int front = max(1, min((int)gridDim.x == p.front_ctas ? total : total / 2, p.front_ctas * S::WARPS));
+  const int behind = ((int)gridDim.x - p.front_ctas) * S::WARPS;
+  const int piece = behind ? max(1, (int)((float)total * p.tail_share) / behind) : 1;
+  const int tail = min(total - front, piece * behind);
+  const int body = total - tail, each = body / front, longer = body - each * front;
+  auto share = [&](int w) {
+    if (w <= front) return w * each + min(w, longer);
+    return min(total, body + (w - front) * piece);
+  };
+  auto worker_of = [&](int step) {
+    if (step >= body) return front + (step - body) / piece;
+    const int split = longer * (each + 1);
+    return step < split ? step / (each + 1) : longer + (step - split) / each;
+  };
+  auto locate = [&](int t) {
     Pair a;
+    int u;
     if (p.blocks) {
-      const int64_t pair = t / listed_steps;
-      a.s = (int)(pair / heads_rows);
       a.steps = listed_steps;
-      const int u = (int)(pair % heads_rows);
-      a.h = u / p.row_tiles;
-      a.rt = u % p.row_tiles;
+      const int pair = t / listed_steps;
       a.base = pair * listed_steps;
+      a.s = pair / heads_rows;
+      u = pair - a.s * heads_rows;
     } else {
-      const int unit = (int)(t / heads_rows);
+      const int unit = t / heads_rows;
       int lo = 0, hi = c.num_seqs - 1;  // the last sequence whose first step is not after t
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -216,27 +252,53 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
       }
       a.s = lo;
       a.steps = prefix[lo + 1] - prefix[lo];
-      const int64_t first = (int64_t)prefix[lo] * heads_rows;
-      const int u = (int)((t - first) / a.steps);
-      a.h = u / p.row_tiles;
-      a.rt = u % p.row_tiles;
-      a.base = first + (int64_t)u * a.steps;
+      const int first = prefix[lo] * heads_rows;
+      u = (t - first) / a.steps;
+      a.base = first + u * a.steps;
     }
+    a.h = u / p.row_tiles;
+    a.rt = u - a.h * p.row_tiles;
     return a;
   };
 
   unsigned char* ring = smem + warp * S::RING_BYTES;
   const uint32_t ring_at = smem_u32(ring);
-  int64_t t = share(worker);
-  const int64_t t_end = share(worker + 1);
-  if (worker < workers) while (t < t_end) {
+  // places of units in the ring: what this lane copies, its key and its value fragments
+  auto place = [&](int token, int unit) {
+    const int x = (unit ^ (token & 6) ^ ((token & 1) << 2)) * 16;
+    return (D == 128 ? token : token >> 1) * 128 + x;
+  };
+  const int copy_token = lane / (D / 16), copy_place = place(copy_token, lane % (D / 16));
+  const int key_place = place(r, cq);
+  const int value_place = D == 128 ? place(2 * cq, r) : place(2 * cq, r >> 1) + (r & 1) * 8;
+  const int value_place1 = D == 128 ? place(2 * cq + 1, r) : place(2 * cq + 1, r >> 1) + (r & 1) * 8;
+  int t = share(worker);
+  const int t_end = share(worker + 1);
+  while (t < t_end) {
     const Pair a = locate(t);
-    const int begin = (int)(t - a.base), end = (int)min((int64_t)a.steps, t_end - a.base);
+    const int begin = t - a.base, end = min(a.steps, t_end - a.base);
     t = a.base + end;
     const int len = held_tokens(c, a.s, p.err);
     const int32_t* list = p.blocks ? p.blocks + ((int64_t)a.s * c.kv_heads + a.h) * p.selected : nullptr;
     const int32_t* table = c.block_table + (int64_t)a.s * c.max_blocks;
     const int entries = p.blocks ? p.selected : (len + bt - 1) / bt;
+
+    // ---- query rows, two elements a register: row nt * 8 + r, channels of the key fragments
+    uint2 raw[NT][KS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = a.rt * S::ROWS + nt * 8 + r;
+      const int l = row / p.group;
+      const int64_t at = a.s * p.q_ss + l * p.q_sl + (a.h * p.group + row - l * p.group) * p.q_sh + 16 * cq;
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const uint16_t* x = q + 64 * (i / 4) + 4 * (i % 4);
+        if (row >= p.rows) raw[nt][i] = make_uint2(0, 0);
+        else if (p.q_aligned) raw[nt][i] = *reinterpret_cast<const uint2*>(x);
+        else raw[nt][i] = make_uint2(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16);
+      }
+    }
 
     // ---- block descriptors: lane i holds entry window + i, `next` the 32 entries after
     struct Entry {
@@ -273,25 +335,15 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
         const int token = __shfl_sync(0xffffffffu, rel < 32 ? now.token : next.token, rel & 31);
         const int row0 = (i & step_mask) * STEP, n = len - token - row0;
         if (block >= 0 && n > 0) {
-          const int64_t at = (((int64_t)block * c.kv_heads + a.h) * bt + row0) * D;
-          const int8_t* k = c.key_code + at + r * D + 16 * cq;
-          const int8_t* v = c.value_code + at + 2 * cq * D + VB * r;
-          const uint32_t to = ring_at + ((i - begin) % S::STAGES) * S::STAGE_BYTES;
+          const int64_t at = (((int64_t)block * c.kv_heads + a.h) * bt + row0) * D + lane * 16;
+          const int8_t *k = c.key_code + at, *v = c.value_code + at;
+          const uint32_t to = ring_at + ((i - begin) % S::STAGES) * S::STEP_BYTES;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {  // (token r or r + 8, low or high half of the channels)
-              const int tok = u * TILE + (x & 1) * 8, ch = (x >> 1) * 64;
-              cp_async16_some(to + u * S::TILE_BYTES + x * 512 + lane * 16, k + tok * D + ch, r + tok < n ? 16 : 0);
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int tok = u * TILE + (x & 1) + (x & 2) * 4;
-              const int bytes = 2 * cq + tok < n ? VB : 0;
-              const uint32_t at_slot = to + u * S::TILE_BYTES + TILE * D + (x * 32 + lane) * VB;
-              if (D == 128) cp_async16_some(at_slot, v + tok * D, bytes);
-              else cp_async8_some(at_slot, v + tok * D, bytes);
-            }
+          for (int x = 0; x < STEP * D / 512; ++x) {  // 512 bytes: the rows of 4 (or 8) tokens
+            const int bytes = x * (512 / D) + copy_token < n ? 16 : 0;
+            const uint32_t at_ring = to + x * 512 + (D == 128 && (x & 1) ? copy_place ^ 64 : copy_place);
+            cp_async16_some(at_ring, k + x * 512, bytes);
+            cp_async16_some(at_ring + STEP * D, v + x * 512, bytes);
           }
         }
       }
@@ -302,47 +354,31 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
     fetch_scales(now);
     bool next_scaled = false;
 
-    // ---- query rows as fp16 operands
+    // ---- query rows as fp16 operands, times the power of two that brings their largest element to [2^13, 2^14)
     uint32_t qb[NT][KS][2];
-    float row_scale[NT];  // of row nt * 8 + r
+    float row_scale[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = a.rt * S::ROWS + nt * 8 + r;
-      const bool real = row < p.rows;
-      const int64_t q0 = a.s * p.q_ss + (real ? row / p.group : 0) * p.q_sl +
-                         (a.h * p.group + (real ? row % p.group : 0)) * p.q_sh;
-      float x[KS][4];
-      float top = 0.f;
+      uint32_t top = 0;  // largest magnitude, as bits of the two halves
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const int64_t at = q0 + 64 * (i / 4) + 16 * cq + 4 * (i % 4);
-        if (p.q_aligned) {
-          const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at);
-          const bool bf = c.dtype == UCB_BF16;
-          x[i][0] = bf ? Dtype<__nv_bfloat16>::lo(w.x) : Dtype<__half>::lo(w.x);
-          x[i][1] = bf ? Dtype<__nv_bfloat16>::hi(w.x) : Dtype<__half>::hi(w.x);
-          x[i][2] = bf ? Dtype<__nv_bfloat16>::lo(w.y) : Dtype<__half>::lo(w.y);
-          x[i][3] = bf ? Dtype<__nv_bfloat16>::hi(w.y) : Dtype<__half>::hi(w.y);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[i][k] = load_element(p, p.q, at + k);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (!real) x[i][k] = 0.f;
-          top = fmaxf(top, fabsf(x[i][k]));
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // power of two that brings the largest element to [2^13, 2^14); both factors are normal numbers
-      const int e = min(126, top > 0.f && top <= 3.4028235e38f ? 140 - (int)(__float_as_uint(top) >> 23) : 0);
+      for (int i = 0; i < KS; ++i)
+        top = __vmaxu2(top, __vmaxu2(raw[nt][i].x & 0x7fff7fffu, raw[nt][i].y & 0x7fff7fffu));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = max(top & 0xffffu, top >> 16);
+      const bool bf = c.dtype == UCB_BF16;
+      const uint32_t exponent = __float_as_uint(bf ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top))) >> 23;
+      // both factors are normal numbers; a row of zeros, infinities or NaN is left as it is
+      const int e = exponent == 0 && top == 0 || exponent == 255 ? 0 : min(126, 140 - (int)exponent);
       const float up = __uint_as_float((uint32_t)(127 + e) << 23);
       row_scale[nt] = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        qb[nt][i][0] = pack_f16x2(x[i][0] * up, x[i][1] * up);
-        qb[nt][i][1] = pack_f16x2(x[i][2] * up, x[i][3] * up);
+        const uint32_t w[2] = {raw[nt][i].x, raw[nt][i].y};
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          qb[nt][i][k] = bf ? pack_f16x2(Dtype<__nv_bfloat16>::lo(w[k]) * up, Dtype<__nv_bfloat16>::hi(w[k]) * up)
+                            : pack_f16x2(Dtype<__half>::lo(w[k]) * up, Dtype<__half>::hi(w[k]) * up);
       }
     }
     float col_scale[NT][2];
@@ -382,14 +418,15 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
         next_scaled = true;
       }
       cp_async_wait<S::STAGES - 2>();
-      issue(i + S::STAGES - 1);  // into the slot of the step before, whose values were used
+      __syncwarp();              // the other lanes' copies of step i, and their reads of the step before
+      issue(i + S::STAGES - 1);  // into the slot of the step before
       const int rel = entry - window;
       const int block = __shfl_sync(0xffffffffu, now.block, rel);
       const int first_token = __shfl_sync(0xffffffffu, now.token, rel) + (i & step_mask) * STEP;
       if (block < 0 || first_token >= len) continue;
       const float ks = __shfl_sync(0xffffffffu, now.ks, rel);
       const float lv = __shfl_sync(0xffffffffu, now.lv, rel);
-      const unsigned char* slot = ring + ((i - begin) % S::STAGES) * S::STAGE_BYTES;
+      const unsigned char* slot = ring + ((i - begin) % S::STAGES) * S::STEP_BYTES;
 
       // ---- logits of 16 tokens (rows) and 8 query rows (columns)
       float s[U][NT][4];
@@ -398,9 +435,9 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
         float part[KS / 4][NT][4];
 #pragma unroll
         for (int half = 0; half < KS / 4; ++half) {
-          const unsigned char* at = slot + u * S::TILE_BYTES + half * 1024 + lane * 16;
+          const unsigned char* at = slot + u * TILE * D + (half ? key_place ^ 64 : key_place);
           const uint4 ka = *reinterpret_cast<const uint4*>(at);
-          const uint4 kb = *reinterpret_cast<const uint4*>(at + 512);
+          const uint4 kb = *reinterpret_cast<const uint4*>(at + 8 * D);
           const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) part[half][nt][0] = part[half][nt][1] = part[half][nt][2] = part[half][nt][3] = 0.f;
@@ -493,7 +530,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
         uint32_t vw[4][D / 32];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const unsigned char* at = slot + u * S::TILE_BYTES + TILE * D + (x * 32 + lane) * VB;
+          const unsigned char* at = slot + STEP * D + (u * TILE + (x >> 1) * 8) * D + (x & 1 ? value_place1 : value_place);
           if (D == 128) {
             const uint4 v = *reinterpret_cast<const uint4*>(at);
             vw[x][0] = v.x, vw[x][1] = v.y, vw[x][D / 32 - 2] = v.z, vw[x][D / 32 - 1] = v.w;
@@ -522,7 +559,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
     // segment stays in its ring, an earlier one that a warp before began goes through global memory.
     const bool whole = begin == 0 && end == a.steps;
     const int which = begin == 0 ? 1 : 0;
-    float* state = t >= t_end ? reinterpret_cast<float*>(ring) : p.spill + worker * S::STATE_FLOATS;
+    float* state = t >= t_end ? reinterpret_cast<float*>(ring) : p.spill + (int64_t)worker * S::STATE_FLOATS;
     __syncwarp();  // every lane is done with the ring before states overwrite it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -555,43 +592,40 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
 #pragma unroll
           for (int i = 0; i < VB; i += 4)
             *reinterpret_cast<float4*>(at + VB * r + i) = make_float4(run[i], run[i + 1], run[i + 2], run[i + 3]);
-          if (r == 0) at[D] = ref[nt][k], at[D + 1] = sum_ref[nt][k], at[D + 2] = l;
+          if (r == 0) *reinterpret_cast<float4*>(at + D) = make_float4(ref[nt][k], sum_ref[nt][k], l, 0.f);
         }
       }
-    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == a.steps, a.s, a.h, a.rt, state};
+    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == a.steps, a.s, a.h, a.rt, t >= t_end ? nullptr : state};
   }
   __syncthreads();
 
+  launch_dependents();
+
   // ---- chains of segments of one pair: complete ones are written, the CTA's first and last may go on
-  // in other CTAs.  A warp's slot 0 continues the pair that was open before it, slot 1 opens one.
+  // in other CTAs.  A warp's slot 0 continues the pair that was open before it, slot 1 opens one; a state outside
+  // the rings ends its chain, since its warp went on to another pair.
   if (threadIdx.x == 0) p.links[blockIdx.x * 4] = -1;
-  int open_w = 0, open_which = 0, open_n = 0;  // the open chain: first segment and count
+  int open_w = 0, open_n = 0;  // the open chain: first warp and count
   bool from_before = false;
   auto emit = [&](const Segment& seg, bool ended) {
     const bool complete = ended && !from_before;
     float* to = p.partials + ((int64_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * S::STATE_FLOATS;
-    for (int item = threadIdx.x; item < S::ROWS * D / 2; item += S::WARPS * 32) {
-      const int in_tile = item / (D / 2), d = item % (D / 2) * 2, row = seg.rt * S::ROWS + in_tile;
+    for (int item = threadIdx.x; item < S::ROWS * D / 4; item += S::WARPS * 32) {
+      const int in_tile = item / (D / 4), d = item % (D / 4) * 4, row = seg.rt * S::ROWS + in_tile;
       if (row >= p.rows) break;
-      float second = 0.f;
-      auto state = [&](int i) { return segments[open_w + i][i ? 0 : open_which].state + in_tile * S::ROW_FLOATS; };
-      const Merged m = merge_states(open_n, [&](int i) {
-        const float* at = state(i);
-        return Merged{at[d], at[D], at[D + 1], at[D + 2]};
+      const unsigned char* states = smem + open_w * S::RING_BYTES + in_tile * (S::ROW_FLOATS * 4);
+      const Merged m = merge_states<D>(0, open_n, 1, d, [&](int i) {
+        return i == open_n - 1 && seg.spilled ? seg.spilled + in_tile * S::ROW_FLOATS
+                                              : reinterpret_cast<const float*>(states + i * S::RING_BYTES);
       });
-      for (int i = 0; i < open_n; ++i) {
-        const float* at = state(i);
-        second = fmaf(at[D] == -INFINITY ? 0.f : fast_exp2(at[D] - m.ref), at[d + 1], second);
-      }
       if (complete) {
-        const float f = normaliser(m.ref, m.sum_ref, m.sum);
         const int64_t out = out_row(p, seg.s, seg.h, row);
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + out * D + d) = pack_out(p, m.value * f, second * f);
+        write_four(p, out * D + d, m);
         if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
       } else {
         float* at = to + in_tile * S::ROW_FLOATS;
-        *reinterpret_cast<float2*>(at + d) = make_float2(m.value, second);
-        if (d == 0) at[D] = m.ref, at[D + 1] = m.sum_ref, at[D + 2] = m.sum;
+        *reinterpret_cast<float4*>(at + d) = m.value;
+        if (d == 0) *reinterpret_cast<float4*>(at + D) = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
       }
     }
   };
@@ -599,7 +633,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
   for (int w = 0; w < S::WARPS; ++w) {
     const Segment s0 = segments[w][0], s1 = segments[w][1];
     if (s0.used) {
-      if (open_n == 0) open_w = w, open_which = 0, from_before = true;
+      if (open_n == 0) open_w = w, from_before = true;
       ++open_n;
       last = s0;
       if (s0.ends) {
@@ -609,40 +643,45 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 1) attention_kern
       }
     }
     if (s1.used) {
-      open_w = w, open_which = 1, open_n = 1, from_before = false;
+      open_w = w, open_n = 1, from_before = false;
       last = s1;
     }
   }
   if (open_n) {
     emit(last, false);
     if (!from_before && threadIdx.x == 0) {  // the pair that starts here ends in a later CTA
-      const Pair a = locate(share(min(workers, ((int64_t)blockIdx.x + 1) * S::WARPS)) - 1);
-      const int64_t step = a.base + a.steps - 1;
-      int* link = p.links + blockIdx.x * 4;
-      link[1] = a.s, link[2] = a.h, link[3] = a.rt;
-      link[0] = (int)(min(workers - 1, ((step + 1) * workers - 1) / total) / S::WARPS);
+      const Pair a = locate(share((blockIdx.x + 1) * S::WARPS) - 1);
+      const int end = worker_of(a.base + a.steps - 1) / S::WARPS;
+      *reinterpret_cast<int4*>(p.links + blockIdx.x * 4) = make_int4(end, a.s, a.h, a.rt);
     }
   }
 }
 
 // Pairs that cross CTAs: block (c, row) merges row `row` of the pair that
-// starts in CTA c: its state there and those that the CTAs up to its last one continue it by.
-template <int D, int NT, int U> __global__ void __launch_bounds__(D) attention_merge_kernel(const AttnParams p) {
+// starts in CTA c: its state there and those that the CTAs up to its last one
+// continue it by, every MERGE_GROUPS-th by one group of D / 4 threads.
+constexpr int MERGE_GROUPS = 4;
+
+template <int D, int NT, int U>
+__global__ void __launch_bounds__(MERGE_GROUPS * D / 4) attention_merge_kernel(const AttnParams p) {
   using S = Shape<D, NT, U>;
-  const int* link = p.links + blockIdx.x * 4;
-  const int end = link[0];
-  if (end < 0) return;
-  const int row = link[3] * S::ROWS + blockIdx.y, d = threadIdx.x;
+  __shared__ float groups[MERGE_GROUPS][D + 4];
+  wait_for_primary();
+  const int4 link = *reinterpret_cast<const int4*>(p.links + blockIdx.x * 4);
+  if (link.x < 0) return;
+  const int row = link.w * S::ROWS + blockIdx.y, d = threadIdx.x % (D / 4) * 4, g = threadIdx.x / (D / 4);
   if (row >= p.rows) return;
-  const Merged m = merge_states(end - (int)blockIdx.x + 1, [&](int i) {
+  Merged m = merge_states<D>(g, link.x - (int)blockIdx.x + 1, MERGE_GROUPS, d, [&](int i) {
     const int64_t slot = (int64_t)(blockIdx.x + i) * 2 + (i == 0);
-    const float* at = p.partials + (slot * S::ROWS + blockIdx.y) * S::ROW_FLOATS;
-    return Merged{at[d], at[D], at[D + 1], at[D + 2]};
+    return p.partials + (slot * S::ROWS + blockIdx.y) * S::ROW_FLOATS;
   });
-  const float value = m.value * normaliser(m.ref, m.sum_ref, m.sum);
-  const int64_t out = out_row(p, link[1], link[2], row);
-  if (p.c.dtype == UCB_BF16) static_cast<__nv_bfloat16*>(p.out)[out * D + d] = __float2bfloat16_rn(value);
-  else static_cast<__half*>(p.out)[out * D + d] = __float2half_rn(value);
+  *reinterpret_cast<float4*>(groups[g] + d) = m.value;
+  if (d == 0) *reinterpret_cast<float4*>(groups[g] + D) = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
+  __syncthreads();
+  if (g > 0) return;
+  m = merge_states<D>(0, MERGE_GROUPS, 1, d, [&](int i) { return static_cast<const float*>(groups[i]); });
+  const int64_t out = out_row(p, link.y, link.z, row);
+  write_four(p, out * D + d, m);
   if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
 }
 
@@ -668,20 +707,24 @@ template <int D, int NT, int U> int launch(AttnParams& p, int sms, cudaStream_t 
     ready[dev & 63] = true;
   }
   const int smem = S::WARPS * S::RING_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
-  p.step_shift = U == 1 ? 0 : p.c.block_tokens == 32 ? 0 : p.c.block_tokens == 64 ? 1 : 2;
+  p.step_shift = (p.c.block_tokens == 16 ? 0 : p.c.block_tokens == 32 ? 1 : p.c.block_tokens == 64 ? 2 : 3) - (U - 1);
   const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
   const int64_t steps = (entries << p.step_shift) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
+  if (steps > 0x3fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: too many tokens in one call");
   const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(sms, wanted));
-  p.spill = p.partials + (int64_t)sms * 2 * S::STATE_FLOATS;
-  p.links = reinterpret_cast<int*>(p.spill + (int64_t)sms * S::WARPS * S::STATE_FLOATS);
+  p.front_ctas = (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, wanted));
+  const int grid = wanted > TAIL_FROM * sms ? 4 * sms : p.front_ctas;
+  p.tail_share = TAIL_SHARE;
+  p.spill = p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS;
+  p.links = reinterpret_cast<int*>(p.spill + (int64_t)CTAS_PER_SM * sms * S::WARPS * S::STATE_FLOATS);
   attention_kernel<D, NT, U><<<grid, S::WARPS * 32, smem, stream>>>(p);
-  attention_merge_kernel<D, NT, U><<<dim3(grid, S::ROWS), D, 0, stream>>>(p);
-  return ucb_host::check_launch("block8 attention_kernel");
+  if (int rc = ucb_host::check_launch("block8 attention_kernel")) return rc;
+  return launch_dependent(attention_merge_kernel<D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), stream, p,
+                          "block8 attention_merge_kernel");
 }
 
 template <int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
-  return p.c.block_tokens == TILE ? launch<D, NT, 1>(p, sms, stream) : launch<D, NT, 2>(p, sms, stream);
+  return launch<D, NT, 1>(p, sms, stream);
 }
 
 }  // namespace
@@ -691,12 +734,12 @@ template <int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t s
 using ucb_host::set_error;
 namespace b8 = ucb::block8;
 
-// For each CTA (one on every multiprocessor): states of two pairs that cross CTAs, one state for each warp, one link.
+// For each CTA: states of two pairs that cross CTAs, one state for each warp, one link.
 extern "C" int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads) {
   if (b8::check_cache(cache, "ucb_block8_attention_workspace_bytes") || queries < 1 || q_heads < 1) return -1;
   const int64_t sms = b8::multiprocessors();
   const int64_t rows = (int64_t)q_heads / cache->kv_heads * queries > 8 ? 16 : 8;
-  return sms > 0 ? sms * ((2 + b8::Shape<128, 1, 1>::WARPS) * rows * (cache->head_dim + 4) * 4 + 16) : -1;
+  return sms > 0 ? sms * b8::CTAS_PER_SM * ((2 + b8::Shape<128, 1, 1>::WARPS) * rows * (cache->head_dim + 4) * 4 + 16) : -1;
 }
 
 extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const void* query, int64_t q_ss, int64_t q_sl,

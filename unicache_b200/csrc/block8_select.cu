@@ -1,5 +1,26 @@
 // The blocks of the 8-bit block cache that a query may need most (ucb_block8_select).
+//
+//   I_hj = sum_d max(q_d low_jd, q_d high_jd) = sum_d max(q_d, 0) high_jd + min(q_d, 0) low_jd
+//   score_j = key_scale_j * max_h (I_hj * qscale_h)
+//
+// over whole numbers: the query heads are rounded to 8 bits by the cache's own
+// rule, so I is exact in the int32 matrix instructions (16 blocks x 8 heads x
+// 32 channels each), and the two fp32 products fix the scores bit for bit.
+// The kernel reads 2 D bytes of bounds for each block: memory bound for
+// many sequences, a few dependent round trips long for one.
+//
+// A cluster of CTAs scores one (sequence, KV head), each CTA its share of the
+// blocks, into the first CTA's shared memory (into global memory where
+// a row of keys does not fit there); that CTA then finds the count-th largest key
+// by four 8-bit radix passes and writes the kept blocks in ascending order.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <utility>
+
 #include "block8.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace ucb {
 namespace block8 {
@@ -9,13 +30,14 @@ struct SelectParams {
   ucb_block8_cache c;
   const void* q;
   int64_t q_ss, q_sh;
-  int q_heads, count, first, recent;
+  int group, count, first, recent;
   int32_t* blocks;
-  uint32_t* keys;  // [num_seqs, kv_heads, max_blocks]
+  uint32_t* spill;  // [num_seqs, kv_heads, max_blocks] when keys do not fit shared memory, else null
   unsigned int* err;
 };
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int MOST_SHARED_KEYS = 49152;  // 192 KB
 
 // Unsigned keys in the order of the scores; NaN above every number, so that a
 // poisoned block is read and shows.
@@ -26,68 +48,252 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
-  const ucb_block8_cache& c = p.c;
-  const int s = blockIdx.x, h = blockIdx.y, d = c.head_dim, group = p.q_heads / c.kv_heads;
-  const int tokens = held_tokens(c, s, p.err);
-  const int n = (tokens + c.block_tokens - 1) / c.block_tokens;
-  uint32_t* keys = p.keys + ((int64_t)s * c.kv_heads + h) * c.max_blocks;
-  int32_t* out = p.blocks + ((int64_t)s * c.kv_heads + h) * p.count;
-  for (int j = threadIdx.x; j < n; j += THREADS) keys[j] = 0;
-  __shared__ float top[THREADS / 32];
-  __shared__ int codes[128];
-  __shared__ unsigned long long best;
-  __shared__ float best_scale;
-  // scores: the largest over the group's heads, kept as floats until the last head
-  float* scores = reinterpret_cast<float*>(keys);
-  for (int g = 0; g < group; ++g) {
-    const T* q = static_cast<const T*>(p.q) + s * p.q_ss + (h * group + g) * p.q_sh;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      unsigned int m = 0;
-      for (int i = 0; i < d; ++i) m = max(m, __float_as_uint(Dtype<T>::to_f(q[i])) & 0x7fffffffu);
-      best_scale = scale_of(__uint_as_float(m));
-    }
-    __syncthreads();
-    const float qs = best_scale, inverse = __fdiv_rn(1.f, qs);
-    if (threadIdx.x < d) codes[threadIdx.x] = code_of(Dtype<T>::to_f(q[threadIdx.x]), inverse);
-    __syncthreads();
-    for (int j = threadIdx.x; j < n; j += THREADS) {
-      const int64_t block = pool_block(c, s, j, p.err);
-      if (block < 0) continue;
-      const int64_t at = (block * c.kv_heads + h) * d;
-      int sum = 0;
-      for (int i = 0; i < d; ++i) sum += max(codes[i] * c.key_low[at + i], codes[i] * c.key_high[at + i]);
-      const float x = __fmul_rn((float)sum, qs), old = scores[j];
-      scores[j] = g == 0 ? x : (x != x || old != old ? x + old : fmaxf(x, old));
-    }
-  }
-  for (int j = threadIdx.x; j < n; j += THREADS) {
-    const int64_t block = pool_block(c, s, j, p.err);
-    const float x = block < 0 ? -INFINITY : __fmul_rn(scores[j], c.key_scale[block * c.kv_heads + h]);
-    keys[j] = j < p.first || j >= n - p.recent ? KEY_FORCED : key_of(x);
-  }
-  // the largest key, lowest block first, `count` times; a taken block's key is 0
-  (void)top;
-  for (int k = 0; k < min(p.count, n); ++k) {
-    __syncthreads();
-    if (threadIdx.x == 0) best = 0;
-    __syncthreads();
-    unsigned long long mine = 0;
-    for (int j = threadIdx.x; j < n; j += THREADS)
-      mine = max(mine, ((unsigned long long)keys[j] << 32) | (0xFFFFFFFFu - (unsigned)j));
-    atomicMax(&best, mine);
-    __syncthreads();
-    if (threadIdx.x == 0) keys[0xFFFFFFFFu - (unsigned)best] = 0;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// D (16 blocks x 8 heads) += A (16 x 32 bytes) B (32 x 8 bytes), signed.
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Exclusive prefix sum over the CTA's threads, and the total.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += u;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int k = 0;
-    for (int j = 0; j < n; ++j)
-      if (keys[j] == 0) out[k++] = j;
-    for (; k < p.count; ++k) out[k] = -1;
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
   }
+  return before + x - v;
+}
+
+template <typename T, int D> __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
+  constexpr int KS = D / 32;  // products of 32 channels on each side
+  extern __shared__ __align__(16) uint32_t row_keys[];
+  __shared__ __align__(16) int8_t q_code[8][2][D + 16];  // [head][min(q, 0) or max(q, 0)][channel], rows on distinct banks
+  __shared__ float q_scale[8];
+  __shared__ int histogram[256];
+  __shared__ int warp_sums[WARPS];
+  __shared__ int found[2];
+  const ucb_block8_cache& c = p.c;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = cluster.num_blocks(), part = cluster.block_rank();
+  auto started = cluster.barrier_arrive();  // waited for before the first key goes to another CTA
+  const int pair = blockIdx.x / parts, s = pair / c.kv_heads, h = pair % c.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cq = lane & 3;
+  const int tokens = held_tokens(c, s, p.err);
+  const int n = (int)(((int64_t)tokens + c.block_tokens - 1) / c.block_tokens);
+  int32_t* out = p.blocks + (int64_t)pair * p.count;
+  uint32_t* keys = p.spill ? p.spill + (int64_t)pair * c.max_blocks : cluster.map_shared_rank(row_keys, 0);
+  const int32_t* table = c.block_table + (int64_t)s * c.max_blocks;
+  const bool all = n <= p.count;  // nothing to choose
+
+  cluster.barrier_wait(std::move(started));
+  if (!all) {
+    const int tiles = (n + 15) / 16, share = (tiles + parts - 1) / parts;
+    const int tile_end = min(tiles, (part + 1) * share);
+    for (int g0 = 0; g0 < p.group; g0 += 8) {
+      // ---- query heads in 8 bits: warp w rounds head g0 + w
+      __syncthreads();
+      {
+        const int g = g0 + warp;
+        constexpr int PER = D / 32;
+        float x[PER];
+        unsigned int top = 0;
+        if (g < p.group) {
+          const T* q = static_cast<const T*>(p.q) + s * p.q_ss + (int64_t)(h * p.group + g) * p.q_sh + lane * PER;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x[i] = Dtype<T>::to_f(q[i]), top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x[i] = 0.f;
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const float scale = scale_of(__uint_as_float(top)), inverse = __fdiv_rn(1.f, scale);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int code = code_of(x[i], inverse);
+          q_code[warp][0][lane * PER + i] = (int8_t)min(code, 0);
+          q_code[warp][1][lane * PER + i] = (int8_t)max(code, 0);
+        }
+        if (lane == 0) q_scale[warp] = scale;
+      }
+      __syncthreads();
+      // operand words in the order of the bounds' 16-byte units: lane (r, cq) takes units cq and cq + 4
+      uint32_t b[2][KS][2];
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int at = (k / 2) * 64 + 16 * cq + (k % 2) * 8;
+          b[side][k][0] = *reinterpret_cast<const uint32_t*>(&q_code[r][side][at]);
+          b[side][k][1] = *reinterpret_cast<const uint32_t*>(&q_code[r][side][at + 4]);
+        }
+      const float scale0 = q_scale[2 * cq], scale1 = q_scale[2 * cq + 1];
+      const bool real0 = g0 + 2 * cq < p.group, real1 = g0 + 2 * cq + 1 < p.group;
+
+      for (int tile = part * share + warp; tile < tile_end; tile += WARPS) {
+        const int mine = tile * 16 + (lane & 15);
+        int block = -1;
+        float ks = 0.f;
+        if (mine < n) {
+          block = table[mine];
+          if (block < 0 || block >= c.num_blocks) {
+            block = -1;
+            atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+          }
+        }
+        if (block >= 0) ks = c.key_scale[(int64_t)block * c.kv_heads + h];
+        const int block0 = __shfl_sync(0xffffffffu, block, r), block1 = __shfl_sync(0xffffffffu, block, r + 8);
+        const int64_t at0 = ((int64_t)max(block0, 0) * c.kv_heads + h) * D + 16 * cq;
+        const int64_t at1 = ((int64_t)max(block1, 0) * c.kv_heads + h) * D + 16 * cq;
+        uint4 x[2][D / 64][2];
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+          for (int half = 0; half < D / 64; ++half) {
+            const int8_t* bounds = (side ? c.key_high : c.key_low) + half * 64;
+            x[side][half][0] = *reinterpret_cast<const uint4*>(bounds + at0);
+            x[side][half][1] = *reinterpret_cast<const uint4*>(bounds + at1);
+          }
+        int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+          for (int half = 0; half < D / 64; ++half) {
+            const uint4 u = x[side][half][0], v = x[side][half][1];
+            mma_s8(sum, u.x, v.x, u.y, v.y, b[side][half * 2][0], b[side][half * 2][1]);
+            mma_s8(sum, u.z, v.z, u.w, v.w, b[side][half * 2 + 1][0], b[side][half * 2 + 1][1]);
+          }
+        // largest over the heads: two columns here, the others in the quad's lanes
+        const float ks0 = __shfl_sync(0xffffffffu, ks, r), ks1 = __shfl_sync(0xffffffffu, ks, r + 8);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float top = -INFINITY;
+          if (real0) top = max_nan(top, __fmul_rn((float)sum[2 * k], scale0));
+          if (real1) top = max_nan(top, __fmul_rn((float)sum[2 * k + 1], scale1));
+          top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int j = tile * 16 + r + 8 * k;
+          if (cq == 0 && j < n) {
+            // groups of more than 8 heads: the raw maximum goes from pass to pass
+            if (g0) top = max_nan(top, __uint_as_float(keys[j]));
+            uint32_t key = __float_as_uint(top);
+            if (g0 + 8 >= p.group) {
+              const bool known = (k ? block1 : block0) >= 0;
+              key = j < p.first || j >= n - p.recent ? KEY_FORCED
+                    : known ? key_of(__fmul_rn(top, k ? ks1 : ks0)) : key_of(-INFINITY);
+            }
+            keys[j] = key;
+          }
+        }
+      }
+    }
+    cluster.sync();  // every CTA's keys are in place
+  }
+  if (part) return;
+
+  if (all) {
+    for (int k = threadIdx.x; k < p.count; k += THREADS) {
+      if (k < n && (table[k] < 0 || table[k] >= c.num_blocks)) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+      out[k] = k < n ? k : -1;
+    }
+    return;
+  }
+  uint32_t* own = p.spill ? keys : row_keys;
+
+  // ---- the count-th largest key: its bits from the top, 8 at a time
+  uint32_t prefix = 0;
+  int need = p.count;  // keys still to take among those that share the prefix
+#pragma unroll
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
+    histogram[threadIdx.x] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += THREADS) {
+      const uint32_t key = own[j];
+      if ((key & mask) == prefix) atomicAdd(&histogram[(key >> shift) & 255], 1);
+    }
+    __syncthreads();
+    // bins from the highest: thread i holds bin 255 - i
+    const int bin = 255 - threadIdx.x, v = histogram[bin];
+    int total;
+    const int before = block_scan(v, warp_sums, total);
+    if (before < need && before + v >= need) {
+      found[0] = bin;
+      found[1] = need - before;
+    }
+    __syncthreads();
+    prefix |= (uint32_t)found[0] << shift;
+    need = found[1];
+    __syncthreads();
+  }
+
+  // ---- kept blocks in ascending order: each thread a contiguous slice; of the keys equal to the last one the
+  // first `need`
+  const int slice = (n + THREADS - 1) / THREADS;
+  const int j0 = min(n, (int)threadIdx.x * slice), j1 = min(n, j0 + slice);
+  int above = 0, equal = 0, total;
+  for (int j = j0; j < j1; ++j) {
+    const uint32_t key = own[j];
+    above += key > prefix;
+    equal += key == prefix;
+  }
+  const int above_before = block_scan(above, warp_sums, total);
+  int equal_seen = block_scan(equal, warp_sums, total);
+  int at = above_before + min(equal_seen, need);
+  for (int j = j0; j < j1; ++j) {
+    const uint32_t key = own[j];
+    if (key > prefix || (key == prefix && equal_seen < need)) out[at++] = j;
+    equal_seen += key == prefix;
+  }
+}
+
+template <typename T, int D> int launch(const SelectParams& p, cudaStream_t stream) {
+  static bool ready[64] = {false};  // the attribute is a device's; setting it twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!ready[dev & 63]) {
+    const cudaError_t e = cudaFuncSetAttribute(select_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               MOST_SHARED_KEYS * 4);
+    if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "ucb_block8_select: %s", cudaGetErrorString(e));
+    ready[dev & 63] = true;
+  }
+  const int64_t pairs = (int64_t)p.c.num_seqs * p.c.kv_heads;
+  // CTAs of a pair: as long as the chip has room for more and each keeps a tile for every warp
+  int parts = 1;
+  while (parts < 8 && pairs * parts * 2 <= 296 && p.c.max_blocks / (parts * 2) >= 16 * WARPS) parts *= 2;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = parts;
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)(pairs * parts));
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = p.spill ? 16 : (size_t)p.c.max_blocks * 4;
+  config.stream = stream;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, select_kernel<T, D>, p);
+  if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "block8 select_kernel: %s", cudaGetErrorString(e));
+  return UCB_OK;
 }
 
 }  // namespace
@@ -99,6 +305,7 @@ namespace b8 = ucb::block8;
 
 extern "C" int64_t ucb_block8_select_workspace_bytes(const ucb_block8_cache* cache) {
   if (b8::check_cache(cache, "ucb_block8_select_workspace_bytes")) return -1;
+  if (cache->max_blocks <= b8::MOST_SHARED_KEYS) return 0;
   return (int64_t)cache->num_seqs * cache->kv_heads * cache->max_blocks * 4;
 }
 
@@ -106,21 +313,22 @@ extern "C" int ucb_block8_select(const ucb_block8_cache* cache, const void* quer
                                  int q_heads, int count, int first, int recent, int32_t* blocks, void* workspace,
                                  void* stream) {
   if (int rc = b8::check_cache(cache, "ucb_block8_select")) return rc;
-  if (!query || !blocks || !workspace) return set_error(UCB_ERR_INVALID, "ucb_block8_select: null pointer");
+  const bool spill = cache->max_blocks > b8::MOST_SHARED_KEYS;
+  if (!query || !blocks || (spill && !workspace)) return set_error(UCB_ERR_INVALID, "ucb_block8_select: null pointer");
   if (q_heads < 1 || q_heads % cache->kv_heads)
     return set_error(UCB_ERR_INVALID, "ucb_block8_select: query heads must be divisible by KV heads");
   if (first < 0 || recent < 0 || count < 1 || (int64_t)first + recent > count)
     return set_error(UCB_ERR_INVALID, "ucb_block8_select: need first + recent <= count and count >= 1");
   if (count > 4096) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_select: at most 4096 blocks");
+  if ((int64_t)cache->num_seqs * cache->kv_heads > 0x0fffffff)
+    return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_select: too many sequences and heads");
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "ucb_block8_select: device error word unavailable");
-  const b8::SelectParams p{*cache, query, q_ss, q_sh, q_heads, count, first, recent, blocks,
-                           static_cast<uint32_t*>(workspace), err};
-  const dim3 grid(cache->num_seqs, cache->kv_heads);
+  const b8::SelectParams p{*cache, query, q_ss, q_sh, q_heads / cache->kv_heads, count, first, recent, blocks,
+                           spill ? static_cast<uint32_t*>(workspace) : nullptr, err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == UCB_BF16)
-    b8::select_kernel<__nv_bfloat16><<<grid, b8::THREADS, 0, s>>>(p);
-  else
-    b8::select_kernel<__half><<<grid, b8::THREADS, 0, s>>>(p);
-  return ucb_host::check_launch("block8 select_kernel");
+  const bool bf = cache->dtype == UCB_BF16;
+  if (cache->head_dim == 128)
+    return bf ? b8::launch<__nv_bfloat16, 128>(p, s) : b8::launch<__half, 128>(p, s);
+  return bf ? b8::launch<__nv_bfloat16, 64>(p, s) : b8::launch<__half, 64>(p, s);
 }

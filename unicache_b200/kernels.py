@@ -1167,11 +1167,14 @@ def rope_table(positions: int, rotary_dim: int, *, theta: float = 10000.0,
 def _call_on(device: torch.device, name: str, *args) -> None:
     """``call`` with ``device`` current: its kernels launch on a stream of that device."""
 
+    function = getattr(_capi.load(), name)
     if torch.cuda.current_device() == device.index:
-        call(name, *args)
+        rc = function(*args)
     else:
         with torch.cuda.device(device):
-            call(name, *args)
+            rc = function(*args)
+    if rc:
+        _capi.check(rc, name)
 
 
 def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_weight: torch.Tensor | None = None,
@@ -1194,61 +1197,74 @@ def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_w
     require_cuda(first, "query" if query is not None else "key")
     device, dtype = first.device, first.dtype
     code = dtype_code(dtype)
-    tokens, head_dim = int(first.shape[0]), int(first.shape[-1])
+    if first.dim() != 3:
+        raise ValueError("query and key must be [tokens, heads, head_dim]")
+    tokens, _, head_dim = first.shape
     if not 2 <= head_dim <= 256:
         raise ValueError("head_dim must be 2 to 256")
-    sides = []
-    for name, x, weight, out in (("query", query, query_weight, query_out), ("key", key, key_weight, key_out)):
-        if x is None:
-            sides.append((None, 0, 0, 0, None, None, None, 0, 0))
-            continue
-        if x.device != device or x.dtype != dtype or x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != head_dim \
-                or x.stride(2) != 1:
-            raise ValueError(f"{name} must be [tokens, heads, head_dim] with unit channel stride, one dtype and device")
-        if weight is not None and (weight.device != device or weight.dtype != dtype or weight.numel() != head_dim
-                                   or not weight.is_contiguous()):
-            raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of the rows' dtype and device")
-        if out is None:
-            out = torch.empty(x.shape, device=device, dtype=dtype)
-        elif out.shape != x.shape or out.device != device or out.dtype != dtype or out.stride(2) != 1:
-            raise ValueError(f"{name}_out must match {name}, with unit channel stride")
-        sides.append((x.data_ptr(), x.stride(0), x.stride(1), x.shape[1], ptr(weight), out, out.data_ptr(),
-                      out.stride(0), out.stride(1)))
-    rotary = table_rows = 0
+    q = _norm_side("query", query, query_weight, query_out, device, dtype, tokens, head_dim)
+    k = _norm_side("key", key, key_weight, key_out, device, dtype, tokens, head_dim)
+    rotary = table_rows = wide = 0
+    tables = (None, None, None)
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise ValueError("the rotation needs cos, sin and positions")
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape \
+        shape = cos.shape
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or shape != sin.shape \
                 or not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError("cos and sin must be contiguous float32 [positions, rotary_dim / 2] tables")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.numel() != tokens \
+        wide = positions.dtype == torch.int64
+        if not (wide or positions.dtype == torch.int32) or positions.numel() != tokens \
                 or not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32 or int64 tensor of one entry per token")
         if cos.device != device or sin.device != device or positions.device != device:
             raise ValueError("cos, sin and positions must be on the rows' device")
-        table_rows, rotary = int(cos.shape[0]), 2 * int(cos.shape[1])
+        table_rows, rotary = shape[0], 2 * shape[1]
         if rotary > head_dim:
             raise ValueError("the tables rotate more channels than head_dim")
-    q, k = sides
-    _call_on(device, "ucb_head_norm_rope", q[0], q[1], q[2], q[3], k[0], k[1], k[2], k[3], q[4], k[4], ptr(cos),
-             ptr(sin), ptr(positions), int(positions is not None and positions.dtype == torch.int64), table_rows,
-             tokens, head_dim, rotary, int(interleaved), code, eps, q[6], q[7], q[8], k[6], k[7], k[8],
+        tables = (cos.data_ptr(), sin.data_ptr(), positions.data_ptr())
+    _call_on(device, "ucb_head_norm_rope", q[0], q[1], q[2], q[3], k[0], k[1], k[2], k[3], q[4], k[4], *tables,
+             wide, table_rows, tokens, head_dim, rotary, interleaved, code, eps, q[6], q[7], q[8], k[6], k[7], k[8],
              stream_of(first))
     return q[5], k[5]
 
 
-# ---------------------------------------------------------------- 8-bit block cache
-def block8_rows(cache, name: str, x: torch.Tensor) -> torch.Tensor:
-    """Check rows [N, H, D] of a block cache write."""
+def _norm_side(name, x, weight, out, device, dtype, tokens, head_dim):
+    """One side's checked (address, token stride, head stride, heads, weight, out, out address and strides)."""
 
-    if x.device != cache.device or x.dtype != cache.dtype or x.dim() != 3 or x.shape[1] != cache.num_kv_heads \
-            or x.shape[2] != cache.head_dim or x.stride(2) != 1:
+    if x is None:
+        return None, 0, 0, 0, None, None, None, 0, 0
+    shape, stride = x.shape, x.stride()
+    if x.device != device or x.dtype != dtype or len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim \
+            or stride[2] != 1:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with unit channel stride, one dtype and device")
+    if weight is not None:
+        if weight.device != device or weight.dtype != dtype or weight.numel() != head_dim or not weight.is_contiguous():
+            raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of the rows' dtype and device")
+        weight = weight.data_ptr()
+    if out is None:
+        out = x.new_empty(shape)
+        out_stride = (shape[1] * head_dim, head_dim)
+    else:
+        out_stride = out.stride()
+        if out.shape != shape or out.device != device or out.dtype != dtype or out_stride[2] != 1:
+            raise ValueError(f"{name}_out must match {name}, with unit channel stride")
+    return x.data_ptr(), stride[0], stride[1], shape[1], weight, out, out.data_ptr(), out_stride[0], out_stride[1]
+
+
+# ---------------------------------------------------------------- 8-bit block cache
+def _block8_rows(cache, name: str, x: torch.Tensor) -> tuple:
+    """Shape and strides of checked rows [N, H, D] of a block cache write."""
+
+    shape, stride = x.shape, x.stride()
+    if x.device != cache.device or x.dtype != cache.dtype or len(shape) != 3 or shape[1] != cache.num_kv_heads \
+            or shape[2] != cache.head_dim or stride[2] != 1:
         raise ValueError(f"{name} must be [rows, kv_heads, head_dim] with unit channel stride, in the cache's dtype and "
                          "on its device")
-    return x
+    return shape, stride
 
 
-def block8_starts(cache, rows: int, starts: torch.Tensor | None) -> int | None:
+def _block8_starts(cache, rows: int, starts: torch.Tensor | None) -> int | None:
     if starts is None:
         if rows != cache.num_seqs:
             raise ValueError("without starts there must be one row for each sequence")
@@ -1262,53 +1278,53 @@ def block8_starts(cache, rows: int, starts: torch.Tensor | None) -> int | None:
 def block8_write(cache, key: torch.Tensor, value: torch.Tensor, starts: torch.Tensor | None = None) -> None:
     """Rows [N, H, D] become the last tokens of the cache's sequences (``Int8BlockCache.write``)."""
 
-    block8_rows(cache, "key", key)
-    block8_rows(cache, "value", value)
-    rows = int(key.shape[0])
-    if int(value.shape[0]) != rows:
+    shape, ks = _block8_rows(cache, "key", key)
+    value_shape, vs = _block8_rows(cache, "value", value)
+    rows = shape[0]
+    if value_shape[0] != rows:
         raise ValueError("key and value must have the same rows")
-    at = block8_starts(cache, rows, starts)
-    _call_on(cache.device, "ucb_block8_write", cache.descriptor, key.data_ptr(), key.stride(0), key.stride(1),
-             value.data_ptr(), value.stride(0), value.stride(1), rows, at, stream_of(cache.lengths))
+    at = _block8_starts(cache, rows, starts)
+    _call_on(cache.device, "ucb_block8_write", cache.descriptor, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0],
+             vs[1], rows, at, stream_of(key))
 
 
 def block8_read(cache, rows: int, starts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The last rows of every sequence restored (``Int8BlockCache.read``)."""
 
-    at = block8_starts(cache, rows, starts)
-    key = torch.empty((rows, cache.num_kv_heads, cache.head_dim), device=cache.device, dtype=cache.dtype)
-    value = torch.empty_like(key)
+    at = _block8_starts(cache, rows, starts)
+    shape = (rows, cache.num_kv_heads, cache.head_dim)
+    key, value = cache.pending_key.new_empty(shape), cache.pending_key.new_empty(shape)
     _call_on(cache.device, "ucb_block8_read", cache.descriptor, rows, at, key.data_ptr(), value.data_ptr(),
              stream_of(cache.lengths))
     return key, value
 
 
-def _block8_query(cache, query: torch.Tensor) -> int:
-    """Query heads of a query [S, Hq, D] or [S, L, Hq, D] of the cache's sequences."""
+def _block8_query(cache, query: torch.Tensor) -> tuple:
+    """Shape and strides of a checked query [S, Hq, D] or [S, L, Hq, D] of the cache's sequences."""
 
-    if query.device != cache.device or query.dtype != cache.dtype or query.shape[0] != cache.num_seqs \
-            or query.shape[-1] != cache.head_dim or query.stride(-1) != 1:
+    shape, stride = query.shape, query.stride()
+    if query.device != cache.device or query.dtype != cache.dtype or len(shape) < 3 or shape[0] != cache.num_seqs \
+            or shape[-1] != cache.head_dim or stride[-1] != 1:
         raise ValueError("query must be [num_seqs, (queries,) q_heads, head_dim] with unit channel stride, in the "
                          "cache's dtype and on its device")
-    q_heads = int(query.shape[-2])
-    if q_heads < 1 or q_heads % cache.num_kv_heads:
+    if shape[-2] < 1 or shape[-2] % cache.num_kv_heads:
         raise ValueError("Query heads must be divisible by KV heads")
-    return q_heads
+    return shape, stride
 
 
 def block8_select(query: torch.Tensor, cache, *, count: int, first: int = 1, recent: int = 2) -> torch.Tensor:
     """The blocks of each sequence and KV head that the query [S, Hq, D] may need most (see
     ``Int8BlockCache.select``): int32 [S, Hkv, count]."""
 
-    if query.dim() != 3:
+    shape, stride = _block8_query(cache, query)
+    if len(shape) != 3:
         raise ValueError("block selection takes one query token a sequence: [num_seqs, q_heads, head_dim]")
-    q_heads = _block8_query(cache, query)
     if not (1 <= count <= 4096 and first >= 0 and recent >= 0 and first + recent <= count):
         raise ValueError("need 1 <= count <= 4096 and first + recent <= count")
-    blocks = torch.empty((cache.num_seqs, cache.num_kv_heads, count), device=cache.device, dtype=torch.int32)
-    workspace = torch.empty(cache.select_bytes, device=cache.device, dtype=torch.uint8)
-    _call_on(cache.device, "ucb_block8_select", cache.descriptor, query.data_ptr(), query.stride(0), query.stride(1),
-             q_heads, count, first, recent, blocks.data_ptr(), workspace.data_ptr(), stream_of(query))
+    blocks = cache.lengths.new_empty((cache.num_seqs, cache.num_kv_heads, count))
+    workspace = cache.key_code.new_empty(cache.select_bytes) if cache.select_bytes else None
+    _call_on(cache.device, "ucb_block8_select", cache.descriptor, query.data_ptr(), stride[0], stride[1], shape[1],
+             count, first, recent, blocks.data_ptr(), ptr(workspace), stream_of(query))
     return blocks
 
 
@@ -1317,27 +1333,31 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
     """Attention of the last query tokens over the cache (see ``Int8BlockCache.attention``): query
     [S, Hq, D] or [S, L, Hq, D] -> (out like query, lse fp32 of its leading dimensions)."""
 
-    if query.dim() not in (3, 4):
+    shape, stride = _block8_query(cache, query)
+    if len(shape) == 3:
+        queries, query_stride = 1, 0
+    elif len(shape) == 4:
+        queries, query_stride = shape[1], stride[1]
+    else:
         raise ValueError("query must be [num_seqs, (queries,) q_heads, head_dim]")
-    q_heads = _block8_query(cache, query)
-    queries, stride = (1, 0) if query.dim() == 3 else (int(query.shape[1]), query.stride(1))
     if not 1 <= queries <= 16:
         raise ValueError("the block cache attention takes 1 to 16 query tokens a sequence; read the cache back and "
                          "use long_query_attention_summary for more")
-    selected = 0
+    selected, at = 0, None
     if blocks is not None:
-        if blocks.device != cache.device or blocks.dtype != torch.int32 or blocks.dim() != 3 \
-                or blocks.shape[0] != cache.num_seqs or blocks.shape[1] != cache.num_kv_heads \
-                or blocks.shape[2] < 1 or not blocks.is_contiguous():
+        listed = blocks.shape
+        if blocks.device != cache.device or blocks.dtype != torch.int32 or len(listed) != 3 \
+                or listed[0] != cache.num_seqs or listed[1] != cache.num_kv_heads \
+                or listed[2] < 1 or not blocks.is_contiguous():
             raise ValueError("blocks must be a contiguous int32 [num_seqs, kv_heads, count] tensor on the cache's device")
-        selected = int(blocks.shape[2])
-    scale = 1.0 / math.sqrt(cache.head_dim) if softmax_scale is None else float(softmax_scale)
-    out = torch.empty(query.shape, device=cache.device, dtype=cache.dtype)
-    lse = torch.empty(query.shape[:-1], device=cache.device, dtype=torch.float32)
+        selected, at = listed[2], blocks.data_ptr()
+    q_heads = shape[-2]
+    scale = cache.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
+    out, lse = query.new_empty(shape), cache.key_scale.new_empty(shape[:-1])
     workspace = cache.attention_workspace(queries, q_heads)
-    _call_on(cache.device, "ucb_block8_attention", cache.descriptor, query.data_ptr(), query.stride(0), stride,
-             query.stride(-2), queries, q_heads, ptr(blocks), selected, scale, out.data_ptr(), lse.data_ptr(),
-             ptr(workspace), stream_of(query))
+    _call_on(cache.device, "ucb_block8_attention", cache.descriptor, query.data_ptr(), stride[0], query_stride, stride[-2],
+             queries, q_heads, at, selected, scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
+             stream_of(query))
     return out, lse
 
 

@@ -207,7 +207,7 @@ class Int8BlockCache:
             if size < 0:
                 raise RuntimeError("the device of the block cache is unavailable")
             self._workspace_bytes[(queries, q_heads)] = size
-        return torch.empty(size, device=self.device, dtype=torch.uint8)
+        return self.key_code.new_empty(size)
 
     # ---------------------------------------------------------------- accounting
     @property
