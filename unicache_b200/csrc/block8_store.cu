@@ -34,6 +34,7 @@ struct WriteParams {
   ucb_block8_cache c;
   const void *key, *value;
   int64_t k_st, k_sh, v_st, v_sh, rows;
+  int aligned;  // rows start on 16 bytes
   const int32_t* starts;
   unsigned int* err;
 };
@@ -58,50 +59,189 @@ __device__ __forceinline__ int seq_of_row(const int32_t* starts, int seqs, int64
   return lo;
 }
 
-// One side (keys or values) of one block and head: rows [0, held) come from the
-// pending rows, rows [held, m) from the call's.
-template <typename T, bool KEY>
-__device__ void write_block(const WriteParams& p, int s, int h, int64_t block, int m, int held, int64_t first_row) {
-  __shared__ unsigned int amax_bits;
-  __shared__ int low[THREADS], high[THREADS];
-  const ucb_block8_cache& c = p.c;
-  const int d = c.head_dim, bt = c.block_tokens;
-  const int ch = threadIdx.x % d, g = threadIdx.x / d, groups = THREADS / d;
-  const int64_t st = KEY ? p.k_st : p.v_st;
-  const T* src = static_cast<const T*>(KEY ? p.key : p.value) + h * (KEY ? p.k_sh : p.v_sh) + ch;
-  T* pend = static_cast<T*>(KEY ? c.pending_key : c.pending_value) + ((int64_t)s * c.kv_heads + h) * bt * d + ch;
-  int8_t* codes = (KEY ? c.key_code : c.value_code) + (block * c.kv_heads + h) * bt * d + ch;
-  auto row = [&](int r) { return r < held ? pend[(int64_t)r * d] : src[(first_row + r - held) * st]; };
-  if (threadIdx.x == 0) amax_bits = 0;
-  __syncthreads();
-  unsigned int top = 0;
-  for (int r = g; r < m; r += groups)  // magnitude bits: their order is the values', with NaN above infinity
-    top = max(top, __float_as_uint(Dtype<T>::to_f(row(r))) & 0x7fffffffu);
-  atomicMax(&amax_bits, top);
-  __syncthreads();
-  const float scale = scale_of(__uint_as_float(amax_bits));
-  const float inverse = __fdiv_rn(1.f, scale);
-  int lo = 127, hi = -127;
-  for (int r = g; r < m; r += groups) {
-    const T x = row(r);
-    const int q = code_of(Dtype<T>::to_f(x), inverse);
-    codes[(int64_t)r * d] = (int8_t)q;
-    lo = min(lo, q);
-    hi = max(hi, q);
-    if (m < bt && r >= held) pend[(int64_t)r * d] = x;
+// Eight adjacent 16-bit elements; rows that do not start on 16 bytes element by element.
+__device__ __forceinline__ uint4 load8(const uint16_t* x, bool aligned) {
+  if (aligned) return *reinterpret_cast<const uint4*>(x);
+  return make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16,
+                    x[6] | (uint32_t)x[7] << 16);
+}
+
+template <bool BF> __device__ __forceinline__ float low_half(uint32_t w) {
+  return BF ? Dtype<__nv_bfloat16>::lo(w) : Dtype<__half>::lo(w);
+}
+template <bool BF> __device__ __forceinline__ float high_half(uint32_t w) {
+  return BF ? Dtype<__nv_bfloat16>::hi(w) : Dtype<__half>::hi(w);
+}
+template <bool BF> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  if (BF) {
+    const __nv_bfloat162 m = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
   }
-  if (threadIdx.x == 0) (KEY ? c.key_scale : c.value_scale)[block * c.kv_heads + h] = scale;
-  if (KEY) {
-    low[threadIdx.x] = lo;
-    high[threadIdx.x] = hi;
-    __syncthreads();
-    if (g == 0) {
-      for (int k = 1; k < groups; ++k) lo = min(lo, low[k * d + ch]), hi = max(hi, high[k * d + ch]);
-      c.key_low[(block * c.kv_heads + h) * d + ch] = (int8_t)lo;
-      c.key_high[(block * c.kv_heads + h) * d + ch] = (int8_t)hi;
+  const __half2 m = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <bool BF> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  if (BF) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+
+// Four codes: rint of the fp32 product by adding 1.5 * 2^23 (two roundings, as code_of has; the products are
+// below 128), whose low byte is the code.  `inverse` 0 stands for a scale that is no number: codes 0.
+template <bool BF> __device__ __forceinline__ uint32_t codes4(uint32_t w0, uint32_t w1, float inverse) {
+  if (inverse == 0.f) return 0;
+  const float x[4] = {low_half<BF>(w0), high_half<BF>(w0), low_half<BF>(w1), high_half<BF>(w1)};
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inverse), 12582912.f));
+  return prmt(prmt(v[0], v[1], 0x0040), prmt(v[2], v[3], 0x0040), 0x5410);
+}
+
+// 1 / scale, 0 for a scale that is no number.
+__device__ __forceinline__ float inverse_of(float scale) { return scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f; }
+
+// Keys and values of one block and head: rows [0, held) are pending ones, rows [held, m) the call's.  The new
+// rows decide whether the block's scale grows: where it does not, the codes
+// of the held rows stand (they depend on the scale alone, and the scale of a
+// larger magnitude is never the smaller), and only the new rows are written.
+template <bool BF, int D, int BT>
+__device__ void write_block(const WriteParams& p, int s, int h, int64_t block, int m, int held, int64_t first_row) {
+  constexpr int UNITS = D / 8, STRIDE = THREADS / UNITS, PASSES = (BT + STRIDE - 1) / STRIDE, WARPS = THREADS / 32;
+  __shared__ uint32_t warp_top[2][WARPS];
+  __shared__ __align__(16) uint32_t warp_low[WARPS][D / 2], warp_high[WARPS][D / 2];
+  const ucb_block8_cache& c = p.c;
+  const int unit = threadIdx.x % UNITS, g = threadIdx.x / UNITS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at = (block * c.kv_heads + h) * (int64_t)(BT * D) + unit * 8;
+  const int64_t scale_at = block * c.kv_heads + h;
+  const int64_t pending_at = ((int64_t)s * c.kv_heads + h) * (BT * D) + unit * 8;
+  const float old[2] = {held ? c.key_scale[scale_at] : 0.f, held ? c.value_scale[scale_at] : 0.f};
+
+  // ---- new rows: loads of both sides together
+  uint4 x[2][PASSES];
+  uint32_t top[2] = {0, 0}, low[4], high[4];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const uint16_t* src = static_cast<const uint16_t*>(side ? p.value : p.key) + h * (side ? p.v_sh : p.k_sh) + unit * 8;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int row = held + g + i * STRIDE;
+      if (row < m) x[side][i] = load8(src + (first_row + row - held) * (side ? p.v_st : p.k_st), p.aligned);
     }
   }
+  constexpr uint32_t INF2 = BF ? 0x7f807f80u : 0x7c007c00u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) low[k] = INF2, high[k] = INF2 | 0x80008000u;
+  auto bounds = [&](uint4 w) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) low[k] = min2<BF>(low[k], v[k]), high[k] = max2<BF>(high[k], v[k]);
+  };
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+    if (held + g + i * STRIDE < m) {
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {  // magnitude bits: their order is the values', with NaN above infinity
+        const uint4 w = x[side][i];
+        top[side] = __vmaxu2(top[side], __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
+                                                 __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+      }
+      bounds(x[0][i]);
+    }
+  auto share_bounds = [&]() {  // over the warp's rows, then one row of shared memory a warp
+#pragma unroll
+    for (int o = UNITS; o < 32; o <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        low[k] = min2<BF>(low[k], __shfl_xor_sync(0xffffffffu, low[k], o));
+        high[k] = max2<BF>(high[k], __shfl_xor_sync(0xffffffffu, high[k], o));
+      }
+    if (lane < UNITS) {
+      *reinterpret_cast<uint4*>(&warp_low[warp][unit * 4]) = make_uint4(low[0], low[1], low[2], low[3]);
+      *reinterpret_cast<uint4*>(&warp_high[warp][unit * 4]) = make_uint4(high[0], high[1], high[2], high[3]);
+    }
+  };
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const uint32_t t = __reduce_max_sync(0xffffffffu, max(top[side] & 0xffffu, top[side] >> 16));
+    if (lane == 0) warp_top[side][warp] = t;
+  }
+  share_bounds();
   __syncthreads();
+  float scale[2], inverse[2];
+  bool grown[2];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) t = max(t, warp_top[side][w]);
+    const float mine = scale_of(low_half<BF>(t));
+    grown[side] = !held || mine > old[side] || (mine != mine && old[side] == old[side]);
+    scale[side] = grown[side] ? mine : old[side];
+    inverse[side] = inverse_of(scale[side]);
+  }
+
+  // ---- codes of the new rows, and the rows themselves while the block is incomplete
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int row = held + g + i * STRIDE;
+      if (row >= m) continue;
+      const uint4 w = x[side][i];
+      *reinterpret_cast<uint2*>((side ? c.value_code : c.key_code) + at + row * D) =
+          make_uint2(codes4<BF>(w.x, w.y, inverse[side]), codes4<BF>(w.z, w.w, inverse[side]));
+      if (m < BT)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(side ? c.pending_value : c.pending_key) + pending_at + row * D) = w;
+    }
+  // ---- a larger scale: the held rows again
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+    if (held && grown[side]) {
+      const uint16_t* src = static_cast<const uint16_t*>(side ? c.pending_value : c.pending_key) + pending_at;
+      int8_t* codes = (side ? c.value_code : c.key_code) + at;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int row = g + i * STRIDE;
+        if (row < held) x[side][i] = *reinterpret_cast<const uint4*>(src + row * D);
+      }
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int row = g + i * STRIDE;
+        if (row >= held) continue;
+        const uint4 w = x[side][i];
+        if (side == 0) bounds(w);
+        *reinterpret_cast<uint2*>(codes + row * D) =
+            make_uint2(codes4<BF>(w.x, w.y, inverse[side]), codes4<BF>(w.z, w.w, inverse[side]));
+      }
+      if (side == 0) {
+        __syncthreads();  // the new rows' bounds were read by no one yet, but other warps' are in place
+        share_bounds();
+        __syncthreads();
+      }
+    }
+  if (threadIdx.x < 2 && grown[threadIdx.x ? 1 : 0])
+    (threadIdx.x ? c.value_scale : c.key_scale)[scale_at] = threadIdx.x ? scale[1] : scale[0];
+  // ---- bounds of the key codes: rounding keeps order, so they are the codes of the channels' bounds
+  for (int pair = threadIdx.x; pair < D / 2; pair += THREADS) {
+    uint32_t lo = warp_low[0][pair], hi = warp_high[0][pair];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) lo = min2<BF>(lo, warp_low[w][pair]), hi = max2<BF>(hi, warp_high[w][pair]);
+    const uint32_t q = codes4<BF>(lo, hi, inverse[0]);  // low of two channels, high of two channels
+    char2 low2 = make_char2((signed char)(q & 255), (signed char)(q >> 8 & 255));
+    char2 high2 = make_char2((signed char)(q >> 16 & 255), (signed char)(q >> 24));
+    char2* low_to = reinterpret_cast<char2*>(c.key_low + scale_at * D) + pair;
+    char2* high_to = reinterpret_cast<char2*>(c.key_high + scale_at * D) + pair;
+    if (!grown[0]) {
+      const char2 a = *low_to, b = *high_to;
+      low2 = make_char2(min(low2.x, a.x), min(low2.y, a.y));
+      high2 = make_char2(max(high2.x, b.x), max(high2.y, b.y));
+    }
+    *low_to = low2;
+    *high_to = high2;
+  }
 }
 
 // Work items of a head: item s < num_seqs is sequence s's first touched block
@@ -109,10 +249,10 @@ __device__ void write_block(const WriteParams& p, int s, int h, int64_t block, i
 // the last overwrites); item num_seqs + i is the whole block in between that
 // holds row i * block_tokens of the call (every such block holds exactly one
 // multiple of block_tokens).
-template <typename T>
+template <bool BF, int D, int BT>
 __global__ void __launch_bounds__(THREADS) write_kernel(const WriteParams p) {
   const ucb_block8_cache& c = p.c;
-  const int bt = c.block_tokens, h = blockIdx.y;
+  const int bt = BT, h = blockIdx.y;
   const bool ends = blockIdx.x < c.num_seqs;
   const int64_t probe = ends ? 0 : (int64_t)(blockIdx.x - c.num_seqs) * bt;
   const int s = ends ? blockIdx.x : seq_of_row(p.starts, c.num_seqs, probe);
@@ -131,13 +271,14 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const WriteParams p) {
     const int64_t t0 = (int64_t)j * bt;
     const int m = (int)min((int64_t)bt, len - t0);
     const int held = (int)max((int64_t)0, min((int64_t)m, old - t0));
-    const int64_t row = a + t0 + held - old;
-    write_block<T, true>(p, s, h, block, m, held, row);
-    write_block<T, false>(p, s, h, block, m, held, row);
+    write_block<BF, D, BT>(p, s, h, block, m, held, a + t0 + held - old);
   };
   if (ends) {
     one(first);
-    if (last > first && len % bt) one(last);
+    if (last > first && len % bt) {
+      __syncthreads();  // the pending rows of the first block are read
+      one(last);
+    }
   } else {
     if (probe < a || probe >= e) return;
     const int64_t j = (old + probe - a) / bt;
@@ -153,37 +294,74 @@ struct ReadParams {
   unsigned int* err;
 };
 
-// One warp per row: four codes of each side at a time over the row's heads.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) read_kernel(const ReadParams p) {
+// A warp restores ROWS consecutive rows: lanes find one row's block each, then all
+// lanes take units of 16 codes of every row's heads, keys and values.
+constexpr int READ_ROWS = 4;
+
+template <bool BF, int D> __global__ void __launch_bounds__(THREADS) read_kernel(const ReadParams p) {
   const ucb_block8_cache& c = p.c;
-  const int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-  if (r >= p.rows) return;
-  const int lane = threadIdx.x & 31, d = c.head_dim, bt = c.block_tokens;
-  const int s = seq_of_row(p.starts, c.num_seqs, r);
-  int64_t a, e;
-  const bool ok = row_range(p.starts, s, p.rows, a, e);
-  const int64_t len = c.lengths[s], t = len - (e - r);
-  if (!ok || r < a || r >= e || len - (e - a) < 0 || len > (int64_t)c.max_blocks * bt) {
-    if (lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-    return;
-  }
-  const int64_t block = pool_block(c, s, (int)(t / bt), p.err);
-  if (block < 0) return;
-  for (int i = lane; i < c.kv_heads * d / 4; i += 32) {
-    const int h = i / (d / 4), ch = i % (d / 4) * 4;
-    const int64_t at = ((block * c.kv_heads + h) * bt + t % bt) * d + ch;
-    const int64_t to = (r * c.kv_heads + h) * d + ch;
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const char4 q = *reinterpret_cast<const char4*>((side ? c.value_code : c.key_code) + at);
-      const float x = (side ? c.value_scale : c.key_scale)[block * c.kv_heads + h];
-      T* out = static_cast<T*>(side ? p.value : p.key) + to;
-      out[0] = Dtype<T>::from_f(q.x * x);
-      out[1] = Dtype<T>::from_f(q.y * x);
-      out[2] = Dtype<T>::from_f(q.z * x);
-      out[3] = Dtype<T>::from_f(q.w * x);
+  const int lane = threadIdx.x & 31, bt = c.block_tokens;
+  const int64_t r0 = ((int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * READ_ROWS;
+  int block = -1, in_block = 0;
+  if (lane < READ_ROWS && r0 + lane < p.rows) {
+    const int64_t r = r0 + lane;
+    const int s = seq_of_row(p.starts, c.num_seqs, r);
+    int64_t a, e;
+    const bool ok = row_range(p.starts, s, p.rows, a, e);
+    const int64_t len = c.lengths[s], t = len - (e - r);
+    if (!ok || r < a || r >= e || len - (e - a) < 0 || len > (int64_t)c.max_blocks * bt) {
+      atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+    } else {
+      block = (int)pool_block(c, s, (int)(t / bt), p.err);
+      in_block = (int)(t % bt);
     }
+  }
+  int where[READ_ROWS], row[READ_ROWS];
+#pragma unroll
+  for (int k = 0; k < READ_ROWS; ++k) {
+    where[k] = __shfl_sync(0xffffffffu, block, k);
+    row[k] = __shfl_sync(0xffffffffu, in_block, k);
+  }
+  const int units = c.kv_heads * (D / 16);
+  for (int i = lane; i < 2 * units; i += 32) {
+    const int side = i >= units, u = side ? i - units : i, h = u / (D / 16), d = u % (D / 16) * 16;
+    const int8_t* codes = side ? c.value_code : c.key_code;
+    const float* scales = side ? c.value_scale : c.key_scale;
+    uint16_t* out = static_cast<uint16_t*>(side ? p.value : p.key);
+    uint4 q[READ_ROWS];
+    float scale[READ_ROWS];
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; ++k) {
+      if (where[k] >= 0) {
+        const int64_t at = (int64_t)where[k] * c.kv_heads + h;
+        q[k] = *reinterpret_cast<const uint4*>(codes + (at * bt + row[k]) * D + d);
+        scale[k] = scales[at];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < READ_ROWS; ++k) {
+      if (where[k] < 0) continue;
+      const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+      uint32_t y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t two = w[j / 2] >> (j % 2 * 16);
+        const float x0 = (float)(int)(signed char)(two & 255) * scale[k], x1 = (float)(int)(signed char)(two >> 8 & 255) * scale[k];
+        y[j] = BF ? pack_bf16x2(x0, x1) : pack_f16x2(x0, x1);
+      }
+      uint4* to = reinterpret_cast<uint4*>(out + ((r0 + k) * c.kv_heads + h) * D + d);
+      to[0] = make_uint4(y[0], y[1], y[2], y[3]);
+      to[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+  }
+}
+
+template <bool BF, int D> void launch_write(const WriteParams& p, dim3 grid, cudaStream_t s) {
+  switch (p.c.block_tokens) {
+    case 16: write_kernel<BF, D, 16><<<grid, THREADS, 0, s>>>(p); break;
+    case 32: write_kernel<BF, D, 32><<<grid, THREADS, 0, s>>>(p); break;
+    case 64: write_kernel<BF, D, 64><<<grid, THREADS, 0, s>>>(p); break;
+    default: write_kernel<BF, D, 128><<<grid, THREADS, 0, s>>>(p);
   }
 }
 
@@ -204,15 +382,18 @@ extern "C" int ucb_block8_write(const ucb_block8_cache* cache, const void* key, 
   if (!key || !value) return set_error(UCB_ERR_INVALID, "ucb_block8_write: null pointer");
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "ucb_block8_write: device error word unavailable");
-  const b8::WriteParams p{*cache, key, value, k_st, k_sh, v_st, v_sh, rows, starts, err};
+  b8::WriteParams p{*cache, key, value, k_st, k_sh, v_st, v_sh, rows, 0, starts, err};
+  p.aligned = ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) == 0 &&
+              ((k_st | k_sh | v_st | v_sh) & 7) == 0;
   const int64_t items = cache->num_seqs + (starts ? (rows + cache->block_tokens - 1) / cache->block_tokens : 0);
   if (items > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_write: too many rows");
   const dim3 grid((unsigned)items, cache->kv_heads);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == UCB_BF16)
-    b8::write_kernel<__nv_bfloat16><<<grid, b8::THREADS, 0, s>>>(p);
+  const bool bf = cache->dtype == UCB_BF16;
+  if (cache->head_dim == 128)
+    bf ? b8::launch_write<true, 128>(p, grid, s) : b8::launch_write<false, 128>(p, grid, s);
   else
-    b8::write_kernel<__half><<<grid, b8::THREADS, 0, s>>>(p);
+    bf ? b8::launch_write<true, 64>(p, grid, s) : b8::launch_write<false, 64>(p, grid, s);
   return ucb_host::check_launch("block8 write_kernel");
 }
 
@@ -226,12 +407,17 @@ extern "C" int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, cons
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "ucb_block8_read: device error word unavailable");
   const b8::ReadParams p{*cache, rows, starts, key, value, err};
-  const int64_t blocks = (rows + b8::THREADS / 32 - 1) / (b8::THREADS / 32);
+  if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15)
+    return set_error(UCB_ERR_INVALID, "ucb_block8_read: outputs must be 16-byte aligned");
+  const int64_t each = b8::THREADS / 32 * b8::READ_ROWS, blocks = (rows + each - 1) / each;
   if (blocks > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_read: too many rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == UCB_BF16)
-    b8::read_kernel<__nv_bfloat16><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p);
+  const bool bf = cache->dtype == UCB_BF16;
+  if (cache->head_dim == 128)
+    bf ? b8::read_kernel<true, 128><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p)
+       : b8::read_kernel<false, 128><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p);
   else
-    b8::read_kernel<__half><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p);
+    bf ? b8::read_kernel<true, 64><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p)
+       : b8::read_kernel<false, 64><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p);
   return ucb_host::check_launch("block8 read_kernel");
 }

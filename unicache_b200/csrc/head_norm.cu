@@ -1,5 +1,7 @@
 // RMS norm of every query and key head and the rotary embedding of its
-// position in one pass over the rows (ucb_head_norm_rope).
+// position in one pass over the rows (ucb_head_norm_rope):
+//   y = x * rsqrt(mean(x^2) + eps) * w,  (a, b) -> (a c - b s, b c + a s)
+// in fp32 with one rounding.  Each row is read and written once: memory bound.
 #include "common.cuh"
 
 namespace ucb {
@@ -76,7 +78,145 @@ __global__ void __launch_bounds__(256) head_norm_rows_kernel(const HeadNormParam
   }
 }
 
+// Eight adjacent elements of a row as fp32.
+template <typename T> __device__ __forceinline__ void load8(const T* src, float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 w = *reinterpret_cast<const uint4*>(src);
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = Dtype<T>::lo(v[i]), x[2 * i + 1] = Dtype<T>::hi(v[i]);
+  } else {
+    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+}
+template <typename T> __device__ __forceinline__ void store8(T* dst, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = Dtype<T>::code == UCB_BF16 ? pack_bf16x2(x[2 * i], x[2 * i + 1]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+// head_dim 8 L for L = 8, 16 or 32 lanes a row, 16-byte aligned rows, and rotation pairs that are neighbours
+// or a whole number of lanes apart: L lanes hold a row, eight channels each,
+// and HEADS rows of one token in flight, so that the token's angles are read
+// once for them.  A partner's channels come from its lane by one shuffle each.
+template <typename T, int L, int HEADS, bool PAIRS>
+__global__ void __launch_bounds__(256) head_norm_lanes_kernel(const HeadNormParams p, int q_units, int units) {
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const int lane = threadIdx.x % L, d = lane * 8;
+  const bool live = unit < p.tokens * units;
+  const int64_t t = live ? unit / units : 0;
+  const int u = live ? (int)(unit - t * units) : 0;
+  const bool is_q = u < q_units;
+  const int head0 = (is_q ? u : u - q_units) * HEADS, heads = live ? (is_q ? p.hq : p.hk) : 0;
+  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.q_st : p.k_st) + d;
+  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.qo_st : p.ko_st) + d;
+  const int64_t sh = is_q ? p.q_sh : p.k_sh, oh = is_q ? p.qo_sh : p.ko_sh;
+  float x[HEADS][8];
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i)
+    if (head0 + i < heads) load8(src + (head0 + i) * sh, x[i]);
+
+  // the lane's angles: its own pairs, or those of its eight channels
+  const int half = p.rot / 2, hop = half / 8;
+  const bool turned = d < p.rot;
+  const bool second = !PAIRS && d >= half;
+  float c[PAIRS ? 4 : 8], s[PAIRS ? 4 : 8];
+  bool bad = false;
+  if (turned) {
+    int64_t pos = position_of(p, t);
+    bad = pos < 0 || pos >= p.table_rows;
+    if (bad) {
+      if (live && lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+      pos = 0;
+    }
+    const int64_t at = pos * half + (PAIRS ? d / 2 : second ? d - half : d);
+#pragma unroll
+    for (int i = 0; i < (PAIRS ? 4 : 8); i += 4) {
+      const float4 cv = *reinterpret_cast<const float4*>(p.cos + at + i), sv = *reinterpret_cast<const float4*>(p.sin + at + i);
+      c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
+      s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
+    }
+  }
+  bad = __shfl_sync(0xffffffffu, bad, 0, L);
+  float w[8];
+  const T* weight = static_cast<const T*>(is_q ? p.qw : p.kw);
+  if (weight) load8(weight + d, w);
+  const int partner = PAIRS ? lane : second ? lane - hop : lane + hop;
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss = fmaf(x[i][k], x[i][k], ss);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = rsqrtf(ss / (float)(8 * L) + p.eps);
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = x[i][k] * r * (weight ? w[k] : 1.f);
+    if (PAIRS) {
+      if (turned) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = y[2 * k], b = y[2 * k + 1];
+          y[2 * k] = fmaf(a, c[k], -b * s[k]);
+          y[2 * k + 1] = fmaf(b, c[k], a * s[k]);
+        }
+      }
+    } else if (p.rot) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float other = __shfl_sync(0xffffffffu, y[k], partner & (L - 1), L);
+        if (turned) y[k] = second ? fmaf(y[k], c[k], other * s[k]) : fmaf(y[k], c[k], -other * s[k]);
+      }
+    }
+    if (bad) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = __int_as_float(0x7fffffff);
+    }
+    if (head0 + i < heads) store8(dst + (head0 + i) * oh, y);
+  }
+}
+
+// Whether every row of one side starts on 16 bytes.
+template <typename T> bool aligned(const void* x, int64_t st, int64_t sh) {
+  return reinterpret_cast<uintptr_t>(x) % 16 == 0 && st * sizeof(T) % 16 == 0 && sh * sizeof(T) % 16 == 0;
+}
+
+template <typename T, int L, int HEADS> int launch_lanes(const HeadNormParams& p, cudaStream_t s) {
+  const int q_units = (p.hq + HEADS - 1) / HEADS, units = q_units + (p.hk + HEADS - 1) / HEADS;
+  const int64_t blocks = (p.tokens * units * L + 255) / 256;
+  if (blocks > 0x7fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_head_norm_rope: too many rows");
+  if (p.interleaved)
+    head_norm_lanes_kernel<T, L, HEADS, true><<<(unsigned)blocks, 256, 0, s>>>(p, q_units, units);
+  else
+    head_norm_lanes_kernel<T, L, HEADS, false><<<(unsigned)blocks, 256, 0, s>>>(p, q_units, units);
+  return ucb_host::check_launch("head_norm_lanes_kernel");
+}
+
+template <typename T, int L> int launch_heads(const HeadNormParams& p, cudaStream_t s) {
+  // Four rows in flight for each group of lanes once that still gives every thread of the chip work.
+  if (p.tokens * (p.hq + p.hk) * L >= 148 * 2048 * 4) return launch_lanes<T, L, 4>(p, s);
+  return launch_lanes<T, L, 1>(p, s);
+}
+
 template <typename T> int launch(const HeadNormParams& p, cudaStream_t s) {
+  const bool tables = reinterpret_cast<uintptr_t>(p.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sin) % 16 == 0;
+  const bool rows = (!p.hq || (aligned<T>(p.q, p.q_st, p.q_sh) && aligned<T>(p.qo, p.qo_st, p.qo_sh))) &&
+                    (!p.hk || (aligned<T>(p.k, p.k_st, p.k_sh) && aligned<T>(p.ko, p.ko_st, p.ko_sh))) &&
+                    reinterpret_cast<uintptr_t>(p.qw) % 16 == 0 && reinterpret_cast<uintptr_t>(p.kw) % 16 == 0;
+  if (rows && tables && p.rot % (p.interleaved ? 8 : 16) == 0) {
+    if (p.d == 128) return launch_heads<T, 16>(p, s);
+    if (p.d == 64) return launch_heads<T, 8>(p, s);
+    if (p.d == 256) return launch_heads<T, 32>(p, s);
+  }
   const int64_t blocks = (p.tokens * (p.hq + p.hk) + 7) / 8;
   if (blocks > 0x7fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_head_norm_rope: too many rows");
   head_norm_rows_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(p);
