@@ -250,7 +250,7 @@ __device__ void write_block(const WriteParams& p, int s, int h, int64_t block, i
 // holds row i * block_tokens of the call (every such block holds exactly one
 // multiple of block_tokens).
 template <bool BF, int D, int BT>
-__global__ void __launch_bounds__(THREADS) write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(const WriteParams p) {
   const ucb_block8_cache& c = p.c;
   const int bt = BT, h = blockIdx.y;
   const bool ends = blockIdx.x < c.num_seqs;
@@ -295,7 +295,7 @@ struct ReadParams {
 };
 
 // A warp restores ROWS consecutive rows: lanes find one row's block each, then all
-// lanes take units of 16 codes of every row's heads, keys and values.
+// lanes take units of 8 codes of every row's heads, keys and values.
 constexpr int READ_ROWS = 4;
 
 template <bool BF, int D> __global__ void __launch_bounds__(THREADS) read_kernel(const ReadParams p) {
@@ -322,36 +322,32 @@ template <bool BF, int D> __global__ void __launch_bounds__(THREADS) read_kernel
     where[k] = __shfl_sync(0xffffffffu, block, k);
     row[k] = __shfl_sync(0xffffffffu, in_block, k);
   }
-  const int units = c.kv_heads * (D / 16);
+  const int units = c.kv_heads * (D / 8);
   for (int i = lane; i < 2 * units; i += 32) {
-    const int side = i >= units, u = side ? i - units : i, h = u / (D / 16), d = u % (D / 16) * 16;
+    const int side = i >= units, u = side ? i - units : i, h = u / (D / 8), d = u % (D / 8) * 8;
     const int8_t* codes = side ? c.value_code : c.key_code;
     const float* scales = side ? c.value_scale : c.key_scale;
     uint16_t* out = static_cast<uint16_t*>(side ? p.value : p.key);
-    uint4 q[READ_ROWS];
+    uint2 q[READ_ROWS];
     float scale[READ_ROWS];
 #pragma unroll
-    for (int k = 0; k < READ_ROWS; ++k) {
+    for (int k = 0; k < READ_ROWS; ++k)
       if (where[k] >= 0) {
         const int64_t at = (int64_t)where[k] * c.kv_heads + h;
-        q[k] = *reinterpret_cast<const uint4*>(codes + (at * bt + row[k]) * D + d);
+        q[k] = *reinterpret_cast<const uint2*>(codes + (at * bt + row[k]) * D + d);
         scale[k] = scales[at];
       }
-    }
 #pragma unroll
     for (int k = 0; k < READ_ROWS; ++k) {
       if (where[k] < 0) continue;
-      const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
-      uint32_t y[8];
+      uint32_t y[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t two = w[j / 2] >> (j % 2 * 16);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t two = (j < 2 ? q[k].x : q[k].y) >> (j % 2 * 16);
         const float x0 = (float)(int)(signed char)(two & 255) * scale[k], x1 = (float)(int)(signed char)(two >> 8 & 255) * scale[k];
         y[j] = BF ? pack_bf16x2(x0, x1) : pack_f16x2(x0, x1);
       }
-      uint4* to = reinterpret_cast<uint4*>(out + ((r0 + k) * c.kv_heads + h) * D + d);
-      to[0] = make_uint4(y[0], y[1], y[2], y[3]);
-      to[1] = make_uint4(y[4], y[5], y[6], y[7]);
+      *reinterpret_cast<uint4*>(out + ((r0 + k) * c.kv_heads + h) * D + d) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
 }

@@ -78,78 +78,74 @@ __global__ void __launch_bounds__(256) head_norm_rows_kernel(const HeadNormParam
   }
 }
 
-// Eight adjacent elements of a row as fp32.
-template <typename T> __device__ __forceinline__ void load8(const T* src, float (&x)[8]) {
+// Four adjacent elements of a row as fp32.
+template <typename T> __device__ __forceinline__ void load4(const T* src, float* x) {
   if constexpr (sizeof(T) == 2) {
-    const uint4 w = *reinterpret_cast<const uint4*>(src);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = Dtype<T>::lo(v[i]), x[2 * i + 1] = Dtype<T>::hi(v[i]);
+    const uint2 w = *reinterpret_cast<const uint2*>(src);
+    x[0] = Dtype<T>::lo(w.x), x[1] = Dtype<T>::hi(w.x), x[2] = Dtype<T>::lo(w.y), x[3] = Dtype<T>::hi(w.y);
   } else {
-    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    const float4 a = *reinterpret_cast<const float4*>(src);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
   }
 }
-template <typename T> __device__ __forceinline__ void store8(T* dst, const float (&x)[8]) {
+template <typename T> __device__ __forceinline__ void store4(T* dst, const float* x) {
   if constexpr (sizeof(T) == 2) {
-    uint32_t v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = Dtype<T>::code == UCB_BF16 ? pack_bf16x2(x[2 * i], x[2 * i + 1]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+    const bool bf = Dtype<T>::code == UCB_BF16;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(bf ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]),
+                                                bf ? pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]));
   } else {
     *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
   }
 }
 
-// head_dim 8 L for L = 8, 16 or 32 lanes a row, 16-byte aligned rows, and rotation pairs that are neighbours
-// or a whole number of lanes apart: L lanes hold a row, eight channels each,
-// and HEADS rows of one token in flight, so that the token's angles are read
-// once for them.  A partner's channels come from its lane by one shuffle each.
+// head_dim 64, 128 or 256 with rows that start on four elements: L = head_dim / 8
+// lanes a row.  A lane holds two runs of four channels that are each
+// other's rotation partners (in the halves' form runs i and i + rotary_dim / 2), so
+// that the rotation needs no exchange and the lane four angles; HEADS rows of one
+// token are in flight and share the angles.
 template <typename T, int L, int HEADS, bool PAIRS>
-__global__ void __launch_bounds__(256) head_norm_lanes_kernel(const HeadNormParams p, int q_units, int units) {
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const int lane = threadIdx.x % L, d = lane * 8;
-  const bool live = unit < p.tokens * units;
-  const int64_t t = live ? unit / units : 0;
-  const int u = live ? (int)(unit - t * units) : 0;
-  const bool is_q = u < q_units;
+__global__ void __launch_bounds__(256) head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units) {
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / L;
+  const int lane = threadIdx.x % L;
+  const uint32_t t = unit / units, u = unit - t * units;
+  const bool live = t < p.tokens, is_q = u < q_units;
+  const int half = p.rot / 2;
+  const bool turned = lane * (PAIRS ? 8 : 4) < (PAIRS ? p.rot : half);
+  const int rest = p.rot + 8 * (lane - half / 4);  // channels that are only normalised
+  const int d0 = PAIRS ? 8 * lane : turned ? 4 * lane : rest, d1 = PAIRS || !turned ? d0 + 4 : d0 + half;
   const int head0 = (is_q ? u : u - q_units) * HEADS, heads = live ? (is_q ? p.hq : p.hk) : 0;
-  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.q_st : p.k_st) + d;
-  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.qo_st : p.ko_st) + d;
+  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.q_st : p.k_st);
+  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.qo_st : p.ko_st);
   const int64_t sh = is_q ? p.q_sh : p.k_sh, oh = is_q ? p.qo_sh : p.ko_sh;
   float x[HEADS][8];
 #pragma unroll
   for (int i = 0; i < HEADS; ++i)
-    if (head0 + i < heads) load8(src + (head0 + i) * sh, x[i]);
-
-  // the lane's angles: its own pairs, or those of its eight channels
-  const int half = p.rot / 2, hop = half / 8;
-  const bool turned = d < p.rot;
-  const bool second = !PAIRS && d >= half;
-  float c[PAIRS ? 4 : 8], s[PAIRS ? 4 : 8];
+    if (head0 + i < heads) {
+      load4(src + (head0 + i) * sh + d0, x[i]);
+      load4(src + (head0 + i) * sh + d1, x[i] + 4);
+    }
+  float c[4], s[4], w[8];
   bool bad = false;
-  if (turned) {
+  if (p.rot && live) {
     int64_t pos = position_of(p, t);
     bad = pos < 0 || pos >= p.table_rows;
     if (bad) {
-      if (live && lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+      if (lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
       pos = 0;
     }
-    const int64_t at = pos * half + (PAIRS ? d / 2 : second ? d - half : d);
-#pragma unroll
-    for (int i = 0; i < (PAIRS ? 4 : 8); i += 4) {
-      const float4 cv = *reinterpret_cast<const float4*>(p.cos + at + i), sv = *reinterpret_cast<const float4*>(p.sin + at + i);
-      c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
-      s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
+    if (turned) {
+      load4(p.cos + pos * half + 4 * lane, c);
+      load4(p.sin + pos * half + 4 * lane, s);
     }
   }
-  bad = __shfl_sync(0xffffffffu, bad, 0, L);
-  float w[8];
   const T* weight = static_cast<const T*>(is_q ? p.qw : p.kw);
-  if (weight) load8(weight + d, w);
-  const int partner = PAIRS ? lane : second ? lane - hop : lane + hop;
+  if (weight) {
+    load4(weight + d0, w);
+    load4(weight + d1, w + 4);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = 1.f;
+  }
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
     float ss = 0.f;
@@ -157,47 +153,38 @@ __global__ void __launch_bounds__(256) head_norm_lanes_kernel(const HeadNormPara
     for (int k = 0; k < 8; ++k) ss = fmaf(x[i][k], x[i][k], ss);
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss / (float)(8 * L) + p.eps);
+    const float r = bad ? __int_as_float(0x7fffffff) : rsqrtf(ss * (1.f / (8 * L)) + p.eps);
     float y[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = x[i][k] * r * (weight ? w[k] : 1.f);
-    if (PAIRS) {
-      if (turned) {
+    for (int k = 0; k < 8; ++k) y[k] = x[i][k] * r * w[k];
+    if (turned) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float a = y[2 * k], b = y[2 * k + 1];
-          y[2 * k] = fmaf(a, c[k], -b * s[k]);
-          y[2 * k + 1] = fmaf(b, c[k], a * s[k]);
-        }
-      }
-    } else if (p.rot) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float other = __shfl_sync(0xffffffffu, y[k], partner & (L - 1), L);
-        if (turned) y[k] = second ? fmaf(y[k], c[k], other * s[k]) : fmaf(y[k], c[k], -other * s[k]);
+      for (int k = 0; k < 4; ++k) {
+        const int first = PAIRS ? 2 * k : k, other = PAIRS ? 2 * k + 1 : k + 4;
+        const float a = y[first], b = y[other];
+        y[first] = fmaf(a, c[k], -b * s[k]);
+        y[other] = fmaf(b, c[k], a * s[k]);
       }
     }
-    if (bad) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = __int_as_float(0x7fffffff);
+    if (head0 + i < heads) {
+      store4(dst + (head0 + i) * oh + d0, y);
+      store4(dst + (head0 + i) * oh + d1, y + 4);
     }
-    if (head0 + i < heads) store8(dst + (head0 + i) * oh, y);
   }
 }
 
-// Whether every row of one side starts on 16 bytes.
+// Whether every row of one side starts on four elements.
 template <typename T> bool aligned(const void* x, int64_t st, int64_t sh) {
-  return reinterpret_cast<uintptr_t>(x) % 16 == 0 && st * sizeof(T) % 16 == 0 && sh * sizeof(T) % 16 == 0;
+  return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 && st % 4 == 0 && sh % 4 == 0;
 }
 
 template <typename T, int L, int HEADS> int launch_lanes(const HeadNormParams& p, cudaStream_t s) {
   const int q_units = (p.hq + HEADS - 1) / HEADS, units = q_units + (p.hk + HEADS - 1) / HEADS;
-  const int64_t blocks = (p.tokens * units * L + 255) / 256;
-  if (blocks > 0x7fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_head_norm_rope: too many rows");
+  const unsigned blocks = (unsigned)((p.tokens * units * L + 255) / 256);
   if (p.interleaved)
-    head_norm_lanes_kernel<T, L, HEADS, true><<<(unsigned)blocks, 256, 0, s>>>(p, q_units, units);
+    head_norm_lanes_kernel<T, L, HEADS, true><<<blocks, 256, 0, s>>>(p, q_units, units);
   else
-    head_norm_lanes_kernel<T, L, HEADS, false><<<(unsigned)blocks, 256, 0, s>>>(p, q_units, units);
+    head_norm_lanes_kernel<T, L, HEADS, false><<<blocks, 256, 0, s>>>(p, q_units, units);
   return ucb_host::check_launch("head_norm_lanes_kernel");
 }
 
@@ -211,8 +198,9 @@ template <typename T> int launch(const HeadNormParams& p, cudaStream_t s) {
   const bool tables = reinterpret_cast<uintptr_t>(p.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sin) % 16 == 0;
   const bool rows = (!p.hq || (aligned<T>(p.q, p.q_st, p.q_sh) && aligned<T>(p.qo, p.qo_st, p.qo_sh))) &&
                     (!p.hk || (aligned<T>(p.k, p.k_st, p.k_sh) && aligned<T>(p.ko, p.ko_st, p.ko_sh))) &&
-                    reinterpret_cast<uintptr_t>(p.qw) % 16 == 0 && reinterpret_cast<uintptr_t>(p.kw) % 16 == 0;
-  if (rows && tables && p.rot % (p.interleaved ? 8 : 16) == 0) {
+                    (reinterpret_cast<uintptr_t>(p.qw) | reinterpret_cast<uintptr_t>(p.kw)) % (4 * sizeof(T)) == 0;
+  // the lanes' 32-bit indexes hold tokens * heads * 32
+  if (rows && tables && p.rot % 8 == 0 && p.tokens <= 0x3ffffff / (p.hq + p.hk)) {
     if (p.d == 128) return launch_heads<T, 16>(p, s);
     if (p.d == 64) return launch_heads<T, 8>(p, s);
     if (p.d == 256) return launch_heads<T, 32>(p, s);
