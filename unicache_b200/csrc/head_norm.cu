@@ -20,6 +20,7 @@ struct HeadNormParams {
 };
 
 constexpr int MAX_HEAD_DIM = 256;
+constexpr int LANES_THREADS = 128;
 
 __device__ __forceinline__ int64_t position_of(const HeadNormParams& p, int64_t t) {
   return p.pos64 ? static_cast<const int64_t*>(p.pos)[t] : (int64_t)static_cast<const int32_t*>(p.pos)[t];
@@ -78,16 +79,19 @@ __global__ void __launch_bounds__(256) head_norm_rows_kernel(const HeadNormParam
   }
 }
 
-// Four adjacent elements of a row as fp32.
-template <typename T> __device__ __forceinline__ void load4(const T* src, float* x) {
-  if constexpr (sizeof(T) == 2) {
-    const uint2 w = *reinterpret_cast<const uint2*>(src);
+// Four adjacent elements, as loaded and as fp32.
+template <typename T> struct Four {
+  uint2 w;
+  __device__ __forceinline__ void load(const T* src) { w = *reinterpret_cast<const uint2*>(src); }
+  __device__ __forceinline__ void to(float* x) const {
     x[0] = Dtype<T>::lo(w.x), x[1] = Dtype<T>::hi(w.x), x[2] = Dtype<T>::lo(w.y), x[3] = Dtype<T>::hi(w.y);
-  } else {
-    const float4 a = *reinterpret_cast<const float4*>(src);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
   }
-}
+};
+template <> struct Four<float> {
+  float4 w;
+  __device__ __forceinline__ void load(const float* src) { w = *reinterpret_cast<const float4*>(src); }
+  __device__ __forceinline__ void to(float* x) const { x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w; }
+};
 template <typename T> __device__ __forceinline__ void store4(T* dst, const float* x) {
   if constexpr (sizeof(T) == 2) {
     const bool bf = Dtype<T>::code == UCB_BF16;
@@ -101,11 +105,13 @@ template <typename T> __device__ __forceinline__ void store4(T* dst, const float
 // head_dim 64, 128 or 256 with rows that start on four elements: L = head_dim / 8
 // lanes a row.  A lane holds two runs of four channels that are each
 // other's rotation partners (in the halves' form runs i and i + rotary_dim / 2), so
-// that the rotation needs no exchange and the lane four angles; HEADS rows of one
-// token are in flight and share the angles.
+// that the rotation needs no exchange and the lane four angles, which the HEADS rows
+// of one token that it has in flight share.  Measured for 16384 tokens x 32
+// heads x 128 (277 MB): 4 rows a lane 57 us (4.9 TB/s), 1 row 85, 2 rows 75,
+// 8 rows 84; 4 rows of two tokens 71; blocks of 256 threads 59.
 template <typename T, int L, int HEADS, bool PAIRS>
-__global__ void __launch_bounds__(256) head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units) {
-  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / L;
+__global__ void __launch_bounds__(LANES_THREADS, 1) head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units) {
+  const uint32_t unit = (blockIdx.x * (uint32_t)LANES_THREADS + threadIdx.x) / L;
   const int lane = threadIdx.x % L;
   const uint32_t t = unit / units, u = unit - t * units;
   const bool live = t < p.tokens, is_q = u < q_units;
@@ -114,61 +120,62 @@ __global__ void __launch_bounds__(256) head_norm_lanes_kernel(const HeadNormPara
   const int rest = p.rot + 8 * (lane - half / 4);  // channels that are only normalised
   const int d0 = PAIRS ? 8 * lane : turned ? 4 * lane : rest, d1 = PAIRS || !turned ? d0 + 4 : d0 + half;
   const int head0 = (is_q ? u : u - q_units) * HEADS, heads = live ? (is_q ? p.hq : p.hk) : 0;
-  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.q_st : p.k_st);
-  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.qo_st : p.ko_st);
   const int64_t sh = is_q ? p.q_sh : p.k_sh, oh = is_q ? p.qo_sh : p.ko_sh;
-  float x[HEADS][8];
+  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.q_st : p.k_st) + head0 * sh;
+  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.qo_st : p.ko_st) + head0 * oh;
+  const int64_t pos = p.rot && live ? position_of(p, t) : 0;
+  Four<T> raw[HEADS][2];
 #pragma unroll
   for (int i = 0; i < HEADS; ++i)
     if (head0 + i < heads) {
-      load4(src + (head0 + i) * sh + d0, x[i]);
-      load4(src + (head0 + i) * sh + d1, x[i] + 4);
+      raw[i][0].load(src + i * sh + d0);
+      raw[i][1].load(src + i * sh + d1);
     }
-  float c[4], s[4], w[8];
-  bool bad = false;
-  if (p.rot && live) {
-    int64_t pos = position_of(p, t);
-    bad = pos < 0 || pos >= p.table_rows;
-    if (bad) {
-      if (lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-      pos = 0;
-    }
-    if (turned) {
-      load4(p.cos + pos * half + 4 * lane, c);
-      load4(p.sin + pos * half + 4 * lane, s);
-    }
-  }
+  float w[8];
   const T* weight = static_cast<const T*>(is_q ? p.qw : p.kw);
   if (weight) {
-    load4(weight + d0, w);
-    load4(weight + d1, w + 4);
+    Four<T> a, b;
+    a.load(weight + d0);
+    b.load(weight + d1);
+    a.to(w);
+    b.to(w + 4);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) w[k] = 1.f;
   }
+  float c[4], s[4];
+  const bool bad = p.rot && live && (pos < 0 || pos >= p.table_rows);
+  if (bad && lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+  if (turned) {
+    const int64_t at = (bad ? 0 : pos) * half + 4 * lane;
+    const float4 cv = *reinterpret_cast<const float4*>(p.cos + at), sv = *reinterpret_cast<const float4*>(p.sin + at);
+    c[0] = cv.x, c[1] = cv.y, c[2] = cv.z, c[3] = cv.w;
+    s[0] = sv.x, s[1] = sv.y, s[2] = sv.z, s[3] = sv.w;
+  }
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    float ss = 0.f;
+    float x[8], ss = 0.f;
+    raw[i][0].to(x);
+    raw[i][1].to(x + 4);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fmaf(x[i][k], x[i][k], ss);
+    for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float r = bad ? __int_as_float(0x7fffffff) : rsqrtf(ss * (1.f / (8 * L)) + p.eps);
-    float y[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = x[i][k] * r * w[k];
+    for (int k = 0; k < 8; ++k) x[k] = x[k] * r * w[k];
     if (turned) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int first = PAIRS ? 2 * k : k, other = PAIRS ? 2 * k + 1 : k + 4;
-        const float a = y[first], b = y[other];
-        y[first] = fmaf(a, c[k], -b * s[k]);
-        y[other] = fmaf(b, c[k], a * s[k]);
+        const float a = x[first], b = x[other];
+        x[first] = fmaf(a, c[k], -b * s[k]);
+        x[other] = fmaf(b, c[k], a * s[k]);
       }
     }
     if (head0 + i < heads) {
-      store4(dst + (head0 + i) * oh + d0, y);
-      store4(dst + (head0 + i) * oh + d1, y + 4);
+      store4(dst + i * oh + d0, x);
+      store4(dst + i * oh + d1, x + 4);
     }
   }
 }
@@ -180,17 +187,18 @@ template <typename T> bool aligned(const void* x, int64_t st, int64_t sh) {
 
 template <typename T, int L, int HEADS> int launch_lanes(const HeadNormParams& p, cudaStream_t s) {
   const int q_units = (p.hq + HEADS - 1) / HEADS, units = q_units + (p.hk + HEADS - 1) / HEADS;
-  const unsigned blocks = (unsigned)((p.tokens * units * L + 255) / 256);
+  const unsigned blocks = (unsigned)((p.tokens * units * L + LANES_THREADS - 1) / LANES_THREADS);
   if (p.interleaved)
-    head_norm_lanes_kernel<T, L, HEADS, true><<<blocks, 256, 0, s>>>(p, q_units, units);
+    head_norm_lanes_kernel<T, L, HEADS, true><<<blocks, LANES_THREADS, 0, s>>>(p, q_units, units);
   else
-    head_norm_lanes_kernel<T, L, HEADS, false><<<blocks, 256, 0, s>>>(p, q_units, units);
+    head_norm_lanes_kernel<T, L, HEADS, false><<<blocks, LANES_THREADS, 0, s>>>(p, q_units, units);
   return ucb_host::check_launch("head_norm_lanes_kernel");
 }
 
 template <typename T, int L> int launch_heads(const HeadNormParams& p, cudaStream_t s) {
-  // Four rows in flight for each group of lanes once that still gives every thread of the chip work.
-  if (p.tokens * (p.hq + p.hk) * L >= 148 * 2048 * 4) return launch_lanes<T, L, 4>(p, s);
+  // Four rows a lane once one row a lane would fill the chip's threads (4999 tokens x 18 heads x 64: 5.8 us against
+  // 7.6 with one row; below that, one row has the shorter way).
+  if (p.tokens * (p.hq + p.hk) * L >= 148 * 2048) return launch_lanes<T, L, 4>(p, s);
   return launch_lanes<T, L, 1>(p, s);
 }
 

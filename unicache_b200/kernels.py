@@ -1243,12 +1243,10 @@ def _norm_side(name, x, weight, out, device, dtype, tokens, head_dim):
             raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of the rows' dtype and device")
         weight = weight.data_ptr()
     if out is None:
-        out = x.new_empty(shape)
-        out_stride = (shape[1] * head_dim, head_dim)
-    else:
-        out_stride = out.stride()
-        if out.shape != shape or out.device != device or out.dtype != dtype or out_stride[2] != 1:
-            raise ValueError(f"{name}_out must match {name}, with unit channel stride")
+        out = torch.empty_like(x)  # dense, channels contiguous as x's are
+    elif out.shape != shape or out.device != device or out.dtype != dtype or out.stride(2) != 1:
+        raise ValueError(f"{name}_out must match {name}, with unit channel stride")
+    out_stride = out.stride()
     return x.data_ptr(), stride[0], stride[1], shape[1], weight, out, out.data_ptr(), out_stride[0], out_stride[1]
 
 
@@ -1353,7 +1351,8 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
         selected, at = listed[2], blocks.data_ptr()
     q_heads = shape[-2]
     scale = cache.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
-    out, lse = query.new_empty(shape), cache.key_scale.new_empty(shape[:-1])
+    out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(shape)
+    lse = cache.key_scale.new_empty(shape[:-1])
     workspace = cache.attention_workspace(queries, q_heads)
     _call_on(cache.device, "ucb_block8_attention", cache.descriptor, query.data_ptr(), stride[0], query_stride, stride[-2],
              queries, q_heads, at, selected, scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
