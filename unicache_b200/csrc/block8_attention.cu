@@ -9,7 +9,8 @@
 // up to a dozen rows the pool's bytes bound it.
 //
 // Work split: the tiles of all (sequence, KV head, row tile) triples in one
-// flat order, every warp of the grid an equal contiguous share (lengths are
+// flat order, each triple's preceded by START empty ones for what its start
+// costs, every warp of the grid an equal contiguous share (lengths are
 // read on the device, so a captured step follows them).  A warp that holds
 // a whole triple writes its output; the others' states (reference maximum, sum,
 // unnormalised rows) are merged in shared memory within a CTA, and across CTAs by
@@ -50,8 +51,6 @@ struct AttnParams {
   int selected;
   int q_aligned;     // query rows can be read 8 bytes at a time
   int step_shift;    // log2(steps in a block)
-  int front_ctas;    // CTAs that are resident at once; those after them have smaller shares
-  float tail_share;  // of all steps, for the latter
   float scale_log2;  // softmax scale * log2(e)
   void* out;
   float* lse;
@@ -62,10 +61,9 @@ struct AttnParams {
 };
 
 constexpr int TILE = 16;     // tokens of one matrix product
+constexpr int START = 4;      // steps that the start of a pair costs a warp, in the flat order
 constexpr int MIN_STEPS = 1;  // a warp's least share, where there is more than that
-constexpr int CTAS_PER_SM = 4;  // at most, in one launch
-constexpr float TAIL_SHARE = 0.06f;
-constexpr int TAIL_FROM = 1000;
+constexpr int CTAS_PER_SM = 2;
 constexpr float LIFT = 6.f;   // log2 of the largest weight when its reference is set
 constexpr float LAZY = 14.f;  // a weight may reach 2^LAZY before its reference moves
 constexpr float LAZY_SUM = 100.f;
@@ -75,7 +73,7 @@ template <int D, int NT, int U> struct Shape {
   static constexpr int ROWS = 8 * NT;
   static constexpr int WARPS = NT == 1 ? 8 : D == 64 ? 6 : 4;
   static constexpr int STEP_BYTES = U * 2 * TILE * D;
-  static constexpr int STAGES = 98304 / (WARPS * STEP_BYTES);
+  static constexpr int STAGES = 65536 / (WARPS * STEP_BYTES);
   static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its reference, the sum's reference, the sum
   static constexpr int STATE_FLOATS = ROWS * ROW_FLOATS;
   static constexpr int RING_BYTES = STAGES * STEP_BYTES;
@@ -192,7 +190,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 
   // ---- the flat order: steps of every sequence (at least one, so that every row is written)
   int total;
-  const int listed_steps = p.selected << p.step_shift;
+  const int listed_steps = (p.selected << p.step_shift) + START;
   if (p.blocks) {
     total = c.num_seqs * listed_steps * heads_rows;
   } else {
@@ -200,7 +198,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int base = 0; base < c.num_seqs; base += S::WARPS * 32) {
       const int i = base + threadIdx.x;
-      int v = i < c.num_seqs ? max(1, (held_tokens(c, i, p.err) + STEP - 1) / STEP) : 0;
+      int v = i < c.num_seqs ? max(1, (held_tokens(c, i, p.err) + STEP - 1) / STEP) + START : 0;
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
@@ -219,18 +217,11 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   }
   const int worker = blockIdx.x * S::WARPS + warp;
   if (lane == 0) segments[warp][0].used = segments[warp][1].used = 0;
-  // shares: `front` workers have an equal part of all but the last `tail` steps, the others `piece` steps each
-  const int front = max(1, min((int)gridDim.x == p.front_ctas ? total : total / 2, p.front_ctas * S::WARPS));
-  const int behind = ((int)gridDim.x - p.front_ctas) * S::WARPS;
-  const int piece = behind ? max(1, (int)((float)total * p.tail_share) / behind) : 1;
-  const int tail = min(total - front, piece * behind);
-  const int body = total - tail, each = body / front, longer = body - each * front;
-  auto share = [&](int w) {
-    if (w <= front) return w * each + min(w, longer);
-    return min(total, body + (w - front) * piece);
-  };
+  // equal shares, the first `longer` of one step more
+  const int workers = max(1, min((int)gridDim.x * S::WARPS, total / MIN_STEPS));
+  const int each = total / workers, longer = total - each * workers;
+  auto share = [&](int w) { return w < workers ? w * each + min(w, longer) : total; };
   auto worker_of = [&](int step) {
-    if (step >= body) return front + (step - body) / piece;
     const int split = longer * (each + 1);
     return step < split ? step / (each + 1) : longer + (step - split) / each;
   };
@@ -276,8 +267,9 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   const int t_end = share(worker + 1);
   while (t < t_end) {
     const Pair a = locate(t);
-    const int begin = t - a.base, end = min(a.steps, t_end - a.base);
-    t = a.base + end;
+    const int begin = max(t - a.base - START, 0), end = min(a.steps, t_end - a.base) - START, steps = a.steps - START;
+    t = a.base + end + START;
+    if (end <= 0) continue;  // the rest of the pair's start: its tiles are the next warp's
     const int len = held_tokens(c, a.s, p.err);
     const int32_t* list = p.blocks ? p.blocks + ((int64_t)a.s * c.kv_heads + a.h) * p.selected : nullptr;
     const int32_t* table = c.block_table + (int64_t)a.s * c.max_blocks;
@@ -557,7 +549,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 
     // ---- the segment's result: lane (r, cq) holds channels VB * r .. of rows 2 cq and 2 cq + 1.  A warp's last
     // segment stays in its ring, an earlier one that a warp before began goes through global memory.
-    const bool whole = begin == 0 && end == a.steps;
+    const bool whole = begin == 0 && end == steps;
     const int which = begin == 0 ? 1 : 0;
     float* state = t >= t_end ? reinterpret_cast<float*>(ring) : p.spill + (int64_t)worker * S::STATE_FLOATS;
     __syncwarp();  // every lane is done with the ring before states overwrite it
@@ -595,7 +587,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
           if (r == 0) *reinterpret_cast<float4*>(at + D) = make_float4(ref[nt][k], sum_ref[nt][k], l, 0.f);
         }
       }
-    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == a.steps, a.s, a.h, a.rt, t >= t_end ? nullptr : state};
+    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == steps, a.s, a.h, a.rt, t >= t_end ? nullptr : state};
   }
   __syncthreads();
 
@@ -605,21 +597,29 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   // in other CTAs.  A warp's slot 0 continues the pair that was open before it, slot 1 opens one; a state outside
   // the rings ends its chain, since its warp went on to another pair.
   if (threadIdx.x == 0) p.links[blockIdx.x * 4] = -1;
-  int open_w = 0, open_n = 0;  // the open chain: first warp and count
-  bool from_before = false;
-  auto emit = [&](const Segment& seg, bool ended) {
+  const Segment& mine = segments[min(lane, 2 * S::WARPS - 1) >> 1][lane & 1];
+  unsigned used = __ballot_sync(0xffffffffu, lane < 2 * S::WARPS && mine.used);
+  while (used) {  // a chain: the segments up to the next one that opens a pair
+    const int first = __ffs(used) - 1;
+    const unsigned opening = used & 0xAAAAAAAAu & ~(1u << first);
+    const unsigned chain = opening ? used & ((1u << (__ffs(opening) - 1)) - 1) : used;
+    used &= ~chain;
+    const int open_w = first >> 1, open_n = __popc(chain), final = 31 - __clz(chain);
+    const Segment last = segments[final >> 1][final & 1];
+    const bool from_before = !(first & 1), ended = last.ends;
+    // the chain ends, here or in a later CTA
     const bool complete = ended && !from_before;
     float* to = p.partials + ((int64_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * S::STATE_FLOATS;
     for (int item = threadIdx.x; item < S::ROWS * D / 4; item += S::WARPS * 32) {
-      const int in_tile = item / (D / 4), d = item % (D / 4) * 4, row = seg.rt * S::ROWS + in_tile;
+      const int in_tile = item / (D / 4), d = item % (D / 4) * 4, row = last.rt * S::ROWS + in_tile;
       if (row >= p.rows) break;
       const unsigned char* states = smem + open_w * S::RING_BYTES + in_tile * (S::ROW_FLOATS * 4);
       const Merged m = merge_states<D>(0, open_n, 1, d, [&](int i) {
-        return i == open_n - 1 && seg.spilled ? seg.spilled + in_tile * S::ROW_FLOATS
-                                              : reinterpret_cast<const float*>(states + i * S::RING_BYTES);
+        return i == open_n - 1 && last.spilled ? last.spilled + in_tile * S::ROW_FLOATS
+                                               : reinterpret_cast<const float*>(states + i * S::RING_BYTES);
       });
       if (complete) {
-        const int64_t out = out_row(p, seg.s, seg.h, row);
+        const int64_t out = out_row(p, last.s, last.h, row);
         write_four(p, out * D + d, m);
         if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
       } else {
@@ -628,28 +628,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
         if (d == 0) *reinterpret_cast<float4*>(at + D) = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
       }
     }
-  };
-  Segment last{};
-  for (int w = 0; w < S::WARPS; ++w) {
-    const Segment s0 = segments[w][0], s1 = segments[w][1];
-    if (s0.used) {
-      if (open_n == 0) open_w = w, from_before = true;
-      ++open_n;
-      last = s0;
-      if (s0.ends) {
-        emit(s0, true);
-        open_n = 0;
-        from_before = false;
-      }
-    }
-    if (s1.used) {
-      open_w = w, open_n = 1, from_before = false;
-      last = s1;
-    }
-  }
-  if (open_n) {
-    emit(last, false);
-    if (!from_before && threadIdx.x == 0) {  // the pair that starts here ends in a later CTA
+    if (!ended && !from_before && threadIdx.x == 0) {  // the pair that starts here ends in a later CTA
       const Pair a = locate(share((blockIdx.x + 1) * S::WARPS) - 1);
       const int end = worker_of(a.base + a.steps - 1) / S::WARPS;
       *reinterpret_cast<int4*>(p.links + blockIdx.x * 4) = make_int4(end, a.s, a.h, a.rt);
@@ -709,12 +688,10 @@ template <int D, int NT, int U> int launch(AttnParams& p, int sms, cudaStream_t 
   const int smem = S::WARPS * S::RING_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
   p.step_shift = (p.c.block_tokens == 16 ? 0 : p.c.block_tokens == 32 ? 1 : p.c.block_tokens == 64 ? 2 : 3) - (U - 1);
   const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
-  const int64_t steps = (entries << p.step_shift) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
+  const int64_t steps = ((entries << p.step_shift) + START) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
   if (steps > 0x3fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: too many tokens in one call");
   const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
-  p.front_ctas = (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, wanted));
-  const int grid = wanted > TAIL_FROM * sms ? 4 * sms : p.front_ctas;
-  p.tail_share = TAIL_SHARE;
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
   p.spill = p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS;
   p.links = reinterpret_cast<int*>(p.spill + (int64_t)CTAS_PER_SM * sms * S::WARPS * S::STATE_FLOATS);
   attention_kernel<D, NT, U><<<grid, S::WARPS * 32, smem, stream>>>(p);
@@ -724,6 +701,11 @@ template <int D, int NT, int U> int launch(AttnParams& p, int sms, cudaStream_t 
 }
 
 template <int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
+  // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 76 us
+  // against 96) and for 16 rows (eight of 5003 tokens, four queries each: 23.4 against 25.4).
+  if constexpr (D == 64 || NT == 2) {
+    if (p.c.block_tokens > TILE) return launch<D, NT, 2>(p, sms, stream);
+  }
   return launch<D, NT, 1>(p, sms, stream);
 }
 
