@@ -12,7 +12,9 @@
 // A cluster of CTAs scores one (sequence, KV head), each CTA its share of the
 // blocks, into the first CTA's shared memory (into global memory where
 // a row of keys does not fit there); that CTA then finds the count-th largest key
-// by four 8-bit radix passes and writes the kept blocks in ascending order.
+// by up to four 8-bit radix passes and writes the kept blocks in ascending order.
+// One sequence is a chain of round trips (lengths, table and query together;
+// bounds; keys), many are bound by the bounds' bytes.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -37,6 +39,7 @@ struct SelectParams {
 };
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int AHEAD = 2;  // tiles of a warp whose table entries are loaded before the lengths are known
 constexpr int MOST_SHARED_KEYS = 49152;  // 192 KB
 
 // Unsigned keys in the order of the scores; NaN above every number, so that a
@@ -62,81 +65,101 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Exclusive prefix sum over the CTA's threads, and the total.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += u;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
-  }
-  return before + x - v;
-}
-
 template <typename T, int D> __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
   constexpr int KS = D / 32;  // products of 32 channels on each side
   extern __shared__ __align__(16) uint32_t row_keys[];
   __shared__ __align__(16) int8_t q_code[8][2][D + 16];  // [head][min(q, 0) or max(q, 0)][channel], rows on distinct banks
   __shared__ float q_scale[8];
-  __shared__ int histogram[256];
-  __shared__ int warp_sums[WARPS];
-  __shared__ int found[2];
+  __shared__ __align__(16) int histogram[4][256];
+  __shared__ int2 warp_counts[WARPS];
   const ucb_block8_cache& c = p.c;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
   auto started = cluster.barrier_arrive();  // waited for before the first key goes to another CTA
   const int pair = blockIdx.x / parts, s = pair / c.kv_heads, h = pair % c.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cq = lane & 3;
-  const int tokens = held_tokens(c, s, p.err);
-  const int n = (int)(((int64_t)tokens + c.block_tokens - 1) / c.block_tokens);
   int32_t* out = p.blocks + (int64_t)pair * p.count;
   uint32_t* keys = p.spill ? p.spill + (int64_t)pair * c.max_blocks : cluster.map_shared_rank(row_keys, 0);
   const int32_t* table = c.block_table + (int64_t)s * c.max_blocks;
-  const bool all = n <= p.count;  // nothing to choose
 
+  // ---- what does not depend on the lengths: query heads (warp w rounds head g0 + w), table entries of the
+  // warp's first tiles
+  constexpr int PER = D / 32;
+  auto load_head = [&](int g, float (&x)[PER]) {
+    const T* q = static_cast<const T*>(p.q) + s * p.q_ss + (int64_t)(h * p.group + g) * p.q_sh + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = g < p.group ? Dtype<T>::to_f(q[i]) : 0.f;
+  };
+  float x[PER];
+  load_head(warp, x);
+  const int tile0 = part * WARPS + warp, tile_step = parts * WARPS;
+  int entry[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    const int j = (tile0 + i * tile_step) * 16 + (lane & 15);
+    entry[i] = j < c.max_blocks ? table[j] : -1;
+  }
+  const int tokens = held_tokens(c, s, p.err);
+  const int n = (int)(((int64_t)tokens + c.block_tokens - 1) / c.block_tokens);
+  const bool all = n <= p.count;  // nothing to choose
+  for (int i = threadIdx.x; i < 4 * 256; i += THREADS) histogram[0][i] = 0;
+
+  // bounds and key scales of a tile's blocks: lane i the scale of block i, lane (r, cq) units cq and cq + 4 of blocks
+  // r and r + 8
+  struct Tile {
+    uint4 x[2][D / 64][2];
+    float ks;
+    int block0, block1;
+  };
+  auto load_tile = [&](int tile, int block) {
+    Tile a;
+    if (tile * 16 + (lane & 15) >= n) block = -1;
+    else if (block < 0 || block >= c.num_blocks) {
+      block = -1;
+      atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+    }
+    a.ks = block >= 0 ? c.key_scale[(int64_t)block * c.kv_heads + h] : 0.f;
+    a.block0 = __shfl_sync(0xffffffffu, block, r);
+    a.block1 = __shfl_sync(0xffffffffu, block, r + 8);
+    const int64_t at0 = ((int64_t)max(a.block0, 0) * c.kv_heads + h) * D + 16 * cq;
+    const int64_t at1 = ((int64_t)max(a.block1, 0) * c.kv_heads + h) * D + 16 * cq;
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half) {
+        const int8_t* bounds = (side ? c.key_high : c.key_low) + half * 64;
+        a.x[side][half][0] = *reinterpret_cast<const uint4*>(bounds + at0);
+        a.x[side][half][1] = *reinterpret_cast<const uint4*>(bounds + at1);
+      }
+    return a;
+  };
+
+  const int tiles = (n + 15) / 16;
+  Tile next;
+  if (!all && tile0 < tiles) next = load_tile(tile0, entry[0]);
   cluster.barrier_wait(std::move(started));
   if (!all) {
-    const int tiles = (n + 15) / 16, share = (tiles + parts - 1) / parts;
-    const int tile_end = min(tiles, (part + 1) * share);
     for (int g0 = 0; g0 < p.group; g0 += 8) {
-      // ---- query heads in 8 bits: warp w rounds head g0 + w
-      __syncthreads();
-      {
-        const int g = g0 + warp;
-        constexpr int PER = D / 32;
-        float x[PER];
-        unsigned int top = 0;
-        if (g < p.group) {
-          const T* q = static_cast<const T*>(p.q) + s * p.q_ss + (int64_t)(h * p.group + g) * p.q_sh + lane * PER;
-#pragma unroll
-          for (int i = 0; i < PER; ++i) x[i] = Dtype<T>::to_f(q[i]), top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-        } else {
-#pragma unroll
-          for (int i = 0; i < PER; ++i) x[i] = 0.f;
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const float scale = scale_of(__uint_as_float(top)), inverse = __fdiv_rn(1.f, scale);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int code = code_of(x[i], inverse);
-          q_code[warp][0][lane * PER + i] = (int8_t)min(code, 0);
-          q_code[warp][1][lane * PER + i] = (int8_t)max(code, 0);
-        }
-        if (lane == 0) q_scale[warp] = scale;
+      // ---- query heads in 8 bits
+      if (g0) {
+        __syncthreads();
+        load_head(g0 + warp, x);
+        if (tile0 < tiles) next = load_tile(tile0, entry[0]);
       }
+      unsigned int top = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+      top = __reduce_max_sync(0xffffffffu, top);
+      const float scale = scale_of(__uint_as_float(top)), inverse = __fdiv_rn(1.f, scale);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int code = code_of(x[i], inverse);
+        q_code[warp][0][lane * PER + i] = (int8_t)min(code, 0);
+        q_code[warp][1][lane * PER + i] = (int8_t)max(code, 0);
+      }
+      if (lane == 0) q_scale[warp] = scale;
       __syncthreads();
-      // operand words in the order of the bounds' 16-byte units: lane (r, cq) takes units cq and cq + 4
+      // operand words in the order of the bounds' 16-byte units
       uint32_t b[2][KS][2];
 #pragma unroll
       for (int side = 0; side < 2; ++side)
@@ -149,41 +172,27 @@ template <typename T, int D> __global__ void __launch_bounds__(THREADS) select_k
       const float scale0 = q_scale[2 * cq], scale1 = q_scale[2 * cq + 1];
       const bool real0 = g0 + 2 * cq < p.group, real1 = g0 + 2 * cq + 1 < p.group;
 
-      for (int tile = part * share + warp; tile < tile_end; tile += WARPS) {
-        const int mine = tile * 16 + (lane & 15);
-        int block = -1;
-        float ks = 0.f;
-        if (mine < n) {
-          block = table[mine];
-          if (block < 0 || block >= c.num_blocks) {
-            block = -1;
-            atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-          }
+      for (int tile = tile0, i = 0; tile < tiles; tile += tile_step, ++i) {
+        const Tile a = next;
+        const int after = tile + tile_step;
+        if (after < tiles) {
+          const int j = after * 16 + (lane & 15);
+          int block = -1;
+          if (i + 1 < AHEAD) block = entry[1];
+          else if (j < n) block = table[j];
+          next = load_tile(after, block);
         }
-        if (block >= 0) ks = c.key_scale[(int64_t)block * c.kv_heads + h];
-        const int block0 = __shfl_sync(0xffffffffu, block, r), block1 = __shfl_sync(0xffffffffu, block, r + 8);
-        const int64_t at0 = ((int64_t)max(block0, 0) * c.kv_heads + h) * D + 16 * cq;
-        const int64_t at1 = ((int64_t)max(block1, 0) * c.kv_heads + h) * D + 16 * cq;
-        uint4 x[2][D / 64][2];
-#pragma unroll
-        for (int side = 0; side < 2; ++side)
-#pragma unroll
-          for (int half = 0; half < D / 64; ++half) {
-            const int8_t* bounds = (side ? c.key_high : c.key_low) + half * 64;
-            x[side][half][0] = *reinterpret_cast<const uint4*>(bounds + at0);
-            x[side][half][1] = *reinterpret_cast<const uint4*>(bounds + at1);
-          }
         int sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int side = 0; side < 2; ++side)
 #pragma unroll
           for (int half = 0; half < D / 64; ++half) {
-            const uint4 u = x[side][half][0], v = x[side][half][1];
+            const uint4 u = a.x[side][half][0], v = a.x[side][half][1];
             mma_s8(sum, u.x, v.x, u.y, v.y, b[side][half * 2][0], b[side][half * 2][1]);
             mma_s8(sum, u.z, v.z, u.w, v.w, b[side][half * 2 + 1][0], b[side][half * 2 + 1][1]);
           }
         // largest over the heads: two columns here, the others in the quad's lanes
-        const float ks0 = __shfl_sync(0xffffffffu, ks, r), ks1 = __shfl_sync(0xffffffffu, ks, r + 8);
+        const float ks0 = __shfl_sync(0xffffffffu, a.ks, r), ks1 = __shfl_sync(0xffffffffu, a.ks, r + 8);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float top = -INFINITY;
@@ -197,7 +206,7 @@ template <typename T, int D> __global__ void __launch_bounds__(THREADS) select_k
             if (g0) top = max_nan(top, __uint_as_float(keys[j]));
             uint32_t key = __float_as_uint(top);
             if (g0 + 8 >= p.group) {
-              const bool known = (k ? block1 : block0) >= 0;
+              const bool known = (k ? a.block1 : a.block0) >= 0;
               key = j < p.first || j >= n - p.recent ? KEY_FORCED
                     : known ? key_of(__fmul_rn(top, k ? ks1 : ks0)) : key_of(-INFINITY);
             }
@@ -219,50 +228,77 @@ template <typename T, int D> __global__ void __launch_bounds__(THREADS) select_k
   }
   uint32_t* own = p.spill ? keys : row_keys;
 
-  // ---- the count-th largest key: its bits from the top, 8 at a time
-  uint32_t prefix = 0;
-  int need = p.count;  // keys still to take among those that share the prefix
-#pragma unroll
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-    histogram[threadIdx.x] = 0;
-    __syncthreads();
+  // ---- the count-th largest key: its bits from the top, 8 at a time; every warp finds the bin by itself.  Done
+  // early when a bin is taken whole.  (Counting a warp's equal digits once, by __match_any_sync, took 5.7 us for 2048 keys
+  // where these atomics take 1.)
+  uint32_t threshold = 0;  // keys from here on, of the equal ones `need`
+  int need = p.count;
+#pragma unroll 1  // instructions of a second pass are at hand, a second copy's are not
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    const uint32_t mask = pass == 0 ? 0u : 0xFFFFFFFFu << (shift + 8);
     for (int j = threadIdx.x; j < n; j += THREADS) {
       const uint32_t key = own[j];
-      if ((key & mask) == prefix) atomicAdd(&histogram[(key >> shift) & 255], 1);
+      if ((key & mask) == threshold) atomicAdd(&histogram[pass][key >> shift & 255], 1);
     }
     __syncthreads();
-    // bins from the highest: thread i holds bin 255 - i
-    const int bin = 255 - threadIdx.x, v = histogram[bin];
-    int total;
-    const int before = block_scan(v, warp_sums, total);
-    if (before < need && before + v >= need) {
-      found[0] = bin;
-      found[1] = need - before;
+    // lane i holds bins 255 - 8 i down to 248 - 8 i
+    const int4 hi = *reinterpret_cast<const int4*>(&histogram[pass][252 - 8 * lane]);
+    const int4 lo = *reinterpret_cast<const int4*>(&histogram[pass][248 - 8 * lane]);
+    const int v[8] = {hi.w, hi.z, hi.y, hi.x, lo.w, lo.z, lo.y, lo.x};
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i];
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += u;
     }
-    __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    need = found[1];
-    __syncthreads();
+    before -= sum;
+    int bin = -1, left = 0, held = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (bin < 0 && before < need && before + v[i] >= need) bin = 255 - 8 * lane - i, left = need - before, held = v[i];
+      before += v[i];
+    }
+    const int owner = __ffs(__ballot_sync(0xffffffffu, bin >= 0)) - 1;
+    bin = __shfl_sync(0xffffffffu, bin, owner);
+    need = __shfl_sync(0xffffffffu, left, owner);
+    held = __shfl_sync(0xffffffffu, held, owner);
+    threshold |= (uint32_t)bin << shift;
+    if (held == need) {  // every key from the threshold on
+      threshold -= threshold > 0;  // no key is 0
+      need = 0;
+      break;
+    }
   }
 
-  // ---- kept blocks in ascending order: each thread a contiguous slice; of the keys equal to the last one the
+  // ---- kept blocks in ascending order: each thread a contiguous slice; of the keys equal to the threshold the
   // first `need`
   const int slice = (n + THREADS - 1) / THREADS;
   const int j0 = min(n, (int)threadIdx.x * slice), j1 = min(n, j0 + slice);
-  int above = 0, equal = 0, total;
+  int above = 0, equal = 0;
   for (int j = j0; j < j1; ++j) {
     const uint32_t key = own[j];
-    above += key > prefix;
-    equal += key == prefix;
+    above += key > threshold;
+    equal += key == threshold;
   }
-  const int above_before = block_scan(above, warp_sums, total);
-  int equal_seen = block_scan(equal, warp_sums, total);
-  int at = above_before + min(equal_seen, need);
+  int above_in = above, equal_in = equal;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, above_in, o), v = __shfl_up_sync(0xffffffffu, equal_in, o);
+    if (lane >= o) above_in += u, equal_in += v;
+  }
+  if (lane == 31) warp_counts[warp] = make_int2(above_in, equal_in);
+  __syncthreads();
+  int above_before = above_in - above, equal_before = equal_in - equal;
+  for (int w = 0; w < warp; ++w) above_before += warp_counts[w].x, equal_before += warp_counts[w].y;
+  int at = above_before + min(equal_before, need);
   for (int j = j0; j < j1; ++j) {
     const uint32_t key = own[j];
-    if (key > prefix || (key == prefix && equal_seen < need)) out[at++] = j;
-    equal_seen += key == prefix;
+    if (key > threshold || (key == threshold && equal_before < need)) out[at++] = j;
+    equal_before += key == threshold;
   }
 }
 
@@ -277,9 +313,9 @@ template <typename T, int D> int launch(const SelectParams& p, cudaStream_t stre
     ready[dev & 63] = true;
   }
   const int64_t pairs = (int64_t)p.c.num_seqs * p.c.kv_heads;
-  // CTAs of a pair: as long as the chip has room for more and each keeps a tile for every warp
+  // CTAs of a pair: until every warp has a tile, as long as the chip has room for more
   int parts = 1;
-  while (parts < 8 && pairs * parts * 2 <= 296 && p.c.max_blocks / (parts * 2) >= 16 * WARPS) parts *= 2;
+  while (parts < 8 && pairs * parts * 2 <= 296 && p.c.max_blocks > parts * 16 * WARPS) parts *= 2;
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
   attribute[0].val.clusterDim.x = parts;
