@@ -41,22 +41,34 @@ __device__ __forceinline__ int held_tokens(const ucb_block8_cache& c, int s, uns
   return n < 0 ? 0 : (int)most;
 }
 
-// Programmatic dependent launch: a kernel launched by launch_dependent may become resident once every CTA of the kernel
-// before it has called launch_dependents (or ended), and reads nothing of it before wait_for_primary returns.
+// Programmatic dependent launch: a kernel launched as `dependent` may become resident once every CTA of the kernel before
+// it in its stream has called launch_dependents (or ended).  It calls wait_for_primary before its first access to global
+// memory, which returns when that kernel is complete and its writes are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename P>
-int launch_dependent(void (*kernel)(const P), dim3 grid, dim3 block, cudaStream_t stream, const P& params, const char* what) {
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+int launch(void (*kernel)(const P), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P& params,
+           const char* what, int cluster = 1, bool dependent = false) {
+  cudaLaunchAttribute attribute[2];
+  int attributes = 0;
+  if (dependent) {
+    attribute[attributes].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[attributes++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attribute[attributes].id = cudaLaunchAttributeClusterDimension;
+    attribute[attributes].val.clusterDim.x = cluster;
+    attribute[attributes].val.clusterDim.y = attribute[attributes].val.clusterDim.z = 1;
+    ++attributes;
+  }
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = block;
+  config.dynamicSmemBytes = smem;
   config.stream = stream;
   config.attrs = attribute;
-  config.numAttrs = 1;
+  config.numAttrs = attributes;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, params);
   if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return UCB_OK;

@@ -674,7 +674,7 @@ int multiprocessors() {
 
 constexpr int MOST_SEQS = 4096;
 
-template <int D, int NT, int U> int launch(AttnParams& p, int sms, cudaStream_t stream) {
+template <int D, int NT, int U> int launch_shape(AttnParams& p, int sms, cudaStream_t stream) {
   using S = Shape<D, NT, U>;
   static bool ready[64] = {false};  // the attribute is a device's; setting it twice is harmless
   int dev = 0;
@@ -694,19 +694,20 @@ template <int D, int NT, int U> int launch(AttnParams& p, int sms, cudaStream_t 
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
   p.spill = p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS;
   p.links = reinterpret_cast<int*>(p.spill + (int64_t)CTAS_PER_SM * sms * S::WARPS * S::STATE_FLOATS);
-  attention_kernel<D, NT, U><<<grid, S::WARPS * 32, smem, stream>>>(p);
-  if (int rc = ucb_host::check_launch("block8 attention_kernel")) return rc;
-  return launch_dependent(attention_merge_kernel<D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), stream, p,
-                          "block8 attention_merge_kernel");
+  if (int rc = block8::launch(attention_kernel<D, NT, U>, dim3(grid), dim3(S::WARPS * 32), smem, stream, p,
+                              "block8 attention_kernel"))
+    return rc;
+  return block8::launch(attention_merge_kernel<D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), 0, stream, p,
+                        "block8 attention_merge_kernel", 1, true);
 }
 
 template <int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
   // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 76 us
   // against 96) and for 16 rows (eight of 5003 tokens, four queries each: 23.4 against 25.4).
   if constexpr (D == 64 || NT == 2) {
-    if (p.c.block_tokens > TILE) return launch<D, NT, 2>(p, sms, stream);
+    if (p.c.block_tokens > TILE) return launch_shape<D, NT, 2>(p, sms, stream);
   }
-  return launch<D, NT, 1>(p, sms, stream);
+  return launch_shape<D, NT, 1>(p, sms, stream);
 }
 
 }  // namespace

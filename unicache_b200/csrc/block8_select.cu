@@ -302,7 +302,7 @@ template <typename T, int D> __global__ void __launch_bounds__(THREADS) select_k
   }
 }
 
-template <typename T, int D> int launch(const SelectParams& p, cudaStream_t stream) {
+template <typename T, int D> int launch_select(const SelectParams& p, cudaStream_t stream) {
   static bool ready[64] = {false};  // the attribute is a device's; setting it twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
@@ -316,20 +316,8 @@ template <typename T, int D> int launch(const SelectParams& p, cudaStream_t stre
   // CTAs of a pair: until every warp has a tile, as long as the chip has room for more
   int parts = 1;
   while (parts < 8 && pairs * parts * 2 <= 296 && p.c.max_blocks > parts * 16 * WARPS) parts *= 2;
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = parts;
-  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)(pairs * parts));
-  config.blockDim = dim3(THREADS);
-  config.dynamicSmemBytes = p.spill ? 16 : (size_t)p.c.max_blocks * 4;
-  config.stream = stream;
-  config.attrs = attribute;
-  config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, select_kernel<T, D>, p);
-  if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "block8 select_kernel: %s", cudaGetErrorString(e));
-  return UCB_OK;
+  return block8::launch(select_kernel<T, D>, dim3((unsigned)(pairs * parts)), dim3(THREADS),
+                        p.spill ? 16 : (size_t)p.c.max_blocks * 4, stream, p, "block8 select_kernel", parts);
 }
 
 }  // namespace
@@ -365,6 +353,6 @@ extern "C" int ucb_block8_select(const ucb_block8_cache* cache, const void* quer
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == UCB_BF16;
   if (cache->head_dim == 128)
-    return bf ? b8::launch<__nv_bfloat16, 128>(p, s) : b8::launch<__half, 128>(p, s);
-  return bf ? b8::launch<__nv_bfloat16, 64>(p, s) : b8::launch<__half, 64>(p, s);
+    return bf ? b8::launch_select<__nv_bfloat16, 128>(p, s) : b8::launch_select<__half, 128>(p, s);
+  return bf ? b8::launch_select<__nv_bfloat16, 64>(p, s) : b8::launch_select<__half, 64>(p, s);
 }

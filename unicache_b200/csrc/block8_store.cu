@@ -352,13 +352,18 @@ template <bool BF, int D> __global__ void __launch_bounds__(THREADS) read_kernel
   }
 }
 
-template <bool BF, int D> void launch_write(const WriteParams& p, dim3 grid, cudaStream_t s) {
+template <bool BF, int D> int launch_write(const WriteParams& p, dim3 grid, cudaStream_t s) {
+  const char* what = "block8 write_kernel";
   switch (p.c.block_tokens) {
-    case 16: write_kernel<BF, D, 16><<<grid, THREADS, 0, s>>>(p); break;
-    case 32: write_kernel<BF, D, 32><<<grid, THREADS, 0, s>>>(p); break;
-    case 64: write_kernel<BF, D, 64><<<grid, THREADS, 0, s>>>(p); break;
-    default: write_kernel<BF, D, 128><<<grid, THREADS, 0, s>>>(p);
+    case 16: return launch(write_kernel<BF, D, 16>, grid, dim3(THREADS), 0, s, p, what);
+    case 32: return launch(write_kernel<BF, D, 32>, grid, dim3(THREADS), 0, s, p, what);
+    case 64: return launch(write_kernel<BF, D, 64>, grid, dim3(THREADS), 0, s, p, what);
+    default: return launch(write_kernel<BF, D, 128>, grid, dim3(THREADS), 0, s, p, what);
   }
+}
+
+template <bool BF, int D> int launch_read(const ReadParams& p, unsigned blocks, cudaStream_t s) {
+  return launch(read_kernel<BF, D>, dim3(blocks), dim3(THREADS), 0, s, p, "block8 read_kernel");
 }
 
 }  // namespace
@@ -386,11 +391,8 @@ extern "C" int ucb_block8_write(const ucb_block8_cache* cache, const void* key, 
   const dim3 grid((unsigned)items, cache->kv_heads);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == UCB_BF16;
-  if (cache->head_dim == 128)
-    bf ? b8::launch_write<true, 128>(p, grid, s) : b8::launch_write<false, 128>(p, grid, s);
-  else
-    bf ? b8::launch_write<true, 64>(p, grid, s) : b8::launch_write<false, 64>(p, grid, s);
-  return ucb_host::check_launch("block8 write_kernel");
+  if (cache->head_dim == 128) return bf ? b8::launch_write<true, 128>(p, grid, s) : b8::launch_write<false, 128>(p, grid, s);
+  return bf ? b8::launch_write<true, 64>(p, grid, s) : b8::launch_write<false, 64>(p, grid, s);
 }
 
 extern "C" int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, const int32_t* starts, void* key,
@@ -409,11 +411,7 @@ extern "C" int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, cons
   if (blocks > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_read: too many rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == UCB_BF16;
-  if (cache->head_dim == 128)
-    bf ? b8::read_kernel<true, 128><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p)
-       : b8::read_kernel<false, 128><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p);
-  else
-    bf ? b8::read_kernel<true, 64><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p)
-       : b8::read_kernel<false, 64><<<(unsigned)blocks, b8::THREADS, 0, s>>>(p);
-  return ucb_host::check_launch("block8 read_kernel");
+  const unsigned grid = (unsigned)blocks;
+  if (cache->head_dim == 128) return bf ? b8::launch_read<true, 128>(p, grid, s) : b8::launch_read<false, 128>(p, grid, s);
+  return bf ? b8::launch_read<true, 64>(p, grid, s) : b8::launch_read<false, 64>(p, grid, s);
 }
