@@ -567,21 +567,35 @@ UCB_API int ucb_compact_rows(const void* src_dev, int64_t row_bytes, const uint8
  * head_dim] (k_heads may be 0; dtype UCB_BF16, UCB_F16 or UCB_F32; strides in
  * elements, channels contiguous): y = x * rsqrt(mean(x^2) + eps) * weight
  * (weights [head_dim] of the same dtype, NULL = ones), then the rotation by
- * row positions[t] of the tables cos_dev, sin_dev (fp32 [table_rows,
+ * row positions[t] of the tables cos, sin (fp32 [table_rows,
  * rotary_dim / 2]): channels (i, i + rotary_dim / 2), or (2i, 2i + 1) when
  * `interleaved`; channels from rotary_dim on are only normalised.  fp32
  * arithmetic, one rounding.  The outputs may be the inputs.  rotary_dim 0: no
  * rotation.  2 <= head_dim <= 256.  positions: int32, or int64 when
  * positions_64.  A position outside the tables sets device error bit 2 and
  * its rows become NaN. */
-UCB_API int ucb_head_norm_rope(const void* query_dev, int64_t q_stride_token, int64_t q_stride_head, int q_heads,
-                               const void* key_dev, int64_t k_stride_token, int64_t k_stride_head, int k_heads,
-                               const void* q_weight_dev, const void* k_weight_dev, const float* cos_dev,
-                               const float* sin_dev, const void* positions_dev, int positions_64,
-                               int64_t table_rows, int64_t tokens, int head_dim, int rotary_dim, int interleaved,
-                               int dtype, float eps, void* q_out_dev, int64_t qo_stride_token,
-                               int64_t qo_stride_head, void* k_out_dev, int64_t ko_stride_token,
-                               int64_t ko_stride_head, void* stream);
+typedef struct ucb_head_norm_args {
+  const void* query;
+  const void* key;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  const void* positions;
+  void* q_out;
+  void* k_out;
+  int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head;
+  int64_t qo_stride_token, qo_stride_head, ko_stride_token, ko_stride_head;
+  int64_t table_rows;
+  int64_t tokens;
+  int32_t q_heads, k_heads;
+  int32_t head_dim, rotary_dim;
+  int32_t interleaved;
+  int32_t positions_64;
+  int32_t dtype;
+  float eps;
+} ucb_head_norm_args;
+UCB_API int ucb_head_norm_rope(const ucb_head_norm_args* args, void* stream);
 
 /* ------------------------------------------------------------------ 8-bit block cache
  * No counterpart in the reference (its quantized segments are frozen and
@@ -650,16 +664,24 @@ UCB_API int ucb_block8_select(const ucb_block8_cache* cache, const void* query_d
 /* Attention of query [num_seqs, queries, q_heads, head_dim] (channels
  * contiguous, 1 <= queries <= 16) over the cache: query i of a sequence is its
  * token lengths[s] - queries + i and sees the tokens up to itself (none: output
- * 0, LSE -inf).  blocks_dev int32 [num_seqs, kv_heads, num_selected] limits it
+ * 0, LSE -inf).  blocks int32 [num_seqs, kv_heads, num_selected] limits it
  * to the tokens of these blocks (negative entries are skipped, no block may
  * be named twice); NULL = all.  out [num_seqs, queries, q_heads, head_dim] in
  * dtype, lse fp32 [num_seqs, queries, q_heads] natural log (or NULL).
- * workspace_dev: ucb_block8_attention_workspace_bytes bytes, 16-byte aligned. */
+ * workspace: ucb_block8_attention_workspace_bytes bytes; it and out 16-byte aligned. */
 UCB_API int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads);
-UCB_API int ucb_block8_attention(const ucb_block8_cache* cache, const void* query_dev, int64_t q_stride_seq,
-                                 int64_t q_stride_query, int64_t q_stride_head, int queries, int q_heads,
-                                 const int32_t* blocks_dev, int num_selected, float softmax_scale, void* out_dev,
-                                 float* lse_dev, void* workspace_dev, void* stream);
+typedef struct ucb_block8_attention_args {
+  const void* query;
+  const int32_t* blocks;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t q_stride_seq, q_stride_query, q_stride_head;
+  int32_t queries, q_heads;
+  int32_t num_selected;
+  float softmax_scale;
+} ucb_block8_attention_args;
+UCB_API int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------------ self test
  * Checks on the current device that mma.sync f16 consumes fp16 subnormal

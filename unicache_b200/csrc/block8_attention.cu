@@ -725,35 +725,35 @@ extern "C" int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* 
   return sms > 0 ? sms * b8::CTAS_PER_SM * ((2 + b8::Shape<128, 1, 1>::WARPS) * rows * (cache->head_dim + 4) * 4 + 16) : -1;
 }
 
-extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const void* query, int64_t q_ss, int64_t q_sl,
-                                    int64_t q_sh, int queries, int q_heads, const int32_t* blocks, int num_selected,
-                                    float softmax_scale, void* out, float* lse, void* workspace, void* stream) {
+extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* a, void* stream) {
   if (int rc = b8::check_cache(cache, "ucb_block8_attention")) return rc;
-  if (!query || !out || !workspace) return set_error(UCB_ERR_INVALID, "ucb_block8_attention: null pointer");
-  if (queries < 1 || queries > 16) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: 1 to 16 query tokens");
-  if (q_heads < 1 || q_heads % cache->kv_heads)
+  if (!a || !a->query || !a->out || !a->workspace)
+    return set_error(UCB_ERR_INVALID, "ucb_block8_attention: null pointer");
+  if (a->queries < 1 || a->queries > 16)
+    return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: 1 to 16 query tokens");
+  if (a->q_heads < 1 || a->q_heads % cache->kv_heads)
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: query heads must be divisible by KV heads");
-  if (blocks && (num_selected < 1 || num_selected > 1 << 20))
+  if (a->blocks && (a->num_selected < 1 || a->num_selected > 1 << 20))
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: a selection needs 1 to 2^20 entries");
-  if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(out)) & 15)
+  if ((reinterpret_cast<uintptr_t>(a->workspace) | reinterpret_cast<uintptr_t>(a->out)) & 15)
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: out and workspace must be 16-byte aligned");
   unsigned int* err = ucb_host::device_error_word();
   const int sms = b8::multiprocessors();
   if (!err || sms < 1) return set_error(UCB_ERR_CUDA, "ucb_block8_attention: no device");
   b8::AttnParams p{};
   p.c = *cache;
-  p.q = query;
-  p.q_ss = q_ss, p.q_sl = q_sl, p.q_sh = q_sh;
-  p.q_aligned = reinterpret_cast<uintptr_t>(query) % 8 == 0 && (q_ss | q_sl | q_sh) % 4 == 0;
-  p.queries = queries, p.q_heads = q_heads;
-  p.group = q_heads / cache->kv_heads;
-  p.rows = p.group * queries;
+  p.q = a->query;
+  p.q_ss = a->q_stride_seq, p.q_sl = a->q_stride_query, p.q_sh = a->q_stride_head;
+  p.q_aligned = reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.q_ss | p.q_sl | p.q_sh) % 4 == 0;
+  p.queries = a->queries, p.q_heads = a->q_heads;
+  p.group = a->q_heads / cache->kv_heads;
+  p.rows = p.group * a->queries;
   const int tile_rows = p.rows > 8 ? 16 : 8;
   p.row_tiles = (p.rows + tile_rows - 1) / tile_rows;
-  p.blocks = blocks, p.selected = num_selected;
-  p.scale_log2 = softmax_scale * 1.44269504088896341f;
-  p.out = out, p.lse = lse;
-  p.partials = static_cast<float*>(workspace);
+  p.blocks = a->blocks, p.selected = a->blocks ? a->num_selected : 0;
+  p.scale_log2 = a->softmax_scale * 1.44269504088896341f;
+  p.out = a->out, p.lse = a->lse;
+  p.partials = static_cast<float*>(a->workspace);
   p.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (cache->head_dim == 128) return tile_rows == 16 ? b8::launch_block<128, 2>(p, sms, s) : b8::launch_block<128, 1>(p, sms, s);

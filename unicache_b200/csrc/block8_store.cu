@@ -402,11 +402,11 @@ extern "C" int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, cons
     return set_error(UCB_ERR_INVALID, "ucb_block8_read: one row for each sequence, or starts");
   if (rows == 0) return UCB_OK;
   if (!key || !value) return set_error(UCB_ERR_INVALID, "ucb_block8_read: null pointer");
+  if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15)
+    return set_error(UCB_ERR_INVALID, "ucb_block8_read: outputs must be 16-byte aligned");
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "ucb_block8_read: device error word unavailable");
   const b8::ReadParams p{*cache, rows, starts, key, value, err};
-  if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15)
-    return set_error(UCB_ERR_INVALID, "ucb_block8_read: outputs must be 16-byte aligned");
   const int64_t each = b8::THREADS / 32 * b8::READ_ROWS, blocks = (rows + each - 1) / each;
   if (blocks > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_read: too many rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

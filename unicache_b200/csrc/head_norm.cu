@@ -224,27 +224,30 @@ template <typename T> int launch(const HeadNormParams& p, cudaStream_t s) {
 
 using ucb_host::set_error;
 
-extern "C" int ucb_head_norm_rope(const void* q, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_st,
-                                  int64_t k_sh, int hk, const void* qw, const void* kw, const float* cos_t,
-                                  const float* sin_t, const void* positions, int positions_64, int64_t table_rows,
-                                  int64_t tokens, int head_dim, int rotary_dim, int interleaved, int dtype, float eps,
-                                  void* qo, int64_t qo_st, int64_t qo_sh, void* ko, int64_t ko_st, int64_t ko_sh,
-                                  void* stream) {
-  if (tokens < 0 || hq < 0 || hk < 0 || hq + hk == 0)
+extern "C" int ucb_head_norm_rope(const ucb_head_norm_args* a, void* stream) {
+  if (!a) return set_error(UCB_ERR_INVALID, "ucb_head_norm_rope: null pointer");
+  if (a->tokens < 0 || a->q_heads < 0 || a->k_heads < 0 || a->q_heads + (int64_t)a->k_heads == 0)
     return set_error(UCB_ERR_INVALID, "ucb_head_norm_rope: bad shape");
-  if (head_dim < 2 || head_dim > ucb::MAX_HEAD_DIM)
+  if (a->q_heads + (int64_t)a->k_heads > 65535)
+    return set_error(UCB_ERR_UNSUPPORTED, "ucb_head_norm_rope: at most 65535 heads");
+  if (a->head_dim < 2 || a->head_dim > ucb::MAX_HEAD_DIM)
     return set_error(UCB_ERR_UNSUPPORTED, "ucb_head_norm_rope: head_dim must be 2..%d", ucb::MAX_HEAD_DIM);
-  if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > head_dim)
+  if (a->rotary_dim < 0 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
     return set_error(UCB_ERR_INVALID, "ucb_head_norm_rope: rotary_dim must be even and at most head_dim");
-  if (tokens == 0) return UCB_OK;
-  if ((hq && (!q || !qo)) || (hk && (!k || !ko)) || (rotary_dim && (!cos_t || !sin_t || !positions)))
+  if (a->tokens == 0) return UCB_OK;
+  if ((a->q_heads && (!a->query || !a->q_out)) || (a->k_heads && (!a->key || !a->k_out)) ||
+      (a->rotary_dim && (!a->cos || !a->sin || !a->positions)))
     return set_error(UCB_ERR_INVALID, "ucb_head_norm_rope: null pointer");
+  if (a->rotary_dim && a->table_rows < 1) return set_error(UCB_ERR_INVALID, "ucb_head_norm_rope: empty tables");
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "ucb_head_norm_rope: device error word unavailable");
-  const ucb::HeadNormParams p{q,     k,     qw,    kw,    qo,    ko,         cos_t, sin_t, positions,  q_st,        q_sh,         k_st, k_sh,
-                              qo_st, qo_sh, ko_st, ko_sh, tokens, table_rows, hq,    hk,    head_dim, rotary_dim, interleaved, positions_64, eps,  err};
+  const ucb::HeadNormParams p{a->query, a->key, a->q_weight, a->k_weight, a->q_out, a->k_out, a->cos, a->sin, a->positions,
+                              a->q_stride_token, a->q_stride_head, a->k_stride_token, a->k_stride_head,
+                              a->qo_stride_token, a->qo_stride_head, a->ko_stride_token, a->ko_stride_head,
+                              a->tokens, a->table_rows, a->q_heads, a->k_heads, a->head_dim, a->rotary_dim,
+                              a->interleaved, a->positions_64, a->eps, err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
+  switch (a->dtype) {
     case UCB_BF16: return ucb::launch<__nv_bfloat16>(p, s);
     case UCB_F16: return ucb::launch<__half>(p, s);
     case UCB_F32: return ucb::launch<float>(p, s);

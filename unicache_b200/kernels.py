@@ -1164,14 +1164,14 @@ def rope_table(positions: int, rotary_dim: int, *, theta: float = 10000.0,
     return angle.cos().float(), angle.sin().float()
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with ``device`` current: its kernels launch on a stream of that device."""
+def _call_on(index: int, name: str, *args) -> None:
+    """``call`` with device ``index`` current: its kernels launch on a stream of that device."""
 
     function = getattr(_capi.load(), name)
-    if torch.cuda.current_device() == device.index:
+    if torch.cuda.current_device() == index:
         rc = function(*args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = function(*args)
     if rc:
         _capi.check(rc, name)
@@ -1195,59 +1195,65 @@ def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_w
     if first is None:
         raise ValueError("head_norm_rope needs a query or a key")
     require_cuda(first, "query" if query is not None else "key")
-    device, dtype = first.device, first.dtype
+    index, dtype, shape = first.get_device(), first.dtype, first.shape
     code = dtype_code(dtype)
-    if first.dim() != 3:
+    if len(shape) != 3:
         raise ValueError("query and key must be [tokens, heads, head_dim]")
-    tokens, _, head_dim = first.shape
+    tokens, _, head_dim = shape
     if not 2 <= head_dim <= 256:
         raise ValueError("head_dim must be 2 to 256")
-    q = _norm_side("query", query, query_weight, query_out, device, dtype, tokens, head_dim)
-    k = _norm_side("key", key, key_weight, key_out, device, dtype, tokens, head_dim)
-    rotary = table_rows = wide = 0
-    tables = (None, None, None)
+    q_at, q_st, q_sh, q_heads, q_weight, query_out, qo_at, qo_st, qo_sh = \
+        _norm_side("query", query, query_weight, query_out, index, dtype, tokens, head_dim)
+    k_at, k_st, k_sh, k_heads, k_weight, key_out, ko_at, ko_st, ko_sh = \
+        _norm_side("key", key, key_weight, key_out, index, dtype, tokens, head_dim)
+    rotary = table_rows = cos_at = sin_at = positions_at = 0
+    wide = False
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise ValueError("the rotation needs cos, sin and positions")
         shape = cos.shape
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or shape != sin.shape \
+        if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(shape) != 2 or shape != sin.shape \
                 or not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError("cos and sin must be contiguous float32 [positions, rotary_dim / 2] tables")
-        wide = positions.dtype == torch.int64
-        if not (wide or positions.dtype == torch.int32) or positions.numel() != tokens \
+        wide = positions.dtype is torch.int64
+        if not (wide or positions.dtype is torch.int32) or positions.numel() != tokens \
                 or not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32 or int64 tensor of one entry per token")
-        if cos.device != device or sin.device != device or positions.device != device:
+        if cos.get_device() != index or sin.get_device() != index or positions.get_device() != index:
             raise ValueError("cos, sin and positions must be on the rows' device")
         table_rows, rotary = shape[0], 2 * shape[1]
         if rotary > head_dim:
             raise ValueError("the tables rotate more channels than head_dim")
-        tables = (cos.data_ptr(), sin.data_ptr(), positions.data_ptr())
-    _call_on(device, "ucb_head_norm_rope", q[0], q[1], q[2], q[3], k[0], k[1], k[2], k[3], q[4], k[4], *tables,
-             wide, table_rows, tokens, head_dim, rotary, interleaved, code, eps, q[6], q[7], q[8], k[6], k[7], k[8],
-             stream_of(first))
-    return q[5], k[5]
+        cos_at, sin_at, positions_at = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    if tokens:
+        args = _capi.HEAD_NORM_ARGS.pack(
+            q_at, k_at, q_weight, k_weight, cos_at, sin_at, positions_at, qo_at, ko_at, q_st, q_sh, k_st, k_sh, qo_st,
+            qo_sh, ko_st, ko_sh, table_rows, tokens, q_heads, k_heads, head_dim, rotary, interleaved, wide, code, eps)
+        _call_on(index, "ucb_head_norm_rope", args, stream_of(first))
+    return query_out, key_out
 
 
-def _norm_side(name, x, weight, out, device, dtype, tokens, head_dim):
-    """One side's checked (address, token stride, head stride, heads, weight, out, out address and strides)."""
+def _norm_side(name, x, weight, out, index, dtype, tokens, head_dim):
+    """One side's checked (address, token stride, head stride, heads, weight, out, out's address and strides)."""
 
     if x is None:
-        return None, 0, 0, 0, None, None, None, 0, 0
+        return 0, 0, 0, 0, 0, None, 0, 0, 0
     shape, stride = x.shape, x.stride()
-    if x.device != device or x.dtype != dtype or len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim \
-            or stride[2] != 1:
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim or stride[2] != 1 or x.dtype is not dtype \
+            or x.get_device() != index:
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with unit channel stride, one dtype and device")
+    weight_at = 0
     if weight is not None:
-        if weight.device != device or weight.dtype != dtype or weight.numel() != head_dim or not weight.is_contiguous():
+        if weight.numel() != head_dim or weight.dtype is not dtype or weight.get_device() != index \
+                or not weight.is_contiguous():
             raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of the rows' dtype and device")
-        weight = weight.data_ptr()
+        weight_at = weight.data_ptr()
     if out is None:
         out = torch.empty_like(x)  # dense, channels contiguous as x's are
-    elif out.shape != shape or out.device != device or out.dtype != dtype or out.stride(2) != 1:
+    elif out.shape != shape or out.get_device() != index or out.dtype is not dtype or out.stride(2) != 1:
         raise ValueError(f"{name}_out must match {name}, with unit channel stride")
     out_stride = out.stride()
-    return x.data_ptr(), stride[0], stride[1], shape[1], weight, out, out.data_ptr(), out_stride[0], out_stride[1]
+    return x.data_ptr(), stride[0], stride[1], shape[1], weight_at, out, out.data_ptr(), out_stride[0], out_stride[1]
 
 
 # ---------------------------------------------------------------- 8-bit block cache
@@ -1255,7 +1261,7 @@ def _block8_rows(cache, name: str, x: torch.Tensor) -> tuple:
     """Shape and strides of checked rows [N, H, D] of a block cache write."""
 
     shape, stride = x.shape, x.stride()
-    if x.device != cache.device or x.dtype != cache.dtype or len(shape) != 3 or shape[1] != cache.num_kv_heads \
+    if x.get_device() != cache.index or x.dtype is not cache.dtype or len(shape) != 3 or shape[1] != cache.num_kv_heads \
             or shape[2] != cache.head_dim or stride[2] != 1:
         raise ValueError(f"{name} must be [rows, kv_heads, head_dim] with unit channel stride, in the cache's dtype and "
                          "on its device")
@@ -1267,7 +1273,7 @@ def _block8_starts(cache, rows: int, starts: torch.Tensor | None) -> int | None:
         if rows != cache.num_seqs:
             raise ValueError("without starts there must be one row for each sequence")
         return None
-    if starts.device != cache.device or starts.dtype != torch.int32 or starts.numel() != cache.num_seqs + 1 \
+    if starts.get_device() != cache.index or starts.dtype is not torch.int32 or starts.numel() != cache.num_seqs + 1 \
             or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 [num_seqs + 1] tensor on the cache's device")
     return starts.data_ptr()
@@ -1282,7 +1288,7 @@ def block8_write(cache, key: torch.Tensor, value: torch.Tensor, starts: torch.Te
     if value_shape[0] != rows:
         raise ValueError("key and value must have the same rows")
     at = _block8_starts(cache, rows, starts)
-    _call_on(cache.device, "ucb_block8_write", cache.descriptor, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0],
+    _call_on(cache.index, "ucb_block8_write", cache.descriptor, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0],
              vs[1], rows, at, stream_of(key))
 
 
@@ -1292,7 +1298,7 @@ def block8_read(cache, rows: int, starts: torch.Tensor | None = None) -> tuple[t
     at = _block8_starts(cache, rows, starts)
     shape = (rows, cache.num_kv_heads, cache.head_dim)
     key, value = cache.pending_key.new_empty(shape), cache.pending_key.new_empty(shape)
-    _call_on(cache.device, "ucb_block8_read", cache.descriptor, rows, at, key.data_ptr(), value.data_ptr(),
+    _call_on(cache.index, "ucb_block8_read", cache.descriptor, rows, at, key.data_ptr(), value.data_ptr(),
              stream_of(cache.lengths))
     return key, value
 
@@ -1301,7 +1307,7 @@ def _block8_query(cache, query: torch.Tensor) -> tuple:
     """Shape and strides of a checked query [S, Hq, D] or [S, L, Hq, D] of the cache's sequences."""
 
     shape, stride = query.shape, query.stride()
-    if query.device != cache.device or query.dtype != cache.dtype or len(shape) < 3 or shape[0] != cache.num_seqs \
+    if query.get_device() != cache.index or query.dtype is not cache.dtype or len(shape) < 3 or shape[0] != cache.num_seqs \
             or shape[-1] != cache.head_dim or stride[-1] != 1:
         raise ValueError("query must be [num_seqs, (queries,) q_heads, head_dim] with unit channel stride, in the "
                          "cache's dtype and on its device")
@@ -1321,7 +1327,7 @@ def block8_select(query: torch.Tensor, cache, *, count: int, first: int = 1, rec
         raise ValueError("need 1 <= count <= 4096 and first + recent <= count")
     blocks = cache.lengths.new_empty((cache.num_seqs, cache.num_kv_heads, count))
     workspace = cache.key_code.new_empty(cache.select_bytes) if cache.select_bytes else None
-    _call_on(cache.device, "ucb_block8_select", cache.descriptor, query.data_ptr(), stride[0], stride[1], shape[1],
+    _call_on(cache.index, "ucb_block8_select", cache.descriptor, query.data_ptr(), stride[0], stride[1], shape[1],
              count, first, recent, blocks.data_ptr(), ptr(workspace), stream_of(query))
     return blocks
 
@@ -1341,10 +1347,10 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
     if not 1 <= queries <= 16:
         raise ValueError("the block cache attention takes 1 to 16 query tokens a sequence; read the cache back and "
                          "use long_query_attention_summary for more")
-    selected, at = 0, None
+    selected = at = 0
     if blocks is not None:
         listed = blocks.shape
-        if blocks.device != cache.device or blocks.dtype != torch.int32 or len(listed) != 3 \
+        if blocks.get_device() != cache.index or blocks.dtype is not torch.int32 or len(listed) != 3 \
                 or listed[0] != cache.num_seqs or listed[1] != cache.num_kv_heads \
                 or listed[2] < 1 or not blocks.is_contiguous():
             raise ValueError("blocks must be a contiguous int32 [num_seqs, kv_heads, count] tensor on the cache's device")
@@ -1354,9 +1360,9 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
     out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(shape)
     lse = cache.key_scale.new_empty(shape[:-1])
     workspace = cache.attention_workspace(queries, q_heads)
-    _call_on(cache.device, "ucb_block8_attention", cache.descriptor, query.data_ptr(), stride[0], query_stride, stride[-2],
-             queries, q_heads, at, selected, scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
-             stream_of(query))
+    args = _capi.BLOCK8_ATTENTION_ARGS.pack(query.data_ptr(), at, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
+                                            stride[0], query_stride, stride[-2], queries, q_heads, selected, scale)
+    _call_on(cache.index, "ucb_block8_attention", cache.descriptor, args, stream_of(query))
     return out, lse
 
 

@@ -83,7 +83,8 @@ class Int8BlockCache:
             dtype=kernels.dtype_code(self.pending_key.dtype))
         # the launch wrappers read these on every call
         for name, attribute in (("_struct", struct), ("descriptor", ctypes.addressof(struct)),
-                                ("device", self.key_code.device), ("dtype", self.pending_key.dtype),
+                                ("device", self.key_code.device), ("index", self.key_code.get_device()),
+                                ("dtype", self.pending_key.dtype),
                                 ("num_seqs", seqs), ("num_kv_heads", heads), ("head_dim", dim),
                                 ("block_size", size), ("max_tokens", width * size), ("_workspace_bytes", {})):
             object.__setattr__(self, name, attribute)
