@@ -22,7 +22,8 @@ from dataclasses import dataclass
 import torch
 
 from . import kernels
-from .adapters.attention import long_query_attention_summary
+from .adapters.attention import int8_block_decode, long_query_attention_summary, sparse_int8_block_decode
+from .storage.int8_block import Int8BlockCache
 from .storage.physical import GQAH2OCache, PackedKIVICache
 from .synthetic import make_kv, make_query
 
@@ -246,3 +247,91 @@ class Qwen2PackedDecode:
 
     def replay(self) -> None:
         self.graph.replay()
+
+
+# ---------------------------------------------------------------- decode over the 8-bit block cache
+class Int8BlockDecode:
+    """Attention layers with head norms decoding over 8-bit block caches.
+
+    Each layer normalises its input, projects it, normalises and rotates the
+    query and key heads (``head_norm_rope``), appends key and value to its
+    ``Int8BlockCache`` and attends over the whole cache or, with ``count``,
+    over that many blocks that the query chooses (``sparse_int8_block_decode``).
+    All layers share one block table and one device tensor of lengths, so a
+    step has no host state and is captured once as a CUDA graph.  Weights and
+    prompts are seeded random; the prompts' keys go through the same norm and
+    rotation and all sequences of a layer through one write.
+    """
+
+    def __init__(self, device, *, prompts: list[int], new_tokens: int, layers: int = 2, hidden: int = 3584,
+                 q_heads: int = 28, kv_heads: int = 4, head_dim: int = 128, block_size: int = 64,
+                 count: int | None = None, theta: float = 1.0e6, seed: int = 7):
+        self.device = torch.device(device)
+        self.hq, self.hkv, self.d, self.count, self.eps = q_heads, kv_heads, head_dim, count, 1.0e-6
+        gen = torch.Generator(device=self.device).manual_seed(seed)
+
+        def normal(*shape, std=1.0, mean=0.0):
+            return (mean + std * torch.randn(*shape, generator=gen, device=self.device)).to(torch.bfloat16)
+
+        batch, longest, tokens = len(prompts), max(prompts) + new_tokens, sum(prompts)
+        self.cos, self.sin = kernels.rope_table(longest, head_dim, theta=theta, device=self.device)
+        starts = torch.tensor([0, *prompts], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
+        where = torch.cat([torch.arange(n, dtype=torch.int32) for n in prompts]).to(self.device)
+        self.w, self.caches = [], []
+        for layer in range(layers):
+            weights = {"norm": normal(hidden, std=0.1, mean=1.0),
+                       "qkv": normal(hidden, (q_heads + 2 * kv_heads) * head_dim, std=hidden ** -0.5),
+                       "q_norm": normal(head_dim, std=0.1, mean=1.0), "k_norm": normal(head_dim, std=0.1, mean=1.0),
+                       "o": normal(q_heads * head_dim, hidden, std=hidden ** -0.5)}
+            shared = {} if layer == 0 else {"block_table": self.caches[0].block_table,
+                                            "num_blocks": int(self.caches[0].key_code.shape[0]),
+                                            "lengths": self.caches[0].lengths}
+            cache = Int8BlockCache.allocate(batch, longest, num_kv_heads=kv_heads, head_dim=head_dim,
+                                            block_size=block_size, device=self.device, **shared)
+            if layer == 0:
+                cache.advance(torch.tensor(prompts, dtype=torch.int32, device=self.device))
+            key, value = normal(tokens, kv_heads, head_dim), normal(tokens, kv_heads, head_dim)
+            _, key = kernels.head_norm_rope(None, key, None, weights["k_norm"], self.cos, self.sin, where, eps=self.eps)
+            cache.write(key, value, starts=starts)
+            self.w.append(weights)
+            self.caches.append(cache)
+        self.x = normal(batch, hidden)
+        self.query = self.attended = None  # the last layer's, of the last step
+        self.graph = None
+
+    def step(self) -> torch.Tensor:
+        """One token of every sequence (device-only, capturable): the hidden states [batch, hidden]."""
+
+        hq, hkv, d = self.hq, self.hkv, self.d
+        lengths = self.caches[0].lengths
+        self.caches[0].advance(1)  # for every layer
+        positions = lengths - 1
+        x = self.x
+        for w, cache in zip(self.w, self.caches):
+            qkv = (kernels.rms_norm(x, w["norm"], self.eps) @ w["qkv"]).view(-1, hq + 2 * hkv, d)
+            query, key = kernels.head_norm_rope(qkv[:, :hq], qkv[:, hq:hq + hkv], w["q_norm"], w["k_norm"], self.cos,
+                                                self.sin, positions, eps=self.eps)
+            cache.write(key, qkv[:, hq + hkv:])
+            if self.count is None:
+                out, _ = int8_block_decode(query, cache)
+            else:
+                _, out, _ = sparse_int8_block_decode(query, cache, count=self.count)
+            x = torch.addmm(x, out.view(-1, hq * d), w["o"])
+        self.query, self.attended = query, out
+        self.x.copy_(x)
+        return self.x
+
+    def capture(self) -> None:
+        """Capture one step as a CUDA graph; ``replay`` then runs a step."""
+
+        stream = torch.cuda.Stream(device=self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream):
+            with torch.cuda.graph(self.graph, stream=stream):
+                self.step()
+        torch.cuda.current_stream(self.device).wait_stream(stream)
+
+    def replay(self) -> torch.Tensor:
+        self.graph.replay()
+        return self.x
