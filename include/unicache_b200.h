@@ -668,7 +668,8 @@ UCB_API int ucb_block8_select(const ucb_block8_cache* cache, const void* query_d
  * to the tokens of these blocks (negative entries are skipped, no block may
  * be named twice); NULL = all.  out [num_seqs, queries, q_heads, head_dim] in
  * dtype, lse fp32 [num_seqs, queries, q_heads] natural log (or NULL).
- * workspace: ucb_block8_attention_workspace_bytes bytes; it and out 16-byte aligned. */
+ * Query rows start on 8 bytes.  workspace: ucb_block8_attention_workspace_bytes
+ * bytes; it and out 16-byte aligned. */
 UCB_API int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads);
 typedef struct ucb_block8_attention_args {
   const void* query;

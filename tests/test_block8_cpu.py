@@ -73,7 +73,7 @@ def test_bad_caches_are_refused_by_every_entry(changes, message):
 
 @pytest.mark.parametrize("change,message", [
     ({0: 0}, "null pointer"), ({2: 0}, "null pointer"), ({4: 0}, "null pointer"), ({4: 4100}, "aligned"),
-    ({2: 4104}, "aligned"), ({8: 0}, "16 query tokens"), ({8: 17}, "16 query tokens"), ({9: 27}, "divisible"),
+    ({2: 4104}, "aligned"), ({0: 4098}, "8 bytes"), ({7: 130}, "8 bytes"), ({8: 0}, "16 query tokens"), ({8: 17}, "16 query tokens"), ({9: 27}, "divisible"),
     ({1: 4096, 10: 0}, "selection")])
 def test_bad_attention_calls_are_refused(change, message):
     lib = _capi.load()

@@ -347,6 +347,9 @@ def test_strided_queries_and_scales():
     cache, _, _, gen = filled(lengths, seed=8)
     wide = make_query(gen, (2, 3, 36, 131), torch.bfloat16)
     check_attention(cache, wide[:, :, 4:32, 1:129], lengths)
+    flat = make_query(gen, (2 * 28 * 128 + 1,), torch.bfloat16)
+    check_attention(cache, flat[1:].view(2, 28, 128), lengths)
+    check_attention(cache, wide[:, 1, 4:32, :128].transpose(0, 1).contiguous().transpose(0, 1), lengths)
     check_attention(cache, wide[:, 1, 4:32, 3:], lengths, scale=0.31)
     check_attention(cache, wide[:, 1, 4:32, :128], lengths, scale=0.0)
     check_attention(cache, wide[:, 1, 4:32, :128], lengths, scale=-0.1)

@@ -46,10 +46,10 @@ struct AttnParams {
   ucb_block8_cache c;
   const void* q;
   int64_t q_ss, q_sl, q_sh;
-  int queries, q_heads, group, rows, row_tiles;  // rows = group * queries of a KV head
+  int queries, q_heads, group, rows, row_tiles, heads_rows;  // rows = group * queries of a KV head
   const int32_t* blocks;
   int selected;
-  int q_aligned;     // query rows can be read 8 bytes at a time
+  uint32_t group_magic, heads_rows_magic, row_tiles_magic;  // floor(2^32 / divisor)
   int step_shift;    // log2(steps in a block)
   float scale_log2;  // softmax scale * log2(e)
   void* out;
@@ -106,12 +106,19 @@ struct Segment {
   const float* spilled;  // null: in the warp's ring
 };
 
-__device__ __forceinline__ uint32_t pack_out(const AttnParams& p, float lo, float hi) {
-  return p.c.dtype == UCB_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+// x / divisor, by the divisor's floor(2^32 / divisor): at most one below.
+__device__ __forceinline__ int divide(int x, int divisor, uint32_t magic) {
+  const int q = (int)__umulhi((uint32_t)x, magic);
+  return q + (x - q * divisor >= divisor);
+}
+
+template <bool BF> __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+  return BF ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
 
 __device__ __forceinline__ int64_t out_row(const AttnParams& p, int s, int h, int row) {
-  return ((int64_t)s * p.queries + row / p.group) * p.q_heads + h * p.group + row % p.group;
+  const int l = divide(row, p.group, p.group_magic);
+  return ((int64_t)s * p.queries + l) * p.q_heads + h * p.group + row - l * p.group;
 }
 
 __device__ __forceinline__ void write_lse(const AttnParams& p, int64_t row, float ref, float sum) {
@@ -120,7 +127,7 @@ __device__ __forceinline__ void write_lse(const AttnParams& p, int64_t row, floa
 
 // 2^(ref - sum_ref) / sum, the factor of an unnormalised row; 0 where no token was seen.
 __device__ __forceinline__ float normaliser(float ref, float sum_ref, float sum) {
-  return sum == 0.f || (ref == -INFINITY && sum == sum) ? 0.f : exp2f(ref - sum_ref) / sum;
+  return sum == 0.f || (ref == -INFINITY && sum == sum) ? 0.f : fast_exp2(ref - sum_ref) * __fdividef(1.f, sum);
 }
 
 // States of one row merged, four channels of it.  A state without a token has references -inf and sum 0; products, not
@@ -166,13 +173,13 @@ template <int D, typename Get> __device__ __forceinline__ Merged merge_states(in
   return m;
 }
 
-__device__ __forceinline__ void write_four(const AttnParams& p, int64_t at, const Merged& m) {
+template <bool BF> __device__ __forceinline__ void write_four(const AttnParams& p, int64_t at, const Merged& m) {
   const float f = normaliser(m.ref, m.sum_ref, m.sum);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
-      make_uint2(pack_out(p, m.value.x * f, m.value.y * f), pack_out(p, m.value.z * f, m.value.w * f));
+      make_uint2(pack_out<BF>(m.value.x * f, m.value.y * f), pack_out<BF>(m.value.z * f, m.value.w * f));
 }
 
-template <int D, int NT, int U>
+template <bool BF, int D, int NT, int U>
 __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kernel(const AttnParams p) {
   using S = Shape<D, NT, U>;
   constexpr int MT = D / 16;          // value products of 16 channels
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   __shared__ int warp_sums[S::WARPS];
   int* prefix = reinterpret_cast<int*>(smem + S::WARPS * S::RING_BYTES);  // [num_seqs + 1], dense only
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cq = lane & 3;
-  const int bt = c.block_tokens, heads_rows = c.kv_heads * p.row_tiles;
+  const int bt = c.block_tokens, heads_rows = p.heads_rows;
   const int step_mask = (1 << p.step_shift) - 1;
 
   // ---- the flat order: steps of every sequence (at least one, so that every row is written)
@@ -227,27 +234,26 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   };
   auto locate = [&](int t) {
     Pair a;
-    int u;
+    const int unit = divide(t, heads_rows, p.heads_rows_magic);
+    int first;
     if (p.blocks) {
+      a.s = unit / listed_steps;
       a.steps = listed_steps;
-      const int pair = t / listed_steps;
-      a.base = pair * listed_steps;
-      a.s = pair / heads_rows;
-      u = pair - a.s * heads_rows;
+      first = a.s * listed_steps;
     } else {
-      const int unit = t / heads_rows;
       int lo = 0, hi = c.num_seqs - 1;  // the last sequence whose first step is not after t
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (prefix[mid] <= unit) lo = mid; else hi = mid - 1;
       }
       a.s = lo;
-      a.steps = prefix[lo + 1] - prefix[lo];
-      const int first = prefix[lo] * heads_rows;
-      u = (t - first) / a.steps;
-      a.base = first + u * a.steps;
+      first = prefix[lo];
+      a.steps = prefix[lo + 1] - first;
     }
-    a.h = u / p.row_tiles;
+    first *= heads_rows;
+    const int u = (t - first) / a.steps;
+    a.base = first + u * a.steps;
+    a.h = divide(u, p.row_tiles, p.row_tiles_magic);
     a.rt = u - a.h * p.row_tiles;
     return a;
   };
@@ -280,16 +286,12 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = a.rt * S::ROWS + nt * 8 + r;
-      const int l = row / p.group;
-      const int64_t at = a.s * p.q_ss + l * p.q_sl + (a.h * p.group + row - l * p.group) * p.q_sh + 16 * cq;
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
+      const int l = divide(row, p.group, p.group_magic);
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + a.s * p.q_ss + l * p.q_sl +
+                          (a.h * p.group + row - l * p.group) * p.q_sh + 16 * cq;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const uint16_t* x = q + 64 * (i / 4) + 4 * (i % 4);
-        if (row >= p.rows) raw[nt][i] = make_uint2(0, 0);
-        else if (p.q_aligned) raw[nt][i] = *reinterpret_cast<const uint2*>(x);
-        else raw[nt][i] = make_uint2(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16);
-      }
+      for (int i = 0; i < KS; ++i)
+        raw[nt][i] = row < p.rows ? *reinterpret_cast<const uint2*>(q + 64 * (i / 4) + 4 * (i % 4)) : make_uint2(0, 0);
     }
 
     // ---- block descriptors: lane i holds entry window + i, `next` the 32 entries after
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       if (e.block >= 0) {
         const int64_t at = (int64_t)e.block * c.kv_heads + a.h;
         e.ks = c.key_scale[at];
-        e.lv = log2f(c.value_scale[at]);
+        e.lv = __log2f(c.value_scale[at]);
       }
     };
     int window = begin >> p.step_shift;
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       }
       cp_async_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int x = 0; x < S::STAGES - 1; ++x) issue(begin + x);
     fetch_scales(now);
     bool next_scaled = false;
@@ -358,8 +360,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
       top = max(top & 0xffffu, top >> 16);
-      const bool bf = c.dtype == UCB_BF16;
-      const uint32_t exponent = __float_as_uint(bf ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top))) >> 23;
+      const uint32_t exponent = __float_as_uint(BF ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top))) >> 23;
       // both factors are normal numbers; a row of zeros, infinities or NaN is left as it is
       const int e = exponent == 0 && top == 0 || exponent == 255 ? 0 : min(126, 140 - (int)exponent);
       const float up = __uint_as_float((uint32_t)(127 + e) << 23);
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
         const uint32_t w[2] = {raw[nt][i].x, raw[nt][i].y};
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          qb[nt][i][k] = bf ? pack_f16x2(Dtype<__nv_bfloat16>::lo(w[k]) * up, Dtype<__nv_bfloat16>::hi(w[k]) * up)
+          qb[nt][i][k] = BF ? pack_f16x2(Dtype<__nv_bfloat16>::lo(w[k]) * up, Dtype<__nv_bfloat16>::hi(w[k]) * up)
                             : pack_f16x2(Dtype<__half>::lo(w[k]) * up, Dtype<__half>::hi(w[k]) * up);
       }
     }
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       for (int k = 0; k < 2; ++k) {
         col_scale[nt][k] = __shfl_sync(0xffffffffu, row_scale[nt], 4 * (2 * cq + k));
         const int row = a.rt * S::ROWS + nt * 8 + 2 * cq + k;
-        col_limit[nt][k] = len - p.queries + 1 + (row < p.rows ? row / p.group : 0);
+        col_limit[nt][k] = len - p.queries + 1 + (row < p.rows ? divide(row, p.group, p.group_magic) : 0);
       }
     const int sure = len - p.queries + 1;  // tokens that every row sees
 
@@ -575,8 +576,8 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
             uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * D + VB * r);
 #pragma unroll
             for (int i = 0; i < VB / 8; ++i)
-              out[i] = make_uint4(pack_out(p, run[8 * i], run[8 * i + 1]), pack_out(p, run[8 * i + 2], run[8 * i + 3]),
-                                  pack_out(p, run[8 * i + 4], run[8 * i + 5]), pack_out(p, run[8 * i + 6], run[8 * i + 7]));
+              out[i] = make_uint4(pack_out<BF>(run[8 * i], run[8 * i + 1]), pack_out<BF>(run[8 * i + 2], run[8 * i + 3]),
+                                  pack_out<BF>(run[8 * i + 4], run[8 * i + 5]), pack_out<BF>(run[8 * i + 6], run[8 * i + 7]));
             if (r == 0) write_lse(p, to, sum_ref[nt][k], l);
           }
         } else {
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       });
       if (complete) {
         const int64_t out = out_row(p, last.s, last.h, row);
-        write_four(p, out * D + d, m);
+        write_four<BF>(p, out * D + d, m);
         if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
       } else {
         float* at = to + in_tile * S::ROW_FLOATS;
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 // continue it by, every MERGE_GROUPS-th by one group of D / 4 threads.
 constexpr int MERGE_GROUPS = 4;
 
-template <int D, int NT, int U>
+template <bool BF, int D, int NT, int U>
 __global__ void __launch_bounds__(MERGE_GROUPS * D / 4) attention_merge_kernel(const AttnParams p) {
   using S = Shape<D, NT, U>;
   __shared__ float groups[MERGE_GROUPS][D + 4];
@@ -660,7 +661,7 @@ __global__ void __launch_bounds__(MERGE_GROUPS * D / 4) attention_merge_kernel(c
   if (g > 0) return;
   m = merge_states<D>(0, MERGE_GROUPS, 1, d, [&](int i) { return static_cast<const float*>(groups[i]); });
   const int64_t out = out_row(p, link.y, link.z, row);
-  write_four(p, out * D + d, m);
+  write_four<BF>(p, out * D + d, m);
   if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
 }
 
@@ -674,13 +675,13 @@ int multiprocessors() {
 
 constexpr int MOST_SEQS = 4096;
 
-template <int D, int NT, int U> int launch_shape(AttnParams& p, int sms, cudaStream_t stream) {
+template <bool BF, int D, int NT, int U> int launch_shape(AttnParams& p, int sms, cudaStream_t stream) {
   using S = Shape<D, NT, U>;
   static bool ready[64] = {false};  // the attribute is a device's; setting it twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
   if (!ready[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_kernel<D, NT, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(attention_kernel<BF, D, NT, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                S::WARPS * S::RING_BYTES + (MOST_SEQS + 1) * 4);
     if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "ucb_block8_attention: %s", cudaGetErrorString(e));
     ready[dev & 63] = true;
@@ -694,20 +695,25 @@ template <int D, int NT, int U> int launch_shape(AttnParams& p, int sms, cudaStr
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
   p.spill = p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS;
   p.links = reinterpret_cast<int*>(p.spill + (int64_t)CTAS_PER_SM * sms * S::WARPS * S::STATE_FLOATS);
-  if (int rc = block8::launch(attention_kernel<D, NT, U>, dim3(grid), dim3(S::WARPS * 32), smem, stream, p,
+  if (int rc = block8::launch(attention_kernel<BF, D, NT, U>, dim3(grid), dim3(S::WARPS * 32), smem, stream, p,
                               "block8 attention_kernel"))
     return rc;
-  return block8::launch(attention_merge_kernel<D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), 0, stream, p,
+  return block8::launch(attention_merge_kernel<BF, D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), 0, stream, p,
                         "block8 attention_merge_kernel", 1, true);
 }
 
-template <int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
+template <bool BF, int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
   // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 76 us
   // against 96) and for 16 rows (eight of 5003 tokens, four queries each: 23.4 against 25.4).
   if constexpr (D == 64 || NT == 2) {
-    if (p.c.block_tokens > TILE) return launch_shape<D, NT, 2>(p, sms, stream);
+    if (p.c.block_tokens > TILE) return launch_shape<BF, D, NT, 2>(p, sms, stream);
   }
-  return launch_shape<D, NT, 1>(p, sms, stream);
+  return launch_shape<BF, D, NT, 1>(p, sms, stream);
+}
+
+template <bool BF> int launch_heads(AttnParams& p, int sms, cudaStream_t stream) {
+  if (p.c.head_dim == 128) return p.rows > 8 ? launch_block<BF, 128, 2>(p, sms, stream) : launch_block<BF, 128, 1>(p, sms, stream);
+  return p.rows > 8 ? launch_block<BF, 64, 2>(p, sms, stream) : launch_block<BF, 64, 1>(p, sms, stream);
 }
 
 }  // namespace
@@ -735,6 +741,9 @@ extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_blo
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: query heads must be divisible by KV heads");
   if (a->blocks && (a->num_selected < 1 || a->num_selected > 1 << 20))
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: a selection needs 1 to 2^20 entries");
+  if (reinterpret_cast<uintptr_t>(a->query) & 7 || (a->q_stride_seq | a->q_stride_query | a->q_stride_head) & 3)
+    return set_error(UCB_ERR_INVALID, "ucb_block8_attention: query rows must start on 8 bytes");
+  if (a->q_heads > 65535) return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: at most 65535 query heads");
   if ((reinterpret_cast<uintptr_t>(a->workspace) | reinterpret_cast<uintptr_t>(a->out)) & 15)
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: out and workspace must be 16-byte aligned");
   unsigned int* err = ucb_host::device_error_word();
@@ -744,18 +753,20 @@ extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_blo
   p.c = *cache;
   p.q = a->query;
   p.q_ss = a->q_stride_seq, p.q_sl = a->q_stride_query, p.q_sh = a->q_stride_head;
-  p.q_aligned = reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.q_ss | p.q_sl | p.q_sh) % 4 == 0;
   p.queries = a->queries, p.q_heads = a->q_heads;
   p.group = a->q_heads / cache->kv_heads;
   p.rows = p.group * a->queries;
   const int tile_rows = p.rows > 8 ? 16 : 8;
   p.row_tiles = (p.rows + tile_rows - 1) / tile_rows;
+  p.heads_rows = cache->kv_heads * p.row_tiles;
+  // floor(2^32 / d), 2^32 - 1 for 1 (one below in the product, as divide() takes it)
+  auto magic = [](int d) { return (uint32_t)std::min<uint64_t>(0xffffffffu, (1ull << 32) / d); };
+  p.group_magic = magic(p.group), p.heads_rows_magic = magic(p.heads_rows), p.row_tiles_magic = magic(p.row_tiles);
   p.blocks = a->blocks, p.selected = a->blocks ? a->num_selected : 0;
   p.scale_log2 = a->softmax_scale * 1.44269504088896341f;
   p.out = a->out, p.lse = a->lse;
   p.partials = static_cast<float*>(a->workspace);
   p.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 128) return tile_rows == 16 ? b8::launch_block<128, 2>(p, sms, s) : b8::launch_block<128, 1>(p, sms, s);
-  return tile_rows == 16 ? b8::launch_block<64, 2>(p, sms, s) : b8::launch_block<64, 1>(p, sms, s);
+  return cache->dtype == UCB_BF16 ? b8::launch_heads<true>(p, sms, s) : b8::launch_heads<false>(p, sms, s);
 }

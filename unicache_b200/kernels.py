@@ -1357,6 +1357,10 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
         selected, at = listed[2], blocks.data_ptr()
     q_heads = shape[-2]
     scale = cache.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if query.data_ptr() & 7 or (stride[0] | query_stride | stride[-2]) & 3:  # the kernel reads rows 8 bytes at a time
+        query = query.clone(memory_format=torch.contiguous_format)
+        stride = query.stride()
+        query_stride = stride[1] if len(shape) == 4 else 0
     out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(shape)
     lse = cache.key_scale.new_empty(shape[:-1])
     workspace = cache.attention_workspace(queries, q_heads)
