@@ -55,7 +55,6 @@ struct AttnParams {
   void* out;
   float* lse;
   float* partials;  // [2 * grid] states of pairs that cross CTAs
-  float* spill;     // [grid * warps] states of segments that are not a warp's last
   int* links;       // [grid][4]: last CTA of the pair that starts in this CTA and goes on (-1: none), s, h, row tile
   unsigned int* err;
 };
@@ -77,6 +76,7 @@ template <int D, int NT, int U> struct Shape {
   static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its reference, the sum's reference, the sum
   static constexpr int STATE_FLOATS = ROWS * ROW_FLOATS;
   static constexpr int RING_BYTES = STAGES * STEP_BYTES;
+  static constexpr int SMEM_BYTES = WARPS * (RING_BYTES + STATE_FLOATS * 4);  // without the prefix sums
   static_assert(RING_BYTES >= STATE_FLOATS * 4, "a state fits a ring");
 };
 
@@ -103,7 +103,8 @@ struct Pair {
 struct Segment {
   int used, ends;  // ends: holds the pair's last step
   int s, h, rt;
-  const float* spilled;  // null: in the warp's ring
+  int end_cta;  // the CTA that holds the pair's last step
+  int apart;    // the state is not in the warp's ring but in its other place
 };
 
 // x / divisor, by the divisor's floor(2^32 / divisor): at most one below.
@@ -136,39 +137,38 @@ struct Merged {
   float4 value;
   float ref, sum_ref, sum;
 };
+// One more state, at references not above m's.
+__device__ __forceinline__ void merge_in(Merged& m, float4 value, float4 meta) {
+  const float f = meta.x == -INFINITY ? 0.f : fast_exp2(meta.x - m.ref);
+  m.value.x = fmaf(f, value.x, m.value.x);
+  m.value.y = fmaf(f, value.y, m.value.y);
+  m.value.z = fmaf(f, value.z, m.value.z);
+  m.value.w = fmaf(f, value.w, m.value.w);
+  m.sum = fmaf(meta.y == -INFINITY ? 0.f : fast_exp2(meta.y - m.sum_ref), meta.z, m.sum);
+}
 template <int D, typename Get> __device__ __forceinline__ Merged merge_states(int first, int n, int stride, int d, Get get) {
   Merged m{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f};
+#pragma unroll 1
   for (int i = first; i < n; i += 4 * stride) {  // four at a time, their loads together
     float4 x[4], y[4];
     float ref = m.ref, sum_ref = m.sum_ref;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (i + k * stride < n) {
-        const float* at = get(i + k * stride);
-        x[k] = *reinterpret_cast<const float4*>(at + D);
-        y[k] = *reinterpret_cast<const float4*>(at + d);
-      }
+    for (int k = 0; k < 4; ++k) {  // past the end, the last one again: not counted below
+      const float* at = get(min(i + k * stride, n - 1));
+      x[k] = *reinterpret_cast<const float4*>(at + D);
+      y[k] = *reinterpret_cast<const float4*>(at + d);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ref = fmaxf(ref, x[k].x);
+      sum_ref = fmaxf(sum_ref, x[k].y);
+    }
+    const float4 old = m.value, meta = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
+    m = Merged{make_float4(0.f, 0.f, 0.f, 0.f), ref, sum_ref, 0.f};
+    merge_in(m, old, meta);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i + k * stride < n) {
-        ref = fmaxf(ref, x[k].x);
-        sum_ref = fmaxf(sum_ref, x[k].y);
-      }
-    float f = m.ref == -INFINITY ? 0.f : fast_exp2(m.ref - ref);
-    m.value = make_float4(m.value.x * f, m.value.y * f, m.value.z * f, m.value.w * f);
-    m.sum *= m.sum_ref == -INFINITY ? 0.f : fast_exp2(m.sum_ref - sum_ref);
-    m.ref = ref;
-    m.sum_ref = sum_ref;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (i + k * stride < n) {
-        f = x[k].x == -INFINITY ? 0.f : fast_exp2(x[k].x - ref);
-        m.value.x = fmaf(f, y[k].x, m.value.x);
-        m.value.y = fmaf(f, y[k].y, m.value.y);
-        m.value.z = fmaf(f, y[k].z, m.value.z);
-        m.value.w = fmaf(f, y[k].w, m.value.w);
-        m.sum = fmaf(x[k].y == -INFINITY ? 0.f : fast_exp2(x[k].y - sum_ref), x[k].z, m.sum);
-      }
+      if (i + k * stride < n) merge_in(m, y[k], x[k]);
   }
   return m;
 }
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Segment segments[S::WARPS][2];
   __shared__ int warp_sums[S::WARPS];
-  int* prefix = reinterpret_cast<int*>(smem + S::WARPS * S::RING_BYTES);  // [num_seqs + 1], dense only
+  int* prefix = reinterpret_cast<int*>(smem + S::SMEM_BYTES);  // [num_seqs + 1], dense only
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cq = lane & 3;
   const int bt = c.block_tokens, heads_rows = p.heads_rows;
   const int step_mask = (1 << p.step_shift) - 1;
@@ -296,21 +296,25 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 
     // ---- block descriptors: lane i holds entry window + i, `next` the 32 entries after
     struct Entry {
-      int block, token;
-      float ks, lv;  // key scale, log2 of the value scale
+      int block, token;  // pool block (-1: skipped) and its first token (-1: no entry)
+      float ks, lv;      // key scale, log2 of the value scale
     };
-    auto fetch = [&](int k) {
-      Entry e{-1, 0, 0.f, 0.f};
+    auto fetch = [&](int k) {  // the table's entry as it is, checked when it is first used
+      Entry e{-1, -1, 0.f, 0.f};
       if (k < entries) {
         const int j = list ? list[k] : k;
         if (j >= 0 && j < c.max_blocks && (int64_t)j * bt < len) {
           e.token = j * bt;
-          const int b = table[j];
-          if (b >= 0 && b < c.num_blocks) e.block = b;
-          else atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+          e.block = table[j];
         }
       }
       return e;
+    };
+    auto check = [&](Entry& e) {  // a block outside the pool is skipped
+      if (e.token >= 0 && (e.block < 0 || e.block >= c.num_blocks)) {
+        atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+        e.block = -1;
+      }
     };
     auto fetch_scales = [&](Entry& e) {
       if (e.block >= 0) {
@@ -320,7 +324,14 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       }
     };
     int window = begin >> p.step_shift;
-    Entry now = fetch(window + lane), next = fetch(window + 32 + lane);
+    Entry now = fetch(window + lane), next{-1, -1, 0.f, 0.f};
+    bool next_scaled = true;
+    if (((end - 1) >> p.step_shift) - window >= 32) {
+      next = fetch(window + 32 + lane);
+      check(next);
+      next_scaled = false;
+    }
+    check(now);
 
     auto issue = [&](int i) {
       if (i < end) {
@@ -346,7 +357,6 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 #pragma unroll 1
     for (int x = 0; x < S::STAGES - 1; ++x) issue(begin + x);
     fetch_scales(now);
-    bool next_scaled = false;
 
     // ---- query rows as fp16 operands, times the power of two that brings their largest element to [2^13, 2^14)
     uint32_t qb[NT][KS][2];
@@ -405,6 +415,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
         now = next;
         window += 32;
         next = fetch(window + 32 + lane);
+        check(next);
         next_scaled = false;
       } else if (!next_scaled && i > begin) {
         fetch_scales(next);
@@ -549,10 +560,11 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
     cp_async_wait<0>();
 
     // ---- the segment's result: lane (r, cq) holds channels VB * r .. of rows 2 cq and 2 cq + 1.  A warp's last
-    // segment stays in its ring, an earlier one that a warp before began goes through global memory.
+    // segment stays in its ring, an earlier one that a warp before began has a place of its own.
     const bool whole = begin == 0 && end == steps;
     const int which = begin == 0 ? 1 : 0;
-    float* state = t >= t_end ? reinterpret_cast<float*>(ring) : p.spill + (int64_t)worker * S::STATE_FLOATS;
+    const bool apart = t < t_end;
+    float* state = reinterpret_cast<float*>(apart ? smem + S::WARPS * S::RING_BYTES + warp * (S::STATE_FLOATS * 4) : ring);
     __syncwarp();  // every lane is done with the ring before states overwrite it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -588,7 +600,8 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
           if (r == 0) *reinterpret_cast<float4*>(at + D) = make_float4(ref[nt][k], sum_ref[nt][k], l, 0.f);
         }
       }
-    if (!whole && lane == 0) segments[warp][which] = Segment{1, end == steps, a.s, a.h, a.rt, t >= t_end ? nullptr : state};
+    if (!whole && lane == 0)
+      segments[warp][which] = Segment{1, end == steps, a.s, a.h, a.rt, worker_of(a.base + a.steps - 1) / S::WARPS, apart};
   }
   __syncthreads();
 
@@ -614,11 +627,20 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
     for (int item = threadIdx.x; item < S::ROWS * D / 4; item += S::WARPS * 32) {
       const int in_tile = item / (D / 4), d = item % (D / 4) * 4, row = last.rt * S::ROWS + in_tile;
       if (row >= p.rows) break;
+      // the chain's states lie a ring apart, the last one perhaps in its warp's other place
       const unsigned char* states = smem + open_w * S::RING_BYTES + in_tile * (S::ROW_FLOATS * 4);
-      const Merged m = merge_states<D>(0, open_n, 1, d, [&](int i) {
-        return i == open_n - 1 && last.spilled ? last.spilled + in_tile * S::ROW_FLOATS
-                                               : reinterpret_cast<const float*>(states + i * S::RING_BYTES);
-      });
+      const unsigned char* end_state = last.apart ? smem + S::WARPS * S::RING_BYTES + ((final >> 1) * S::ROWS + in_tile) * (S::ROW_FLOATS * 4)
+                                                  : states + (open_n - 1) * S::RING_BYTES;
+      auto state = [&](int i) { return reinterpret_cast<const float*>(i < open_n - 1 ? states + i * S::RING_BYTES : end_state); };
+      Merged m{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f};
+#pragma unroll 2
+      for (int i = 0; i < open_n; ++i) {
+        const float2 x = *reinterpret_cast<const float2*>(state(i) + D);
+        m.ref = fmaxf(m.ref, x.x);
+        m.sum_ref = fmaxf(m.sum_ref, x.y);
+      }
+#pragma unroll 2
+      for (int i = 0; i < open_n; ++i) merge_in(m, *reinterpret_cast<const float4*>(state(i) + d), *reinterpret_cast<const float4*>(state(i) + D));
       if (complete) {
         const int64_t out = out_row(p, last.s, last.h, row);
         write_four<BF>(p, out * D + d, m);
@@ -629,11 +651,8 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
         if (d == 0) *reinterpret_cast<float4*>(at + D) = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
       }
     }
-    if (!ended && !from_before && threadIdx.x == 0) {  // the pair that starts here ends in a later CTA
-      const Pair a = locate(share((blockIdx.x + 1) * S::WARPS) - 1);
-      const int end = worker_of(a.base + a.steps - 1) / S::WARPS;
-      *reinterpret_cast<int4*>(p.links + blockIdx.x * 4) = make_int4(end, a.s, a.h, a.rt);
-    }
+    if (!ended && !from_before && threadIdx.x == 0)  // the pair that starts here ends in a later CTA
+      *reinterpret_cast<int4*>(p.links + blockIdx.x * 4) = make_int4(last.end_cta, last.s, last.h, last.rt);
   }
 }
 
@@ -682,19 +701,18 @@ template <bool BF, int D, int NT, int U> int launch_shape(AttnParams& p, int sms
   cudaGetDevice(&dev);
   if (!ready[dev & 63]) {
     const cudaError_t e = cudaFuncSetAttribute(attention_kernel<BF, D, NT, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               S::WARPS * S::RING_BYTES + (MOST_SEQS + 1) * 4);
+                                               S::SMEM_BYTES + (MOST_SEQS + 1) * 4);
     if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "ucb_block8_attention: %s", cudaGetErrorString(e));
     ready[dev & 63] = true;
   }
-  const int smem = S::WARPS * S::RING_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
+  const int smem = S::SMEM_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
   p.step_shift = (p.c.block_tokens == 16 ? 0 : p.c.block_tokens == 32 ? 1 : p.c.block_tokens == 64 ? 2 : 3) - (U - 1);
   const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
   const int64_t steps = ((entries << p.step_shift) + START) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
   if (steps > 0x3fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: too many tokens in one call");
   const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
-  p.spill = p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS;
-  p.links = reinterpret_cast<int*>(p.spill + (int64_t)CTAS_PER_SM * sms * S::WARPS * S::STATE_FLOATS);
+  p.links = reinterpret_cast<int*>(p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS);
   if (int rc = block8::launch(attention_kernel<BF, D, NT, U>, dim3(grid), dim3(S::WARPS * 32), smem, stream, p,
                               "block8 attention_kernel"))
     return rc;
@@ -723,12 +741,12 @@ template <bool BF> int launch_heads(AttnParams& p, int sms, cudaStream_t stream)
 using ucb_host::set_error;
 namespace b8 = ucb::block8;
 
-// For each CTA: states of two pairs that cross CTAs, one state for each warp, one link.
+// For each CTA: states of two pairs that cross CTAs, one link.
 extern "C" int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads) {
   if (b8::check_cache(cache, "ucb_block8_attention_workspace_bytes") || queries < 1 || q_heads < 1) return -1;
   const int64_t sms = b8::multiprocessors();
   const int64_t rows = (int64_t)q_heads / cache->kv_heads * queries > 8 ? 16 : 8;
-  return sms > 0 ? sms * b8::CTAS_PER_SM * ((2 + b8::Shape<128, 1, 1>::WARPS) * rows * (cache->head_dim + 4) * 4 + 16) : -1;
+  return sms > 0 ? sms * b8::CTAS_PER_SM * (2 * rows * (cache->head_dim + 4) * 4 + 16) : -1;
 }
 
 extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* a, void* stream) {

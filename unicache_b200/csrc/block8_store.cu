@@ -48,13 +48,18 @@ __device__ __forceinline__ bool row_range(const int32_t* starts, int s, int64_t 
   return a >= 0 && a <= e && e <= rows;
 }
 
-// The sequence whose rows hold row r (starts ascending).
+// The sequence whose rows hold row r (starts ascending), found by the whole warp: a round trip for every factor of 32
+// in the number of sequences.
 __device__ __forceinline__ int seq_of_row(const int32_t* starts, int seqs, int64_t r) {
   if (!starts) return (int)r;
-  int lo = 0, hi = seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (starts[mid] <= r) lo = mid; else hi = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = seqs;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const bool before = lane * step < n && starts[lo + lane * step] <= r;
+    const int skip = (max(__popc(__ballot_sync(0xffffffffu, before)), 1) - 1) * step;
+    lo += skip;
+    n = min(step, n - skip);
   }
   return lo;
 }
@@ -107,8 +112,11 @@ __device__ __forceinline__ float inverse_of(float scale) { return scale < INFINI
 // rows decide whether the block's scale grows: where it does not, the codes
 // of the held rows stand (they depend on the scale alone, and the scale of a
 // larger magnitude is never the smaller), and only the new rows are written.
-template <bool BF, int D, int BT>
-__device__ void write_block(const WriteParams& p, int s, int h, int64_t block, int m, int held, int64_t first_row) {
+// FRESH: a block without held rows.
+template <bool BF, int D, int BT, bool FRESH>
+__device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, int64_t block, int m, int held,
+                                            int64_t first_row) {
+  if (FRESH) held = 0;
   constexpr int UNITS = D / 8, STRIDE = THREADS / UNITS, PASSES = (BT + STRIDE - 1) / STRIDE, WARPS = THREADS / 32;
   __shared__ uint32_t warp_top[2][WARPS];
   __shared__ __align__(16) uint32_t warp_low[WARPS][D / 2], warp_high[WARPS][D / 2];
@@ -265,24 +273,25 @@ __global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(c
   }
   if (n == 0) return;
   const int first = (int)(old / bt), last = (int)((len - 1) / bt);
-  auto one = [&](int j) {
+  if (!ends) {
+    if (probe < a || probe >= e) return;
+    const int64_t j = (old + probe - a) / bt;
+    if (j <= first || (j + 1) * bt > len) return;
+    const int64_t block = pool_block(c, s, (int)j, p.err);
+    if (block >= 0) write_block<BF, D, BT, true>(p, s, h, block, bt, 0, a + j * bt - old);
+    return;
+  }
+  int j = first;
+#pragma unroll 1  // one copy of write_block
+  while (true) {
     const int64_t block = pool_block(c, s, j, p.err);
-    if (block < 0) return;
     const int64_t t0 = (int64_t)j * bt;
     const int m = (int)min((int64_t)bt, len - t0);
     const int held = (int)max((int64_t)0, min((int64_t)m, old - t0));
-    write_block<BF, D, BT>(p, s, h, block, m, held, a + t0 + held - old);
-  };
-  if (ends) {
-    one(first);
-    if (last > first && len % bt) {
-      __syncthreads();  // the pending rows of the first block are read
-      one(last);
-    }
-  } else {
-    if (probe < a || probe >= e) return;
-    const int64_t j = (old + probe - a) / bt;
-    if (j > first && (j + 1) * bt <= len) one((int)j);
+    if (block >= 0) write_block<BF, D, BT, false>(p, s, h, block, m, held, a + t0 + held - old);
+    if (j != first || last == first || len % bt == 0) break;
+    j = last;
+    __syncthreads();  // the pending rows of the first block are read
   }
 }
 
@@ -303,9 +312,12 @@ template <bool BF, int D> __global__ void __launch_bounds__(THREADS) read_kernel
   const int lane = threadIdx.x & 31, bt = c.block_tokens;
   const int64_t r0 = ((int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * READ_ROWS;
   int block = -1, in_block = 0;
+  if (r0 >= p.rows) return;
+  const int s0 = seq_of_row(p.starts, c.num_seqs, r0);
   if (lane < READ_ROWS && r0 + lane < p.rows) {
     const int64_t r = r0 + lane;
-    const int s = seq_of_row(p.starts, c.num_seqs, r);
+    int s = p.starts ? s0 : (int)r;
+    while (p.starts && s + 1 < c.num_seqs && p.starts[s + 1] <= r) ++s;
     int64_t a, e;
     const bool ok = row_range(p.starts, s, p.rows, a, e);
     const int64_t len = c.lengths[s], t = len - (e - r);
