@@ -2,6 +2,8 @@
 // position in one pass over the rows (ucb_head_norm_rope):
 //   y = x * rsqrt(mean(x^2) + eps) * w,  (a, b) -> (a c - b s, b c + a s)
 // in fp32 with one rounding.  Each row is read and written once: memory bound.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace ucb {
@@ -106,77 +108,97 @@ template <typename T> __device__ __forceinline__ void store4(T* dst, const float
 // lanes a row.  A lane holds two runs of four channels that are each
 // other's rotation partners (in the halves' form runs i and i + rotary_dim / 2), so
 // that the rotation needs no exchange and the lane four angles, which the HEADS rows
-// of one token that it has in flight share.  Measured for 16384 tokens x 32
-// heads x 128 (277 MB): 4 rows a lane 57 us (4.9 TB/s), 1 row 85, 2 rows 75,
-// 8 rows 84; 4 rows of two tokens 71; blocks of 256 threads 59.
-template <typename T, int L, int HEADS, bool PAIRS>
-__global__ void __launch_bounds__(LANES_THREADS, 1) head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units) {
-  const uint32_t unit = (blockIdx.x * (uint32_t)LANES_THREADS + threadIdx.x) / L;
+// of one token that it has in flight share.  With STREAM a group of lanes goes from
+// token to token, the next one's rows and angles in flight.  Measured for
+// 16384 tokens x 32 heads x 128 (277 MB): 53 us (5.2 TB/s) with STREAM, one token
+// a group 57; 2 rows a lane 75, 1 row 85, 8 rows 84; blocks of 256 threads 59.
+template <typename T, int L, int HEADS, bool PAIRS, bool STREAM>
+__global__ void __launch_bounds__(LANES_THREADS, 1)
+    head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units, uint32_t token_step) {
+  const uint32_t group = (blockIdx.x * (uint32_t)LANES_THREADS + threadIdx.x) / L;
   const int lane = threadIdx.x % L;
-  const uint32_t t = unit / units, u = unit - t * units;
-  const bool live = t < p.tokens, is_q = u < q_units;
+  const uint32_t t0 = group / units, u = group - t0 * units;
+  const bool is_q = u < q_units;
   const int half = p.rot / 2;
   const bool turned = lane * (PAIRS ? 8 : 4) < (PAIRS ? p.rot : half);
   const int rest = p.rot + 8 * (lane - half / 4);  // channels that are only normalised
   const int d0 = PAIRS ? 8 * lane : turned ? 4 * lane : rest, d1 = PAIRS || !turned ? d0 + 4 : d0 + half;
-  const int head0 = (is_q ? u : u - q_units) * HEADS, heads = live ? (is_q ? p.hq : p.hk) : 0;
+  const int head0 = (is_q ? u : u - q_units) * HEADS;
+  const int rows = t0 < token_step ? (is_q ? p.hq : p.hk) - head0 : 0;  // of this group; 0 past the last group
   const int64_t sh = is_q ? p.q_sh : p.k_sh, oh = is_q ? p.qo_sh : p.ko_sh;
-  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.q_st : p.k_st) + head0 * sh;
-  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.qo_st : p.ko_st) + head0 * oh;
-  const int64_t pos = p.rot && live ? position_of(p, t) : 0;
-  Four<T> raw[HEADS][2];
-#pragma unroll
-  for (int i = 0; i < HEADS; ++i)
-    if (head0 + i < heads) {
-      raw[i][0].load(src + i * sh + d0);
-      raw[i][1].load(src + i * sh + d1);
-    }
-  float w[8];
+  const int64_t st = is_q ? p.q_st : p.k_st, ot = is_q ? p.qo_st : p.ko_st;
+  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + head0 * sh;
+  T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + head0 * oh;
+  Four<T> w[2];
   const T* weight = static_cast<const T*>(is_q ? p.qw : p.kw);
-  if (weight) {
-    Four<T> a, b;
-    a.load(weight + d0);
-    b.load(weight + d1);
-    a.to(w);
-    b.to(w + 4);
-  } else {
+  if (weight) w[0].load(weight + d0), w[1].load(weight + d1);
+
+  struct Ahead {
+    Four<T> raw[HEADS][2];
+    float4 c, s;
+    bool bad;
+  };
+  auto position = [&](uint32_t t) { return p.rot && t < p.tokens ? position_of(p, t) : 0; };
+  auto fetch = [&](uint32_t t, int64_t pos) {
+    Ahead a;
+    a.bad = false;
+    if (t >= p.tokens) return a;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = 1.f;
-  }
-  float c[4], s[4];
-  const bool bad = p.rot && live && (pos < 0 || pos >= p.table_rows);
-  if (bad && lane == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-  if (turned) {
-    const int64_t at = (bad ? 0 : pos) * half + 4 * lane;
-    const float4 cv = *reinterpret_cast<const float4*>(p.cos + at), sv = *reinterpret_cast<const float4*>(p.sin + at);
-    c[0] = cv.x, c[1] = cv.y, c[2] = cv.z, c[3] = cv.w;
-    s[0] = sv.x, s[1] = sv.y, s[2] = sv.z, s[3] = sv.w;
-  }
-#pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    float x[8], ss = 0.f;
-    raw[i][0].to(x);
-    raw[i][1].to(x + 4);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = bad ? __int_as_float(0x7fffffff) : rsqrtf(ss * (1.f / (8 * L)) + p.eps);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = x[k] * r * w[k];
+    for (int i = 0; i < HEADS; ++i)
+      if (i < rows) {
+        a.raw[i][0].load(src + t * st + i * sh + d0);
+        a.raw[i][1].load(src + t * st + i * sh + d1);
+      }
+    a.bad = p.rot && (pos < 0 || pos >= p.table_rows);
     if (turned) {
+      const int64_t at = (a.bad ? 0 : pos) * half + 4 * lane;
+      a.c = *reinterpret_cast<const float4*>(p.cos + at);
+      a.s = *reinterpret_cast<const float4*>(p.sin + at);
+    }
+    return a;
+  };
+  uint32_t t = t0;
+  Ahead next = fetch(t, position(t));
+  int64_t pos = STREAM ? position(t + token_step) : 0;
+#pragma unroll 1
+  while (t < p.tokens) {
+    const Ahead now = next;
+    if (STREAM) {
+      next = fetch(t + token_step, pos);
+      pos = position(t + 2 * token_step);
+    }
+    if (now.bad && lane == 0 && rows > 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+    const float c[4] = {now.c.x, now.c.y, now.c.z, now.c.w}, s[4] = {now.s.x, now.s.y, now.s.z, now.s.w};
+    float wf[8];
+    if (weight) w[0].to(wf), w[1].to(wf + 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int first = PAIRS ? 2 * k : k, other = PAIRS ? 2 * k + 1 : k + 4;
-        const float a = x[first], b = x[other];
-        x[first] = fmaf(a, c[k], -b * s[k]);
-        x[other] = fmaf(b, c[k], a * s[k]);
+    for (int i = 0; i < HEADS; ++i) {
+      float x[8], ss = 0.f;
+      now.raw[i][0].to(x);
+      now.raw[i][1].to(x + 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, L);
+      const float r = now.bad ? __int_as_float(0x7fffffff) : rsqrtf(ss * (1.f / (8 * L)) + p.eps);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = weight ? x[k] * r * wf[k] : x[k] * r;
+      if (turned) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int first = PAIRS ? 2 * k : k, other = PAIRS ? 2 * k + 1 : k + 4;
+          const float a = x[first], b = x[other];
+          x[first] = fmaf(a, c[k], -b * s[k]);
+          x[other] = fmaf(b, c[k], a * s[k]);
+        }
+      }
+      if (i < rows) {
+        store4(dst + t * ot + i * oh + d0, x);
+        store4(dst + t * ot + i * oh + d1, x + 4);
       }
     }
-    if (head0 + i < heads) {
-      store4(dst + i * oh + d0, x);
-      store4(dst + i * oh + d1, x + 4);
-    }
+    if (!STREAM) break;
+    t += token_step;
   }
 }
 
@@ -185,21 +207,33 @@ template <typename T> bool aligned(const void* x, int64_t st, int64_t sh) {
   return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 && st % 4 == 0 && sh % 4 == 0;
 }
 
-template <typename T, int L, int HEADS> int launch_lanes(const HeadNormParams& p, cudaStream_t s) {
-  const int q_units = (p.hq + HEADS - 1) / HEADS, units = q_units + (p.hk + HEADS - 1) / HEADS;
-  const unsigned blocks = (unsigned)((p.tokens * units * L + LANES_THREADS - 1) / LANES_THREADS);
-  if (p.interleaved)
-    head_norm_lanes_kernel<T, L, HEADS, true><<<blocks, LANES_THREADS, 0, s>>>(p, q_units, units);
-  else
-    head_norm_lanes_kernel<T, L, HEADS, false><<<blocks, LANES_THREADS, 0, s>>>(p, q_units, units);
+template <typename T, int L, int HEADS, bool STREAM> int launch_lanes(const HeadNormParams& p, cudaStream_t s) {
+  const uint32_t q_units = (p.hq + HEADS - 1) / HEADS, units = q_units + (p.hk + HEADS - 1) / HEADS;
+  const auto kernel = p.interleaved ? head_norm_lanes_kernel<T, L, HEADS, true, STREAM>
+                                    : head_norm_lanes_kernel<T, L, HEADS, false, STREAM>;
+  uint32_t step = (uint32_t)p.tokens;  // tokens that are worked on at once
+  if (STREAM) {  // as many as are resident, in equal turns
+    static int resident[2] = {0, 0};
+    int& ctas = resident[p.interleaved != 0];
+    if (ctas == 0 && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, LANES_THREADS, 0) != cudaSuccess)
+      return ucb_host::check_launch("head_norm_lanes_kernel");
+    const int64_t most = std::max<int64_t>(1, (int64_t)ctas * 148 * (LANES_THREADS / L) / units);
+    const int64_t turns = (p.tokens + most - 1) / most;
+    step = (uint32_t)((p.tokens + turns - 1) / turns);
+  }
+  const unsigned blocks = (unsigned)(((int64_t)step * units * L + LANES_THREADS - 1) / LANES_THREADS);
+  kernel<<<blocks, LANES_THREADS, 0, s>>>(p, q_units, units, step);
   return ucb_host::check_launch("head_norm_lanes_kernel");
 }
 
 template <typename T, int L> int launch_heads(const HeadNormParams& p, cudaStream_t s) {
   // Four rows a lane once one row a lane would fill the chip's threads (4999 tokens x 18 heads x 64: 5.8 us against
-  // 7.6 with one row; below that, one row has the shorter way).
-  if (p.tokens * (p.hq + p.hk) * L >= 148 * 2048) return launch_lanes<T, L, 4>(p, s);
-  return launch_lanes<T, L, 1>(p, s);
+  // 7.6 with one row; below that, one row has the shorter way); from token to token once that makes several turns
+  // (where it makes two or three, 6.8 us for the same case).
+  const int64_t lanes = p.tokens * (p.hq + p.hk) * L;
+  if (lanes >= 148 * 2048 * 8) return launch_lanes<T, L, 4, true>(p, s);
+  if (lanes >= 148 * 2048) return launch_lanes<T, L, 4, false>(p, s);
+  return launch_lanes<T, L, 1, false>(p, s);
 }
 
 template <typename T> int launch(const HeadNormParams& p, cudaStream_t s) {
