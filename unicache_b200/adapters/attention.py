@@ -279,5 +279,4 @@ def sparse_int8_block_decode(query: torch.Tensor, cache: Int8BlockCache, *, coun
     """Attention of query [num_seqs, q_heads, head_dim] over ``count`` blocks of each sequence and KV
     head (``Int8BlockCache.select``): (blocks, out, lse)."""
 
-    blocks = kernels.block8_select(query, cache, count=count, first=first, recent=recent)
-    return (blocks, *kernels.block8_attention(query, cache, blocks=blocks, softmax_scale=softmax_scale))
+    return kernels.block8_sparse_attention(query, cache, count=count, first=first, recent=recent, softmax_scale=softmax_scale)

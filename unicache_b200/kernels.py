@@ -1338,6 +1338,26 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
     [S, Hq, D] or [S, L, Hq, D] -> (out like query, lse fp32 of its leading dimensions)."""
 
     shape, stride = _block8_query(cache, query)
+    if blocks is not None:
+        listed = blocks.shape
+        if blocks.get_device() != cache.index or blocks.dtype is not torch.int32 or len(listed) != 3 \
+                or listed[0] != cache.num_seqs or listed[1] != cache.num_kv_heads \
+                or listed[2] < 1 or not blocks.is_contiguous():
+            raise ValueError("blocks must be a contiguous int32 [num_seqs, kv_heads, count] tensor on the cache's device")
+    return _block8_attend(query, cache, shape, stride, blocks, softmax_scale)
+
+
+def block8_sparse_attention(query: torch.Tensor, cache, *, count: int, first: int = 1, recent: int = 2,
+                            softmax_scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``block8_select``, then ``block8_attention`` over what it chose: (blocks, out, lse)."""
+
+    blocks = block8_select(query, cache, count=count, first=first, recent=recent)
+    return (blocks, *_block8_attend(query, cache, query.shape, query.stride(), blocks, softmax_scale))
+
+
+def _block8_attend(query, cache, shape, stride, blocks, softmax_scale):
+    """The attention launches of a checked query and selection."""
+
     if len(shape) == 3:
         queries, query_stride = 1, 0
     elif len(shape) == 4:
@@ -1347,24 +1367,18 @@ def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None 
     if not 1 <= queries <= 16:
         raise ValueError("the block cache attention takes 1 to 16 query tokens a sequence; read the cache back and "
                          "use long_query_attention_summary for more")
-    selected = at = 0
-    if blocks is not None:
-        listed = blocks.shape
-        if blocks.get_device() != cache.index or blocks.dtype is not torch.int32 or len(listed) != 3 \
-                or listed[0] != cache.num_seqs or listed[1] != cache.num_kv_heads \
-                or listed[2] < 1 or not blocks.is_contiguous():
-            raise ValueError("blocks must be a contiguous int32 [num_seqs, kv_heads, count] tensor on the cache's device")
-        selected, at = listed[2], blocks.data_ptr()
     q_heads = shape[-2]
     scale = cache.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if query.data_ptr() & 7 or (stride[0] | query_stride | stride[-2]) & 3:  # the kernel reads rows 8 bytes at a time
-        query = query.clone(memory_format=torch.contiguous_format)
-        stride = query.stride()
+    address, contiguous = query.data_ptr(), query.is_contiguous()
+    if address & 7 or (stride[0] | query_stride | stride[-2]) & 3:  # the kernel reads rows 8 bytes at a time
+        query, contiguous = query.clone(memory_format=torch.contiguous_format), True
+        address, stride = query.data_ptr(), query.stride()
         query_stride = stride[1] if len(shape) == 4 else 0
-    out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(shape)
+    out = torch.empty_like(query) if contiguous else query.new_empty(shape)
     lse = cache.key_scale.new_empty(shape[:-1])
     workspace = cache.attention_workspace(queries, q_heads)
-    args = _capi.BLOCK8_ATTENTION_ARGS.pack(query.data_ptr(), at, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
+    selected, at = (0, 0) if blocks is None else (blocks.shape[2], blocks.data_ptr())
+    args = _capi.BLOCK8_ATTENTION_ARGS.pack(address, at, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
                                             stride[0], query_stride, stride[-2], queries, q_heads, selected, scale)
     _call_on(cache.index, "ucb_block8_attention", cache.descriptor, args, stream_of(query))
     return out, lse
