@@ -643,7 +643,8 @@ UCB_API int ucb_block8_write(const ucb_block8_cache* cache, const void* key_dev,
                              int64_t value_stride_head, int64_t rows, const int32_t* starts_dev, void* stream);
 
 /* The restored last rows of every sequence (as above) in dtype, contiguous
- * [rows, kv_heads, head_dim]. */
+ * [rows, kv_heads, head_dim], 16-byte aligned; a row that a write would
+ * refuse is NaN and sets device error bit 2. */
 UCB_API int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, const int32_t* starts_dev, void* key_out_dev,
                             void* value_out_dev, void* stream);
 
@@ -665,8 +666,9 @@ UCB_API int ucb_block8_select(const ucb_block8_cache* cache, const void* query_d
  * contiguous, 1 <= queries <= 16) over the cache: query i of a sequence is its
  * token lengths[s] - queries + i and sees the tokens up to itself (none: output
  * 0, LSE -inf).  blocks int32 [num_seqs, kv_heads, num_selected] limits it
- * to the tokens of these blocks (negative entries are skipped, no block may
- * be named twice); NULL = all.  out [num_seqs, queries, q_heads, head_dim] in
+ * to the tokens of these blocks (entries that are negative or past the
+ * sequence are skipped, no block may be named twice); NULL = all.  A table
+ * entry outside the pool is skipped and sets device error bit 2.  out [num_seqs, queries, q_heads, head_dim] in
  * dtype, lse fp32 [num_seqs, queries, q_heads] natural log (or NULL).
  * Query rows start on 8 bytes.  workspace: ucb_block8_attention_workspace_bytes
  * bytes; it and out 16-byte aligned. */

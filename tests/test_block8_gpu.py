@@ -241,8 +241,9 @@ def test_bad_tables_lengths_and_starts_are_flagged_and_write_nothing():
             assert kernels.device_status() & 2
             cache.select(query, count=4)
             assert kernels.device_status() & 2
-            cache.read(3)
+            key, value = cache.read(3)
             assert kernels.device_status() & 2
+            assert key[1].isnan().all() and value[1].isnan().all() and key[[0, 2]].isfinite().all()
     assert kernels.device_status() == 0
 
 

@@ -67,12 +67,13 @@ constexpr float LIFT = 6.f;   // log2 of the largest weight when its reference i
 constexpr float LAZY = 14.f;  // a weight may reach 2^LAZY before its reference moves
 constexpr float LAZY_SUM = 100.f;
 
-// U tiles of 16 tokens a step, two CTAs a multiprocessor.
-template <int D, int NT, int U> struct Shape {
+// U tiles of 16 tokens a step.  OWN: a CTA has one pair to itself, all of a multiprocessor's registers and no second
+// kernel after it; else two CTAs a multiprocessor.
+template <int D, int NT, int U, bool OWN> struct Shape {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int WARPS = NT == 1 ? 8 : D == 64 ? 6 : 4;
+  static constexpr int WARPS = OWN || NT == 1 ? 8 : D == 64 ? 6 : 4;
   static constexpr int STEP_BYTES = U * 2 * TILE * D;
-  static constexpr int STAGES = 65536 / (WARPS * STEP_BYTES);
+  static constexpr int STAGES = (OWN ? 131072 : 65536) / (WARPS * STEP_BYTES);
   static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its reference, the sum's reference, the sum
   static constexpr int STATE_FLOATS = ROWS * ROW_FLOATS;
   static constexpr int RING_BYTES = STAGES * STEP_BYTES;
@@ -179,9 +180,9 @@ template <bool BF> __device__ __forceinline__ void write_four(const AttnParams& 
       make_uint2(pack_out<BF>(m.value.x * f, m.value.y * f), pack_out<BF>(m.value.z * f, m.value.w * f));
 }
 
-template <bool BF, int D, int NT, int U>
-__global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kernel(const AttnParams p) {
-  using S = Shape<D, NT, U>;
+template <bool BF, int D, int NT, int U, bool OWN>
+__global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2) attention_kernel(const AttnParams p) {
+  using S = Shape<D, NT, U, OWN>;
   constexpr int MT = D / 16;          // value products of 16 channels
   constexpr int KS = D / 16;          // key products of 16 channels
   constexpr int VB = D / 8;           // bytes of a value row that a lane holds
@@ -197,15 +198,20 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
 
   // ---- the flat order: steps of every sequence (at least one, so that every row is written)
   int total;
-  const int listed_steps = (p.selected << p.step_shift) + START;
-  if (p.blocks) {
+  const int start = OWN ? 0 : START;
+  const int listed_steps = (p.selected << p.step_shift) + start;
+  auto steps_of = [&](int s) { return max(1, (held_tokens(c, s, p.err) + STEP - 1) / STEP) + start; };
+  const int own_s = divide(blockIdx.x, heads_rows, p.heads_rows_magic);
+  if (OWN) {
+    total = p.blocks ? listed_steps : steps_of(own_s);
+  } else if (p.blocks) {
     total = c.num_seqs * listed_steps * heads_rows;
   } else {
     int carry = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int base = 0; base < c.num_seqs; base += S::WARPS * 32) {
       const int i = base + threadIdx.x;
-      int v = i < c.num_seqs ? max(1, (held_tokens(c, i, p.err) + STEP - 1) / STEP) + START : 0;
+      int v = i < c.num_seqs ? steps_of(i) : 0;
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
@@ -222,10 +228,10 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
     }
     total = carry * heads_rows;
   }
-  const int worker = blockIdx.x * S::WARPS + warp;
+  const int worker = OWN ? warp : blockIdx.x * S::WARPS + warp;
   if (lane == 0) segments[warp][0].used = segments[warp][1].used = 0;
   // equal shares, the first `longer` of one step more
-  const int workers = max(1, min((int)gridDim.x * S::WARPS, total / MIN_STEPS));
+  const int workers = max(1, min(OWN ? S::WARPS : (int)gridDim.x * S::WARPS, total / MIN_STEPS));
   const int each = total / workers, longer = total - each * workers;
   auto share = [&](int w) { return w < workers ? w * each + min(w, longer) : total; };
   auto worker_of = [&](int step) {
@@ -236,6 +242,11 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
     Pair a;
     const int unit = divide(t, heads_rows, p.heads_rows_magic);
     int first;
+    if (OWN) {
+      const int u = blockIdx.x - own_s * heads_rows;
+      a.h = divide(u, p.row_tiles, p.row_tiles_magic);
+      return Pair{own_s, a.h, u - a.h * p.row_tiles, total, 0};
+    }
     if (p.blocks) {
       a.s = unit / listed_steps;
       a.steps = listed_steps;
@@ -273,8 +284,8 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   const int t_end = share(worker + 1);
   while (t < t_end) {
     const Pair a = locate(t);
-    const int begin = max(t - a.base - START, 0), end = min(a.steps, t_end - a.base) - START, steps = a.steps - START;
-    t = a.base + end + START;
+    const int begin = max(t - a.base - start, 0), end = min(a.steps, t_end - a.base) - start, steps = a.steps - start;
+    t = a.base + end + start;
     if (end <= 0) continue;  // the rest of the pair's start: its tiles are the next warp's
     const int len = held_tokens(c, a.s, p.err);
     const int32_t* list = p.blocks ? p.blocks + ((int64_t)a.s * c.kv_heads + a.h) * p.selected : nullptr;
@@ -354,6 +365,16 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
       }
       cp_async_commit();
     };
+    // After step i, whose slot every lane has read: the step STAGES after it goes into that slot, and step i + 1 is waited
+    // for.  Where all warps stream, one slot less is in flight: that uses the bandwidth up, and a deeper queue only makes
+    // every first access wait (172 us against 187 for a gigabyte).  A pair on its own waits for round trips.
+    auto advance = [&](int i) {
+      __syncwarp();
+      if (!OWN) cp_async_wait<S::STAGES - 2>();
+      issue(i + S::STAGES);
+      if (OWN) cp_async_wait<S::STAGES - 1>();
+      __syncwarp();  // the other lanes' copies
+    };
 #pragma unroll 1
     for (int x = 0; x < S::STAGES - 1; ++x) issue(begin + x);
     fetch_scales(now);
@@ -408,7 +429,9 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
         for (int k = 0; k < 4; ++k) o[nt][j][k] = 0.f;
     }
 
-    for (int i = begin; i < end; ++i) {
+#pragma unroll 1
+    for (int i = begin - 1; i < end; advance(i++)) {
+      if (i < begin) continue;
       const int entry = i >> p.step_shift;
       if (entry - window >= 32) {
         if (!next_scaled) fetch_scales(next);
@@ -421,9 +444,6 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
         fetch_scales(next);
         next_scaled = true;
       }
-      cp_async_wait<S::STAGES - 2>();
-      __syncwarp();              // the other lanes' copies of step i, and their reads of the step before
-      issue(i + S::STAGES - 1);  // into the slot of the step before
       const int rel = entry - window;
       const int block = __shfl_sync(0xffffffffu, now.block, rel);
       const int first_token = __shfl_sync(0xffffffffu, now.token, rel) + (i & step_mask) * STEP;
@@ -605,12 +625,12 @@ __global__ void __launch_bounds__(Shape<D, NT, U>::WARPS * 32, 2) attention_kern
   }
   __syncthreads();
 
-  launch_dependents();
+  if (!OWN) launch_dependents();
 
   // ---- chains of segments of one pair: complete ones are written, the CTA's first and last may go on
   // in other CTAs.  A warp's slot 0 continues the pair that was open before it, slot 1 opens one; a state outside
   // the rings ends its chain, since its warp went on to another pair.
-  if (threadIdx.x == 0) p.links[blockIdx.x * 4] = -1;
+  if (threadIdx.x == 0 && !OWN) p.links[blockIdx.x * 4] = -1;
   const Segment& mine = segments[min(lane, 2 * S::WARPS - 1) >> 1][lane & 1];
   unsigned used = __ballot_sync(0xffffffffu, lane < 2 * S::WARPS && mine.used);
   while (used) {  // a chain: the segments up to the next one that opens a pair
@@ -663,7 +683,7 @@ constexpr int MERGE_GROUPS = 4;
 
 template <bool BF, int D, int NT, int U>
 __global__ void __launch_bounds__(MERGE_GROUPS * D / 4) attention_merge_kernel(const AttnParams p) {
-  using S = Shape<D, NT, U>;
+  using S = Shape<D, NT, U, false>;
   __shared__ float groups[MERGE_GROUPS][D + 4];
   wait_for_primary();
   const int4 link = *reinterpret_cast<const int4*>(p.links + blockIdx.x * 4);
@@ -694,39 +714,54 @@ int multiprocessors() {
 
 constexpr int MOST_SEQS = 4096;
 
-template <bool BF, int D, int NT, int U> int launch_shape(AttnParams& p, int sms, cudaStream_t stream) {
-  using S = Shape<D, NT, U>;
+template <bool BF, int D, int NT, int U, bool OWN> int launch_shape(AttnParams& p, int sms, cudaStream_t stream) {
+  using S = Shape<D, NT, U, OWN>;
   static bool ready[64] = {false};  // the attribute is a device's; setting it twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
   if (!ready[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_kernel<BF, D, NT, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               S::SMEM_BYTES + (MOST_SEQS + 1) * 4);
+    const cudaError_t e = cudaFuncSetAttribute(attention_kernel<BF, D, NT, U, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               S::SMEM_BYTES + (OWN ? 0 : (MOST_SEQS + 1) * 4));
     if (e != cudaSuccess) return ucb_host::set_error(UCB_ERR_CUDA, "ucb_block8_attention: %s", cudaGetErrorString(e));
     ready[dev & 63] = true;
   }
-  const int smem = S::SMEM_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
   p.step_shift = (p.c.block_tokens == 16 ? 0 : p.c.block_tokens == 32 ? 1 : p.c.block_tokens == 64 ? 2 : 3) - (U - 1);
-  const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
-  const int64_t steps = ((entries << p.step_shift) + START) * p.c.num_seqs * p.c.kv_heads * p.row_tiles;
-  if (steps > 0x3fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: too many tokens in one call");
-  const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
-  p.links = reinterpret_cast<int*>(p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS);
-  if (int rc = block8::launch(attention_kernel<BF, D, NT, U>, dim3(grid), dim3(S::WARPS * 32), smem, stream, p,
-                              "block8 attention_kernel"))
-    return rc;
-  return block8::launch(attention_merge_kernel<BF, D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), 0, stream, p,
-                        "block8 attention_merge_kernel", 1, true);
+  const int64_t pairs = (int64_t)p.c.num_seqs * p.heads_rows;
+  if constexpr (OWN) {
+    return block8::launch(attention_kernel<BF, D, NT, U, true>, dim3((unsigned)pairs), dim3(S::WARPS * 32), S::SMEM_BYTES,
+                          stream, p, "block8 attention_kernel");
+  } else {
+    const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
+    const int64_t steps = ((entries << p.step_shift) + START) * pairs;
+    if (steps > 0x3fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: too many tokens in one call");
+    const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
+    p.links = reinterpret_cast<int*>(p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS);
+    const int smem = S::SMEM_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
+    if (int rc = block8::launch(attention_kernel<BF, D, NT, U, false>, dim3(grid), dim3(S::WARPS * 32), smem, stream, p,
+                                "block8 attention_kernel"))
+      return rc;
+    return block8::launch(attention_merge_kernel<BF, D, NT, U>, dim3(grid, S::ROWS), dim3(MERGE_GROUPS * D / 4), 0, stream, p,
+                          "block8 attention_merge_kernel", 1, true);
+  }
 }
 
+// Tokens of capacity up to which a pair is one CTA's, where all are resident: one launch and no merge.  Device time with
+// and without: 18 x 1000 tokens x 8 heads 12.4 and 16.4 us, 8 x 1000 x 4 10.9 and 10.6, one of 100 x 4 4.9 and 7.8, one of
+// 700 9.2 and 8.6, one of 1000 10.9 and 8.6; the second launch costs the host 2.4 us (12.2 and 14.6 a call).
+constexpr int OWN_TOKENS = 1024;
+
 template <bool BF, int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
+  const int64_t tokens = (int64_t)(p.blocks ? p.selected : p.c.max_blocks) * p.c.block_tokens;
+  const bool own = tokens <= OWN_TOKENS && (int64_t)p.c.num_seqs * p.heads_rows <= sms;
+  const bool pairs = p.c.block_tokens > TILE;
+  if (own) return pairs ? launch_shape<BF, D, NT, 2, true>(p, sms, stream) : launch_shape<BF, D, NT, 1, true>(p, sms, stream);
   // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 76 us
   // against 96) and for 16 rows (eight of 5003 tokens, four queries each: 23.4 against 25.4).
   if constexpr (D == 64 || NT == 2) {
-    if (p.c.block_tokens > TILE) return launch_shape<BF, D, NT, 2>(p, sms, stream);
+    if (pairs) return launch_shape<BF, D, NT, 2, false>(p, sms, stream);
   }
-  return launch_shape<BF, D, NT, 1>(p, sms, stream);
+  return launch_shape<BF, D, NT, 1, false>(p, sms, stream);
 }
 
 template <bool BF> int launch_heads(AttnParams& p, int sms, cudaStream_t stream) {

@@ -351,10 +351,10 @@ template <bool BF, int D> __global__ void __launch_bounds__(THREADS) read_kernel
       }
 #pragma unroll
     for (int k = 0; k < READ_ROWS; ++k) {
-      if (where[k] < 0) continue;
-      uint32_t y[4];
+      if (r0 + k >= p.rows) continue;
+      uint32_t y[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // NaN where the row is in no block
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4 && where[k] >= 0; ++j) {
         const uint32_t two = (j < 2 ? q[k].x : q[k].y) >> (j % 2 * 16);
         const float x0 = (float)(int)(signed char)(two & 255) * scale[k], x1 = (float)(int)(signed char)(two >> 8 & 255) * scale[k];
         y[j] = BF ? pack_bf16x2(x0, x1) : pack_f16x2(x0, x1);
