@@ -686,6 +686,11 @@ typedef struct ucb_block8_attention_args {
 } ucb_block8_attention_args;
 UCB_API int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* args, void* stream);
 
+/* ucb_block8_select of args->num_selected blocks into args->blocks (written in
+ * this call), then ucb_block8_attention over them; one query token. */
+UCB_API int ucb_block8_sparse_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* args, int first,
+                                        int recent, void* select_workspace_dev, void* stream);
+
 /* ------------------------------------------------------------------ self test
  * Checks on the current device that mma.sync f16 consumes fp16 subnormal
  * operands exactly (the decode kernel feeds small integer codes as subnormals).

@@ -64,7 +64,9 @@ def test_bad_caches_are_refused_by_every_entry(changes, message):
     for rc in (lib.ucb_block8_write(cache, one, 512, 128, one, 512, 128, 2, None, None),
                lib.ucb_block8_read(cache, 2, None, one, one, None),
                lib.ucb_block8_select(cache, one, 3584, 128, 28, 4, 1, 2, one, None, None),
-               lib.ucb_block8_attention(cache, args, None)):
+               lib.ucb_block8_attention(cache, args, None),
+               lib.ucb_block8_sparse_attention(cache, _capi.BLOCK8_ATTENTION_ARGS.pack(
+                   4096, 4096, 4096, 4096, 4096, 3584, 0, 128, 1, 28, 4, 0.1), 1, 2, None, None)):
         assert rc in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED)
         assert message in lib.ucb_last_error().decode()
     assert lib.ucb_block8_select_workspace_bytes(cache) == -1
@@ -93,6 +95,10 @@ def test_bad_selections_and_rows_are_refused():
                                                    (28, 4, 3, 2, "count"), (28, 4, -1, 2, "count"),
                                                    (28, 5000, 1, 2, "4096 blocks")):
         rc = lib.ucb_block8_select(cache, one, 3584, 128, q_heads, count, first, recent, one, None, None)
+        assert rc in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED) and message in lib.ucb_last_error().decode()
+    for blocks, queries, count, message in ((0, 1, 4, "null pointer"), (4096, 2, 4, "one query"), (4096, 1, 2, "count")):
+        args = _capi.BLOCK8_ATTENTION_ARGS.pack(4096, blocks, 4096, 4096, 4096, 3584, 0, 128, queries, 28, count, 0.1)
+        rc = lib.ucb_block8_sparse_attention(cache, args, 1, 2, None, None)
         assert rc in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED) and message in lib.ucb_last_error().decode()
     assert lib.ucb_block8_write(cache, one, 512, 128, one, 512, 128, 3, None, None) == _capi.UCB_ERR_INVALID
     assert lib.ucb_block8_write(cache, None, 512, 128, one, 512, 128, 2, None, None) == _capi.UCB_ERR_INVALID

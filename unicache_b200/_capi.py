@@ -196,6 +196,7 @@ SIGNATURES = {
                                   c_void_p, c_void_p]),
     "ucb_block8_attention_workspace_bytes": (c_int64, [c_void_p, c_int, c_int]),
     "ucb_block8_attention": (c_int, [c_void_p, ctypes.c_char_p, c_void_p]),
+    "ucb_block8_sparse_attention": (c_int, [c_void_p, ctypes.c_char_p, c_int, c_int, c_void_p, c_void_p]),
     "ucb_selftest_mma_subnormal": (c_int, [ctypes.POINTER(c_float), c_void_p]),
     "ucb_host_device_pointer": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "ucb_copy_ranges": (c_int, [c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64),

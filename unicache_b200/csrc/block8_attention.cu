@@ -34,6 +34,12 @@
 // reference moves): every contribution to the output above 2^-20 of the largest
 // keeps 11 bits, whatever the blocks' scales are.  The sum of weights is kept
 // in fp32 against a reference of its own.
+//
+// Measured (B200, device): 1.07 GB of codes (32 x 32768 tokens, 4 KV heads of
+// 128) in 172-175 us, 6.2 TB/s, 95% of the copy rate (194 us over 0.15 s,
+// where the card is at its power cap); 135 MB in 33 us, of which the stream
+// takes 18; 404 MB at head_dim 64 in 74 us (483 instructions a step of 16 tokens
+// and half the bytes); one sequence of 700 tokens 9.1 us.
 #include <algorithm>
 
 #include "block8.cuh"
@@ -822,4 +828,15 @@ extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_blo
   p.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return cache->dtype == UCB_BF16 ? b8::launch_heads<true>(p, sms, s) : b8::launch_heads<false>(p, sms, s);
+}
+
+extern "C" int ucb_block8_sparse_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* a, int first,
+                                           int recent, void* select_workspace, void* stream) {
+  if (!a || !a->blocks) return set_error(UCB_ERR_INVALID, "ucb_block8_sparse_attention: null pointer");
+  if (a->queries != 1)
+    return set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_sparse_attention: one query token chooses blocks");
+  if (int rc = ucb_block8_select(cache, a->query, a->q_stride_seq, a->q_stride_head, a->q_heads, a->num_selected, first,
+                                 recent, const_cast<int32_t*>(a->blocks), select_workspace, stream))
+    return rc;
+  return ucb_block8_attention(cache, a, stream);
 }

