@@ -1302,7 +1302,7 @@ def block8_read(cache, rows: int, starts: torch.Tensor | None = None) -> tuple[t
 
     at = _block8_starts(cache, rows, starts)
     shape = (rows, cache.num_kv_heads, cache.head_dim)
-    key, value = cache.pending_key.new_empty(shape), cache.pending_key.new_empty(shape)
+    key, value = cache.empty(cache.dtype, shape), cache.empty(cache.dtype, shape)
     _call_on(cache.index, "ucb_block8_read", cache.descriptor, rows, at, key.data_ptr(), value.data_ptr(),
              stream_of(cache.lengths))
     return key, value

@@ -211,11 +211,13 @@ class Int8BlockCache:
         return self.key_code.new_empty(size)
 
     def empty(self, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
-        """An uninitialised tensor of a launch's output; one element per shape seen serves as its pattern (0.6 us a call
-        less than naming type and device)."""
+        """An uninitialised tensor of a launch's output, by the pattern of one expanded element (0.6 us a call less than
+        naming type and device)."""
 
         pattern = self._shapes.get((dtype, shape))
         if pattern is None:
+            if len(self._shapes) >= 64:
+                self._shapes.clear()
             pattern = self._shapes[(dtype, shape)] = torch.empty(1, device=self.device, dtype=dtype).expand(shape)
         return torch.empty_like(pattern, memory_format=torch.contiguous_format)
 
