@@ -17,7 +17,7 @@
 // a second small kernel.
 //
 // Loads: every warp copies its own steps by cp.async, whole 128-byte lines an instruction,
-// into a private ring of shared memory: a deep queue without barriers.  The
+// into a private ring of shared memory, without barriers.  The
 // order of channels within a product of 16 (and of tokens) is free as long as both
 // operands have it, so the fragments are 16-byte units of the pool's rows:
 // key lane (r, c) reads units c and c + 4 of tokens r and r + 8, value lane
@@ -36,7 +36,7 @@
 // in fp32 against a reference of its own.
 //
 // Measured (B200, device): 1.07 GB of codes (32 x 32768 tokens, 4 KV heads of
-// 128) in 172-175 us, 6.2 TB/s, 95% of the copy rate (194 us over 0.15 s,
+// 128) in 173-176 us, 6.2 TB/s, 95% of the copy rate (194 us over 0.15 s,
 // where the card is at its power cap); 135 MB in 33 us, of which the stream
 // takes 18; 404 MB at head_dim 64 in 74 us (483 instructions a step of 16 tokens
 // and half the bytes); one sequence of 700 tokens 9.1 us.
@@ -65,13 +65,15 @@ struct AttnParams {
   unsigned int* err;
 };
 
-constexpr int TILE = 16;     // tokens of one matrix product
-constexpr int START = 4;      // steps that the start of a pair costs a warp, in the flat order
-constexpr int MIN_STEPS = 1;  // a warp's least share, where there is more than that
+constexpr int TILE = 16;  // tokens of one matrix product
+// Steps that the start of a pair costs a warp, in the flat order.  Device time with 0, 2, 4 and 8 of them: 8 sequences of up
+// to 5003 tokens x 4 queries 29.9, 20.4, 20.4 and 20.6 us; 48 of 1 to 16384 tokens 84.5, 75.5, 74.4 and 75.3; 32 equal
+// ones 35.1, 33.3, 32.9 and 32.7; one length of 131072 tokens 176, 173, 173 and 174.
+constexpr int START = 4;
 constexpr int CTAS_PER_SM = 2;
-constexpr float LIFT = 6.f;   // log2 of the largest weight when its reference is set
-constexpr float LAZY = 14.f;  // a weight may reach 2^LAZY before its reference moves
-constexpr float LAZY_SUM = 100.f;
+constexpr float LIFT = 6.f;        // log2 of the largest weight when its reference is set
+constexpr float LAZY = 14.f;       // a weight may reach 2^LAZY before its reference moves
+constexpr float LAZY_SUM = 100.f;  // the same of the fp32 sum
 
 // U tiles of 16 tokens a step.  OWN: a CTA has one pair to itself, all of a multiprocessor's registers and no second
 // kernel after it; else two CTAs a multiprocessor.
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
   const int worker = OWN ? warp : blockIdx.x * S::WARPS + warp;
   if (lane == 0) segments[warp][0].used = segments[warp][1].used = 0;
   // equal shares, the first `longer` of one step more
-  const int workers = max(1, min(OWN ? S::WARPS : (int)gridDim.x * S::WARPS, total / MIN_STEPS));
+  const int workers = max(1, min(OWN ? S::WARPS : (int)gridDim.x * S::WARPS, total));
   const int each = total / workers, longer = total - each * workers;
   auto share = [&](int w) { return w < workers ? w * each + min(w, longer) : total; };
   auto worker_of = [&](int step) {
@@ -740,7 +742,7 @@ template <bool BF, int D, int NT, int U, bool OWN> int launch_shape(AttnParams& 
     const int64_t entries = p.blocks ? p.selected : p.c.max_blocks;
     const int64_t steps = ((entries << p.step_shift) + START) * pairs;
     if (steps > 0x3fffffff) return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "ucb_block8_attention: too many tokens in one call");
-    const int64_t wanted = (steps + S::WARPS * MIN_STEPS - 1) / (S::WARPS * MIN_STEPS);
+    const int64_t wanted = (steps + S::WARPS - 1) / S::WARPS;
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(CTAS_PER_SM * sms, wanted));
     p.links = reinterpret_cast<int*>(p.partials + (int64_t)CTAS_PER_SM * sms * 2 * S::STATE_FLOATS);
     const int smem = S::SMEM_BYTES + (p.blocks ? 0 : (p.c.num_seqs + 1) * 4);
@@ -753,8 +755,9 @@ template <bool BF, int D, int NT, int U, bool OWN> int launch_shape(AttnParams& 
 }
 
 // Tokens of capacity up to which a pair is one CTA's, where all are resident: one launch and no merge.  Device time with
-// and without: 18 x 1000 tokens x 8 heads 12.4 and 16.4 us, 8 x 1000 x 4 10.9 and 10.6, one of 100 x 4 4.9 and 7.8, one of
-// 700 9.2 and 8.6, one of 1000 10.9 and 8.6; the second launch costs the host 2.4 us (12.2 and 14.6 a call).
+// and without: 18 x 1000 tokens x 8 heads 12.4 and 16.4 us, 8 x 1000 x 4 11.0 and 10.6, one of 100 x 4 5.0 and 7.7, one of
+// 700 9.3 and 8.6, one of 1000 10.9 and 8.6; the second launch costs the host 2.1 us (12.1 and 14.2 a call), so that a
+// call from the host is the shorter one also where the device is not.
 constexpr int OWN_TOKENS = 1024;
 
 template <bool BF, int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
@@ -762,8 +765,8 @@ template <bool BF, int D, int NT> int launch_block(AttnParams& p, int sms, cudaS
   const bool own = tokens <= OWN_TOKENS && (int64_t)p.c.num_seqs * p.heads_rows <= sms;
   const bool pairs = p.c.block_tokens > TILE;
   if (own) return pairs ? launch_shape<BF, D, NT, 2, true>(p, sms, stream) : launch_shape<BF, D, NT, 1, true>(p, sms, stream);
-  // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 76 us
-  // against 96) and for 16 rows (eight of 5003 tokens, four queries each: 23.4 against 25.4).
+  // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 74 us
+  // against 92) and for 16 rows (eight of up to 5003 tokens, four queries each: 20.4 against 22.0).
   if constexpr (D == 64 || NT == 2) {
     if (pairs) return launch_shape<BF, D, NT, 2, false>(p, sms, stream);
   }

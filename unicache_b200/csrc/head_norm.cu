@@ -227,9 +227,9 @@ template <typename T, int L, int HEADS, bool STREAM> int launch_lanes(const Head
 }
 
 template <typename T, int L> int launch_heads(const HeadNormParams& p, cudaStream_t s) {
-  // Four rows a lane once one row a lane would fill the chip's threads (4999 tokens x 18 heads x 64: 5.8 us against
-  // 7.6 with one row; below that, one row has the shorter way); from token to token once that makes several turns
-  // (where it makes two or three, 6.8 us for the same case).
+  // Four rows a lane once one row a lane would fill the chip's threads (4999 tokens x 18 heads x 64: 5.6 us against
+  // 8.0 with one row; below that, one row has the shorter way); from token to token once that makes several turns
+  // (where it makes two or three, 6.6 us for the same case).
   const int64_t lanes = p.tokens * (p.hq + p.hk) * L;
   if (lanes >= 148 * 2048 * 8) return launch_lanes<T, L, 4, true>(p, s);
   if (lanes >= 148 * 2048) return launch_lanes<T, L, 4, false>(p, s);

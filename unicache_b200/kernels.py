@@ -1376,8 +1376,7 @@ def _block8_attend(query, cache, shape, stride, blocks, softmax_scale, select=No
     else:
         raise ValueError("query must be [num_seqs, (queries,) q_heads, head_dim]")
     if not 1 <= queries <= 16:
-        raise ValueError("the block cache attention takes 1 to 16 query tokens a sequence; read the cache back and "
-                         "use long_query_attention_summary for more")
+        raise ValueError("the block cache attention takes 1 to 16 query tokens a sequence")
     q_heads = shape[-2]
     scale = cache.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     address, contiguous = query.data_ptr(), query.is_contiguous()
