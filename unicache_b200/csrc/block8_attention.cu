@@ -12,7 +12,7 @@
 // flat order, each triple's preceded by START empty ones for what its start
 // costs, every warp of the grid an equal contiguous share (lengths are
 // read on the device, so a captured step follows them).  A warp that holds
-// a whole triple writes its output; the others' states (reference maximum, sum,
+// a whole triple writes its output; the others' states (unit, reference, sum,
 // unnormalised rows) are merged in shared memory within a CTA, and across CTAs by
 // a second small kernel.
 //
@@ -29,11 +29,13 @@
 // 1152); a query row is scaled by a power of two to at most 2^14 and held in
 // fp16 (bf16 and fp16 rows exactly, but for elements 2^-28 of the row's largest);
 // logits, sums and outputs in fp32.  A weight is rounded to fp16 for the value
-// product only, after its block's value scale has been added to its exponent, and
+// product only, after its block's value scale has been multiplied into it,
 // relative to the largest such product so far (at 2^6, up to 2^14 before the
-// reference moves): every contribution to the output above 2^-20 of the largest
+// unit moves): every contribution to the output above 2^-20 of the largest
 // keeps 11 bits, whatever the blocks' scales are.  The sum of weights is kept
-// in fp32 against a reference of its own.
+// in fp32 against the reference alone.  The output's unit is held as its distance
+// from the reference (`gap`, a number of the size of the scales' logarithms), never as
+// a logit plus a logarithm, which would round the scale to the spacing of fp32 at the logit.
 //
 // Measured (B200, device): 1.07 GB of codes (32 x 32768 tokens, 4 KV heads of
 // 128) in 173-176 us, 6.2 TB/s, 95% of the copy rate (194 us over 0.15 s,
@@ -71,9 +73,9 @@ constexpr int TILE = 16;  // tokens of one matrix product
 // ones 35.1, 33.3, 32.9 and 32.7; one length of 131072 tokens 176, 173, 173 and 174.
 constexpr int START = 4;
 constexpr int CTAS_PER_SM = 2;
-constexpr float LIFT = 6.f;        // log2 of the largest weight when its reference is set
-constexpr float LAZY = 14.f;       // a weight may reach 2^LAZY before its reference moves
-constexpr float LAZY_SUM = 100.f;  // the same of the fp32 sum
+constexpr float LIFT = 6.f;        // log2 of the largest scaled weight when the output's unit is set
+constexpr float LAZY = 14.f;       // a scaled weight may reach 2^LAZY before the unit moves
+constexpr float LAZY_SUM = 100.f;  // an unscaled one 2^LAZY_SUM before the reference does
 
 // U tiles of 16 tokens a step.  OWN: a CTA has one pair to itself, all of a multiprocessor's registers and no second
 // kernel after it; else two CTAs a multiprocessor.
@@ -82,7 +84,7 @@ template <int D, int NT, int U, bool OWN> struct Shape {
   static constexpr int WARPS = OWN || NT == 1 ? 8 : D == 64 ? 6 : 4;
   static constexpr int STEP_BYTES = U * 2 * TILE * D;
   static constexpr int STAGES = (OWN ? 131072 : 65536) / (WARPS * STEP_BYTES);
-  static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its reference, the sum's reference, the sum
+  static constexpr int ROW_FLOATS = D + 4;  // unnormalised row, its gap, its reference, the sum
   static constexpr int STATE_FLOATS = ROWS * ROW_FLOATS;
   static constexpr int RING_BYTES = STAGES * STEP_BYTES;
   static constexpr int SMEM_BYTES = WARPS * (RING_BYTES + STATE_FLOATS * 4);  // without the prefix sums
@@ -131,50 +133,54 @@ __device__ __forceinline__ int64_t out_row(const AttnParams& p, int s, int h, in
   return ((int64_t)s * p.queries + l) * p.q_heads + h * p.group + row - l * p.group;
 }
 
+// A state's sum of weights is in units of 2^ref, its unnormalised values are in units of 2^(ref + gap).  Without a token the
+// reference is NO_REF and the sum 0, without a value above zero the gap is NO_GAP: finite, so that differences of them are
+// numbers (or -inf) and need no branch, and far below what either can be.
+constexpr float NO_REF = -3.402823466e38f, NO_GAP = -1e30f;
+
 __device__ __forceinline__ void write_lse(const AttnParams& p, int64_t row, float ref, float sum) {
-  if (p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (ref == -INFINITY ? sum : (ref + log2f(sum)) * 0.693147180559945309f);
+  if (p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.693147180559945309f;
 }
 
-// 2^(ref - sum_ref) / sum, the factor of an unnormalised row; 0 where no token was seen.
-__device__ __forceinline__ float normaliser(float ref, float sum_ref, float sum) {
-  return sum == 0.f || (ref == -INFINITY && sum == sum) ? 0.f : fast_exp2(ref - sum_ref) * __fdividef(1.f, sum);
+// 2^gap / sum, the factor of an unnormalised row; 0 where no token was seen.
+__device__ __forceinline__ float normaliser(float gap, float sum) {
+  return sum == 0.f ? 0.f : fast_exp2(gap) * __fdividef(1.f, sum);
 }
 
-// States of one row merged, four channels of it.  A state without a token has references -inf and sum 0; products, not
-// branches, so that a NaN comes through.  `get(i)` points to state i's row: D channels, then reference, sum reference, sum.
+// States of one row merged, four channels of it; products, not branches, so that a NaN comes through.
+// `get(i)` points to state i's row: D channels, then gap, reference, sum.
 struct Merged {
   float4 value;
-  float ref, sum_ref, sum;
+  float gap, ref, sum;
 };
-// One more state, at references not above m's.
+// One more state; m's units are not below its own.
 __device__ __forceinline__ void merge_in(Merged& m, float4 value, float4 meta) {
-  const float f = meta.x == -INFINITY ? 0.f : fast_exp2(meta.x - m.ref);
+  const float fall = meta.y - m.ref, f = fast_exp2(fall + (meta.x - m.gap));
   m.value.x = fmaf(f, value.x, m.value.x);
   m.value.y = fmaf(f, value.y, m.value.y);
   m.value.z = fmaf(f, value.z, m.value.z);
   m.value.w = fmaf(f, value.w, m.value.w);
-  m.sum = fmaf(meta.y == -INFINITY ? 0.f : fast_exp2(meta.y - m.sum_ref), meta.z, m.sum);
+  m.sum = fmaf(fast_exp2(fall), meta.z, m.sum);
 }
 template <int D, typename Get> __device__ __forceinline__ Merged merge_states(int first, int n, int stride, int d, Get get) {
-  Merged m{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f};
+  Merged m{make_float4(0.f, 0.f, 0.f, 0.f), NO_GAP, NO_REF, 0.f};
 #pragma unroll 1
   for (int i = first; i < n; i += 4 * stride) {  // four at a time, their loads together
     float4 x[4], y[4];
-    float ref = m.ref, sum_ref = m.sum_ref;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {  // past the end, the last one again: not counted below
       const float* at = get(min(i + k * stride, n - 1));
       x[k] = *reinterpret_cast<const float4*>(at + D);
       y[k] = *reinterpret_cast<const float4*>(at + d);
     }
+    const Merged old = m;
+    float ref = fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y));
+    ref = fmaxf(ref, old.ref);
+    float gap = fmaxf(old.gap + (old.ref - ref), NO_GAP);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      ref = fmaxf(ref, x[k].x);
-      sum_ref = fmaxf(sum_ref, x[k].y);
-    }
-    const float4 old = m.value, meta = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
-    m = Merged{make_float4(0.f, 0.f, 0.f, 0.f), ref, sum_ref, 0.f};
-    merge_in(m, old, meta);
+    for (int k = 0; k < 4; ++k) gap = fmaxf(gap, x[k].x + (x[k].y - ref));
+    m = Merged{make_float4(0.f, 0.f, 0.f, 0.f), gap, ref, 0.f};
+    merge_in(m, old.value, make_float4(old.gap, old.ref, old.sum, 0.f));
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (i + k * stride < n) merge_in(m, y[k], x[k]);
@@ -183,7 +189,7 @@ template <int D, typename Get> __device__ __forceinline__ Merged merge_states(in
 }
 
 template <bool BF> __device__ __forceinline__ void write_four(const AttnParams& p, int64_t at, const Merged& m) {
-  const float f = normaliser(m.ref, m.sum_ref, m.sum);
+  const float f = normaliser(m.gap, m.sum);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
       make_uint2(pack_out<BF>(m.value.x * f, m.value.y * f), pack_out<BF>(m.value.z * f, m.value.w * f));
 }
@@ -425,11 +431,12 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
       }
     const int sure = len - p.queries + 1;  // tokens that every row sees
 
-    // Unnormalised output and its reference (of s + log2 value scale), sum of weights and its own (of s).
-    float o[NT][MT][4], ref[NT][2], sum[NT][2], sum_ref[NT][2];
+    // Sum of weights in units of 2^ref, unnormalised output in units of 2^(ref + gap).
+    float o[NT][MT][4], gap[NT][2], sum[NT][2], ref[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      ref[nt][0] = ref[nt][1] = sum_ref[nt][0] = sum_ref[nt][1] = -INFINITY;
+      gap[nt][0] = gap[nt][1] = NO_GAP;
+      ref[nt][0] = ref[nt][1] = NO_REF;
       sum[nt][0] = sum[nt][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < MT; ++j)
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
         for (int k = 0; k < 2; ++k) {
           top[nt][k] = fmaxf(s[0][nt][k], s[0][nt][k + 2]);
           if (U == 2) top[nt][k] = fmaxf(top[nt][k], fmaxf(s[U - 1][nt][k], s[U - 1][nt][k + 2]));
-          move |= top[nt][k] > fminf(ref[nt][k] - lv + LAZY, sum_ref[nt][k] + LAZY_SUM);
+          move |= top[nt][k] - ref[nt][k] > fminf(gap[nt][k] - lv + LAZY, LAZY_SUM);
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -518,12 +525,13 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            const float to = fmaxf(ref[nt][k], m + lv - LIFT), sum_to = fmaxf(sum_ref[nt][k], m);
+            const float to = fmaxf(ref[nt][k], m), fall = ref[nt][k] - to;
+            const float gap_to = fmaxf(fmaxf(gap[nt][k] + fall, (m - to) + lv - LIFT), NO_GAP);
             // a NaN that the sums already hold stays: 0 * NaN
-            const float f = ref[nt][k] == -INFINITY ? 0.f : fast_exp2(ref[nt][k] - to);
-            sum[nt][k] *= sum_ref[nt][k] == -INFINITY ? 0.f : fast_exp2(sum_ref[nt][k] - sum_to);
+            const float f = fast_exp2(fall + (gap[nt][k] - gap_to));
+            sum[nt][k] *= fast_exp2(fall);
+            gap[nt][k] = gap_to;
             ref[nt][k] = to;
-            sum_ref[nt][k] = sum_to;
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               o[nt][j][k] *= f;
@@ -536,20 +544,20 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
       uint32_t pb[U][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float base[2], sum_base[2];
+        float scale[2];  // the value scale in the output's unit (weights below 2^-126 are 0: no factor above 2^126 is needed)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          base[k] = ref[nt][k] == -INFINITY ? (lv == lv ? INFINITY : lv) : ref[nt][k] - lv;
-          sum_base[k] = sum_ref[nt][k] == -INFINITY ? 0.f : sum_ref[nt][k];
+          const float lift = lv - gap[nt][k];
+          scale[k] = fast_exp2(lift > 126.f ? 126.f : lift);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            w[k] = fast_exp2(s[u][nt][k] - base[k & 1]);
-            if (masked && s[u][nt][k] == -INFINITY) w[k] = 0.f;  // whatever the block's scale is
-            sum[nt][k & 1] += fast_exp2(s[u][nt][k] - sum_base[k & 1]);
+            const float e = fast_exp2(s[u][nt][k] - ref[nt][k & 1]);
+            sum[nt][k & 1] += e;
+            w[k] = masked && s[u][nt][k] == -INFINITY ? 0.f : e * scale[k & 1];  // 0 whatever the block's scale is
           }
           pb[u][nt][0] = movmatrix_trans(pack_f16x2(w[0], w[1]));
           pb[u][nt][1] = movmatrix_trans(pack_f16x2(w[2], w[3]));
@@ -603,7 +611,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int in_tile = nt * 8 + 2 * cq + k, row = a.rt * S::ROWS + in_tile;
-        const float f = whole ? normaliser(ref[nt][k], sum_ref[nt][k], l) : 1.f;
+        const float f = whole ? normaliser(gap[nt][k], l) : 1.f;
         float run[VB];
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
@@ -618,14 +626,14 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
             for (int i = 0; i < VB / 8; ++i)
               out[i] = make_uint4(pack_out<BF>(run[8 * i], run[8 * i + 1]), pack_out<BF>(run[8 * i + 2], run[8 * i + 3]),
                                   pack_out<BF>(run[8 * i + 4], run[8 * i + 5]), pack_out<BF>(run[8 * i + 6], run[8 * i + 7]));
-            if (r == 0) write_lse(p, to, sum_ref[nt][k], l);
+            if (r == 0) write_lse(p, to, ref[nt][k], l);
           }
         } else {
           float* at = state + in_tile * S::ROW_FLOATS;
 #pragma unroll
           for (int i = 0; i < VB; i += 4)
             *reinterpret_cast<float4*>(at + VB * r + i) = make_float4(run[i], run[i + 1], run[i + 2], run[i + 3]);
-          if (r == 0) *reinterpret_cast<float4*>(at + D) = make_float4(ref[nt][k], sum_ref[nt][k], l, 0.f);
+          if (r == 0) *reinterpret_cast<float4*>(at + D) = make_float4(gap[nt][k], ref[nt][k], l, 0.f);
         }
       }
     if (!whole && lane == 0)
@@ -660,23 +668,24 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
       const unsigned char* end_state = last.apart ? smem + S::WARPS * S::RING_BYTES + ((final >> 1) * S::ROWS + in_tile) * (S::ROW_FLOATS * 4)
                                                   : states + (open_n - 1) * S::RING_BYTES;
       auto state = [&](int i) { return reinterpret_cast<const float*>(i < open_n - 1 ? states + i * S::RING_BYTES : end_state); };
-      Merged m{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f};
+      Merged m{make_float4(0.f, 0.f, 0.f, 0.f), NO_GAP, NO_REF, 0.f};
 #pragma unroll 2
       for (int i = 0; i < open_n; ++i) {
         const float2 x = *reinterpret_cast<const float2*>(state(i) + D);
-        m.ref = fmaxf(m.ref, x.x);
-        m.sum_ref = fmaxf(m.sum_ref, x.y);
+        const float top = fmaxf(m.ref, x.y);
+        m.gap = fmaxf(m.gap + (m.ref - top), x.x + (x.y - top));
+        m.ref = top;
       }
 #pragma unroll 2
       for (int i = 0; i < open_n; ++i) merge_in(m, *reinterpret_cast<const float4*>(state(i) + d), *reinterpret_cast<const float4*>(state(i) + D));
       if (complete) {
         const int64_t out = out_row(p, last.s, last.h, row);
         write_four<BF>(p, out * D + d, m);
-        if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
+        if (d == 0) write_lse(p, out, m.ref, m.sum);
       } else {
         float* at = to + in_tile * S::ROW_FLOATS;
         *reinterpret_cast<float4*>(at + d) = m.value;
-        if (d == 0) *reinterpret_cast<float4*>(at + D) = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
+        if (d == 0) *reinterpret_cast<float4*>(at + D) = make_float4(m.gap, m.ref, m.sum, 0.f);
       }
     }
     if (!ended && !from_before && threadIdx.x == 0)  // the pair that starts here ends in a later CTA
@@ -703,13 +712,13 @@ __global__ void __launch_bounds__(MERGE_GROUPS * D / 4) attention_merge_kernel(c
     return p.partials + (slot * S::ROWS + blockIdx.y) * S::ROW_FLOATS;
   });
   *reinterpret_cast<float4*>(groups[g] + d) = m.value;
-  if (d == 0) *reinterpret_cast<float4*>(groups[g] + D) = make_float4(m.ref, m.sum_ref, m.sum, 0.f);
+  if (d == 0) *reinterpret_cast<float4*>(groups[g] + D) = make_float4(m.gap, m.ref, m.sum, 0.f);
   __syncthreads();
   if (g > 0) return;
   m = merge_states<D>(0, MERGE_GROUPS, 1, d, [&](int i) { return static_cast<const float*>(groups[i]); });
   const int64_t out = out_row(p, link.y, link.z, row);
   write_four<BF>(p, out * D + d, m);
-  if (d == 0) write_lse(p, out, m.sum_ref, m.sum);
+  if (d == 0) write_lse(p, out, m.ref, m.sum);
 }
 
 int multiprocessors() {
