@@ -607,9 +607,14 @@ UCB_API int ucb_head_norm_rope(const ucb_head_norm_args* args, void* stream);
  * key_low / key_high hold the smallest and largest key code of each channel
  * over the block's tokens.  Token t of sequence s lies in row t % block_tokens
  * of block block_table[s][t / block_tokens].  pending_key / pending_value keep
- * the unquantised rows of each sequence's incomplete block, so a block that
- * grows row by row is always the quantisation of all its rows.  lengths are
- * read on the device: a write expects them already advanced by its rows.
+ * the unquantised rows of the last block that a write touched, so a block that
+ * grows row by row is after each write the quantisation of all its rows; their last row
+ * holds the writer's record of whose rows they are and how many.  lengths are
+ * read on the device: a write expects them already advanced by its rows.  Rows are
+ * withdrawn (rejected drafts, a warm-up step) by taking the lengths back: to any point of
+ * the last block written, to its start, to an earlier block's end or to nothing.  The next write
+ * then gives scale, codes and bounds of the rows that count.  Until it, attention
+ * and selection see the remaining rows under the block's old scale and bounds.
  * head_dim 64 or 128; block_tokens 16, 32, 64 or 128; num_seqs <= 4096; all
  * tensors contiguous; codes, bounds and pending rows 16-byte aligned. */
 typedef struct ucb_block8_cache {
@@ -637,7 +642,9 @@ typedef struct ucb_block8_cache {
  * tokens [lengths[s] - n, lengths[s]); starts_dev int32 [num_seqs + 1], or
  * NULL for one row each.  Every touched block is requantised from all its rows when its
  * scale grows.  Lengths beyond the table, blocks outside the pool and row
- * ranges outside [0, rows) set device error bit 2 and write nothing. */
+ * ranges outside [0, rows) set device error bit 2 and write nothing, and so
+ * does a write into a block whose earlier rows are not pending any more (withdrawn
+ * over a block's end) or were never written. */
 UCB_API int ucb_block8_write(const ucb_block8_cache* cache, const void* key_dev, int64_t key_stride_token,
                              int64_t key_stride_head, const void* value_dev, int64_t value_stride_token,
                              int64_t value_stride_head, int64_t rows, const int32_t* starts_dev, void* stream);

@@ -115,14 +115,25 @@ template <bool BF> __device__ __forceinline__ uint32_t codes4(uint32_t w0, uint3
 // 1 / scale, 0 for a scale that is no number.
 __device__ __forceinline__ float inverse_of(float scale) { return scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f; }
 
-// Keys and values of one block and head: rows [0, held) are pending ones, rows [held, m) the call's.  The new
-// rows decide whether the block's scale grows: where it does not, the codes
+// Whose rows the pending ones of a sequence and head are: the block's place in the sequence and how many of its rows were
+// written.  The record lies in their last row, which no held row needs (a block with that row is complete).  Anything else there
+// is no record: pending rows that were not written by this kernel are taken as they are.
+constexpr uint32_t RECORD = 0x38424c4bu;
+__device__ __forceinline__ uint4 make_record(int j, int m) {
+  return make_uint4(RECORD, (uint32_t)j, (uint32_t)m, ~(RECORD ^ (uint32_t)j ^ (uint32_t)m << 16));
+}
+__device__ __forceinline__ bool is_record(uint4 r) { return r.x == RECORD && r.w == ~(RECORD ^ r.y ^ r.z << 16); }
+
+// Keys and values of block j of sequence s and one head: rows [0, held) are pending ones, rows [held, m) the call's.
+// The new rows decide whether the block's scale grows: where it does not, the codes
 // of the held rows stand (they depend on the scale alone, and the scale of a
-// larger magnitude is never the smaller), and only the new rows are written.
-// FRESH: a block without held rows.
+// larger magnitude is never the smaller), and only the new rows are written.  Where rows
+// of the block were withdrawn since (the record counts more than `held`), scale and bounds
+// come from the held rows again (one token to each of 32 sequences, the one before it withdrawn: 3.9 us against 3.7).  False where the held rows are not there any more, or never were.
+// FRESH: a block without held rows.  KEEP: the last block that the call touches, whose rows stay pending.
 template <bool BF, int D, int BT, bool FRESH>
-__device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, int64_t block, int m, int held,
-                                            int64_t first_row) {
+__device__ __forceinline__ bool write_block(const WriteParams& p, int s, int h, int64_t block, int j, int m, int held,
+                                            int64_t first_row, bool keep) {
   if (FRESH) held = 0;
   constexpr int UNITS = D / 8, STRIDE = THREADS / UNITS, PASSES = (BT + STRIDE - 1) / STRIDE, WARPS = THREADS / 32;
   __shared__ uint32_t warp_top[2][WARPS];
@@ -133,8 +144,11 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
   const int64_t scale_at = block * c.kv_heads + h;
   const int64_t pending_at = ((int64_t)s * c.kv_heads + h) * (BT * D) + unit * 8;
   const float old[2] = {held ? c.key_scale[scale_at] : 0.f, held ? c.value_scale[scale_at] : 0.f};
+  uint4* record_at = reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.pending_key) +
+                                              ((int64_t)s * c.kv_heads + h) * (BT * D) + (BT - 1) * D);
+  const uint4 record = held ? *record_at : make_uint4(0, 0, 0, 0);
 
-  // ---- new rows: loads of both sides together
+  // ---- new rows: loads of both sides together.  x holds row g + i * STRIDE of the block.
   uint4 x[2][PASSES];
   uint32_t top[2] = {0, 0}, low[4], high[4];
 #pragma unroll
@@ -142,10 +156,28 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
     const uint16_t* src = static_cast<const uint16_t*>(side ? p.value : p.key) + h * (side ? p.v_sh : p.k_sh) + unit * 8;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const int row = held + g + i * STRIDE;
-      if (row < m) x[side][i] = load8(src + (first_row + row - held) * (side ? p.v_st : p.k_st), p.aligned);
+      const int row = g + i * STRIDE;
+      if (row >= held && row < m) x[side][i] = load8(src + (first_row + row - held) * (side ? p.v_st : p.k_st), p.aligned);
     }
   }
+  auto load_held = [&](int side) {
+    const uint16_t* src = static_cast<const uint16_t*>(side ? c.pending_value : c.pending_key) + pending_at;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int row = g + i * STRIDE;
+      if (row < held) x[side][i] = *reinterpret_cast<const uint4*>(src + row * D);
+    }
+  };
+  bool again = false;  // rows were withdrawn
+  if (held && is_record(record)) {
+    if (record.y != (uint32_t)j || record.z < (uint32_t)held) {
+      if (threadIdx.x == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+      return false;
+    }
+    again = record.z > (uint32_t)held;
+    if (again) load_held(0), load_held(1);
+  }
+  const int from = again ? 0 : held;
   constexpr uint32_t INF2 = BF ? 0x7f807f80u : 0x7c007c00u;
 #pragma unroll
   for (int k = 0; k < 4; ++k) low[k] = INF2, high[k] = INF2 | 0x80008000u;
@@ -156,7 +188,7 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
   };
 #pragma unroll
   for (int i = 0; i < PASSES; ++i)
-    if (held + g + i * STRIDE < m) {
+    if (g + i * STRIDE >= from && g + i * STRIDE < m) {
 #pragma unroll
       for (int side = 0; side < 2; ++side) {  // magnitude bits: their order is the values', with NaN above infinity
         const uint4 w = x[side][i];
@@ -186,58 +218,45 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
   share_bounds();
   __syncthreads();
   float scale[2], inverse[2];
-  bool grown[2];
+  bool changed[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     uint32_t t = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) t = max(t, warp_top[side][w]);
     const float mine = scale_of(low_half<BF>(t));
-    grown[side] = !held || mine > old[side] || (mine != mine && old[side] == old[side]);
-    scale[side] = grown[side] ? mine : old[side];
+    changed[side] = !held || (again ? !(mine == old[side]) : mine > old[side] || (mine != mine && old[side] == old[side]));
+    scale[side] = changed[side] ? mine : old[side];
     inverse[side] = inverse_of(scale[side]);
   }
 
-  // ---- codes of the new rows, and the rows themselves while the block is incomplete
+  // ---- a larger scale: the held rows too
+  if (held && !again) {
+    if (changed[0]) {
+      load_held(0);
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+        if (g + i * STRIDE < held) bounds(x[0][i]);
+      __syncthreads();  // the new rows' bounds were read by no one yet, but other warps' are in place
+      share_bounds();
+      __syncthreads();
+    }
+    if (changed[1]) load_held(1);
+  }
+  // ---- codes, and the new rows themselves where more of the block may come, or come again
 #pragma unroll
   for (int side = 0; side < 2; ++side)
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const int row = held + g + i * STRIDE;
-      if (row >= m) continue;
+      const int row = g + i * STRIDE;
+      if (row >= m || (row < held && !changed[side])) continue;
       const uint4 w = x[side][i];
       *reinterpret_cast<uint2*>((side ? c.value_code : c.key_code) + at + row * D) =
           make_uint2(codes4<BF>(w.x, w.y, inverse[side]), codes4<BF>(w.z, w.w, inverse[side]));
-      if (m < BT)
+      if (keep && row >= held && row < BT - 1)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(side ? c.pending_value : c.pending_key) + pending_at + row * D) = w;
     }
-  // ---- a larger scale: the held rows again
-#pragma unroll
-  for (int side = 0; side < 2; ++side)
-    if (held && grown[side]) {
-      const uint16_t* src = static_cast<const uint16_t*>(side ? c.pending_value : c.pending_key) + pending_at;
-      int8_t* codes = (side ? c.value_code : c.key_code) + at;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int row = g + i * STRIDE;
-        if (row < held) x[side][i] = *reinterpret_cast<const uint4*>(src + row * D);
-      }
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int row = g + i * STRIDE;
-        if (row >= held) continue;
-        const uint4 w = x[side][i];
-        if (side == 0) bounds(w);
-        *reinterpret_cast<uint2*>(codes + row * D) =
-            make_uint2(codes4<BF>(w.x, w.y, inverse[side]), codes4<BF>(w.z, w.w, inverse[side]));
-      }
-      if (side == 0) {
-        __syncthreads();  // the new rows' bounds were read by no one yet, but other warps' are in place
-        share_bounds();
-        __syncthreads();
-      }
-    }
-  if (threadIdx.x < 2 && grown[threadIdx.x ? 1 : 0])
+  if (threadIdx.x < 2 && changed[threadIdx.x ? 1 : 0])
     (threadIdx.x ? c.value_scale : c.key_scale)[scale_at] = threadIdx.x ? scale[1] : scale[0];
   // ---- bounds of the key codes: rounding keeps order, so they are the codes of the channels' bounds
   for (int pair = threadIdx.x; pair < D / 2; pair += THREADS) {
@@ -249,7 +268,7 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
     char2 high2 = make_char2((signed char)(q >> 16 & 255), (signed char)(q >> 24));
     char2* low_to = reinterpret_cast<char2*>(c.key_low + scale_at * D) + pair;
     char2* high_to = reinterpret_cast<char2*>(c.key_high + scale_at * D) + pair;
-    if (!grown[0]) {
+    if (!changed[0] && !again) {
       const char2 a = *low_to, b = *high_to;
       low2 = make_char2(min(low2.x, a.x), min(low2.y, a.y));
       high2 = make_char2(max(high2.x, b.x), max(high2.y, b.y));
@@ -257,10 +276,13 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
     *low_to = low2;
     *high_to = high2;
   }
+  // every thread read the old record before the barrier; the rows of a block that the call leaves behind are not kept
+  if (!FRESH && threadIdx.x == 0) *record_at = make_record(j, keep ? m : 0);
+  return true;
 }
 
 // Work items of a head: item s < num_seqs is sequence s's first touched block
-// and then its last, incomplete one (one CTA, since the first reads the pending rows that
+// and then its last one (one CTA, since the first reads the pending rows that
 // the last overwrites); item num_seqs + i is the whole block in between that
 // holds row i * block_tokens of the call (every such block holds exactly one
 // multiple of block_tokens).
@@ -285,9 +307,9 @@ __global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(c
   if (!ends) {
     if (probe < a || probe >= e) return;
     const int64_t j = (old + probe - a) / bt;
-    if (j <= first || (j + 1) * bt > len) return;
+    if (j <= first || j >= last) return;
     const int64_t block = pool_block(c, s, (int)j, p.err);
-    if (block >= 0) write_block<BF, D, BT, true>(p, s, h, block, bt, 0, a + j * bt - old);
+    if (block >= 0) write_block<BF, D, BT, true>(p, s, h, block, (int)j, bt, 0, a + j * bt - old, false);
     return;
   }
   int j = first;
@@ -297,8 +319,8 @@ __global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(c
     const int64_t t0 = (int64_t)j * bt;
     const int m = (int)min((int64_t)bt, len - t0);
     const int held = (int)max((int64_t)0, min((int64_t)m, old - t0));
-    if (block >= 0) write_block<BF, D, BT, false>(p, s, h, block, m, held, a + t0 + held - old);
-    if (j != first || last == first || len % bt == 0) break;
+    if (block >= 0 && !write_block<BF, D, BT, false>(p, s, h, block, j, m, held, a + t0 + held - old, j == last)) break;
+    if (j == last) break;
     j = last;
     __syncthreads();  // the pending rows of the first block are read
   }

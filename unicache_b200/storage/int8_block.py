@@ -29,10 +29,10 @@ class Int8BlockCache:
 
     A block's scale is max(amax / 127, 2^-120) over its tokens so far and all
     channels of one head, a code clamp(rint(x * (1 / scale)), -127, 127).  The
-    unquantised rows of each sequence's incomplete block stay in
-    ``pending_key`` / ``pending_value``: the cache is at any time, bit for
-    bit, the quantisation of all rows written so far, whatever the order in
-    which they came.  A NaN or an infinity poisons its block (the scale becomes NaN or
+    unquantised rows of the last block that a write touched stay in
+    ``pending_key`` / ``pending_value``: after each write of a sequence's rows it is, bit for
+    bit, the quantisation of those that count, whatever the portions in
+    which they came and whatever was withdrawn (``advance``) between them.  A NaN or an infinity poisons its block (the scale becomes NaN or
     infinite), so it shows in the attention's output.
 
     ``lengths`` counts the tokens of each sequence and is advanced by the caller
@@ -158,7 +158,13 @@ class Int8BlockCache:
     # ---------------------------------------------------------------- use
     def advance(self, tokens) -> None:
         """Add ``tokens`` (a number or an int32 [num_seqs] tensor) to the lengths
-        before the write of that many rows: once for all caches that share them."""
+        before the write of that many rows: once for all caches that share them.
+
+        Negative numbers withdraw the last rows, such as rejected drafts: as far as the start of
+        the last block written, or back to the end of an earlier block.  From the middle
+        of an earlier block on there is no way forward: its unquantised rows are gone, and a write
+        there is refused (device error bit 2).  So a draft that may be rejected in part ends with
+        its block at the latest."""
 
         self.lengths.add_(tokens)
 
@@ -166,8 +172,9 @@ class Int8BlockCache:
         """Rows [N, kv_heads, head_dim] become the last tokens of the sequences:
         rows ``starts[s]`` to ``starts[s + 1]`` (int32 [num_seqs + 1] on the
         device) of sequence s, or one row each without ``starts``.  ``lengths`` already
-        counts them.  Lengths past the table, blocks outside the pool and malformed
-        starts write nothing and set device error bit 2 (``kernels.device_status``)."""
+        counts them.  Lengths past the table, blocks outside the pool, malformed
+        starts and blocks whose earlier rows are not there (``advance``) write nothing and set
+        device error bit 2 (``kernels.device_status``)."""
 
         kernels.block8_write(self, key, value, starts)
 
