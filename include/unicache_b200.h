@@ -641,10 +641,11 @@ typedef struct ucb_block8_cache {
  * rows [starts[s], starts[s+1]) are the last tokens of sequence s, that is
  * tokens [lengths[s] - n, lengths[s]); starts_dev int32 [num_seqs + 1], or
  * NULL for one row each.  Every touched block is requantised from all its rows when its
- * scale grows.  Lengths beyond the table, blocks outside the pool and row
- * ranges outside [0, rows) set device error bit 2 and write nothing, and so
- * does a write into a block whose earlier rows are not pending any more (withdrawn
- * over a block's end) or were never written. */
+ * scale grows.  What cannot be written is skipped, sets device error bit 2, and the rest is written: a
+ * sequence whose length is beyond the table or below its rows, or whose row range is outside [0,
+ * rows) (where starts do not ascend, whole blocks of the sequences after may be missing too);
+ * a block that the table places outside the pool; and a block whose earlier rows
+ * are not pending any more (withdrawn over a block's end) or were never written. */
 UCB_API int ucb_block8_write(const ucb_block8_cache* cache, const void* key_dev, int64_t key_stride_token,
                              int64_t key_stride_head, const void* value_dev, int64_t value_stride_token,
                              int64_t value_stride_head, int64_t rows, const int32_t* starts_dev, void* stream);

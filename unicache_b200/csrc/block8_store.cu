@@ -129,10 +129,10 @@ __device__ __forceinline__ bool is_record(uint4 r) { return r.x == RECORD && r.w
 // of the held rows stand (they depend on the scale alone, and the scale of a
 // larger magnitude is never the smaller), and only the new rows are written.  Where rows
 // of the block were withdrawn since (the record counts more than `held`), scale and bounds
-// come from the held rows again (one token to each of 32 sequences, the one before it withdrawn: 3.9 us against 3.7).  False where the held rows are not there any more, or never were.
+// come from the held rows again (one token to each of 32 sequences, the one before it withdrawn: 3.9 us against 3.7).  Nothing is written where the held rows are not there any more, or never were.
 // FRESH: a block without held rows.  KEEP: the last block that the call touches, whose rows stay pending.
 template <bool BF, int D, int BT, bool FRESH>
-__device__ __forceinline__ bool write_block(const WriteParams& p, int s, int h, int64_t block, int j, int m, int held,
+__device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, int64_t block, int j, int m, int held,
                                             int64_t first_row, bool keep) {
   if (FRESH) held = 0;
   constexpr int UNITS = D / 8, STRIDE = THREADS / UNITS, PASSES = (BT + STRIDE - 1) / STRIDE, WARPS = THREADS / 32;
@@ -172,7 +172,7 @@ __device__ __forceinline__ bool write_block(const WriteParams& p, int s, int h, 
   if (held && is_record(record)) {
     if (record.y != (uint32_t)j || record.z < (uint32_t)held) {
       if (threadIdx.x == 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-      return false;
+      return;
     }
     again = record.z > (uint32_t)held;
     if (again) load_held(0), load_held(1);
@@ -278,7 +278,6 @@ __device__ __forceinline__ bool write_block(const WriteParams& p, int s, int h, 
   }
   // every thread read the old record before the barrier; the rows of a block that the call leaves behind are not kept
   if (!FRESH && threadIdx.x == 0) *record_at = make_record(j, keep ? m : 0);
-  return true;
 }
 
 // Work items of a head: item s < num_seqs is sequence s's first touched block
@@ -319,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(c
     const int64_t t0 = (int64_t)j * bt;
     const int m = (int)min((int64_t)bt, len - t0);
     const int held = (int)max((int64_t)0, min((int64_t)m, old - t0));
-    if (block >= 0 && !write_block<BF, D, BT, false>(p, s, h, block, j, m, held, a + t0 + held - old, j == last)) break;
+    if (block >= 0) write_block<BF, D, BT, false>(p, s, h, block, j, m, held, a + t0 + held - old, j == last);
     if (j == last) break;
     j = last;
     __syncthreads();  // the pending rows of the first block are read

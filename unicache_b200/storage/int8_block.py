@@ -172,9 +172,9 @@ class Int8BlockCache:
         """Rows [N, kv_heads, head_dim] become the last tokens of the sequences:
         rows ``starts[s]`` to ``starts[s + 1]`` (int32 [num_seqs + 1] on the
         device) of sequence s, or one row each without ``starts``.  ``lengths`` already
-        counts them.  Lengths past the table, blocks outside the pool, malformed
-        starts and blocks whose earlier rows are not there (``advance``) write nothing and set
-        device error bit 2 (``kernels.device_status``)."""
+        counts them.  Sequences with a length past the table or malformed starts, and blocks
+        outside the pool or whose earlier rows are not there (``advance``), are skipped and set
+        device error bit 2 (``kernels.device_status``); the rest is written."""
 
         kernels.block8_write(self, key, value, starts)
 
