@@ -609,7 +609,9 @@ UCB_API int ucb_head_norm_rope(const ucb_head_norm_args* args, void* stream);
  * of block block_table[s][t / block_tokens].  pending_key / pending_value keep
  * the unquantised rows of the last block that a write touched, so a block that
  * grows row by row is after each write the quantisation of all its rows; their last row
- * holds the writer's record of whose rows they are and how many.  lengths are
+ * holds the writer's record of whose rows they are and how many.  Several sequences may have a
+ * complete block in common that none of them writes into; an incomplete one belongs to
+ * one sequence, as its pending rows do.  lengths are
  * read on the device: a write expects them already advanced by its rows.  Rows are
  * withdrawn (rejected drafts, a warm-up step) by taking the lengths back: to any point of
  * the last block written, to its start, to an earlier block's end or to nothing.  The next write
