@@ -764,14 +764,17 @@ template <bool BF, int D, int NT, int U, bool OWN> int launch_shape(AttnParams& 
 }
 
 // Tokens of capacity up to which a pair is one CTA's, where all are resident: one launch and no merge.  Device time with
-// and without: 18 x 1000 tokens x 8 heads 12.4 and 16.4 us, 8 x 1000 x 4 11.0 and 10.6, one of 100 x 4 5.0 and 7.7, one of
-// 700 9.3 and 8.6, one of 1000 10.9 and 8.6; the second launch costs the host 2.1 us (12.1 and 14.2 a call), so that a
-// call from the host is the shorter one also where the device is not.
-constexpr int OWN_TOKENS = 1024;
+// and without, 7 rows of 128 channels: 4 pairs of 64 tokens 4.4 and 6.2 us, 512 7.8 and 8.4, 700 9.1 and 8.5, 1000 10.6 and
+// 8.5; 32 pairs of 700 9.2 and 10.2, 1000 10.8 and 10.6; 72 pairs of 1000 10.9 and 12.6; 144 of 1000 x 64 channels 8.6 and
+// 11.6.  A call from the host takes 11.2 and 13.4, the second launch.  So a pair has its own CTA where that is the shorter on
+// the device, and a little beyond: as far as it loses less there (at most 1.4 us, 32 pairs of 1000 tokens in blocks of 16)
+// than it saves the host.  More pairs fill more of the chip, so the limit rises with them.
+constexpr int OWN_TOKENS = 768, OWN_TOKENS_A_PAIR = 8, MOST_OWN_TOKENS = 1024;
 
 template <bool BF, int D, int NT> int launch_block(AttnParams& p, int sms, cudaStream_t stream) {
   const int64_t tokens = (int64_t)(p.blocks ? p.selected : p.c.max_blocks) * p.c.block_tokens;
-  const bool own = tokens <= OWN_TOKENS && (int64_t)p.c.num_seqs * p.heads_rows <= sms;
+  const int64_t triples = (int64_t)p.c.num_seqs * p.heads_rows;
+  const bool own = triples <= sms && tokens <= std::min<int64_t>(MOST_OWN_TOKENS, OWN_TOKENS + OWN_TOKENS_A_PAIR * triples);
   const bool pairs = p.c.block_tokens > TILE;
   if (own) return pairs ? launch_shape<BF, D, NT, 2, true>(p, sms, stream) : launch_shape<BF, D, NT, 1, true>(p, sms, stream);
   // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 74 us
