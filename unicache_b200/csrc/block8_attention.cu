@@ -721,14 +721,6 @@ __global__ void __launch_bounds__(MERGE_GROUPS * D / 4) attention_merge_kernel(c
   if (d == 0) write_lse(p, out, m.ref, m.sum);
 }
 
-int multiprocessors() {
-  static int counts[64] = {0};
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (counts[dev] == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) counts[dev] = n;
-  return counts[dev];
-}
-
 constexpr int MOST_SEQS = 4096;
 
 template <bool BF, int D, int NT, int U, bool OWN> int launch_shape(AttnParams& p, int sms, cudaStream_t stream) {
@@ -800,7 +792,7 @@ namespace b8 = ucb::block8;
 // For each CTA: states of two pairs that cross CTAs, one link.
 extern "C" int64_t ucb_block8_attention_workspace_bytes(const ucb_block8_cache* cache, int queries, int q_heads) {
   if (b8::check_cache(cache, "ucb_block8_attention_workspace_bytes") || queries < 1 || q_heads < 1) return -1;
-  const int64_t sms = b8::multiprocessors();
+  const int64_t sms = ucb_host::multiprocessors();
   const int64_t rows = (int64_t)q_heads / cache->kv_heads * queries > 8 ? 16 : 8;
   return sms > 0 ? sms * b8::CTAS_PER_SM * (2 * rows * (cache->head_dim + 4) * 4 + 16) : -1;
 }
@@ -821,7 +813,7 @@ extern "C" int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_blo
   if ((reinterpret_cast<uintptr_t>(a->workspace) | reinterpret_cast<uintptr_t>(a->out)) & 15)
     return set_error(UCB_ERR_INVALID, "ucb_block8_attention: out and workspace must be 16-byte aligned");
   unsigned int* err = ucb_host::device_error_word();
-  const int sms = b8::multiprocessors();
+  const int sms = ucb_host::multiprocessors();
   if (!err || sms < 1) return set_error(UCB_ERR_CUDA, "ucb_block8_attention: no device");
   b8::AttnParams p{};
   p.c = *cache;

@@ -315,9 +315,10 @@ template <typename T, int D> int launch_select(const SelectParams& p, cudaStream
     ready[dev & 63] = true;
   }
   const int64_t pairs = (int64_t)p.c.num_seqs * p.c.kv_heads;
-  // CTAs of a pair: until every warp has a tile, as long as the chip has room for more
+  // CTAs of a pair: until every warp has a tile, as long as the chip has room for more (two on a multiprocessor)
+  const int64_t room = 2 * ucb_host::multiprocessors();
   int parts = 1;
-  while (parts < 8 && pairs * parts * 2 <= 296 && p.c.max_blocks > parts * 16 * WARPS) parts *= 2;
+  while (parts < 8 && pairs * parts * 2 <= room && p.c.max_blocks > parts * 16 * WARPS) parts *= 2;
   return block8::launch(select_kernel<T, D>, dim3((unsigned)(pairs * parts)), dim3(THREADS),
                         p.spill ? 16 : (size_t)p.c.max_blocks * 4, stream, p, "block8 select_kernel", parts);
 }

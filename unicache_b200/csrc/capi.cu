@@ -44,6 +44,14 @@ unsigned int* device_error_word() {
   return g_error_word_ptr[dev];
 }
 
+int multiprocessors() {
+  static int counts[kMaxDevices] = {0};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  if (counts[dev] == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) counts[dev] = n;
+  return counts[dev];
+}
+
 }  // namespace ucb_host
 
 extern "C" const char* ucb_last_error(void) { return g_last_error; }

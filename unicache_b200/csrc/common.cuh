@@ -246,4 +246,5 @@ namespace ucb_host {
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
 unsigned int* device_error_word();
+int multiprocessors();  // of the current device; 0 when it cannot be asked
 }  // namespace ucb_host

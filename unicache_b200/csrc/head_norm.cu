@@ -213,11 +213,13 @@ template <typename T, int L, int HEADS, bool STREAM> int launch_lanes(const Head
                                     : head_norm_lanes_kernel<T, L, HEADS, false, STREAM>;
   uint32_t step = (uint32_t)p.tokens;  // tokens that are worked on at once
   if (STREAM) {  // as many as are resident, in equal turns
-    static int resident[2] = {0, 0};
-    int& ctas = resident[p.interleaved != 0];
+    static int resident[64][2] = {{0}};  // CTAs on a multiprocessor, by device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int& ctas = resident[dev & 63][p.interleaved != 0];
     if (ctas == 0 && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, LANES_THREADS, 0) != cudaSuccess)
       return ucb_host::check_launch("head_norm_lanes_kernel");
-    const int64_t most = std::max<int64_t>(1, (int64_t)ctas * 148 * (LANES_THREADS / L) / units);
+    const int64_t most = std::max<int64_t>(1, (int64_t)ctas * ucb_host::multiprocessors() * (LANES_THREADS / L) / units);
     const int64_t turns = (p.tokens + most - 1) / most;
     step = (uint32_t)((p.tokens + turns - 1) / turns);
   }
@@ -230,9 +232,9 @@ template <typename T, int L> int launch_heads(const HeadNormParams& p, cudaStrea
   // Four rows a lane once one row a lane would fill the chip's threads (4999 tokens x 18 heads x 64: 5.6 us against
   // 8.0 with one row; below that, one row has the shorter way); from token to token once that makes several turns
   // (where it makes two or three, 6.6 us for the same case).
-  const int64_t lanes = p.tokens * (p.hq + p.hk) * L;
-  if (lanes >= 148 * 2048 * 8) return launch_lanes<T, L, 4, true>(p, s);
-  if (lanes >= 148 * 2048) return launch_lanes<T, L, 4, false>(p, s);
+  const int64_t lanes = p.tokens * (p.hq + p.hk) * L, threads = (int64_t)ucb_host::multiprocessors() * 2048;
+  if (lanes >= threads * 8) return launch_lanes<T, L, 4, true>(p, s);
+  if (lanes >= threads) return launch_lanes<T, L, 4, false>(p, s);
   return launch_lanes<T, L, 1, false>(p, s);
 }
 

@@ -211,7 +211,8 @@ class Int8BlockCache:
 
         size = self._workspace_bytes.get((queries, q_heads))
         if size is None:
-            size = int(_capi.load().ucb_block8_attention_workspace_bytes(self.descriptor, queries, q_heads))
+            with torch.cuda.device(self.index):  # the multiprocessors of the device that the launch will be on
+                size = int(_capi.load().ucb_block8_attention_workspace_bytes(self.descriptor, queries, q_heads))
             if size < 0:
                 raise RuntimeError("the device of the block cache is unavailable")
             self._workspace_bytes[(queries, q_heads)] = size
