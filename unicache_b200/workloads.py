@@ -324,6 +324,11 @@ class Int8BlockDecode:
     def capture(self) -> None:
         """Capture one step as a CUDA graph; ``replay`` then runs a step."""
 
+        if self.query is None:  # a first step does every first-call set-up; its rows are withdrawn
+            before = self.x.clone()
+            self.step()
+            self.caches[0].advance(-1)
+            self.x.copy_(before)
         stream = torch.cuda.Stream(device=self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
         self.graph = torch.cuda.CUDAGraph()
