@@ -653,8 +653,8 @@ UCB_API int ucb_block8_write(const ucb_block8_cache* cache, const void* key_dev,
                              int64_t value_stride_head, int64_t rows, const int32_t* starts_dev, void* stream);
 
 /* The restored last rows of every sequence (as above) in dtype, contiguous
- * [rows, kv_heads, head_dim], 16-byte aligned; a row that a write would
- * refuse is NaN and sets device error bit 2. */
+ * [rows, kv_heads, head_dim], 16-byte aligned; the rows of a sequence with a bad
+ * length or range and of a block outside the pool are NaN and set device error bit 2. */
 UCB_API int ucb_block8_read(const ucb_block8_cache* cache, int64_t rows, const int32_t* starts_dev, void* key_out_dev,
                             void* value_out_dev, void* stream);
 

@@ -38,10 +38,12 @@
 // a logit plus a logarithm, which would round the scale to the spacing of fp32 at the logit.
 //
 // Measured (B200, device): 1.07 GB of codes (32 x 32768 tokens, 4 KV heads of
-// 128) in 173-176 us, 6.2 TB/s, 95% of the copy rate (194 us over 0.15 s,
-// where the card is at its power cap); 135 MB in 33 us, of which the stream
-// takes 18; 404 MB at head_dim 64 in 74 us (483 instructions a step of 16 tokens
-// and half the bytes); one sequence of 700 tokens 9.1 us.
+// 128) in 173-177 us a call over a dozen calls, 6.2 TB/s, 94% of the copy rate; 194 us over 0.15 s and 207 over two
+// seconds (79%), where the card is at its power cap and its clock at 1.65 GHz.  135 MB in 33 us, of which the stream
+// takes 18; 404 MB at head_dim 64, 48 ragged sequences, in 74 us, of which the stream takes 62; one sequence of 700
+// tokens 9.0 us.  16 tokens cost 479 warp instructions at 128 channels and 253 at 64 (two tiles a step), prologue and merges
+// included.  Both halves of a weight in fp16 (22 bits) take 183 us instead of 174 for the gigabyte, 34.9 instead
+// of 33.3 for 135 MB and 76.5 instead of 74: below the outputs' own rounding, so the weights have one.
 #include <algorithm>
 
 #include "block8.cuh"
@@ -69,8 +71,8 @@ struct AttnParams {
 
 constexpr int TILE = 16;  // tokens of one matrix product
 // Steps that the start of a pair costs a warp, in the flat order.  Device time with 0, 2, 4 and 8 of them: 8 sequences of up
-// to 5003 tokens x 4 queries 29.9, 20.4, 20.4 and 20.6 us; 48 of 1 to 16384 tokens 84.5, 75.5, 74.4 and 75.3; 32 equal
-// ones 35.1, 33.3, 32.9 and 32.7; one length of 131072 tokens 176, 173, 173 and 174.
+// to 5003 tokens x 4 queries 31.4, 20.7, 20.9 and 21.0 us; 48 of 1 to 16384 tokens 83.4, 74.4, 73.8 and 74.4; 16 of 8192
+// 35.3, 33.2, 32.9 and 32.9; 32 of 32768 174.7, 172.6, 172.5 and 172.7.
 constexpr int START = 4;
 constexpr int CTAS_PER_SM = 2;
 constexpr float LIFT = 6.f;        // log2 of the largest scaled weight when the output's unit is set
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(Shape<D, NT, U, OWN>::WARPS * 32, OWN ? 1 : 2)
     };
     // After step i, whose slot every lane has read: the step STAGES after it goes into that slot, and step i + 1 is waited
     // for.  Where all warps stream, one slot less is in flight: that uses the bandwidth up, and a deeper queue only makes
-    // every first access wait (172 us against 187 for a gigabyte).  A pair on its own waits for round trips.
+    // every first access wait (172.5 us against 175.4 for a gigabyte).  A pair on its own waits for round trips.
     auto advance = [&](int i) {
       __syncwarp();
       if (!OWN) cp_async_wait<S::STAGES - 2>();
@@ -770,7 +772,7 @@ template <bool BF, int D, int NT> int launch_block(AttnParams& p, int sms, cudaS
   const bool pairs = p.c.block_tokens > TILE;
   if (own) return pairs ? launch_shape<BF, D, NT, 2, true>(p, sms, stream) : launch_shape<BF, D, NT, 1, true>(p, sms, stream);
   // Two tiles a step where the registers hold them: at D = 64 (48 sequences of up to 16384 tokens x 8 heads: 74 us
-  // against 92) and for 16 rows (eight of up to 5003 tokens, four queries each: 20.4 against 22.0).
+  // against 91) and for 16 rows (eight of up to 5003 tokens, four queries each: 20.9 against 21.8).
   if constexpr (D == 64 || NT == 2) {
     if (pairs) return launch_shape<BF, D, NT, 2, false>(p, sms, stream);
   }

@@ -1,8 +1,8 @@
 // Writes to and reads from the 8-bit block cache (ucb_block8_write / _read):
 //   scale = max(amax / 127, 2^-120),  code = clamp(rint(x * (1 / scale)), -127, 127)
-// Memory bound for prompts (2 bytes in and 1 out a value, and back): 45875
-// tokens x 4 heads x 128, keys and values, written in 28.5 us (4.9 TB/s) and
-// restored in 27.5.  One token of each of 32 sequences is a chain of round
+// Prompts move 2 bytes in and 1 out a value, and back: 45880
+// tokens x 4 heads x 128, keys and values, written in 27.5 us (5.1 TB/s, 75% of the issue slots busy) and
+// restored in 27.2 (waiting for table, scale and codes, one after the other).  One token of each of 32 sequences is a chain of round
 // trips: 3.7 us.  A CTA holds a whole block of one head in registers, so each row is
 // read once; the block's largest magnitude and its channels' bounds are reduced
 // through one barrier.
@@ -286,7 +286,7 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
 // holds row i * block_tokens of the call (every such block holds exactly one
 // multiple of block_tokens).
 // Four CTAs a multiprocessor where a block fits 64 registers a thread: store of the
-// prompts above 28.4 us against 30.1 with three.
+// prompts above 27.6 us against 30.5 with three.
 template <bool BF, int D, int BT>
 __global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(const WriteParams p) {
   const ucb_block8_cache& c = p.c;
