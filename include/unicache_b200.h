@@ -701,6 +701,58 @@ UCB_API int ucb_block8_attention(const ucb_block8_cache* cache, const ucb_block8
 UCB_API int ucb_block8_sparse_attention(const ucb_block8_cache* cache, const ucb_block8_attention_args* args, int first,
                                         int recent, void* select_workspace_dev, void* stream);
 
+/* ------------------------------------------------------------------ pool of blocks
+ * No counterpart in the reference (its segments own their memory).  The
+ * blocks of 8-bit block caches that share table and lengths (the layers of a
+ * model), given to sequences and taken back on the device:
+ * block_table[s][0 .. held[s]) name the blocks of sequence s, the entries
+ * behind are -1; references[b] counts the entries that name block b, 0 = free.
+ * Only these calls change table, held and references.  A free block that is taken is
+ * the lowest one, sequences (pairs) and their blocks are served in ascending order.
+ * num_seqs <= 4096; num_blocks < 2^31; block_tokens 16, 32, 64 or 128;
+ * references 16-byte aligned.  What is refused on the device (below) sets device
+ * error bit 2. */
+typedef struct ucb_block_pool {
+  int32_t* block_table; /* [num_seqs, max_blocks] */
+  int32_t* lengths;     /* [num_seqs] */
+  int32_t* held;        /* [num_seqs] */
+  int32_t* references;  /* [num_blocks] */
+  int64_t num_blocks;
+  int32_t num_seqs;
+  int32_t max_blocks;
+  int32_t block_tokens;
+  int32_t reserved;
+} ucb_block_pool;
+
+/* lengths[s] += tokens[s] (int32 [num_seqs] on the device; NULL: `each` for every
+ * sequence), and blocks for what is longer than those that s holds.  Blocks behind
+ * a shorter length stay held.  Where the pool runs out, the length counts all the
+ * same, the entries stay -1 (writes to them are skipped) and the error bit is
+ * set; so it is for a length below 0 (taken as 0) or past the table. */
+UCB_API int ucb_block_pool_advance(const ucb_block_pool* pool, const int32_t* tokens_dev, int each, void* stream);
+
+/* The sequences' entries become -1, their lengths 0; a block that no entry names any more is free.
+ * sequences_dev int32 [count]; one named twice is released once, one outside is skipped (error bit). */
+UCB_API int ucb_block_pool_release(const ucb_block_pool* pool, const int32_t* sequences_dev, int count, void* stream);
+
+/* children[i] becomes a copy of parents[i] (int32 [count], count <= num_seqs): it is released,
+ * shares the parent's complete blocks and gets a block of its own for the incomplete one,
+ * whose rows, scales, bounds and pending rows are copied in every cache.  caches_dev: `layers` descriptors in device
+ * memory that share the pool's table and lengths, kv_heads the largest number of their KV heads.  A pair of a sequence with
+ * itself is nothing.  A pair is skipped (error bit) when it names a sequence outside, a child that an earlier
+ * pair names, a parent that is a child of the call, or a parent whose length its blocks do not hold.  A child for whose block the
+ * pool has no room is left empty (error bit).  workspace: ucb_block_pool_fork_workspace_bytes(count), 16-byte aligned. */
+UCB_API int64_t ucb_block_pool_fork_workspace_bytes(int count);
+UCB_API int ucb_block_pool_fork(const ucb_block_pool* pool, const int32_t* parents_dev, const int32_t* children_dev, int count,
+                                const ucb_block8_cache* caches_dev, int layers, int kv_heads, void* workspace_dev, void* stream);
+
+/* Moves the live blocks to the pool's front: with n of them, the i-th lowest live block at n or behind goes to
+ * the i-th lowest free block in front of n, in every cache; table and references follow.  live_dev int32 [1]: n.
+ * workspace: ucb_block_pool_compact_workspace_bytes(pool), 4-byte aligned. */
+UCB_API int64_t ucb_block_pool_compact_workspace_bytes(const ucb_block_pool* pool);
+UCB_API int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_block8_cache* caches_dev, int layers, int kv_heads,
+                                   int32_t* live_dev, void* workspace_dev, void* stream);
+
 /* ------------------------------------------------------------------ self test
  * Checks on the current device that mma.sync f16 consumes fp16 subnormal
  * operands exactly (the decode kernel feeds small integer codes as subnormals).

@@ -27,6 +27,7 @@ from .operators import (
     kivi_fake_quant_value,
 )
 from .storage import (
+    BlockPool,
     CacheMutationResult,
     GQAH2OCache,
     HostPackedKIVI,

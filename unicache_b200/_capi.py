@@ -107,6 +107,20 @@ class UcbBlock8Cache(ctypes.Structure):
     ]
 
 
+class UcbBlockPool(ctypes.Structure):
+    _fields_ = [
+        ("block_table", c_void_p),
+        ("lengths", c_void_p),
+        ("held", c_void_p),
+        ("references", c_void_p),
+        ("num_blocks", c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("block_tokens", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # ucb_head_norm_args and ucb_block8_attention_args in their field order, packed with 0 for a null pointer (a packed
 # record costs 0.7 us a call where as many separate arguments cost 3.4).
 HEAD_NORM_ARGS = struct.Struct("=9Q10q7if")
@@ -197,6 +211,12 @@ SIGNATURES = {
     "ucb_block8_attention_workspace_bytes": (c_int64, [c_void_p, c_int, c_int]),
     "ucb_block8_attention": (c_int, [c_void_p, ctypes.c_char_p, c_void_p]),
     "ucb_block8_sparse_attention": (c_int, [c_void_p, ctypes.c_char_p, c_int, c_int, c_void_p, c_void_p]),
+    "ucb_block_pool_advance": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
+    "ucb_block_pool_release": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
+    "ucb_block_pool_fork_workspace_bytes": (c_int64, [c_int]),
+    "ucb_block_pool_fork": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "ucb_block_pool_compact_workspace_bytes": (c_int64, [c_void_p]),
+    "ucb_block_pool_compact": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "ucb_selftest_mma_subnormal": (c_int, [ctypes.POINTER(c_float), c_void_p]),
     "ucb_host_device_pointer": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "ucb_copy_ranges": (c_int, [c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64),

@@ -1,0 +1,565 @@
+// Blocks of the 8-bit block cache given to sequences, shared, copied and moved
+// (ucb_block_pool_*).  The state is whole numbers on the device: the table, each
+// sequence's length and number of blocks, and for each block how many table
+// entries name it.  A free block (no entry) is always the lowest one, so every
+// result is defined; what has to be found in order is found by one cluster of CTAs
+// that ranks the pool's free blocks.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "block8.cuh"
+
+namespace ucb {
+namespace block8 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int MAX_SEQS = 4096;
+constexpr int EACH = MAX_SEQS / PLAN_THREADS;  // sequences (pairs) a thread
+constexpr int MAX_CLUSTER = 8;
+constexpr int LANE_BLOCKS = 32;  // blocks a lane holds at once, a bit each
+
+struct PoolParams {
+  ucb_block_pool pool;
+  unsigned int* err;
+};
+
+// Sum of the threads' values in front of this one, and of all.
+template <typename V> __device__ __forceinline__ V scan_block(V mine, V* warp_sum, V& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  V v = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
+  __syncthreads();  // warp_sum may still be read
+  if (lane == 31) warp_sum[warp] = v;
+  __syncthreads();
+  V w = lane < PLAN_THREADS / 32 ? warp_sum[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V x = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += x;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const V before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  return v - mine + (warp ? before : 0);
+}
+
+// The references from `first` on, `per` of them: bit i set where block first + i is referred to by no entry.  Blocks past the
+// pool have no bit.
+__device__ __forceinline__ uint32_t free_bits(const int32_t* references, int64_t n, int64_t first, int per) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < LANE_BLOCKS / 4; ++k) {
+    const int64_t at = first + 4 * k;
+    if (4 * k >= per || at >= n) continue;
+    int4 v = make_int4(1, 1, 1, 1);
+    if (at + 4 <= n) {
+      v = *reinterpret_cast<const int4*>(references + at);
+    } else {
+      v.x = references[at];
+      if (at + 1 < n) v.y = references[at + 1];
+      if (at + 2 < n) v.z = references[at + 2];
+    }
+    bits |= ((v.x == 0) | (v.y == 0) << 1 | (v.z == 0) << 2 | (v.w == 0) << 3) << (4 * k);
+  }
+  return bits;
+}
+
+// A cluster's pass over the pool in ascending order: in each round a lane has `per` adjacent blocks.
+struct Pass {
+  int rank, ctas, per;
+  int64_t round_blocks;
+  __device__ explicit Pass(int64_t n) {
+    cg::cluster_group cluster = cg::this_cluster();
+    rank = cluster.block_rank(), ctas = cluster.num_blocks();
+    const int64_t threads = (int64_t)ctas * PLAN_THREADS, each = (n + threads - 1) / threads;
+    per = (int)min((int64_t)LANE_BLOCKS, (each + 3) / 4 * 4);
+    round_blocks = threads * per;
+  }
+  __device__ int64_t first(int64_t round) const {
+    return round * round_blocks + ((int64_t)rank * PLAN_THREADS + threadIdx.x) * per;
+  }
+};
+
+struct RankSpace {
+  int warp_sum[32];
+  int cta_total[2];  // by turns: the peers may still read the last round's
+};
+
+// How many of the round's marked blocks are in front of this thread's `mine`, and the round's in all, over the cluster.
+__device__ __forceinline__ int rank_round(RankSpace& space, const Pass& pass, int mine, int turn, int& total) {
+  int before = scan_block(mine, space.warp_sum, total);
+  if (pass.ctas == 1) return before;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (threadIdx.x == 0) space.cta_total[turn & 1] = total;
+  cluster.sync();
+  total = 0;
+  for (int r = 0; r < pass.ctas; ++r) {
+    const int t = *cluster.map_shared_rank(&space.cta_total[turn & 1], r);
+    if (r < pass.rank) before += t;
+    total += t;
+  }
+  return before;
+}
+
+// ---------------------------------------------------------------- release
+struct ReleaseParams {
+  PoolParams p;
+  const int32_t* sequences;
+};
+
+// One CTA a sequence.  Whoever takes the number of its blocks gives them back, so a sequence named twice is released once.
+__global__ void __launch_bounds__(256) release_kernel(const ReleaseParams q) {
+  const ucb_block_pool& pool = q.p.pool;
+  __shared__ int blocks;
+  const int s = q.sequences[blockIdx.x];
+  if (s < 0 || s >= pool.num_seqs) {
+    if (threadIdx.x == 0) atomicOr(q.p.err, DEVERR_BAD_DESCRIPTOR);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    blocks = min(atomicExch(&pool.held[s], 0), pool.max_blocks);
+    pool.lengths[s] = 0;
+  }
+  __syncthreads();
+  int32_t* row = pool.block_table + (int64_t)s * pool.max_blocks;
+  for (int j = threadIdx.x; j < blocks; j += blockDim.x) {
+    const int b = row[j];
+    row[j] = -1;
+    if (b >= 0 && b < pool.num_blocks) {
+      atomicSub(&pool.references[b], 1);
+    } else {
+      atomicOr(q.p.err, DEVERR_BAD_DESCRIPTOR);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- advance
+struct AdvanceParams {
+  PoolParams p;
+  const int32_t* tokens;
+  int each;
+};
+
+__global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvanceParams q) {
+  const ucb_block_pool& pool = q.p.pool;
+  __shared__ int64_t base[MAX_SEQS], wide_sum[32];  // blocks wanted by the sequences in front of each
+  __shared__ RankSpace space;
+  const int seqs = pool.num_seqs, bt = pool.block_tokens;
+  const Pass pass(pool.num_blocks);
+  int length[EACH], held[EACH], want[EACH];
+  int64_t mine = 0, wanted;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int s = threadIdx.x * EACH + i;
+    length[i] = held[i] = want[i] = 0;
+    if (s >= seqs) continue;
+    const int64_t t = (int64_t)pool.lengths[s] + (q.tokens ? q.tokens[s] : q.each), most = (int64_t)pool.max_blocks * bt;
+    bad |= t < 0 || t > most;
+    length[i] = (int)max((int64_t)0, min(t, (int64_t)0x7fffffff));
+    held[i] = pool.held[s];
+    want[i] = max(0, (int)((min((int64_t)length[i], most) + bt - 1) / bt) - held[i]);
+    mine += want[i];
+  }
+  int64_t at = scan_block(mine, wide_sum, wanted);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int s = threadIdx.x * EACH + i;
+    if (s < seqs) base[s] = at;
+    at += want[i];
+  }
+  __syncthreads();
+  int64_t found = 0;
+  for (int round = 0; found < wanted && round * pass.round_blocks < pool.num_blocks; ++round) {
+    const int64_t first = pass.first(round);
+    uint32_t bits = free_bits(pool.references, pool.num_blocks, first, pass.per);
+    int total;
+    int64_t r = found + rank_round(space, pass, __popc(bits), round, total);
+    for (; bits && r < wanted; bits &= bits - 1, ++r) {
+      int lo = 0, n = seqs;  // the last sequence whose blocks begin at r or before: the one that wants this one
+      while (n > 1) {
+        const int half = n / 2;
+        if (base[lo + half] <= r) lo += half, n -= half; else n = half;
+      }
+      const int block = (int)(first + __ffs(bits) - 1);
+      pool.references[block] = 1;
+      pool.block_table[(int64_t)lo * pool.max_blocks + pool.held[lo] + (r - base[lo])] = block;
+    }
+    found += total;
+  }
+  if (pass.ctas > 1) cg::this_cluster().sync(); else __syncthreads();  // lengths and numbers of blocks are read
+  if (pass.rank) return;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int s = threadIdx.x * EACH + i;
+    if (s >= seqs) continue;
+    pool.lengths[s] = length[i];
+    const int64_t given = max((int64_t)0, min((int64_t)want[i], found - base[s]));
+    if (given) pool.held[s] = held[i] + (int)given;
+    bad |= given < want[i];
+  }
+  if (bad) atomicOr(q.p.err, DEVERR_BAD_DESCRIPTOR);
+}
+
+// ---------------------------------------------------------------- fork
+struct ForkParams {
+  PoolParams p;
+  const int32_t *parents, *children;
+  int count;
+  int4* jobs;  // of each pair: source and target block of its incomplete block (-1: nothing to copy), parent, child
+};
+
+enum PairState : int { SKIPPED = -2, WHOLE = -1 };  // otherwise the rank of the block that the pair takes
+
+__global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(const ForkParams q) {
+  const ucb_block_pool& pool = q.p.pool;
+  __shared__ int state[MAX_SEQS];      // first the lowest pair that names a sequence as its child, then each pair's state
+  __shared__ int pair_of[MAX_SEQS];    // the pair that takes the block of a rank
+  __shared__ RankSpace space;
+  const int bt = pool.block_tokens, W = pool.max_blocks;
+  const Pass pass(pool.num_blocks);
+  launch_dependents();
+  for (int i = threadIdx.x; i < MAX_SEQS; i += PLAN_THREADS) state[i] = 0x7fffffff;
+  __syncthreads();
+  int parent[EACH], child[EACH], mine[EACH];
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = threadIdx.x * EACH + e;
+    mine[e] = SKIPPED;
+    if (i >= q.count) continue;
+    parent[e] = q.parents[i], child[e] = q.children[i];
+    if (parent[e] < 0 || parent[e] >= pool.num_seqs || child[e] < 0 || child[e] >= pool.num_seqs) {
+      bad = true;
+    } else if (parent[e] != child[e]) {
+      mine[e] = WHOLE;
+      atomicMin(&state[child[e]], i);
+    }
+  }
+  __syncthreads();
+  int copies = 0, wanted;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = threadIdx.x * EACH + e;
+    if (mine[e] == SKIPPED) continue;
+    const int length = pool.lengths[parent[e]];
+    if (state[child[e]] != i || state[parent[e]] != 0x7fffffff || length < 0 || length > (int64_t)W * bt ||
+        (length + bt - 1) / bt > pool.held[parent[e]]) {
+      mine[e] = SKIPPED, bad = true;
+    } else if (length % bt) {
+      mine[e] = copies++;
+    }
+  }
+  const int before = scan_block(copies, space.warp_sum, wanted);  // its barriers: every owner is read
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = threadIdx.x * EACH + e;
+    if (i >= q.count) continue;
+    if (mine[e] >= 0) pair_of[mine[e] += before] = i;
+    state[i] = mine[e];
+  }
+  __syncthreads();
+  // the children's blocks are given back, a warp a pair
+  const int lane = threadIdx.x & 31, warp = pass.rank * (PLAN_THREADS / 32) + (threadIdx.x >> 5);
+  const int warps = pass.ctas * (PLAN_THREADS / 32);
+  for (int i = warp; i < q.count; i += warps) {
+    if (state[i] == SKIPPED) continue;
+    const int c = q.children[i], held = min(pool.held[c], W);
+    int32_t* row = pool.block_table + (int64_t)c * W;
+    for (int j = lane; j < held; j += 32) {
+      const int b = row[j];
+      row[j] = -1;
+      if (b >= 0 && b < pool.num_blocks) atomicSub(&pool.references[b], 1); else bad = true;
+    }
+  }
+  if (pass.ctas > 1) cg::this_cluster().sync(); else __syncthreads();
+  // blocks for the copies
+  int64_t found = 0;
+  for (int round = 0; found < wanted && round * pass.round_blocks < pool.num_blocks; ++round) {
+    const int64_t first = pass.first(round);
+    uint32_t bits = free_bits(pool.references, pool.num_blocks, first, pass.per);
+    int total;
+    int64_t r = found + rank_round(space, pass, __popc(bits), round, total);
+    for (; bits && r < wanted; bits &= bits - 1, ++r) {
+      const int block = (int)(first + __ffs(bits) - 1);
+      pool.references[block] = 1;
+      q.jobs[pair_of[r]].y = block;
+    }
+    found += total;
+  }
+  if (pass.ctas > 1) cg::this_cluster().sync(); else __syncthreads();
+  // the children's rows
+  for (int i = warp; i < q.count; i += warps) {
+    const int s = state[i], from = q.parents[i], to = q.children[i];
+    if (s == SKIPPED) {
+      if (lane == 0) q.jobs[i].y = -1;
+      continue;
+    }
+    const int length = pool.lengths[from], shared = length / bt;
+    const bool fits = s == WHOLE || s < found;
+    const int32_t* source = pool.block_table + (int64_t)from * W;
+    int32_t* row = pool.block_table + (int64_t)to * W;
+    for (int j = lane; fits && j < shared; j += 32) {
+      const int b = source[j];
+      row[j] = b;
+      if (b >= 0 && b < pool.num_blocks) atomicAdd(&pool.references[b], 1); else bad = true;
+    }
+    if (lane == 0) {
+      int4 job = make_int4(-1, -1, from, to);
+      if (s >= 0 && fits) {
+        const int b = source[shared], block = q.jobs[i].y;
+        row[shared] = block;
+        if (b >= 0 && b < pool.num_blocks) job.x = b, job.y = block; else bad = true;
+      }
+      q.jobs[i] = job;
+      pool.lengths[to] = fits ? length : 0;
+      pool.held[to] = fits ? shared + (s >= 0) : 0;
+      bad |= !fits;
+    }
+  }
+  if (bad) atomicOr(q.p.err, DEVERR_BAD_DESCRIPTOR);
+}
+
+// Copies of the bytes of one block, 16 at a time.
+__device__ __forceinline__ void copy16(void* to, const void* from, int64_t bytes, int thread, int threads) {
+  const uint4* src = static_cast<const uint4*>(from);
+  uint4* dst = static_cast<uint4*>(to);
+  const int64_t n = bytes / 16;
+  constexpr int AHEAD = 8;
+  for (int64_t i = thread; i < n; i += (int64_t)AHEAD * threads) {
+    uint4 x[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i + (int64_t)k * threads < n) x[k] = src[i + (int64_t)k * threads];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i + (int64_t)k * threads < n) dst[i + (int64_t)k * threads] = x[k];
+  }
+}
+
+struct ForkCopyParams {
+  const int4* jobs;
+  const int32_t* lengths;
+  const ucb_block8_cache* caches;
+};
+
+// Pair blockIdx.x, layer blockIdx.y; blockIdx.z is a head's keys or values: the rows that count, and the rows themselves
+// with the record of whose they are.
+__global__ void __launch_bounds__(256) fork_copy_kernel(const ForkCopyParams q) {
+  const ucb_block8_cache c = q.caches[blockIdx.y];
+  const int h = blockIdx.z >> 1, value = blockIdx.z & 1;
+  wait_for_primary();
+  const int4 job = q.jobs[blockIdx.x];
+  if (job.y < 0 || h >= c.kv_heads) return;
+  const int rows = q.lengths[job.z] % c.block_tokens;
+  const int64_t block = (int64_t)c.block_tokens * c.head_dim;
+  const int64_t from = (int64_t)job.x * c.kv_heads + h, to = (int64_t)job.y * c.kv_heads + h;
+  int8_t* code = value ? c.value_code : c.key_code;
+  copy16(code + to * block, code + from * block, (int64_t)rows * c.head_dim, threadIdx.x, blockDim.x);
+  char* pending = static_cast<char*>(value ? c.pending_value : c.pending_key);
+  char* pending_to = pending + ((int64_t)job.w * c.kv_heads + h) * block * 2;
+  const char* pending_from = pending + ((int64_t)job.z * c.kv_heads + h) * block * 2;
+  copy16(pending_to, pending_from, (int64_t)rows * c.head_dim * 2, threadIdx.x, blockDim.x);
+  if (!value) {
+    const int64_t record = (int64_t)(c.block_tokens - 1) * c.head_dim * 2;
+    copy16(pending_to + record, pending_from + record, c.head_dim * 2, threadIdx.x, blockDim.x);
+    copy16(c.key_low + to * c.head_dim, c.key_low + from * c.head_dim, c.head_dim, threadIdx.x, blockDim.x);
+    copy16(c.key_high + to * c.head_dim, c.key_high + from * c.head_dim, c.head_dim, threadIdx.x, blockDim.x);
+  }
+  float* scale = value ? c.value_scale : c.key_scale;
+  if (threadIdx.x == 0) scale[to] = scale[from];
+}
+
+// ---------------------------------------------------------------- compact
+struct CompactParams {
+  PoolParams p;
+  int32_t* live;    // the number of live blocks, for the caller
+  int32_t* moves;   // the number of moved ones
+  int32_t* holes;   // targets in ascending order
+  int32_t* movers;  // sources in ascending order
+  int32_t* place;   // of a moved block
+  const ucb_block8_cache* caches;
+  int layers;
+};
+
+__global__ void __launch_bounds__(PLAN_THREADS) compact_kernel(const CompactParams q) {
+  const ucb_block_pool& pool = q.p.pool;
+  __shared__ RankSpace space;
+  const Pass pass(pool.num_blocks);
+  launch_dependents();
+  int64_t live = pool.num_blocks;
+  int turn = 0, total;
+  for (int round = 0; round * pass.round_blocks < pool.num_blocks; ++round) {
+    rank_round(space, pass, __popc(free_bits(pool.references, pool.num_blocks, pass.first(round), pass.per)), turn++, total);
+    live -= total;
+  }
+  // the i-th live block behind the live count goes to the i-th hole in front of it: as many are the ones as the others
+  int64_t holes = 0, movers = 0;
+  for (int round = 0; round * pass.round_blocks < pool.num_blocks; ++round) {
+    const int64_t first = pass.first(round), front = max((int64_t)0, min((int64_t)32, live - first));
+    const int64_t inside = max((int64_t)0, min((int64_t)pass.per, pool.num_blocks - first));
+    const uint32_t before_live = front >= 32 ? 0xffffffffu : (1u << front) - 1, in_pool = inside >= 32 ? 0xffffffffu : (1u << inside) - 1;
+    const uint32_t free = free_bits(pool.references, pool.num_blocks, first, pass.per);
+    uint32_t hole = free & before_live, mover = ~free & in_pool & ~before_live;
+    int64_t r = holes + rank_round(space, pass, __popc(hole), turn++, total);
+    holes += total;
+    for (; hole; hole &= hole - 1, ++r) q.holes[r] = (int)(first + __ffs(hole) - 1);
+    r = movers + rank_round(space, pass, __popc(mover), turn++, total);
+    movers += total;
+    for (; mover; mover &= mover - 1, ++r) q.movers[r] = (int)(first + __ffs(mover) - 1);
+  }
+  if (pass.ctas > 1) cg::this_cluster().sync(); else __syncthreads();
+  for (int64_t i = (int64_t)pass.rank * PLAN_THREADS + threadIdx.x; i < movers; i += (int64_t)pass.ctas * PLAN_THREADS) {
+    const int from = q.movers[i], to = q.holes[i];
+    pool.references[to] = pool.references[from];
+    pool.references[from] = 0;
+    q.place[from] = to;
+  }
+  if (pass.rank == 0 && threadIdx.x == 0) *q.live = (int)live, *q.moves = (int)movers;
+}
+
+// The moved blocks of every layer, keys and values apart, and the table's entries.
+__global__ void __launch_bounds__(256) compact_copy_kernel(const CompactParams q) {
+  const ucb_block_pool& pool = q.p.pool;
+  wait_for_primary();
+  const int live = *q.live, moves = *q.moves;
+  if (moves == 0) return;
+  const int64_t items = (int64_t)moves * q.layers * 2;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int value = item & 1;
+    const int64_t k = (item >> 1) / q.layers;
+    const ucb_block8_cache& c = q.caches[(item >> 1) % q.layers];
+    const int64_t from = q.movers[k], to = q.holes[k], heads = c.kv_heads, block = heads * c.block_tokens * c.head_dim;
+    int8_t* code = value ? c.value_code : c.key_code;
+    int8_t* bound = value ? c.key_high : c.key_low;
+    float* scale = value ? c.value_scale : c.key_scale;
+    copy16(code + to * block, code + from * block, block, threadIdx.x, blockDim.x);
+    copy16(bound + to * heads * c.head_dim, bound + from * heads * c.head_dim, heads * c.head_dim, threadIdx.x, blockDim.x);
+    for (int h = threadIdx.x; h < heads; h += blockDim.x) scale[to * heads + h] = scale[from * heads + h];
+  }
+  for (int s = blockIdx.x; s < pool.num_seqs; s += gridDim.x) {
+    int32_t* row = pool.block_table + (int64_t)s * pool.max_blocks;
+    const int held = min(pool.held[s], pool.max_blocks);
+    for (int j = threadIdx.x; j < held; j += blockDim.x) {
+      const int b = row[j];
+      if (b >= live && b < pool.num_blocks) row[j] = q.place[b];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+int check_pool(const ucb_block_pool* p, const char* what) {
+  using ucb_host::set_error;
+  if (!p || !p->block_table || !p->lengths || !p->held || !p->references)
+    return set_error(UCB_ERR_INVALID, "%s: null pointer", what);
+  if (p->num_seqs < 1 || p->max_blocks < 1 || p->num_blocks < 1) return set_error(UCB_ERR_INVALID, "%s: bad shape", what);
+  if (p->num_seqs > MAX_SEQS) return set_error(UCB_ERR_UNSUPPORTED, "%s: at most %d sequences", what, MAX_SEQS);
+  if (p->num_blocks > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 blocks", what);
+  if (p->block_tokens != 16 && p->block_tokens != 32 && p->block_tokens != 64 && p->block_tokens != 128)
+    return set_error(UCB_ERR_UNSUPPORTED, "%s: block_tokens must be 16, 32, 64 or 128", what);
+  if ((int64_t)p->max_blocks * p->block_tokens > 0x7fffffff)
+    return set_error(UCB_ERR_UNSUPPORTED, "%s: a sequence holds at most 2^31 - 1 tokens", what);
+  if (reinterpret_cast<uintptr_t>(p->references) & 15)
+    return set_error(UCB_ERR_INVALID, "%s: references must be 16-byte aligned", what);
+  return UCB_OK;
+}
+
+// One CTA ranks 32768 blocks at once; the wider cluster serves larger pools.
+int plan_cluster(int64_t blocks) {
+  int ctas = 1;
+  while (ctas < MAX_CLUSTER && (int64_t)ctas * PLAN_THREADS * LANE_BLOCKS < blocks) ctas *= 2;
+  return ctas;
+}
+
+int check_layers(const void* caches, int layers, int kv_heads, const char* what) {
+  if (!caches || layers < 1 || kv_heads < 1) return ucb_host::set_error(UCB_ERR_INVALID, "%s: no caches", what);
+  if (layers > 65535 || kv_heads > 32767)
+    return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "%s: at most 65535 caches of 32767 KV heads", what);
+  if (reinterpret_cast<uintptr_t>(caches) & 7) return ucb_host::set_error(UCB_ERR_INVALID, "%s: caches must be 8-byte aligned", what);
+  return UCB_OK;
+}
+
+}  // namespace
+}  // namespace block8
+}  // namespace ucb
+
+using ucb_host::set_error;
+namespace b8 = ucb::block8;
+
+extern "C" int ucb_block_pool_release(const ucb_block_pool* pool, const int32_t* sequences, int count, void* stream) {
+  const char* what = "ucb_block_pool_release";
+  if (int rc = b8::check_pool(pool, what)) return rc;
+  if (count < 0) return set_error(UCB_ERR_INVALID, "%s: bad count", what);
+  if (count == 0) return UCB_OK;
+  if (!sequences) return set_error(UCB_ERR_INVALID, "%s: null pointer", what);
+  unsigned int* err = ucb_host::device_error_word();
+  if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
+  const b8::ReleaseParams q{{*pool, err}, sequences};
+  return b8::launch(b8::release_kernel, dim3(count), dim3(256), 0, static_cast<cudaStream_t>(stream), q, "block pool release_kernel");
+}
+
+extern "C" int ucb_block_pool_advance(const ucb_block_pool* pool, const int32_t* tokens, int each, void* stream) {
+  const char* what = "ucb_block_pool_advance";
+  if (int rc = b8::check_pool(pool, what)) return rc;
+  unsigned int* err = ucb_host::device_error_word();
+  if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
+  const b8::AdvanceParams q{{*pool, err}, tokens, each};
+  return b8::launch(b8::advance_kernel, dim3(b8::plan_cluster(pool->num_blocks)), dim3(b8::PLAN_THREADS), 0,
+                    static_cast<cudaStream_t>(stream), q, "block pool advance_kernel", b8::plan_cluster(pool->num_blocks));
+}
+
+extern "C" int64_t ucb_block_pool_fork_workspace_bytes(int count) { return count < 0 ? -1 : (int64_t)count * 16; }
+
+extern "C" int ucb_block_pool_fork(const ucb_block_pool* pool, const int32_t* parents, const int32_t* children, int count,
+                                   const ucb_block8_cache* caches, int layers, int kv_heads, void* workspace, void* stream) {
+  const char* what = "ucb_block_pool_fork";
+  if (int rc = b8::check_pool(pool, what)) return rc;
+  if (count < 0 || count > pool->num_seqs) return set_error(UCB_ERR_INVALID, "%s: at most one pair for each sequence", what);
+  if (int rc = b8::check_layers(caches, layers, kv_heads, what)) return rc;
+  if (count == 0) return UCB_OK;
+  if (!parents || !children || !workspace) return set_error(UCB_ERR_INVALID, "%s: null pointer", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_error(UCB_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+  unsigned int* err = ucb_host::device_error_word();
+  if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const b8::ForkParams q{{*pool, err}, parents, children, count, static_cast<int4*>(workspace)};
+  const int ctas = b8::plan_cluster(pool->num_blocks);
+  if (int rc = b8::launch(b8::fork_kernel, dim3(ctas), dim3(b8::PLAN_THREADS), 0, s, q, "block pool fork_kernel", ctas)) return rc;
+  const b8::ForkCopyParams c{q.jobs, pool->lengths, caches};
+  return b8::launch(b8::fork_copy_kernel, dim3(count, layers, 2 * kv_heads), dim3(256), 0, s, c, "block pool fork_copy_kernel", 1, true);
+}
+
+// The number of moves, then holes and movers (half of the pool at most each), then every block's place.
+extern "C" int64_t ucb_block_pool_compact_workspace_bytes(const ucb_block_pool* pool) {
+  if (b8::check_pool(pool, "ucb_block_pool_compact_workspace_bytes")) return -1;
+  return 4 * (4 + 2 * (pool->num_blocks / 2) + pool->num_blocks);
+}
+
+extern "C" int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_block8_cache* caches, int layers, int kv_heads,
+                                      int32_t* live, void* workspace, void* stream) {
+  const char* what = "ucb_block_pool_compact";
+  if (int rc = b8::check_pool(pool, what)) return rc;
+  if (int rc = b8::check_layers(caches, layers, kv_heads, what)) return rc;
+  if (!live || !workspace) return set_error(UCB_ERR_INVALID, "%s: null pointer", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 3) return set_error(UCB_ERR_INVALID, "%s: workspace must be 4-byte aligned", what);
+  unsigned int* err = ucb_host::device_error_word();
+  if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int32_t* w = static_cast<int32_t*>(workspace);
+  const int64_t half = pool->num_blocks / 2;
+  const b8::CompactParams q{{*pool, err}, live, w, w + 4, w + 4 + half, w + 4 + 2 * half, caches, layers};
+  const int ctas = b8::plan_cluster(pool->num_blocks);
+  if (int rc = b8::launch(b8::compact_kernel, dim3(ctas), dim3(b8::PLAN_THREADS), 0, s, q, "block pool compact_kernel", ctas)) return rc;
+  const int sms = ucb_host::multiprocessors();
+  if (sms < 1) return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
+  const int64_t items = std::max<int64_t>(half * layers * 2, pool->num_seqs);
+  const unsigned grid = (unsigned)std::min<int64_t>(items, (int64_t)sms * 8);
+  return b8::launch(b8::compact_copy_kernel, dim3(std::max(1u, grid)), dim3(256), 0, s, q, "block pool compact_copy_kernel", 1, true);
+}

@@ -1,5 +1,6 @@
 """Physical storage layouts and their B200 kernels (counterpart of unicache/storage)."""
 
+from .block_pool import BlockPool
 from .hierarchy import HostPackedKIVI, QuantizedHostArchive, QuantizedWorkingSetTransition, to_host
 from .int8_block import Int8BlockCache
 from .kivi_b200 import (
@@ -20,6 +21,7 @@ from .physical import (
 from .tensor_backend import CacheMutationResult, TensorCacheStorageBackend
 
 __all__ = [
+    "BlockPool",
     "CacheMutationResult",
     "GQAH2OCache",
     "HostPackedKIVI",
