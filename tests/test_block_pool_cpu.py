@@ -32,10 +32,10 @@ def descriptor(**changes):
 def test_bad_pools_are_refused_by_every_entry(changes, message):
     lib, one = _capi.load(), ctypes.c_void_p(4096)
     pool = ctypes.addressof(struct := descriptor(**changes))
-    for rc in (lib.ucb_block_pool_advance(pool, None, 1, None), lib.ucb_block_pool_release(pool, one, 1, None),
-               lib.ucb_block_pool_fork(pool, one, one, 1, one, 1, 4, one, None),
-               lib.ucb_block_pool_compact(pool, one, 1, 4, one, one, None)):
-        assert rc in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED) and message in lib.ucb_last_error().decode()
+    for call in (lambda: lib.ucb_block_pool_advance(pool, None, 1, None), lambda: lib.ucb_block_pool_release(pool, one, 1, None),
+                 lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 1, 4, one, None),
+                 lambda: lib.ucb_block_pool_compact(pool, one, 1, 4, one, one, None)):
+        assert call() in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED) and message in lib.ucb_last_error().decode()
     assert lib.ucb_block_pool_compact_workspace_bytes(pool) == -1
     assert struct is not None
 
@@ -43,18 +43,18 @@ def test_bad_pools_are_refused_by_every_entry(changes, message):
 def test_bad_calls_are_refused():
     lib, one = _capi.load(), ctypes.c_void_p(4096)
     pool = ctypes.addressof(struct := descriptor())
-    for rc, message in (
-            (lib.ucb_block_pool_release(pool, None, 1, None), "null pointer"), (lib.ucb_block_pool_release(pool, one, -1, None), "count"),
-            (lib.ucb_block_pool_fork(pool, one, one, 5, one, 1, 4, one, None), "one pair"),
-            (lib.ucb_block_pool_fork(pool, None, one, 1, one, 1, 4, one, None), "null pointer"),
-            (lib.ucb_block_pool_fork(pool, one, one, 1, None, 1, 4, one, None), "no caches"),
-            (lib.ucb_block_pool_fork(pool, one, one, 1, one, 0, 4, one, None), "no caches"),
-            (lib.ucb_block_pool_fork(pool, one, one, 1, one, 65536, 4, one, None), "65535"),
-            (lib.ucb_block_pool_fork(pool, one, one, 1, one, 1, 4, ctypes.c_void_p(4104), None), "aligned"),
-            (lib.ucb_block_pool_compact(pool, one, 1, 4, None, one, None), "null pointer"),
-            (lib.ucb_block_pool_compact(pool, None, 1, 4, one, one, None), "no caches"),
-            (lib.ucb_block_pool_compact(pool, one, 1, 4, one, ctypes.c_void_p(4098), None), "aligned")):
-        assert rc in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED) and message in lib.ucb_last_error().decode()
+    for call, message in (
+            (lambda: lib.ucb_block_pool_release(pool, None, 1, None), "null pointer"), (lambda: lib.ucb_block_pool_release(pool, one, -1, None), "count"),
+            (lambda: lib.ucb_block_pool_fork(pool, one, one, 5, one, 1, 4, one, None), "one pair"),
+            (lambda: lib.ucb_block_pool_fork(pool, None, one, 1, one, 1, 4, one, None), "null pointer"),
+            (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, None, 1, 4, one, None), "no caches"),
+            (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 0, 4, one, None), "no caches"),
+            (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 65536, 4, one, None), "65535"),
+            (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 1, 4, ctypes.c_void_p(4104), None), "aligned"),
+            (lambda: lib.ucb_block_pool_compact(pool, one, 1, 4, None, one, None), "null pointer"),
+            (lambda: lib.ucb_block_pool_compact(pool, None, 1, 4, one, one, None), "no caches"),
+            (lambda: lib.ucb_block_pool_compact(pool, one, 1, 4, one, ctypes.c_void_p(4098), None), "aligned")):
+        assert call() in (_capi.UCB_ERR_INVALID, _capi.UCB_ERR_UNSUPPORTED) and message in lib.ucb_last_error().decode()
     assert lib.ucb_block_pool_release(pool, None, 0, None) == _capi.UCB_OK  # nothing to do
     assert lib.ucb_block_pool_fork(pool, None, None, 0, one, 1, 4, None, None) == _capi.UCB_OK
     assert lib.ucb_block_pool_fork_workspace_bytes(3) == 48 and lib.ucb_block_pool_compact_workspace_bytes(pool) == 80
