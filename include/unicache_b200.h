@@ -753,6 +753,51 @@ UCB_API int64_t ucb_block_pool_compact_workspace_bytes(const ucb_block_pool* poo
 UCB_API int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_block8_cache* caches_dev, int layers, int kv_heads,
                                    int32_t* live_dev, void* workspace_dev, void* stream);
 
+/* ------------------------------------------------------------------ draft verification
+ * No counterpart in the reference (it decodes one token at a time).  logits
+ * [seqs, drafts_n + 1, vocab] (dtype UCB_BF16, UCB_F16 or UCB_F32; vocabulary contiguous)
+ * are the target's at the drafted tokens and behind the last one; drafts [seqs, drafts_n]
+ * int32, or int64 when drafts_64; draft_probs [seqs, drafts_n, vocab] (probs_dtype) the distributions that they were
+ * drawn from, NULL for tokens that were not drawn; uniforms [seqs, drafts_n + 1] in [0, 1).
+ * temperature [seqs] on the device, or NULL: temperature_all.  counts [seqs]: the first so many drafts of a
+ * sequence are meant (NULL: all; outside 0 .. drafts_n: limited, error bit).
+ *
+ * With p_j = softmax(logits_j / temperature), draft x_j stays while uniforms_j * q_j(x_j) < p_j(x_j) (q = 1 without
+ * draft_probs).  At the first j that falls the next token comes from max(p_j - q_j, 0) (without draft_probs: p_j without
+ * x_j; where nothing is left, p_j), after all of them from the row behind: the first token whose
+ * running sum is above uniforms[drafts_n] times the sum, in 64 bits.  Temperature 0 (or less): a draft stays where it
+ * is the arg max, which is also the next token; the lowest index of equals.  A draft outside the vocabulary falls, the next token
+ * comes from p_j (error bit).  A row with a NaN or an infinity, or without a token above -inf, has no distribution: its draft falls,
+ * a next token from it is -1 (error bit).  Rows, drafts and distributions behind a sequence's count are not read.
+ *
+ * tokens [seqs, drafts_n + 1]: the drafts that stay, the next token, -1 behind; accepted [seqs]: how many stay;
+ * logprobs fp32 [seqs, drafts_n + 1]: ln p of these tokens (at temperature 1 for temperature 0), 0 behind, NaN for a
+ * next token of -1.  lengths (or NULL) [seqs] are lowered by the drafts that fell.  drafts_n <= 31.
+ * workspace: ucb_verify_drafts_workspace_bytes bytes, 16-byte aligned. */
+typedef struct ucb_verify_args {
+  const void* logits;
+  const void* drafts;
+  const void* draft_probs;
+  const float* uniforms;
+  const float* temperature;
+  const int32_t* counts;
+  int32_t* lengths;
+  int32_t* tokens;
+  int32_t* accepted;
+  float* logprobs;
+  void* workspace;
+  int64_t logits_stride_seq, logits_stride_row;
+  int64_t probs_stride_seq, probs_stride_row;
+  int64_t drafts_stride_seq, uniforms_stride_seq;
+  int32_t seqs, drafts_n, vocab;
+  int32_t dtype, probs_dtype;
+  int32_t drafts_64;
+  int32_t reserved;
+  float temperature_all;
+} ucb_verify_args;
+UCB_API int64_t ucb_verify_drafts_workspace_bytes(int seqs, int drafts, int vocab, int dtype);
+UCB_API int ucb_verify_drafts(const ucb_verify_args* args, void* stream);
+
 /* ------------------------------------------------------------------ self test
  * Checks on the current device that mma.sync f16 consumes fp16 subnormal
  * operands exactly (the decode kernel feeds small integer codes as subnormals).

@@ -121,10 +121,11 @@ class UcbBlockPool(ctypes.Structure):
     ]
 
 
-# ucb_head_norm_args and ucb_block8_attention_args in their field order, packed with 0 for a null pointer (a packed
+# ucb_head_norm_args, ucb_block8_attention_args and ucb_verify_args in their field order, packed with 0 for a null pointer (a packed
 # record costs 0.7 us a call where as many separate arguments cost 3.4).
 HEAD_NORM_ARGS = struct.Struct("=9Q10q7if")
 BLOCK8_ATTENTION_ARGS = struct.Struct("=5Q3q3if")
+VERIFY_ARGS = struct.Struct("=11Q6q7if")
 
 # name -> (restype, argtypes); the exact set declared in include/unicache_b200.h.
 SIGNATURES = {
@@ -217,6 +218,8 @@ SIGNATURES = {
     "ucb_block_pool_fork": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "ucb_block_pool_compact_workspace_bytes": (c_int64, [c_void_p]),
     "ucb_block_pool_compact": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "ucb_verify_drafts_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int]),
+    "ucb_verify_drafts": (c_int, [ctypes.c_char_p, c_void_p]),
     "ucb_selftest_mma_subnormal": (c_int, [ctypes.POINTER(c_float), c_void_p]),
     "ucb_host_device_pointer": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "ucb_copy_ranges": (c_int, [c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64),

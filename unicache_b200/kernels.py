@@ -1397,6 +1397,84 @@ def _block8_attend(query, cache, shape, stride, blocks, softmax_scale, select=No
     return out, lse
 
 
+# ---------------------------------------------------------------- draft verification
+@functools.lru_cache(maxsize=1024)
+def _verify_workspace(index: int, seqs: int, drafts: int, vocab: int, dtype: int) -> int:
+    with torch.cuda.device(index):  # the multiprocessors of the device that the launch will be on
+        size = int(_capi.load().ucb_verify_drafts_workspace_bytes(seqs, drafts, vocab, dtype))
+    if size < 0:
+        raise ValueError("verify_drafts takes at most 31 drafts a sequence")
+    return size
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Tensor, *,
+                  draft_probs: torch.Tensor | None = None, temperature: float | torch.Tensor | None = None,
+                  counts: torch.Tensor | None = None, lengths: torch.Tensor | None = None):
+    """Which drafted tokens stay, and the token behind them: (tokens int32 [S, n + 1], accepted int32 [S],
+    logprobs fp32 [S, n + 1]).
+
+    ``logits`` [S, n + 1, V] (bf16, fp16 or fp32): the target's at the n drafted tokens and behind the last one; ``drafts`` int32 or
+    int64 [S, n], n up to 31; ``uniforms`` fp32 [S, n + 1], independent random numbers from [0, 1).  With p_j = softmax(logits_j /
+    temperature) and q_j = ``draft_probs`` [S, n, V], the distributions that the drafts were drawn from at the same temperature, draft
+    x_j stays while uniforms_j q_j(x_j) < p_j(x_j).  At the first one that does not, the next token is drawn from
+    max(p_j - q_j, 0); after all of them from the last row (n = 0: a plain draw).  So the tokens are distributed as the target's own.
+    Without ``draft_probs`` the drafts count as certain (looked up, not drawn): x_j stays with probability p_j(x_j).  The draw
+    takes the first token whose running sum exceeds ``uniforms[:, n]`` times the sum, in 64 bits.
+
+    ``temperature``: a number or fp32 [S], default 1; 0 is greedy: a draft stays where it is the arg max (the lowest index of equals).
+    ``counts`` int32 [S]: how many drafts a sequence has; what lies behind is not read.  ``tokens`` holds the drafts that stay, the next
+    token and -1; ``accepted`` counts the drafts that stay; ``logprobs`` are ln p of these tokens (of temperature 1 for greedy
+    sequences), 0 behind them.  ``lengths`` int32 [S] (``Int8BlockCache.lengths``, which count all drafts) are lowered
+    in place by the drafts that fell.
+
+    A draft outside the vocabulary falls, and logits with a NaN, an infinity or nothing above -inf give the next token -1: both set
+    device error bit 2 (``device_status``), and so does a count outside 0 to n."""
+
+    require_cuda(logits, "logits")
+    index, shape, code = logits.get_device(), logits.shape, dtype_code(logits.dtype)
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1 or (shape[2] > 1 and logits.stride(2) != 1):
+        raise ValueError("logits must be [sequences, drafts + 1, vocabulary] with unit vocabulary stride")
+    seqs, rows, vocab = shape
+    n = rows - 1
+    if drafts.shape != (seqs, n) or drafts.get_device() != index or drafts.dtype not in (torch.int32, torch.int64) \
+            or (n > 1 and drafts.stride(1) != 1):
+        raise ValueError("drafts must be int32 or int64 [sequences, drafts] with unit stride on the logits' device")
+    if uniforms.shape != (seqs, rows) or uniforms.get_device() != index or uniforms.dtype is not torch.float32 \
+            or (n > 0 and uniforms.stride(1) != 1):
+        raise ValueError("uniforms must be float32 [sequences, drafts + 1] with unit stride on the logits' device")
+    probs_at = probs_code = probs_seq = probs_row = 0
+    if draft_probs is not None:
+        if draft_probs.shape != (seqs, n, vocab) or draft_probs.get_device() != index or (vocab > 1 and draft_probs.stride(2) != 1):
+            raise ValueError("draft_probs must be [sequences, drafts, vocabulary] with unit vocabulary stride on the logits' device")
+        if n:
+            probs_at, probs_code = draft_probs.data_ptr(), dtype_code(draft_probs.dtype)
+            probs_seq, probs_row, _ = draft_probs.stride()
+    heat_at, heat = 0, 1.0
+    if isinstance(temperature, torch.Tensor):
+        if temperature.shape != (seqs,) or temperature.get_device() != index or temperature.dtype is not torch.float32 \
+                or not temperature.is_contiguous():
+            raise ValueError("temperature must be a number or a contiguous float32 [sequences] tensor on the logits' device")
+        heat_at = temperature.data_ptr()
+    elif temperature is not None:
+        heat = float(temperature)
+        if not 0.0 <= heat < 3.0e38:
+            raise ValueError("temperature must be finite and not negative")
+    for name, x in (("counts", counts), ("lengths", lengths)):
+        if x is not None and (x.shape != (seqs,) or x.get_device() != index or x.dtype is not torch.int32 or not x.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 [sequences] tensor on the logits' device")
+    workspace = logits.new_empty(_verify_workspace(index, seqs, n, vocab, code), dtype=torch.uint8) if seqs else None
+    tokens, accepted = uniforms.new_empty((seqs, rows), dtype=torch.int32), uniforms.new_empty(seqs, dtype=torch.int32)
+    logprobs = uniforms.new_empty((seqs, rows))
+    if seqs:
+        seq_stride, row_stride, _ = logits.stride()
+        args = _capi.VERIFY_ARGS.pack(
+            logits.data_ptr(), drafts.data_ptr(), probs_at, uniforms.data_ptr(), heat_at, ptr(counts) or 0, ptr(lengths) or 0,
+            tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(), seq_stride, row_stride, probs_seq,
+            probs_row, drafts.stride(0), uniforms.stride(0), seqs, n, vocab, code, probs_code, drafts.dtype is torch.int64, 0, heat)
+        _call_on(index, "ucb_verify_drafts", args, stream_of(logits))
+    return tokens, accepted, logprobs
+
+
 # ---------------------------------------------------------------- host transfers
 def host_device_pointer(host: torch.Tensor) -> int:
     """Device-visible address of a pinned host tensor (mapped pinned memory)."""
