@@ -597,6 +597,18 @@ typedef struct ucb_head_norm_args {
 } ucb_head_norm_args;
 UCB_API int ucb_head_norm_rope(const ucb_head_norm_args* args, void* stream);
 
+/* The same with a position on each of several axes (time, height and width of image and video tokens):
+ * args->positions [count, tokens], an axis every position_stride entries; rotation pair i turns by the position on
+ * axis axis[i / 16] >> 2 (i % 16) & 3, in row positions[axis][t] of the tables.  count 1 to 4, rotary_dim above 0.
+ * Positions on an axis that no pair turns by are not read. */
+typedef struct ucb_rope_axes {
+  int64_t position_stride;
+  uint32_t axis[8];
+  int32_t count;
+  int32_t reserved;
+} ucb_rope_axes;
+UCB_API int ucb_head_norm_rope_axes(const ucb_head_norm_args* args, const ucb_rope_axes* axes, void* stream);
+
 /* ------------------------------------------------------------------ 8-bit block cache
  * No counterpart in the reference (its quantized segments are frozen and
  * grouped along tokens or channels).  Keys and values of num_seqs sequences

@@ -18,7 +18,7 @@ from .adapters import (
     sparse_int8_block_decode,
 )
 from .core import PhysicalCacheRequest
-from .kernels import head_norm_rope, rope_table, verify_drafts
+from .kernels import head_norm_rope, rope_axes, rope_table, verify_drafts
 from .operators import (
     H2OPhysicalGQAOperator,
     KIVIPackedQuantizationOperator,

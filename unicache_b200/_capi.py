@@ -125,6 +125,7 @@ class UcbBlockPool(ctypes.Structure):
 # record costs 0.7 us a call where as many separate arguments cost 3.4).
 HEAD_NORM_ARGS = struct.Struct("=9Q10q7if")
 BLOCK8_ATTENTION_ARGS = struct.Struct("=5Q3q3if")
+ROPE_AXES = struct.Struct("=q8I2i")
 VERIFY_ARGS = struct.Struct("=11Q6q7if")
 
 # name -> (restype, argtypes); the exact set declared in include/unicache_b200.h.
@@ -203,6 +204,7 @@ SIGNATURES = {
     "ucb_compact_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                  ctypes.POINTER(c_int64), c_void_p]),
     "ucb_head_norm_rope": (c_int, [ctypes.c_char_p, c_void_p]),
+    "ucb_head_norm_rope_axes": (c_int, [ctypes.c_char_p, ctypes.c_char_p, c_void_p]),
     "ucb_block8_write": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
                                  c_void_p]),
     "ucb_block8_read": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),

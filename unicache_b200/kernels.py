@@ -1164,6 +1164,32 @@ def rope_table(positions: int, rotary_dim: int, *, theta: float = 10000.0,
     return angle.cos().float(), angle.sin().float()
 
 
+def rope_axes(sections: list, *, alternating: bool = False) -> tuple:
+    """The axis of every rotation pair, for ``head_norm_rope``: ``sections`` pairs by each axis, one after the other, or by
+    turns as long as each of them lasts."""
+
+    sections = [int(n) for n in sections]
+    if not sections or any(n < 0 for n in sections):
+        raise ValueError("sections must be numbers of rotation pairs, one for each axis")
+    if not alternating:
+        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    return tuple(a for turn in range(max(sections)) for a, n in enumerate(sections) if turn < n)
+
+
+@functools.lru_cache(maxsize=256)
+def _packed_axes(axes: tuple, count: int, stride: int) -> bytes:
+    """The ``ucb_rope_axes`` record of checked axes: two bits a pair."""
+
+    if not 1 <= count <= 4:
+        raise ValueError("positions must be [axes, tokens] of 1 to 4 axes")
+    words = [0] * 8
+    for i, axis in enumerate(axes):
+        if not 0 <= axis < count:
+            raise ValueError("axes must name rows of positions")
+        words[i // 16] |= int(axis) << 2 * (i % 16)
+    return _capi.ROPE_AXES.pack(stride, *words, count, 0)
+
+
 _ENTRIES: dict = {}  # bound entry points of the calls below
 
 
@@ -1186,13 +1212,16 @@ def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_w
                    key_weight: torch.Tensor | None = None, cos: torch.Tensor | None = None,
                    sin: torch.Tensor | None = None, positions: torch.Tensor | None = None, *, eps: float = 1e-6,
                    interleaved: bool = False, query_out: torch.Tensor | None = None,
-                   key_out: torch.Tensor | None = None):
+                   key_out: torch.Tensor | None = None, axes: tuple | None = None):
     """RMS norm of every head of query [T, Hq, D] and key [T, Hkv, D] (either may be None), then the
     rotation by row ``positions[t]`` of ``cos`` / ``sin`` (fp32 [P, R / 2], see ``rope_table``):
     channels (i, i + R / 2), or (2i, 2i + 1) when ``interleaved``; channels from R on
     are only normalised.  Weights [D] in the rows' dtype, None = ones; without tables no rotation.
     Token and head strides are free (views of one projection's output), channels contiguous; the
     outputs may be the inputs.  Arithmetic in fp32, one rounding.  Returns (query, key).
+
+    ``axes``, R / 2 numbers (``rope_axes``): ``positions`` is [A, T], positions on up to four axes such as the time, height
+    and width of image and video tokens, and rotation pair i turns by ``positions[axes[i], t]``.
 
     A position outside the tables makes its rows NaN and sets device error bit 2 (``device_status``)."""
 
@@ -1213,6 +1242,8 @@ def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_w
         _norm_side("key", key, key_weight, key_out, index, dtype, tokens, head_dim)
     rotary = table_rows = cos_at = sin_at = positions_at = 0
     wide = False
+    if axes is not None and positions is None:
+        raise ValueError("axes need positions and tables")
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise ValueError("the rotation needs cos, sin and positions")
@@ -1221,7 +1252,15 @@ def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_w
                 or not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError("cos and sin must be contiguous float32 [positions, rotary_dim / 2] tables")
         wide = positions.dtype is torch.int64
-        if not (wide or positions.dtype is torch.int32) or positions.numel() != tokens \
+        if axes is not None:
+            where = positions.shape
+            if not (wide or positions.dtype is torch.int32) or len(where) != 2 or where[1] != tokens \
+                    or (tokens > 1 and positions.stride(1) != 1):
+                raise ValueError("positions must be an int32 or int64 tensor [axes, tokens] with unit token stride")
+            if len(axes) != shape[1]:
+                raise ValueError("axes must name one axis for each rotation pair")
+            axes = _packed_axes(tuple(axes), where[0], positions.stride(0))
+        elif not (wide or positions.dtype is torch.int32) or positions.numel() != tokens \
                 or not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32 or int64 tensor of one entry per token")
         if cos.get_device() != index or sin.get_device() != index or positions.get_device() != index:
@@ -1229,12 +1268,17 @@ def head_norm_rope(query: torch.Tensor | None, key: torch.Tensor | None, query_w
         table_rows, rotary = shape[0], 2 * shape[1]
         if rotary > head_dim:
             raise ValueError("the tables rotate more channels than head_dim")
+        if axes is not None and rotary == 0:
+            raise ValueError("axes need a rotation")
         cos_at, sin_at, positions_at = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
     if tokens:
         args = _capi.HEAD_NORM_ARGS.pack(
             q_at, k_at, q_weight, k_weight, cos_at, sin_at, positions_at, qo_at, ko_at, q_st, q_sh, k_st, k_sh, qo_st,
             qo_sh, ko_st, ko_sh, table_rows, tokens, q_heads, k_heads, head_dim, rotary, interleaved, wide, code, eps)
-        _call_on(index, "ucb_head_norm_rope", args, stream_of(first))
+        if axes is None:
+            _call_on(index, "ucb_head_norm_rope", args, stream_of(first))
+        else:
+            _call_on(index, "ucb_head_norm_rope_axes", args, axes, stream_of(first))
     return query_out, key_out
 
 
