@@ -222,6 +222,37 @@ def test_nothing_left_of_the_target_falls_back_to_it():
     assert accepted.tolist() == [0] * 3
 
 
+@pytest.mark.parametrize("vocab", [257, 5000, 151936])
+def test_draft_distributions_that_are_the_target_but_for_a_few_tokens(vocab):
+    """Most of max(p - q, 0) is then rounding of q, on one side of the border or the other: the draw is over that as well."""
+
+    need_gpu()
+    seqs, n = 12, 1
+    logits, drafts, uniforms, _ = inputs(seqs, n, vocab, seed=vocab, dtype=torch.float32, probs=None)
+    p = torch.softmax(logits[:, :1].double(), -1)
+    q = p.float()
+    for s in range(seqs):
+        order = p[s, 0].argsort(descending=True)
+        a, b = int(order[0]), int(order[1 + 20 * (s % 4)])
+        q[s, 0, a], q[s, 0, b] = p[s, 0, b], p[s, 0, a]  # offered far too often
+        drafts[s, 0] = b
+    uniforms[:, 0] = 1.0 - 2.0 ** -24
+    _, accepted, _ = check(logits, drafts, uniforms, q)
+    assert accepted.tolist() == [0] * seqs
+    for s in range(seqs):  # and nothing but rounding: only the draft is offered a little too often
+        q[s] = p[s].float()
+        q[s, 0, drafts[s, 0]] *= 1.0 + 2.0 ** -18
+    uniforms[:, 1] = torch.linspace(0.01, 0.99, seqs, device="cuda")
+    tokens, accepted, _ = verify_drafts(logits, drafts, uniforms, draft_probs=q)
+    for s in range(seqs):
+        left = (p[s, 0] - q[s, 0].double()).clamp(min=0)
+        if int(accepted[s]) == 0 and float(left.sum()) > 0:
+            # p itself, in 64 bits, is off by 2^-52 of it: as much as 2^-27 of what rounding left
+            running = left.cumsum(0) / left.sum()
+            token, u = int(tokens[s, 0]), float(uniforms[s, 1])
+            assert left[token] > 0 and float(running[token]) >= u - 1e-6 and float(running[token] - left[token] / left.sum()) <= u + 1e-6
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_large_logits_and_temperatures(dtype):
     need_gpu()

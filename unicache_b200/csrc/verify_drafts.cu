@@ -12,6 +12,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "block8.cuh"
 
@@ -22,7 +23,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int MAX_ROWS = 32;  // of a sequence: its drafts and the one behind them
-constexpr int ROW_THREADS = 256, ROW_AHEAD = 4;
+constexpr int ROW_THREADS = 256, ROW_AHEAD = 4, ROW_VECTORS = ROW_THREADS * ROW_AHEAD;  // of a part of a row
 constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_CLUSTER = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -40,55 +41,71 @@ struct VerifyParams {
 };
 
 // A row of the vocabulary as 16-byte vectors from the aligned address at or before its start: vector k holds the elements
-// k * VEC - shift and on; the first and the last one may have places outside.
+// k * VEC - shift and on.  Vectors [full_begin, full_end) lie inside; one before and one behind them may have some elements.
 template <typename T> struct Row {
   static constexpr int VEC = 16 / sizeof(T);
   const T* x;
-  int shift, vocab, vectors;
+  int shift, vocab, vectors, full_begin, full_end;
   __device__ Row(const void* base, int64_t at, int vocab_) : x(static_cast<const T*>(base) + at), vocab(vocab_) {
     shift = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
     vectors = (int)(((int64_t)vocab + shift + VEC - 1) / VEC);
+    full_begin = shift ? 1 : 0;
+    full_end = (int)(((int64_t)vocab + shift) / VEC);
   }
   __device__ __forceinline__ int first(int k) const { return k * VEC - shift; }
-  __device__ __forceinline__ void load(int k, float (&v)[VEC]) const {  // -inf outside
-    const int i = first(k);
-    if (i >= 0 && i + VEC <= vocab) {
-      const uint4 w = *reinterpret_cast<const uint4*>(x + i);
-      if constexpr (sizeof(T) == 2) {
-        v[0] = Dtype<T>::lo(w.x), v[1] = Dtype<T>::hi(w.x), v[2] = Dtype<T>::lo(w.y), v[3] = Dtype<T>::hi(w.y);
-        v[4] = Dtype<T>::lo(w.z), v[5] = Dtype<T>::hi(w.z), v[6] = Dtype<T>::lo(w.w), v[7] = Dtype<T>::hi(w.w);
-      } else {
-        v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
-      }
+  __device__ __forceinline__ uint4 raw(int k) const { return *reinterpret_cast<const uint4*>(x + first(k)); }  // a full one
+  static __device__ __forceinline__ void to_float(uint4 w, float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 2) {
+      v[0] = Dtype<T>::lo(w.x), v[1] = Dtype<T>::hi(w.x), v[2] = Dtype<T>::lo(w.y), v[3] = Dtype<T>::hi(w.y);
+      v[4] = Dtype<T>::lo(w.z), v[5] = Dtype<T>::hi(w.z), v[6] = Dtype<T>::lo(w.w), v[7] = Dtype<T>::hi(w.w);
     } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = i + e >= 0 && i + e < vocab ? Dtype<T>::to_f(x[i + e]) : -INFINITY;
+      v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
     }
+  }
+  static __device__ __forceinline__ uint4 nothing() {  // -inf throughout
+    const uint32_t w = sizeof(T) == 4 ? 0xff800000u : Dtype<T>::code == UCB_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    return make_uint4(w, w, w, w);
+  }
+  // Any vector as bits, -inf outside the row.
+  __device__ __forceinline__ uint4 load(int k) const {
+    if (k >= full_begin && k < full_end) return raw(k);
+    union {
+      uint4 w;
+      T e[VEC];
+    } u;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int i = first(k) + e;
+      u.e[e] = i >= 0 && i < vocab ? x[i] : Dtype<T>::from_f(-INFINITY);
+    }
+    return u.w;
   }
 };
 
-// N elements of a row of draft probabilities from i on, 0 outside the vocabulary.
-template <typename Q, int N> __device__ __forceinline__ void load_probs(const Q* q, int i, int vocab, float (&v)[N]) {
-  constexpr int BYTES = N * sizeof(Q), ALIGN = BYTES < 16 ? BYTES : 16;
-  if (i >= 0 && i + N <= vocab && reinterpret_cast<uintptr_t>(q + i) % ALIGN == 0) {
-    union {
-      uint4 w16[(BYTES + 15) / 16];
-      uint2 w8;
-      Q e[N];
-    } u;
-    if constexpr (BYTES >= 16) {
+// N elements of a row of draft probabilities from i on, as they lie in memory; 0 outside the vocabulary.
+template <typename Q, int N> struct Probs {
+  static constexpr int BYTES = N * sizeof(Q), ALIGN = BYTES < 16 ? BYTES : 16;
+  union {
+    uint4 w16[(BYTES + 15) / 16];
+    uint2 w8;
+    Q e[N];
+  };
+  __device__ __forceinline__ Probs() {}
+  __device__ __forceinline__ void load(const Q* q, int i, int vocab) {
+    if (i >= 0 && i + N <= vocab && reinterpret_cast<uintptr_t>(q + i) % ALIGN == 0) {
+      if constexpr (BYTES >= 16) {
 #pragma unroll
-      for (int k = 0; k < BYTES / 16; ++k) u.w16[k] = reinterpret_cast<const uint4*>(q + i)[k];
+        for (int k = 0; k < BYTES / 16; ++k) w16[k] = reinterpret_cast<const uint4*>(q + i)[k];
+      } else {
+        w8 = *reinterpret_cast<const uint2*>(q + i);
+      }
     } else {
-      u.w8 = *reinterpret_cast<const uint2*>(q + i);
+#pragma unroll
+      for (int k = 0; k < N; ++k) e[k] = i + k >= 0 && i + k < vocab ? q[i + k] : Dtype<Q>::from_f(0.f);
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = Dtype<Q>::to_f(u.e[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = i + e >= 0 && i + e < vocab ? Dtype<Q>::to_f(q[i + e]) : 0.f;
   }
-}
+  __device__ __forceinline__ float operator[](int k) const { return Dtype<Q>::to_f(e[k]); }
+};
 
 __device__ __forceinline__ float temperature_of(const ucb_verify_args& a, int s) { return a.temperature ? a.temperature[s] : a.temperature_all; }
 
@@ -115,75 +132,213 @@ __device__ __forceinline__ void better(float& v, int& i, float v2, int i2) {
   if (v2 > v || (v2 == v && i2 < i)) v = v2, i = i2;
 }
 
-// One CTA a part of a row.
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float low_of(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float high_of(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+
+// One CTA a part of a row, all of it loaded at once: its maximum first, then the exponentials against that.
 template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC, WARPS = ROW_THREADS / 32;
   const ucb_verify_args& a = p.a;
   block8::launch_dependents();
   const int rows = a.drafts_n + 1, split = blockIdx.x % p.splits, r = blockIdx.x / p.splits, s = r / rows, j = r % rows;
   if (j > count_of(a, s)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Row<T> row(a.logits, s * a.logits_stride_seq + j * a.logits_stride_row, a.vocab);
+  const int begin = split * ROW_VECTORS + threadIdx.x;
+  uint4 raw[ROW_AHEAD];
+#pragma unroll
+  for (int u = 0; u < ROW_AHEAD; ++u) {
+    const int k = begin + u * ROW_THREADS;
+    if (k < row.vectors) raw[u] = row.load(k);
+    else raw[u] = Row<T>::nothing();
+  }
   const float temperature = temperature_of(a, s), c = LOG2E / heat_of(temperature);
-  const bool greedy = temperature <= 0.f;
-  const int each = (row.vectors + p.splits - 1) / p.splits, begin = split * each, end = min(row.vectors, begin + each);
-  float top = -INFINITY, sum = 0.f, best_value = -INFINITY;
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < ROW_AHEAD; ++u) {
+    float x[VEC];
+    Row<T>::to_float(raw[u], x);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) top = fmaxf(top, x[e]);
+  }
+  __shared__ float warp_top[WARPS], warp_sum[WARPS];
+  __shared__ int warp_best[WARPS];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, warp_top[w]);
+  const float from = top == -INFINITY ? 0.f : -top;  // where there is nothing above -inf the exponentials are 0, or NaN
+  const uint64_t from2 = pair_of(from, from), c2 = pair_of(c, c);
+  uint64_t sum2 = 0;
+#pragma unroll
+  for (int u = 0; u < ROW_AHEAD; ++u) {
+    float x[VEC];
+    Row<T>::to_float(raw[u], x);
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      const uint64_t y = mul_pair(add_pair(pair_of(x[e], x[e + 1]), from2), c2);
+      sum2 = add_pair(sum2, pair_of(fast_exp2(low_of(y)), fast_exp2(high_of(y))));
+    }
+  }
+  float sum = low_of(sum2) + high_of(sum2);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   int best = 0x7fffffff;
-  for (int k = begin + threadIdx.x; k < end; k += ROW_THREADS * ROW_AHEAD) {
-    float x[ROW_AHEAD][VEC];
+  if (temperature <= 0.f) {  // the first of the largest
 #pragma unroll
-    for (int u = 0; u < ROW_AHEAD; ++u) {
-      if (k + u * ROW_THREADS < end) {
-        row.load(k + u * ROW_THREADS, x[u]);
-      } else {
+    for (int u = ROW_AHEAD - 1; u >= 0; --u) {
+      float x[VEC];
+      Row<T>::to_float(raw[u], x);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[u][e] = -INFINITY;
-      }
+      for (int e = VEC - 1; e >= 0; --e)
+        if (x[e] == top) best = row.first(begin + u * ROW_THREADS) + e;
     }
-    float t = top;
-#pragma unroll
-    for (int u = 0; u < ROW_AHEAD; ++u)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) t = fmaxf(t, x[u][e]);
-    if (greedy) {
-#pragma unroll
-      for (int u = 0; u < ROW_AHEAD; ++u)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (x[u][e] > best_value) best_value = x[u][e], best = row.first(k + u * ROW_THREADS) + e;
-    }
-    if (t > top) sum *= fast_exp2((top - t) * c);
-    top = t;
-    const float from = t == -INFINITY ? 0.f : t;
-#pragma unroll
-    for (int u = 0; u < ROW_AHEAD; ++u)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) sum += fast_exp2((x[u][e] - from) * c);
+    best = __reduce_min_sync(0xffffffffu, best);
   }
-  __shared__ Partial part[WARPS];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(0xffffffffu, top, o), q = __shfl_xor_sync(0xffffffffu, sum, o);
-    if (greedy) {
-      const float v = __shfl_xor_sync(0xffffffffu, best_value, o);
-      const int i = __shfl_xor_sync(0xffffffffu, best, o);
-      better(best_value, best, v, i);
-    }
-    join(top, sum, t, q, c);
-  }
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = {top, sum, best, 0};
+  if (lane == 0) warp_sum[warp] = sum, warp_best[warp] = best;
   __syncthreads();
   if (threadIdx.x) return;
-  for (int w = 1; w < WARPS; ++w) {
-    better(best_value, best, part[w].top, part[w].best);
-    join(top, sum, part[w].top, part[w].sum, c);
-  }
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) sum += warp_sum[w], best = min(best, warp_best[w]);
   p.partials[blockIdx.x] = {top, sum, best, 0};
 }
 
+// exp(d * T^-1) of the draw: 2^(k / 16) from a table, k the nearest whole number of the exponent in sixteenths, times a
+// polynomial in what is left of it (Taylor's to the fifth power, off by 1.4e-13 at most).  12 instructions of the fp64
+// pipe with the sum, against some 20 of the library's, which takes any argument.
+struct Exponential {
+  double top, scale;  // 16 log2(e) / T
+  float floor;        // below it, e^-700 of the largest, is nothing
+  const double* table;
+  __device__ Exponential(float top_, double inverse, const double* table_) : top(top_), table(table_) {
+    scale = inverse * (16.0 * 1.4426950408889634074);
+    floor = fmaxf(__double2float_ru(top - 700.0 / inverse), -3.40282347e38f);
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    constexpr double A = 0.69314718055994530942 / 16.0, MAGIC = 6755399441055744.0;  // 1.5 * 2^52: its last bit is 1
+    const double d = (double)fmaxf(x, floor) - top, t = fma(d, scale, MAGIC), f = fma(d, scale, MAGIC - t);
+    const int k = __double2loint(t);
+    double e = fma(f, A * A * A * A * A / 120.0, A * A * A * A / 24.0);
+    e = fma(f, e, A * A * A / 6.0);
+    e = fma(f, e, A * A / 2.0);
+    e = fma(f, e, A);
+    e = fma(f, e, 1.0);
+    const double step = table[k & 15];
+    e *= __hiloint2double(__double2hiint(step) + (k >> 4 << 20), __double2loint(step));
+    return x < floor ? 0.0 : e;
+  }
+};
+
 enum Weights { ALL, LEFT, OTHERS };  // p; what the draft's distribution leaves of it; p without the draft
 
+// Of some elements: the sum of their e; and for LEFT what remains of them, the e of those of which something does, and the e
+// of those next to the border.
+struct __align__(16) Sums {
+  double all, left, e_left, border;
+};
+
+// Whether something remains: above 0, or no number.  By the bits, no compare on the fp64 pipe.
+__device__ __forceinline__ bool remains(double rest) { return ((uint32_t)__double2hiint(rest) ^ 0x80000000u) > 0x7ff00000u; }
+
+// The weight of summed elements; `correction` is the right unit less the one that they were summed with.
+__device__ __forceinline__ double weight_of(const Sums& s, Weights kind, double correction) {
+  return kind != LEFT ? s.all : s.e_left == 0.0 ? s.left : fma(s.e_left, correction, s.left);
+}
+
+struct Verdict {
+  double unit, correction, total, before;  // before: the weight in front of the owner's part
+  int owner;                               // the part that holds the drawn token; -1: none
+  Weights kind;
+  bool again;
+};
+
+// One warp: from the sums of all parts, the part with the drawn token, or that the pass has to be made again.
+__device__ void judge(const Sums* sums, int parts, Weights kind, double unit, double share, bool first_time, Verdict& verdict) {
+  constexpr int EACH = DRAW_WARPS * DRAW_CLUSTER / 32;
+  const int lane = threadIdx.x & 31;
+  Sums s = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (lane * EACH + i < parts) {
+      const Sums x = sums[lane * EACH + i];
+      s.all += x.all, s.left += x.left, s.e_left += x.e_left, s.border += x.border;
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.all += __shfl_xor_sync(0xffffffffu, s.all, o);
+    s.left += __shfl_xor_sync(0xffffffffu, s.left, o);
+    s.e_left += __shfl_xor_sync(0xffffffffu, s.e_left, o);
+    s.border += __shfl_xor_sync(0xffffffffu, s.border, o);
+  }
+  double right = unit;
+  bool again = false;
+  if (kind == LEFT) {
+    right = 1.0 / s.all;
+    // elements within 2^-21 of the border were summed apart: what they may be off by has to be below 2^-36 of the whole, and the
+    // fp32 sum no further off
+    constexpr double NEAR = 1.0 / (1 << 21), NOTHING = NEAR / (1 << 15);
+    const bool none = s.e_left == 0.0 && s.left == 0.0;
+    again = first_time && (fabs(right - unit) > NEAR * right ||
+                           s.border * right * NEAR > (none ? 0.0 : NOTHING * weight_of(s, kind, right - unit)));
+    if (none && !again) kind = ALL;  // nothing remains: from p itself, whose sums are here
+  } else if (kind == OTHERS && s.all == 0.0) {
+    kind = ALL, again = true;
+  }
+  double v[EACH], all = 0.0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    v[i] = lane * EACH + i < parts ? weight_of(sums[lane * EACH + i], kind, right - unit) : 0.0;
+    all += v[i];
+  }
+  double run = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += x;
+  }
+  const double total = __shfl_sync(0xffffffffu, run, 31), target = share * total;
+  double at = __shfl_up_sync(0xffffffffu, run, 1);
+  if (lane == 0) at = 0.0;
+  // the first part that reaches above the target; where rounding leaves none, the last one with a weight
+  int found = parts, last = -1;
+  double found_at = 0.0, last_at = 0.0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (v[i] > 0.0) {
+      if (found == parts && at + v[i] > target) found = lane * EACH + i, found_at = at;
+      last = lane * EACH + i, last_at = at;
+    }
+    at += v[i];
+  }
+  const int first = __reduce_min_sync(0xffffffffu, found), final = __reduce_max_sync(0xffffffffu, last);
+  const int which = first < parts ? first : final;
+  if (lane == 0) {
+    verdict.unit = right, verdict.correction = right - unit, verdict.total = total, verdict.owner = which;
+    verdict.kind = kind, verdict.again = again;
+  }
+  if (which >= 0 && lane == which / EACH) verdict.before = first < parts ? found_at : last_at;
+}
+
 // One cluster a sequence: the tests, then the next token.
-template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS) verify_draw_kernel(const VerifyParams p) {
+template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS, 2) verify_draw_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC;
   const ucb_verify_args& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
@@ -191,11 +346,34 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = a.drafts_n + 1, count = count_of(a, s);
   __shared__ Partial part[MAX_ROWS];
   __shared__ int accepted_at;
-  __shared__ double warp_sum[2][DRAW_WARPS], all_sum[DRAW_WARPS * DRAW_CLUSTER], drawn[3];
+  __shared__ double sixteenths[16];
+  __shared__ Sums warp_sums[2][DRAW_WARPS], all_sums[DRAW_WARPS * DRAW_CLUSTER];
+  __shared__ Verdict verdict;
   const float temperature = temperature_of(a, s);
   const bool greedy = temperature <= 0.f;
   const float c = LOG2E / heat_of(temperature);
   const double inverse = 1.0 / (double)heat_of(temperature);
+  const T* logits = static_cast<const T*>(a.logits) + s * a.logits_stride_seq;
+  const Q* probs = static_cast<const Q*>(a.draft_probs) + s * a.probs_stride_seq;
+  auto draft_of = [&](int j) {
+    const int64_t at = s * a.drafts_stride_seq + j;
+    return a.drafts_64 ? static_cast<const int64_t*>(a.drafts)[at] : (int64_t)static_cast<const int32_t*>(a.drafts)[at];
+  };
+  // what the tests need of the inputs, a lane a draft: before the rows' sums are there
+  int64_t draft = -1;
+  float draft_logit = 0.f, draft_uniform = 0.f, draft_q = 1.f;
+  bool outside = false;
+  if (warp == 0 && lane < count) {
+    draft = draft_of(lane);
+    draft_uniform = a.uniforms[s * a.uniforms_stride_seq + lane];
+    outside = draft < 0 || draft >= a.vocab;
+    if (!outside) {
+      draft_logit = Dtype<T>::to_f(logits[lane * a.logits_stride_row + draft]);
+      if (a.draft_probs) draft_q = Dtype<Q>::to_f(probs[lane * a.probs_stride_row + draft]);
+    }
+  }
+  const double share = (double)a.uniforms[s * a.uniforms_stride_seq + a.drafts_n];
+  if (threadIdx.x < 16) sixteenths[threadIdx.x] = exp2(threadIdx.x / 16.0);
   block8::wait_for_primary();
   for (int j = warp; j <= count; j += DRAW_WARPS) {
     float top = -INFINITY, sum = 0.f, best_value = -INFINITY;
@@ -216,51 +394,40 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
     if (lane == 0) part[j] = {top, sum, best, 0};
   }
   __syncthreads();
-  // ---- the drafts, a lane each
-  const T* logits = static_cast<const T*>(a.logits) + s * a.logits_stride_seq;
-  const Q* probs = static_cast<const Q*>(a.draft_probs) + s * a.probs_stride_seq;
-  auto draft_of = [&](int j) {
-    const int64_t at = s * a.drafts_stride_seq + j;
-    return a.drafts_64 ? static_cast<const int64_t*>(a.drafts)[at] : (int64_t)static_cast<const int32_t*>(a.drafts)[at];
-  };
-  auto logprob_of = [&](int j, int64_t x) {
-    return ((double)Dtype<T>::to_f(logits[j * a.logits_stride_row + x]) - (double)part[j].top) * inverse - log((double)part[j].sum);
-  };
+  // ---- the drafts
+  auto logprob_of = [&](int j, float x) { return ((double)x - (double)part[j].top) * inverse - log((double)part[j].sum); };
   if (warp == 0) {
-    bool stays = false, outside = false;
-    int64_t x = -1;
-    double logprob = 0.0;
-    if (lane < count) {
-      x = draft_of(lane);
-      outside = x < 0 || x >= a.vocab;
-      if (!outside) {
-        logprob = logprob_of(lane, x);
-        const double q = a.draft_probs ? (double)Dtype<Q>::to_f(probs[lane * a.probs_stride_row + x]) : 1.0;
-        stays = greedy ? x == part[lane].best && part[lane].sum < INFINITY : (double)a.uniforms[s * a.uniforms_stride_seq + lane] * q < exp(logprob);
-      }
+    bool stays = false;
+    if (lane < count && !outside) {
+      const Partial& x = part[lane];
+      // the sum is off by some 1e-7 in any case, and so may the exponential be
+      stays = greedy ? draft == x.best && x.sum < INFINITY
+                     : (double)draft_uniform * draft_q * (double)x.sum < (double)fast_exp2((draft_logit - x.top) * c);
     }
     const unsigned falls = ~__ballot_sync(0xffffffffu, stays);
     const int accepted = min(count, falls ? __ffs(falls) - 1 : 32);
     if (lane == 0) accepted_at = accepted;
-    if (rank == 0) {
-      if (lane < rows && lane != accepted) {
-        a.tokens[s * rows + lane] = lane < accepted ? (int)x : -1;
-        a.logprobs[s * rows + lane] = lane < accepted ? (float)logprob : 0.f;
-      }
-      if (lane == 0) {
-        a.accepted[s] = accepted;
-        if (a.lengths) a.lengths[s] -= count - accepted;
-        if (a.counts && a.counts[s] != count) outside = true;
-      }
-      if (outside && lane <= accepted) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-    }
   }
   __syncthreads();
+  if (rank == 0 && warp == 0) {
+    const int accepted = accepted_at;
+    if (lane < rows && lane != accepted) {
+      a.tokens[s * rows + lane] = lane < accepted ? (int)draft : -1;
+      a.logprobs[s * rows + lane] = lane < accepted ? (float)logprob_of(lane, draft_logit) : 0.f;
+    }
+    if (lane == 0) {
+      a.accepted[s] = accepted;
+      if (a.lengths) a.lengths[s] -= count - accepted;
+      if (a.counts && a.counts[s] != count) outside = true;
+    }
+    if (outside && lane <= accepted) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+  }
   const int j = accepted_at;
   const float sum = part[j].sum;
   auto answer = [&](int token) {
     a.tokens[s * rows + j] = token;
-    a.logprobs[s * rows + j] = token < 0 ? __int_as_float(0x7fffffff) : (float)logprob_of(j, token);
+    a.logprobs[s * rows + j] =
+        token < 0 ? __int_as_float(0x7fffffff) : (float)logprob_of(j, Dtype<T>::to_f(logits[j * a.logits_stride_row + token]));
     if (token < 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
   };
   const bool none = !(sum > 0.f && sum < INFINITY);  // a NaN or an infinity among the logits, or nothing but -inf
@@ -268,145 +435,160 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
     if (rank == 0 && threadIdx.x == 0) answer(none ? -1 : part[j].best);
     return;
   }
-  // ---- the draw, over the whole row in fp64
+  // ---- the draw, over the whole row in fp64: a thread has `each` adjacent vectors
   const Row<T> row(logits, j * a.logits_stride_row, a.vocab);
   const Q* left = probs + j * a.probs_stride_row;
-  const int64_t draft = j < count ? draft_of(j) : -1;
-  const bool named = draft >= 0 && draft < a.vocab;
-  Weights kind = !named ? ALL : a.draft_probs ? LEFT : OTHERS;
-  const double top = part[j].top;
-  double unit = 1.0;  // 1 / the sum of the exponentials, where p itself is needed
-  const int parts = ctas * DRAW_WARPS, mine = rank * DRAW_WARPS + warp, each = (row.vectors + parts - 1) / parts;
-  const int begin = min(row.vectors, mine * each), end = min(row.vectors, begin + each);
-  auto weights = [&](int k, Weights of, double (&w)[VEC]) {
-    float x[VEC], q[VEC];
-    row.load(k, x);
-    if (of == LEFT) load_probs<Q, VEC>(left, row.first(k), a.vocab, q);
+  const int64_t draft_here = j < count ? draft_of(j) : -1;
+  const int fallen = draft_here >= 0 && draft_here < a.vocab ? (int)draft_here : -1;
+  Weights kind = fallen < 0 ? ALL : a.draft_probs ? LEFT : OTHERS;
+  const Exponential exponential(part[j].top, inverse, sixteenths);
+  const int parts = ctas * DRAW_WARPS, mine = rank * DRAW_WARPS + warp;
+  const int each = (row.vectors + parts * 32 - 1) / (parts * 32);
+  const int begin = min(row.vectors, (mine * 32 + lane) * each), end = min(row.vectors, begin + each);
+  // What the draft leaves of p, max(e / Z - q, 0) with Z the sum of all e, would need a pass for Z first.  The pass takes the fp32
+  // sum instead, 1 / `unit`: as long as the same elements remain, the sums of what they leave and of their e give those for Z
+  // itself.  Elements that are so near to the border that they may change sides are summed too; where they could matter
+  // (they hardly ever do), the pass is made again with Z.
+  double unit = kind == LEFT ? 1.0 / (double)sum : 1.0;
+  Sums mine_sums;
+  for (int turn = 0;; turn ^= 1) {
+    mine_sums = {0.0, 0.0, 0.0, 0.0};
+    uint4 next_x = begin < end ? row.load(begin) : make_uint4(0, 0, 0, 0);
+    Probs<Q, VEC> next_q;
+    if (kind == LEFT && begin < end) next_q.load(left, row.first(begin), a.vocab);
+    for (int k = begin; k < end; ++k) {
+      float x[VEC];
+      Row<T>::to_float(next_x, x);
+      const Probs<Q, VEC> q = next_q;
+      if (k + 1 < end) {
+        next_x = row.load(k + 1);
+        if (kind == LEFT) next_q.load(left, row.first(k + 1), a.vocab);
+      }
+      double e[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[e] = exp(((double)x[e] - top) * inverse);
-      if (of == LEFT) {
-        const double rest = w[e] * unit - (double)q[e];
-        w[e] = rest <= 0.0 ? 0.0 : rest;  // a NaN stays
-      } else if (of == OTHERS && row.first(k) + e == draft) {
-        w[e] = 0.0;
+      for (int i = 0; i < VEC; ++i) e[i] = exponential(x[i]);
+      if (kind == LEFT) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const double qi = (double)q[i], rest = fma(e[i], unit, -qi);
+          if (remains(rest)) mine_sums.left += rest, mine_sums.e_left += e[i];
+          if ((__double2hiint(rest) & 0x7ff00000) + (21 << 20) < (__double2hiint(qi) & 0x7ff00000)) mine_sums.border += e[i];
+        }
+      } else if (kind == OTHERS) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (row.first(k) + i == fallen) e[i] = 0.0;
+      }
+#pragma unroll
+      for (int o = 1; o < VEC; o *= 2)
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2 * o) e[i] += e[i + o];
+      mine_sums.all += e[0];
+    }
+    Sums w = mine_sums;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      w.all += __shfl_xor_sync(0xffffffffu, w.all, o);
+      if (kind == LEFT) {
+        w.left += __shfl_xor_sync(0xffffffffu, w.left, o);
+        w.e_left += __shfl_xor_sync(0xffffffffu, w.e_left, o);
+        w.border += __shfl_xor_sync(0xffffffffu, w.border, o);
       }
     }
-  };
-  int turn = 0;
-  // The sum over the row, and of the parts in front of the one that holds `share` of it; the part.
-  auto add_up = [&](Weights of, double share, double& before, int& owner) {
-    double mine_sum = 0.0;
-    for (int k = begin + lane; k < end; k += 32) {
-      double w[VEC];
-      weights(k, of, w);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) mine_sum += w[e];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine_sum += __shfl_xor_sync(0xffffffffu, mine_sum, o);
-    if (lane == 0) warp_sum[turn][warp] = mine_sum;
+    if (lane == 0) warp_sums[turn][warp] = w;
     cluster.sync();
     for (int i = threadIdx.x; i < parts; i += DRAW_THREADS)
-      all_sum[i] = *cluster.map_shared_rank(&warp_sum[turn][i % DRAW_WARPS], i / DRAW_WARPS);
-    turn ^= 1;
+      all_sums[i] = *cluster.map_shared_rank(&warp_sums[turn][i % DRAW_WARPS], i / DRAW_WARPS);
     __syncthreads();
-    if (warp == 0) {
-      constexpr int EACH = DRAW_WARPS * DRAW_CLUSTER / 32;
-      double v[EACH], lane_sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) v[i] = lane * EACH + i < parts ? all_sum[lane * EACH + i] : 0.0, lane_sum += v[i];
-      double run = lane_sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double x = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += x;
-      }
-      const double total = __shfl_sync(0xffffffffu, run, 31), target = share * total;
-      double at = __shfl_up_sync(0xffffffffu, run, 1);
-      if (lane == 0) at = 0.0;
-      // the first part that reaches above the target; where rounding leaves none, the last one with a weight
-      int found = parts, last = -1;
-      double found_at = 0.0, last_at = 0.0;
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        if (v[i] > 0.0) {
-          if (found == parts && at + v[i] > target) found = lane * EACH + i, found_at = at;
-          last = lane * EACH + i, last_at = at;
-        }
-        at += v[i];
-      }
-      const int first = __reduce_min_sync(0xffffffffu, found), final = __reduce_max_sync(0xffffffffu, last);
-      const int which = first < parts ? first : final;
-      if (lane == 0) drawn[0] = total, drawn[1] = which;
-      __syncwarp();
-      if (which >= 0 && lane == which / EACH) drawn[2] = first < parts ? found_at : last_at;
-    }
+    if (warp == 0) judge(all_sums, parts, kind, unit, share, turn == 0, verdict);
     __syncthreads();
-    const double total = drawn[0];
-    before = drawn[2], owner = (int)drawn[1];
-    return total;
-  };
-  const double share = (double)a.uniforms[s * a.uniforms_stride_seq + a.drafts_n];
-  double before, total;
-  int owner;
-  if (kind == LEFT) unit = 1.0 / add_up(ALL, share, before, owner);
-  total = add_up(kind, share, before, owner);
-  if (kind != ALL && total == 0.0) {  // nothing is left: from p itself
-    kind = ALL;
-    total = add_up(ALL, share, before, owner);
+    kind = verdict.kind, unit = verdict.unit;
+    if (!verdict.again) break;
   }
+  const double total = verdict.total;
   cluster.sync();  // no CTA ends while others read its sums
   if (!(total > 0.0 && total < INFINITY)) {
     if (rank == 0 && threadIdx.x == 0) answer(-1);
     return;
   }
-  if (mine != owner) return;
-  const double target = share * total;
-  double run = before;
-  int last = -1;
-  for (int k0 = begin; k0 < end; k0 += 32) {
-    const int k = k0 + lane;
-    double w[VEC], sum = 0.0;
-    if (k < end) {
-      weights(k, kind, w);
-    } else {
+  if (mine != verdict.owner) return;
+  auto weights = [&](int k, double (&w)[VEC]) {
+    float x[VEC];
+    Probs<Q, VEC> q;
+    Row<T>::to_float(row.load(k), x);
+    if (kind == LEFT) q.load(left, row.first(k), a.vocab);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) w[e] = 0.0;
+    for (int i = 0; i < VEC; ++i) {
+      w[i] = exponential(x[i]);
+      if (kind == LEFT) {
+        const double rest = fma(w[i], unit, -(double)q[i]);
+        w[i] = remains(rest) ? rest : 0.0;
+      } else if (kind == OTHERS && row.first(k) + i == fallen) {
+        w[i] = 0.0;
+      }
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) sum += w[e];
-    double upto = sum;
+  };
+  // ---- the lane, then the token; each time the first that reaches above the target, else the last with a weight
+  const double target = share * total;
+  auto find = [&](double weight, double& at) {  // `at`: in front of the lanes, then of the lane that is found
+    double upto = weight;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    double at = __shfl_up_sync(0xffffffffu, upto, 1);
-    at = run + (lane ? at : 0.0);
-    int token = -1, positive = -1;
+    double mine_at = __shfl_up_sync(0xffffffffu, upto, 1);
+    mine_at = at + (lane ? mine_at : 0.0);
+    const unsigned reach = __ballot_sync(0xffffffffu, weight > 0.0 && mine_at + weight > target);
+    const unsigned some = __ballot_sync(0xffffffffu, weight > 0.0);
+    const int which = reach ? __ffs(reach) - 1 : some ? 31 - __clz(some) : 0;
+    at = __shfl_sync(0xffffffffu, mine_at, which);
+    return make_int2(reach | some ? which : -1, reach != 0);
+  };
+  double at = verdict.before;
+  const int which = max(0, find(weight_of(mine_sums, kind, verdict.correction), at).x);
+  const int from = __shfl_sync(0xffffffffu, begin, which), to = __shfl_sync(0xffffffffu, end, which);
+  int token = -1;
+  for (int k0 = from; k0 < to; k0 += 32) {
+    const int k = k0 + lane;
+    double w[VEC], all = 0.0;
+    if (k < to) {
+      weights(k, w);
+    } else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (w[e] > 0.0) {
-        positive = row.first(k) + e;
-        if (token < 0 && at + w[e] > target) token = positive;
+      for (int e = 0; e < VEC; ++e) w[e] = 0.0;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) all += w[e];
+    double here = at;
+    const int2 found = find(all, here);
+    if (found.x >= 0) {
+      int mine_token = -1;
+      double run = here;
+      bool reached = false;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (w[e] > 0.0 && !reached) {
+          mine_token = row.first(k) + e;
+          reached = run + w[e] > target;
+        }
+        run += w[e];
       }
-      at += w[e];
+      token = __shfl_sync(0xffffffffu, mine_token, found.x);
     }
-    last = max(last, __reduce_max_sync(0xffffffffu, positive));
-    const unsigned found = __ballot_sync(0xffffffffu, token >= 0);
-    if (found) {
-      last = __shfl_sync(0xffffffffu, token, __ffs(found) - 1);
-      break;
-    }
-    run += __shfl_sync(0xffffffffu, upto, 31);
+    if (found.y) break;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    at += all;
   }
-  if (lane == 0) answer(last);
+  if (lane == 0) answer(token);
 }
 
 template <typename T, typename Q> int launch_draw(const VerifyParams& p, cudaStream_t s) {
-  return block8::launch(verify_draw_kernel<T, Q>, dim3((unsigned)p.a.seqs * DRAW_CLUSTER), dim3(DRAW_THREADS), 0, s, p,
-                        "verify_draw_kernel", DRAW_CLUSTER, true);
+  int ctas = DRAW_CLUSTER;
+  while (ctas > 1 && (int64_t)p.a.seqs * ctas > 2 * ucb_host::multiprocessors()) ctas /= 2;
+  return block8::launch(verify_draw_kernel<T, Q>, dim3((unsigned)p.a.seqs * ctas), dim3(DRAW_THREADS), 0, s, p,
+                        "verify_draw_kernel", ctas, true);
 }
 
 template <typename T> int launch_all(const VerifyParams& p, cudaStream_t s) {
@@ -419,13 +601,10 @@ template <typename T> int launch_all(const VerifyParams& p, cudaStream_t s) {
   }
 }
 
-// Parts of a row: CTAs for every multiprocessor, none with less than one round of its threads' loads.
-int splits_of(int64_t rows, int vocab, int dtype) {
-  const int sms = ucb_host::multiprocessors();
-  if (sms < 1) return -1;
-  const int64_t vectors = (vocab + 7) / (dtype == UCB_F32 ? 4 : 8) + 1;
-  const int64_t most = std::max<int64_t>(1, vectors / ROW_THREADS), wanted = (sms * 6 + rows - 1) / rows;
-  return (int)std::min<int64_t>(64, std::min(most, wanted));
+// Parts of a row; one more vector than elements need where rows do not start on 16 bytes.
+int64_t splits_of(int vocab, int dtype) {
+  const int64_t vectors = vocab / (dtype == UCB_F32 ? 4 : 8) + 2;
+  return (vectors + ROW_VECTORS - 1) / ROW_VECTORS;
 }
 
 }  // namespace
@@ -437,8 +616,7 @@ namespace uv = ucb::verify;
 
 extern "C" int64_t ucb_verify_drafts_workspace_bytes(int seqs, int drafts, int vocab, int dtype) {
   if (seqs < 1 || drafts < 0 || drafts >= uv::MAX_ROWS || vocab < 1) return -1;
-  const int splits = uv::splits_of((int64_t)seqs * (drafts + 1), vocab, dtype);
-  return splits < 1 ? -1 : (int64_t)seqs * (drafts + 1) * splits * (int64_t)sizeof(uv::Partial);
+  return (int64_t)seqs * (drafts + 1) * uv::splits_of(vocab, dtype) * (int64_t)sizeof(uv::Partial);
 }
 
 extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
@@ -457,9 +635,9 @@ extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
     return set_error(UCB_ERR_UNSUPPORTED, "%s: unsupported dtype", what);
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
-  const int splits = uv::splits_of((int64_t)a->seqs * (a->drafts_n + 1), a->vocab, a->dtype);
-  if (splits < 1) return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
-  const uv::VerifyParams p{*a, static_cast<uv::Partial*>(a->workspace), splits, err};
+  const int64_t splits = uv::splits_of(a->vocab, a->dtype);
+  if (splits * a->seqs * (a->drafts_n + 1) > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "%s: too many rows or tokens", what);
+  const uv::VerifyParams p{*a, static_cast<uv::Partial*>(a->workspace), (int)splits, err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case UCB_BF16: return uv::launch_all<__nv_bfloat16>(p, s);
