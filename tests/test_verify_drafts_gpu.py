@@ -263,6 +263,21 @@ def test_large_logits_and_temperatures(dtype):
     check((logits + 20000.0).to(dtype), drafts, uniforms, None, heat)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_the_lowest_value_are_uniform(dtype):
+    """A mask of the type's lowest value that leaves nothing; -inf beside it still has no probability."""
+
+    need_gpu()
+    vocab = 700
+    logits = torch.full((40, 2, vocab), torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    logits[20:, :, 10:] = -math.inf
+    drafts = torch.full((40, 1), 3, device="cuda")
+    uniforms = torch.rand(40, 2, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    for heat in (None, 0.2, 30.0, 0.0):
+        tokens, _, _ = check(logits, drafts, uniforms, None, heat)
+        assert (tokens[20:] < 10).all()
+
+
 def test_strides_alignment_and_shared_rows():
     need_gpu()
     seqs, n, vocab = 5, 3, 1001

@@ -24,7 +24,8 @@ namespace cg = cooperative_groups;
 
 constexpr int MAX_ROWS = 32;  // of a sequence: its drafts and the one behind them
 constexpr int ROW_THREADS = 256, ROW_AHEAD = 4, ROW_VECTORS = ROW_THREADS * ROW_AHEAD;  // of a part of a row
-constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_CLUSTER = 8;
+constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_CLUSTER = 8, DRAW_CTAS = 1;
+constexpr float LOWEST = -3.40282347e38f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Partial {
@@ -222,28 +223,47 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
 }
 
 // exp(d * T^-1) of the draw: 2^(k / 16) from a table, k the nearest whole number of the exponent in sixteenths, times a
-// polynomial in what is left of it (Taylor's to the fifth power, off by 1.4e-13 at most).  12 instructions of the fp64
-// pipe with the sum, against some 20 of the library's, which takes any argument.
-struct Exponential {
+// polynomial in what is left of it (Taylor's to the fifth power, off by 1.4e-13 at most).  What is below e^-350 is taken as something
+// between e^-350 and e^-700: with masked elements it is below NOTHING wherever weights are compared.
+constexpr double NOTHING = 1e-145;
+constexpr double SIXTEENTH = 0.69314718055994530942 / 16.0;
+struct Steps {
+  double power[6], magic;
+};
+// The magic number is 1.5 * 2^52, whose last bit is 1.
+__constant__ Steps STEPS = {{1.0, SIXTEENTH, SIXTEENTH * SIXTEENTH / 2.0, SIXTEENTH * SIXTEENTH * SIXTEENTH / 6.0,
+                             SIXTEENTH * SIXTEENTH * SIXTEENTH * SIXTEENTH / 24.0,
+                             SIXTEENTH * SIXTEENTH * SIXTEENTH * SIXTEENTH * SIXTEENTH / 120.0},
+                            6755399441055744.0};
+template <typename T> struct Exponential {
   double top, scale;  // 16 log2(e) / T
-  float floor;        // below it, e^-700 of the largest, is nothing
+  float floor;        // no more than 700 T below the top
+  bool halved;        // of the elements' halves: next to fp32's lowest number nothing lies between an element and -inf
   const double* table;
-  __device__ Exponential(float top_, double inverse, const double* table_) : top(top_), table(table_) {
-    scale = inverse * (16.0 * 1.4426950408889634074);
-    floor = fmaxf(__double2float_ru(top - 700.0 / inverse), -3.40282347e38f);
+  __device__ Exponential(float top_, double heat, const double* table_) : table(table_) {
+    halved = sizeof(T) == 4 && top_ < 0.5f * LOWEST;
+    if (halved) top_ *= 0.5f, heat *= 0.5;
+    top = top_;
+    // where T is so small that the next smaller number is below e^-350 already, any T for which it is will do
+    heat = fmax(heat, (top - (double)nextafterf(top_, -INFINITY)) / 350.0);
+    scale = 16.0 * 1.4426950408889634074 / heat;
+    floor = fmaxf(__double2float_rd(top - 350.0 * heat), LOWEST);
   }
-  __device__ __forceinline__ double operator()(float x) const {
-    constexpr double A = 0.69314718055994530942 / 16.0, MAGIC = 6755399441055744.0;  // 1.5 * 2^52: its last bit is 1
-    const double d = (double)fmaxf(x, floor) - top, t = fma(d, scale, MAGIC), f = fma(d, scale, MAGIC - t);
+  template <int N> __device__ __forceinline__ void prepare(float (&x)[N]) const {
+    if (sizeof(T) == 4 && halved)
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] *= 0.5f;
+  }
+  __device__ __forceinline__ double operator()(float x) const {  // of a prepared element
+    const double d = (double)fmaxf(x, floor) - top, t = fma(d, scale, STEPS.magic), f = fma(d, scale, STEPS.magic - t);
     const int k = __double2loint(t);
-    double e = fma(f, A * A * A * A * A / 120.0, A * A * A * A / 24.0);
-    e = fma(f, e, A * A * A / 6.0);
-    e = fma(f, e, A * A / 2.0);
-    e = fma(f, e, A);
-    e = fma(f, e, 1.0);
+    double e = fma(f, STEPS.power[5], STEPS.power[4]);
+    e = fma(f, e, STEPS.power[3]);
+    e = fma(f, e, STEPS.power[2]);
+    e = fma(f, e, STEPS.power[1]);
+    e = fma(f, e, STEPS.power[0]);
     const double step = table[k & 15];
-    e *= __hiloint2double(__double2hiint(step) + (k >> 4 << 20), __double2loint(step));
-    return x < floor ? 0.0 : e;
+    return e * __hiloint2double(__double2hiint(step) + ((k & ~15) << 16), __double2loint(step));
   }
 };
 
@@ -258,9 +278,88 @@ struct __align__(16) Sums {
 // Whether something remains: above 0, or no number.  By the bits, no compare on the fp64 pipe.
 __device__ __forceinline__ bool remains(double rest) { return ((uint32_t)__double2hiint(rest) ^ 0x80000000u) > 0x7ff00000u; }
 
+// A warp's pass over vectors [begin, end) of a row, the lanes side by side: `load` brings a lane's vector k to a buffer, `use` takes it.
+// Two groups of vectors by turns, one in flight while the other is used; the row's ends, which not every lane has, one by one.
+template <int GROUP, typename Buffer, typename RowT, typename Load, typename Use>
+__device__ __forceinline__ void pass_over(const RowT& row, int begin, int end, Load load, Use use) {
+  const int lane = threadIdx.x & 31, first = max(begin, row.full_begin), last = min(end, row.full_end);
+  const int steps = max(0, last - first + 31) / 32;
+  Buffer a[GROUP], b[GROUP];
+  auto load_group = [&](Buffer(&x)[GROUP], int i) {
+#pragma unroll
+    for (int u = 0; u < GROUP; ++u)
+      if (first + 32 * (i + u) + lane < last) load(x[u], first + 32 * (i + u) + lane);
+  };
+  auto use_group = [&](Buffer(&x)[GROUP], int i) {
+#pragma unroll
+    for (int u = 0; u < GROUP; ++u)
+      if (first + 32 * (i + u) + lane < last) use(x[u], first + 32 * (i + u) + lane);
+  };
+  load_group(a, 0);
+  for (int i = 0; i < steps; i += 2 * GROUP) {
+    load_group(b, i + GROUP);
+    use_group(a, i);
+    load_group(a, i + 2 * GROUP);
+    if (i + GROUP < steps) use_group(b, i + GROUP);
+  }
+  if (lane == 0 && begin == 0 && end > 0 && row.full_begin == 1) load(a[0], 0), use(a[0], 0);
+  if (lane == 0 && end == row.vectors && begin < end && row.full_end >= row.full_begin && row.full_end < row.vectors)
+    load(a[0], row.full_end), use(a[0], row.full_end);
+}
+
+// The e of this lane's share of the warp's vectors [begin, end) without that of element `but`.
+template <typename T> __device__ __forceinline__ Sums sum_others(const Row<T>& row, int begin, int end,
+                                                                 const Exponential<T>& exponential, int but) {
+  constexpr int VEC = Row<T>::VEC;
+  double sum = 0.0;
+  pass_over<2, uint4>(row, begin, end, [&](uint4& raw, int k) { raw = row.load(k); }, [&](const uint4& raw, int k) {
+    float x[VEC];
+    Row<T>::to_float(raw, x);
+    exponential.prepare(x);
+    if ((unsigned)(but - row.first(k)) < VEC)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (row.first(k) + i == but) x[i] = -INFINITY;
+    double e[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = exponential(x[i]);
+#pragma unroll
+    for (int o = 1; o < VEC; o *= 2)
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2 * o) e[i] += e[i + o];
+    sum += e[0];
+  });
+  return {sum, 0.0, 0.0, 0.0};
+}
+
+// The e of this lane's share of them, and what remains of it.
+template <typename T, typename Q> __device__ __forceinline__ Sums sum_left(const Row<T>& row, const Q* left, int begin, int end,
+                                                                           const Exponential<T>& exponential, double unit) {
+  constexpr int VEC = Row<T>::VEC;
+  struct Both {
+    uint4 x;
+    Probs<Q, VEC> q;
+  };
+  Sums s = {0.0, 0.0, 0.0, 0.0};
+  pass_over<1, Both>(row, begin, end, [&](Both& both, int k) { both.x = row.load(k), both.q.load(left, row.first(k), row.vocab); },
+                     [&](const Both& both, int) {
+    float x[VEC];
+    Row<T>::to_float(both.x, x);
+    exponential.prepare(x);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const double e = exponential(x[i]), q = (double)both.q[i], rest = fma(e, unit, -q);
+      s.all += e;
+      if (remains(rest)) s.left += rest, s.e_left += e;
+      if ((__double2hiint(rest) & 0x7ff00000) + (20 << 20) < (__double2hiint(q) & 0x7ff00000)) s.border += e;
+    }
+  });
+  return s;
+}
+
 // The weight of summed elements; `correction` is the right unit less the one that they were summed with.
 __device__ __forceinline__ double weight_of(const Sums& s, Weights kind, double correction) {
-  return kind != LEFT ? s.all : s.e_left == 0.0 ? s.left : fma(s.e_left, correction, s.left);
+  return kind != LEFT ? s.all : fma(s.e_left, correction, s.left);
 }
 
 struct Verdict {
@@ -292,14 +391,14 @@ __device__ void judge(const Sums* sums, int parts, Weights kind, double unit, do
   bool again = false;
   if (kind == LEFT) {
     right = 1.0 / s.all;
-    // elements within 2^-21 of the border were summed apart: what they may be off by has to be below 2^-36 of the whole, and the
-    // fp32 sum no further off
-    constexpr double NEAR = 1.0 / (1 << 21), NOTHING = NEAR / (1 << 15);
-    const bool none = s.e_left == 0.0 && s.left == 0.0;
-    again = first_time && (fabs(right - unit) > NEAR * right ||
-                           s.border * right * NEAR > (none ? 0.0 : NOTHING * weight_of(s, kind, right - unit)));
+    // elements within 2^-20 of the border were summed apart: what they may be off by together has to be below 2^-35 of the
+    // whole, and the fp32 sum no further off than they were looked for
+    constexpr double NEAR = 1.0 / (1 << 20), TOLERATED = NEAR / (1 << 15);
+    const bool none = s.left < NOTHING;
+    const double off = fabs(right - unit) / right, whole = none ? 0.0 : weight_of(s, kind, right - unit);
+    again = first_time && (off > NEAR || s.border * right * off > TOLERATED * whole);
     if (none && !again) kind = ALL;  // nothing remains: from p itself, whose sums are here
-  } else if (kind == OTHERS && s.all == 0.0) {
+  } else if (kind == OTHERS && s.all < NOTHING) {
     kind = ALL, again = true;
   }
   double v[EACH], all = 0.0;
@@ -322,7 +421,7 @@ __device__ void judge(const Sums* sums, int parts, Weights kind, double unit, do
   double found_at = 0.0, last_at = 0.0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    if (v[i] > 0.0) {
+    if (v[i] > NOTHING) {
       if (found == parts && at + v[i] > target) found = lane * EACH + i, found_at = at;
       last = lane * EACH + i, last_at = at;
     }
@@ -338,7 +437,7 @@ __device__ void judge(const Sums* sums, int parts, Weights kind, double unit, do
 }
 
 // One cluster a sequence: the tests, then the next token.
-template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS, 2) verify_draw_kernel(const VerifyParams p) {
+template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS, DRAW_CTAS) verify_draw_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC;
   const ucb_verify_args& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
@@ -349,6 +448,8 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   __shared__ double sixteenths[16];
   __shared__ Sums warp_sums[2][DRAW_WARPS], all_sums[DRAW_WARPS * DRAW_CLUSTER];
   __shared__ Verdict verdict;
+  __shared__ int firsts[DRAW_WARPS], lasts[DRAW_WARPS], fallback_token;
+  __shared__ float fallback_logit;
   const float temperature = temperature_of(a, s);
   const bool greedy = temperature <= 0.f;
   const float c = LOG2E / heat_of(temperature);
@@ -372,7 +473,7 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
       if (a.draft_probs) draft_q = Dtype<Q>::to_f(probs[lane * a.probs_stride_row + draft]);
     }
   }
-  const double share = (double)a.uniforms[s * a.uniforms_stride_seq + a.drafts_n];
+  const double share = fmax((double)a.uniforms[s * a.uniforms_stride_seq + a.drafts_n], 1e-130);  // 0: what is above NOTHING
   if (threadIdx.x < 16) sixteenths[threadIdx.x] = exp2(threadIdx.x / 16.0);
   block8::wait_for_primary();
   for (int j = warp; j <= count; j += DRAW_WARPS) {
@@ -424,68 +525,34 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   }
   const int j = accepted_at;
   const float sum = part[j].sum;
-  auto answer = [&](int token) {
+  auto answer = [&](int token, float logit) {
     a.tokens[s * rows + j] = token;
-    a.logprobs[s * rows + j] =
-        token < 0 ? __int_as_float(0x7fffffff) : (float)logprob_of(j, Dtype<T>::to_f(logits[j * a.logits_stride_row + token]));
+    a.logprobs[s * rows + j] = token < 0 ? __int_as_float(0x7fffffff) : (float)logprob_of(j, logit);
     if (token < 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
   };
   const bool none = !(sum > 0.f && sum < INFINITY);  // a NaN or an infinity among the logits, or nothing but -inf
   if (none || greedy) {
-    if (rank == 0 && threadIdx.x == 0) answer(none ? -1 : part[j].best);
+    if (rank == 0 && threadIdx.x == 0) answer(none ? -1 : part[j].best, part[j].top);
     return;
   }
-  // ---- the draw, over the whole row in fp64: a thread has `each` adjacent vectors
+  // ---- the draw, over the whole row in fp64: a warp has `each` adjacent vectors
   const Row<T> row(logits, j * a.logits_stride_row, a.vocab);
   const Q* left = probs + j * a.probs_stride_row;
   const int64_t draft_here = j < count ? draft_of(j) : -1;
   const int fallen = draft_here >= 0 && draft_here < a.vocab ? (int)draft_here : -1;
   Weights kind = fallen < 0 ? ALL : a.draft_probs ? LEFT : OTHERS;
-  const Exponential exponential(part[j].top, inverse, sixteenths);
+  const Exponential<T> exponential(part[j].top, (double)heat_of(temperature), sixteenths);
   const int parts = ctas * DRAW_WARPS, mine = rank * DRAW_WARPS + warp;
-  const int each = (row.vectors + parts * 32 - 1) / (parts * 32);
-  const int begin = min(row.vectors, (mine * 32 + lane) * each), end = min(row.vectors, begin + each);
+  const int each = (row.vectors + parts - 1) / parts;
+  auto begin_of = [&](int part) { return (int)min((int64_t)row.vectors, (int64_t)part * each); };
   // What the draft leaves of p, max(e / Z - q, 0) with Z the sum of all e, would need a pass for Z first.  The pass takes the fp32
   // sum instead, 1 / `unit`: as long as the same elements remain, the sums of what they leave and of their e give those for Z
   // itself.  Elements that are so near to the border that they may change sides are summed too; where they could matter
   // (they hardly ever do), the pass is made again with Z.
   double unit = kind == LEFT ? 1.0 / (double)sum : 1.0;
-  Sums mine_sums;
   for (int turn = 0;; turn ^= 1) {
-    mine_sums = {0.0, 0.0, 0.0, 0.0};
-    uint4 next_x = begin < end ? row.load(begin) : make_uint4(0, 0, 0, 0);
-    Probs<Q, VEC> next_q;
-    if (kind == LEFT && begin < end) next_q.load(left, row.first(begin), a.vocab);
-    for (int k = begin; k < end; ++k) {
-      float x[VEC];
-      Row<T>::to_float(next_x, x);
-      const Probs<Q, VEC> q = next_q;
-      if (k + 1 < end) {
-        next_x = row.load(k + 1);
-        if (kind == LEFT) next_q.load(left, row.first(k + 1), a.vocab);
-      }
-      double e[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = exponential(x[i]);
-      if (kind == LEFT) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const double qi = (double)q[i], rest = fma(e[i], unit, -qi);
-          if (remains(rest)) mine_sums.left += rest, mine_sums.e_left += e[i];
-          if ((__double2hiint(rest) & 0x7ff00000) + (21 << 20) < (__double2hiint(qi) & 0x7ff00000)) mine_sums.border += e[i];
-        }
-      } else if (kind == OTHERS) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (row.first(k) + i == fallen) e[i] = 0.0;
-      }
-#pragma unroll
-      for (int o = 1; o < VEC; o *= 2)
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2 * o) e[i] += e[i + o];
-      mine_sums.all += e[0];
-    }
-    Sums w = mine_sums;
+    Sums w = kind == LEFT ? sum_left<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, unit)
+                      : sum_others<T>(row, begin_of(mine), begin_of(mine + 1), exponential, kind == OTHERS ? fallen : -1);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       w.all += __shfl_xor_sync(0xffffffffu, w.all, o);
@@ -506,87 +573,97 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
     if (!verdict.again) break;
   }
   const double total = verdict.total;
-  cluster.sync();  // no CTA ends while others read its sums
-  if (!(total > 0.0 && total < INFINITY)) {
-    if (rank == 0 && threadIdx.x == 0) answer(-1);
-    return;
-  }
-  if (mine != verdict.owner) return;
-  auto weights = [&](int k, double (&w)[VEC]) {
-    float x[VEC];
-    Probs<Q, VEC> q;
-    Row<T>::to_float(row.load(k), x);
-    if (kind == LEFT) q.load(left, row.first(k), a.vocab);
+  cluster.barrier_arrive();  // this CTA has read the others' sums
+  if (!(total > NOTHING && total < INFINITY)) {
+    if (rank == 0 && threadIdx.x == 0) answer(-1, 0.f);
+  } else if (verdict.owner / DRAW_WARPS == rank) {
+    // ---- the token, in the part that holds it: a warp for each 32 of its vectors.  Each time what is looked for is the first
+    // that reaches above the target, or where rounding leaves none, the last with a weight.
+    const double target = share * total;
+    const int begin = begin_of(verdict.owner), end = begin_of(verdict.owner + 1);
+    double before = verdict.before;
+    int last = -1;  // the last with a weight so far: every warp's the same
+    for (int base = begin; base < end; base += DRAW_THREADS) {
+      const int k = base + threadIdx.x;
+      double w[VEC], all = 0.0;
+      float x[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      w[i] = exponential(x[i]);
-      if (kind == LEFT) {
-        const double rest = fma(w[i], unit, -(double)q[i]);
-        w[i] = remains(rest) ? rest : 0.0;
-      } else if (kind == OTHERS && row.first(k) + i == fallen) {
-        w[i] = 0.0;
+      for (int i = 0; i < VEC; ++i) w[i] = 0.0, x[i] = 0.f;
+      if (k < end) {
+        Probs<Q, VEC> q;
+        Row<T>::to_float(row.load(k), x);
+        if (kind == LEFT) q.load(left, row.first(k), a.vocab);
+        float prepared[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) prepared[i] = x[i];
+        exponential.prepare(prepared);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          w[i] = exponential(prepared[i]);
+          if (kind == LEFT) {
+            const double rest = fma(w[i], unit, -(double)q[i]);
+            w[i] = remains(rest) ? rest : 0.0;
+          } else if (kind == OTHERS && row.first(k) + i == fallen) {
+            w[i] = 0.0;
+          }
+          if (w[i] < NOTHING) w[i] = 0.0;
+          all += w[i];
+        }
       }
-    }
-  };
-  // ---- the lane, then the token; each time the first that reaches above the target, else the last with a weight
-  const double target = share * total;
-  auto find = [&](double weight, double& at) {  // `at`: in front of the lanes, then of the lane that is found
-    double upto = weight;
+      double upto = all;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    double mine_at = __shfl_up_sync(0xffffffffu, upto, 1);
-    mine_at = at + (lane ? mine_at : 0.0);
-    const unsigned reach = __ballot_sync(0xffffffffu, weight > 0.0 && mine_at + weight > target);
-    const unsigned some = __ballot_sync(0xffffffffu, weight > 0.0);
-    const int which = reach ? __ffs(reach) - 1 : some ? 31 - __clz(some) : 0;
-    at = __shfl_sync(0xffffffffu, mine_at, which);
-    return make_int2(reach | some ? which : -1, reach != 0);
-  };
-  double at = verdict.before;
-  const int which = max(0, find(weight_of(mine_sums, kind, verdict.correction), at).x);
-  const int from = __shfl_sync(0xffffffffu, begin, which), to = __shfl_sync(0xffffffffu, end, which);
-  int token = -1;
-  for (int k0 = from; k0 < to; k0 += 32) {
-    const int k = k0 + lane;
-    double w[VEC], all = 0.0;
-    if (k < to) {
-      weights(k, w);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) w[e] = 0.0;
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) all += w[e];
-    double here = at;
-    const int2 found = find(all, here);
-    if (found.x >= 0) {
-      int mine_token = -1;
-      double run = here;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      __syncthreads();  // the last round's sums are read
+      if (lane == 31) all_sums[warp].all = upto;
+      __syncthreads();
+      double at = before;
+      for (int i = 0; i < DRAW_WARPS; ++i) {
+        if (i == warp) at = before;
+        before += all_sums[i].all;
+      }
+      double mine_at = __shfl_up_sync(0xffffffffu, upto, 1);
+      mine_at = at + (lane ? mine_at : 0.0);
+      // its tokens in order
+      int token = -1;
+      float logit = 0.f;
       bool reached = false;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (w[e] > 0.0 && !reached) {
-          mine_token = row.first(k) + e;
-          reached = run + w[e] > target;
+      for (int i = 0; i < VEC; ++i) {
+        if (w[i] > 0.0 && !reached) {
+          token = row.first(k) + i, logit = x[i];
+          reached = mine_at + w[i] > target;
         }
-        run += w[e];
+        mine_at += w[i];
       }
-      token = __shfl_sync(0xffffffffu, mine_token, found.x);
-    }
-    if (found.y) break;
+      const unsigned reach = __ballot_sync(0xffffffffu, reached), some = __ballot_sync(0xffffffffu, token >= 0);
+      // the first warp that reaches it has the token; without one the last of the last warp with a weight stands
+      if (lane == 0) firsts[warp] = reach ? warp : DRAW_WARPS, lasts[warp] = some ? warp : -1;
+      __syncthreads();
+      int first = DRAW_WARPS, latest = -1;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    at += all;
+      for (int i = 0; i < DRAW_WARPS; ++i) first = min(first, firsts[i]), latest = max(latest, lasts[i]);
+      if (first < DRAW_WARPS) {
+        if (warp == first && lane == __ffs(reach) - 1) answer(token, logit);
+        last = -1;
+        break;
+      }
+      if (latest >= 0) {
+        last = latest;
+        if (warp == latest && lane == 31 - __clz(some)) fallback_token = token, fallback_logit = logit;
+      }
+    }
+    __syncthreads();
+    if (last >= 0 && threadIdx.x == 0) answer(fallback_token, fallback_logit);
   }
-  if (lane == 0) answer(token);
+  cluster.barrier_wait();  // no CTA ends while others read its sums
 }
 
 template <typename T, typename Q> int launch_draw(const VerifyParams& p, cudaStream_t s) {
   int ctas = DRAW_CLUSTER;
-  while (ctas > 1 && (int64_t)p.a.seqs * ctas > 2 * ucb_host::multiprocessors()) ctas /= 2;
+  while (ctas > 1 && (int64_t)p.a.seqs * ctas > DRAW_CTAS * ucb_host::multiprocessors()) ctas /= 2;
   return block8::launch(verify_draw_kernel<T, Q>, dim3((unsigned)p.a.seqs * ctas), dim3(DRAW_THREADS), 0, s, p,
                         "verify_draw_kernel", ctas, true);
 }
