@@ -9,8 +9,6 @@
 // sum off by d names another token with a probability of up to d times the number of
 // tokens, which is percents for fp32.  So the one row of each sequence that is drawn from
 // is summed in fp64, exponentials included, by a cluster of CTAs.
-#include <cooperative_groups.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -20,11 +18,10 @@ namespace ucb {
 namespace verify {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int MAX_ROWS = 32;  // of a sequence: its drafts and the one behind them
 constexpr int ROW_THREADS = 256, ROW_AHEAD = 4, ROW_VECTORS = ROW_THREADS * ROW_AHEAD;  // of a part of a row
-constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_CLUSTER = 8, DRAW_CTAS = 1;
+constexpr int DRAW_THREADS = 256, DRAW_WARPS = DRAW_THREADS / 32, DRAW_CTAS = 3;
+constexpr int MAX_PARTS = 1024;  // of the row that is drawn from, a warp each
 constexpr float LOWEST = -3.40282347e38f;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -34,10 +31,20 @@ struct Partial {
   int unused;
 };
 
+enum Weights : int { ALL, LEFT, OTHERS, ANSWERED };  // p; what the draft's distribution leaves of it; p without the draft; no draw
+
+// Of some elements: the sum of their e; and for LEFT what remains of them, the e of those of which something does, and the e
+// of those next to the border.
+struct __align__(16) Sums {
+  double all, left, e_left, border;
+};
+
 struct VerifyParams {
   ucb_verify_args a;
   Partial* partials;  // [seqs * rows][splits]
-  int splits;
+  Sums* sums;         // [seqs][ctas * DRAW_WARPS]
+  unsigned int* done;  // [seqs]: CTAs whose sums are there
+  int splits, ctas, part_vectors;
   unsigned int* err;
 };
 
@@ -160,6 +167,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
   const int rows = a.drafts_n + 1, split = blockIdx.x % p.splits, r = blockIdx.x / p.splits, s = r / rows, j = r % rows;
   if (j > count_of(a, s)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (j == 0 && split == 0 && threadIdx.x == 0) p.done[s] = 0;  // for the next kernel
   const Row<T> row(a.logits, s * a.logits_stride_seq + j * a.logits_stride_row, a.vocab);
   const int begin = split * ROW_VECTORS + threadIdx.x;
   uint4 raw[ROW_AHEAD];
@@ -228,13 +236,17 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
 constexpr double NOTHING = 1e-145;
 constexpr double SIXTEENTH = 0.69314718055994530942 / 16.0;
 struct Steps {
-  double power[6], magic;
+  double power[6], magic, sixteenth[16];  // 2^(j / 16)
 };
 // The magic number is 1.5 * 2^52, whose last bit is 1.
 __constant__ Steps STEPS = {{1.0, SIXTEENTH, SIXTEENTH * SIXTEENTH / 2.0, SIXTEENTH * SIXTEENTH * SIXTEENTH / 6.0,
                              SIXTEENTH * SIXTEENTH * SIXTEENTH * SIXTEENTH / 24.0,
                              SIXTEENTH * SIXTEENTH * SIXTEENTH * SIXTEENTH * SIXTEENTH / 120.0},
-                            6755399441055744.0};
+                            6755399441055744.0,
+                            {1.00000000000000000000, 1.04427378242741384032, 1.09050773266525765921, 1.13878863475669165370,
+                             1.18920711500272106672, 1.24185781207348404859, 1.29683955465100966593, 1.35425554693689272830,
+                             1.41421356237309504880, 1.47682614593949931139, 1.54221082540794082361, 1.61049033194925430818,
+                             1.68179283050742908606, 1.75625216037329948311, 1.83400808640934246349, 1.91520656139714729387}};
 template <typename T> struct Exponential {
   double top, scale;  // 16 log2(e) / T
   float floor;        // no more than 700 T below the top
@@ -267,93 +279,60 @@ template <typename T> struct Exponential {
   }
 };
 
-enum Weights { ALL, LEFT, OTHERS };  // p; what the draft's distribution leaves of it; p without the draft
-
-// Of some elements: the sum of their e; and for LEFT what remains of them, the e of those of which something does, and the e
-// of those next to the border.
-struct __align__(16) Sums {
-  double all, left, e_left, border;
-};
 
 // Whether something remains: above 0, or no number.  By the bits, no compare on the fp64 pipe.
 __device__ __forceinline__ bool remains(double rest) { return ((uint32_t)__double2hiint(rest) ^ 0x80000000u) > 0x7ff00000u; }
 
-// A warp's pass over vectors [begin, end) of a row, the lanes side by side: `load` brings a lane's vector k to a buffer, `use` takes it.
-// Two groups of vectors by turns, one in flight while the other is used; the row's ends, which not every lane has, one by one.
-template <int GROUP, typename Buffer, typename RowT, typename Load, typename Use>
-__device__ __forceinline__ void pass_over(const RowT& row, int begin, int end, Load load, Use use) {
-  const int lane = threadIdx.x & 31, first = max(begin, row.full_begin), last = min(end, row.full_end);
-  const int steps = max(0, last - first + 31) / 32;
-  Buffer a[GROUP], b[GROUP];
-  auto load_group = [&](Buffer(&x)[GROUP], int i) {
-#pragma unroll
-    for (int u = 0; u < GROUP; ++u)
-      if (first + 32 * (i + u) + lane < last) load(x[u], first + 32 * (i + u) + lane);
-  };
-  auto use_group = [&](Buffer(&x)[GROUP], int i) {
-#pragma unroll
-    for (int u = 0; u < GROUP; ++u)
-      if (first + 32 * (i + u) + lane < last) use(x[u], first + 32 * (i + u) + lane);
-  };
-  load_group(a, 0);
-  for (int i = 0; i < steps; i += 2 * GROUP) {
-    load_group(b, i + GROUP);
-    use_group(a, i);
-    load_group(a, i + 2 * GROUP);
-    if (i + GROUP < steps) use_group(b, i + GROUP);
-  }
-  if (lane == 0 && begin == 0 && end > 0 && row.full_begin == 1) load(a[0], 0), use(a[0], 0);
-  if (lane == 0 && end == row.vectors && begin < end && row.full_end >= row.full_begin && row.full_end < row.vectors)
-    load(a[0], row.full_end), use(a[0], row.full_end);
-}
-
-// The e of this lane's share of the warp's vectors [begin, end) without that of element `but`.
-template <typename T> __device__ __forceinline__ Sums sum_others(const Row<T>& row, int begin, int end,
-                                                                 const Exponential<T>& exponential, int but) {
+// The sums of a warp's vectors [begin, end), the lanes side by side, the same in every lane.  One loop of little code: most calls go
+// through it once or a few times, and what costs most then is to fetch the instructions.
+template <typename T, typename Q> __device__ __forceinline__ Sums sum_vectors(const Row<T>& row, const Q* left, int begin, int end,
+                                                                              const Exponential<T>& exponential, Weights kind,
+                                                                              double unit, int fallen) {
   constexpr int VEC = Row<T>::VEC;
-  double sum = 0.0;
-  pass_over<2, uint4>(row, begin, end, [&](uint4& raw, int k) { raw = row.load(k); }, [&](const uint4& raw, int k) {
+  const int but = kind == OTHERS ? fallen : -1;
+  Sums s = {0.0, 0.0, 0.0, 0.0};
+  int k = begin + (threadIdx.x & 31);
+  uint4 next_x = make_uint4(0, 0, 0, 0);
+  Probs<Q, VEC> next_q;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) next_q.e[i] = Dtype<Q>::from_f(0.f);
+  auto fetch = [&]() {
+    next_x = row.load(k);
+    if (kind == LEFT) next_q.load(left, row.first(k), row.vocab);
+  };
+  if (k < end) fetch();
+#pragma unroll 1
+  while (k < end) {
     float x[VEC];
-    Row<T>::to_float(raw, x);
+    Row<T>::to_float(next_x, x);
     exponential.prepare(x);
+    const Probs<Q, VEC> now_q = next_q;
     if ((unsigned)(but - row.first(k)) < VEC)
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         if (row.first(k) + i == but) x[i] = -INFINITY;
-    double e[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) e[i] = exponential(x[i]);
-#pragma unroll
-    for (int o = 1; o < VEC; o *= 2)
-#pragma unroll
-      for (int i = 0; i < VEC; i += 2 * o) e[i] += e[i + o];
-    sum += e[0];
-  });
-  return {sum, 0.0, 0.0, 0.0};
-}
-
-// The e of this lane's share of them, and what remains of it.
-template <typename T, typename Q> __device__ __forceinline__ Sums sum_left(const Row<T>& row, const Q* left, int begin, int end,
-                                                                           const Exponential<T>& exponential, double unit) {
-  constexpr int VEC = Row<T>::VEC;
-  struct Both {
-    uint4 x;
-    Probs<Q, VEC> q;
-  };
-  Sums s = {0.0, 0.0, 0.0, 0.0};
-  pass_over<1, Both>(row, begin, end, [&](Both& both, int k) { both.x = row.load(k), both.q.load(left, row.first(k), row.vocab); },
-                     [&](const Both& both, int) {
-    float x[VEC];
-    Row<T>::to_float(both.x, x);
-    exponential.prepare(x);
+    k += 32;
+    if (k < end) fetch();
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const double e = exponential(x[i]), q = (double)both.q[i], rest = fma(e, unit, -q);
+      const double e = exponential(x[i]);
       s.all += e;
-      if (remains(rest)) s.left += rest, s.e_left += e;
-      if ((__double2hiint(rest) & 0x7ff00000) + (20 << 20) < (__double2hiint(q) & 0x7ff00000)) s.border += e;
+      if (kind == LEFT) {
+        const double q = (double)now_q[i], rest = fma(e, unit, -q);
+        if (remains(rest)) s.left += rest, s.e_left += e;
+        if ((__double2hiint(rest) & 0x7ff00000) + (20 << 20) < (__double2hiint(q) & 0x7ff00000)) s.border += e;
+      }
     }
-  });
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.all += __shfl_xor_sync(0xffffffffu, s.all, o);
+    if (kind == LEFT) {
+      s.left += __shfl_xor_sync(0xffffffffu, s.left, o);
+      s.e_left += __shfl_xor_sync(0xffffffffu, s.e_left, o);
+      s.border += __shfl_xor_sync(0xffffffffu, s.border, o);
+    }
+  }
   return s;
 }
 
@@ -363,109 +342,109 @@ __device__ __forceinline__ double weight_of(const Sums& s, Weights kind, double 
 }
 
 struct Verdict {
-  double unit, correction, total, before;  // before: the weight in front of the owner's part
-  int owner;                               // the part that holds the drawn token; -1: none
+  double unit, total, before;  // before: the weight in front of the owner's part
+  int owner;                   // the part that holds the drawn token; -1: none
   Weights kind;
   bool again;
 };
 
-// One warp: from the sums of all parts, the part with the drawn token, or that the pass has to be made again.
-__device__ void judge(const Sums* sums, int parts, Weights kind, double unit, double share, bool first_time, Verdict& verdict) {
-  constexpr int EACH = DRAW_WARPS * DRAW_CLUSTER / 32;
-  const int lane = threadIdx.x & 31;
-  Sums s = {0.0, 0.0, 0.0, 0.0};
+// The whole CTA: from the sums of all parts, the part with the drawn token, or that they have to be made again.  A thread has a few
+// adjacent parts.
+__device__ __forceinline__ void judge(const Sums* sums, int parts, Weights kind, double unit, double share, bool first_time,
+                                      Verdict& verdict) {
+  __shared__ Sums warp_sums[DRAW_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (parts + DRAW_THREADS - 1) / DRAW_THREADS;
+  const int begin = min(parts, (int)threadIdx.x * each), end = min(parts, begin + each);
+  if (threadIdx.x == 0) verdict.owner = -1, verdict.again = false;
+  Sums own = {0.0, 0.0, 0.0, 0.0};
+  for (int i = begin; i < end; ++i) own.all += sums[i].all, own.left += sums[i].left, own.e_left += sums[i].e_left, own.border += sums[i].border;
+  Sums upto = own;  // and the threads in front
 #pragma unroll
-  for (int i = 0; i < EACH; ++i)
-    if (lane * EACH + i < parts) {
-      const Sums x = sums[lane * EACH + i];
-      s.all += x.all, s.left += x.left, s.e_left += x.e_left, s.border += x.border;
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const double all = __shfl_up_sync(0xffffffffu, upto.all, o), left = __shfl_up_sync(0xffffffffu, upto.left, o);
+    const double e_left = __shfl_up_sync(0xffffffffu, upto.e_left, o), border = __shfl_up_sync(0xffffffffu, upto.border, o);
+    if (lane >= o) upto.all += all, upto.left += left, upto.e_left += e_left, upto.border += border;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  Sums whole = {0.0, 0.0, 0.0, 0.0}, front = whole;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s.all += __shfl_xor_sync(0xffffffffu, s.all, o);
-    s.left += __shfl_xor_sync(0xffffffffu, s.left, o);
-    s.e_left += __shfl_xor_sync(0xffffffffu, s.e_left, o);
-    s.border += __shfl_xor_sync(0xffffffffu, s.border, o);
+  for (int i = 0; i < DRAW_WARPS; ++i) {
+    if (i == warp) front = whole;
+    const Sums x = warp_sums[i];
+    whole.all += x.all, whole.left += x.left, whole.e_left += x.e_left, whole.border += x.border;
   }
   double right = unit;
-  bool again = false;
   if (kind == LEFT) {
-    right = 1.0 / s.all;
+    right = 1.0 / whole.all;
     // elements within 2^-20 of the border were summed apart: what they may be off by together has to be below 2^-35 of the
     // whole, and the fp32 sum no further off than they were looked for
     constexpr double NEAR = 1.0 / (1 << 20), TOLERATED = NEAR / (1 << 15);
-    const bool none = s.left < NOTHING;
-    const double off = fabs(right - unit) / right, whole = none ? 0.0 : weight_of(s, kind, right - unit);
-    again = first_time && (off > NEAR || s.border * right * off > TOLERATED * whole);
+    const bool none = whole.left < NOTHING;
+    const double off = fabs(right - unit), remaining = none ? 0.0 : weight_of(whole, kind, right - unit);
+    const bool again = first_time && (off > NEAR * right || whole.border * off > TOLERATED * remaining);
+    if (again && threadIdx.x == 0) verdict.again = true;
     if (none && !again) kind = ALL;  // nothing remains: from p itself, whose sums are here
-  } else if (kind == OTHERS && s.all < NOTHING) {
-    kind = ALL, again = true;
+  } else if (kind == OTHERS && whole.all < NOTHING) {
+    kind = ALL;
+    if (threadIdx.x == 0) verdict.again = true;
   }
-  double v[EACH], all = 0.0;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    v[i] = lane * EACH + i < parts ? weight_of(sums[lane * EACH + i], kind, right - unit) : 0.0;
-    all += v[i];
-  }
-  double run = all;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double x = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += x;
-  }
-  const double total = __shfl_sync(0xffffffffu, run, 31), target = share * total;
-  double at = __shfl_up_sync(0xffffffffu, run, 1);
-  if (lane == 0) at = 0.0;
-  // the first part that reaches above the target; where rounding leaves none, the last one with a weight
+  const double correction = right - unit, total = weight_of(whole, kind, correction), target = share * total;
+  front.all += upto.all - own.all, front.left += upto.left - own.left, front.e_left += upto.e_left - own.e_left;
+  // The first part that reaches above the target.  The threads' own weights in front may, rounded apart, leave none or two: the lowest
+  // part of those, and else the last one with a weight.
+  double at = weight_of(front, kind, correction), found_at = at, last_at = at;
   int found = parts, last = -1;
-  double found_at = 0.0, last_at = 0.0;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    if (v[i] > NOTHING) {
-      if (found == parts && at + v[i] > target) found = lane * EACH + i, found_at = at;
-      last = lane * EACH + i, last_at = at;
+  for (int i = begin; i < end; ++i) {
+    const double v = weight_of(sums[i], kind, correction);
+    if (v > NOTHING) {
+      if (found == parts && at + v > target) found = i, found_at = at;
+      last = i, last_at = at;
     }
-    at += v[i];
+    at += v;
   }
+  __shared__ int firsts[DRAW_WARPS], lasts[DRAW_WARPS];
   const int first = __reduce_min_sync(0xffffffffu, found), final = __reduce_max_sync(0xffffffffu, last);
-  const int which = first < parts ? first : final;
-  if (lane == 0) {
-    verdict.unit = right, verdict.correction = right - unit, verdict.total = total, verdict.owner = which;
-    verdict.kind = kind, verdict.again = again;
-  }
-  if (which >= 0 && lane == which / EACH) verdict.before = first < parts ? found_at : last_at;
+  if (lane == 0) firsts[warp] = first, lasts[warp] = final;
+  __syncthreads();
+  int which = parts, fallback = -1;
+#pragma unroll
+  for (int i = 0; i < DRAW_WARPS; ++i) which = min(which, firsts[i]), fallback = max(fallback, lasts[i]);
+  const bool reached = which < parts;
+  if (!reached) which = fallback;
+  if (threadIdx.x == 0) verdict.unit = right, verdict.total = total, verdict.kind = kind;
+  if (which >= begin && which < end) verdict.owner = which, verdict.before = reached ? found_at : last_at;
+  __syncthreads();
 }
 
-// One cluster a sequence: the tests, then the next token.
+// ln p of a token from its logit.
+__device__ __forceinline__ float logprob_of(float logit, const Partial& row, double inverse) {
+  return (float)(((double)logit - (double)row.top) * inverse - (double)logf(row.sum));
+}
+
+// Some CTAs a sequence, each with some parts of the row that the next token is drawn from, a part a warp.  Which row that is every
+// one of them finds by the tests; the first writes down what they say, and whichever is the last to have its sums finds the token.
 template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS, DRAW_CTAS) verify_draw_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC;
   const ucb_verify_args& a = p.a;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = cluster.block_rank(), ctas = cluster.num_blocks(), s = blockIdx.x / ctas;
+  const int s = blockIdx.x / p.ctas, cta = blockIdx.x % p.ctas;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = a.drafts_n + 1, count = count_of(a, s);
   __shared__ Partial part[MAX_ROWS];
-  __shared__ int accepted_at;
+  __shared__ int accepted_at, fallen_draft;
   __shared__ double sixteenths[16];
-  __shared__ Sums warp_sums[2][DRAW_WARPS], all_sums[DRAW_WARPS * DRAW_CLUSTER];
-  __shared__ Verdict verdict;
-  __shared__ int firsts[DRAW_WARPS], lasts[DRAW_WARPS], fallback_token;
-  __shared__ float fallback_logit;
-  const float temperature = temperature_of(a, s);
+  __shared__ bool is_last;
+  const float temperature = temperature_of(a, s), heat = heat_of(temperature), c = LOG2E / heat;
   const bool greedy = temperature <= 0.f;
-  const float c = LOG2E / heat_of(temperature);
-  const double inverse = 1.0 / (double)heat_of(temperature);
+  const double inverse = 1.0 / (double)heat;
   const T* logits = static_cast<const T*>(a.logits) + s * a.logits_stride_seq;
   const Q* probs = static_cast<const Q*>(a.draft_probs) + s * a.probs_stride_seq;
-  auto draft_of = [&](int j) {
-    const int64_t at = s * a.drafts_stride_seq + j;
-    return a.drafts_64 ? static_cast<const int64_t*>(a.drafts)[at] : (int64_t)static_cast<const int32_t*>(a.drafts)[at];
-  };
   // what the tests need of the inputs, a lane a draft: before the rows' sums are there
   int64_t draft = -1;
   float draft_logit = 0.f, draft_uniform = 0.f, draft_q = 1.f;
   bool outside = false;
   if (warp == 0 && lane < count) {
-    draft = draft_of(lane);
+    const int64_t at = s * a.drafts_stride_seq + lane;
+    draft = a.drafts_64 ? static_cast<const int64_t*>(a.drafts)[at] : (int64_t)static_cast<const int32_t*>(a.drafts)[at];
     draft_uniform = a.uniforms[s * a.uniforms_stride_seq + lane];
     outside = draft < 0 || draft >= a.vocab;
     if (!outside) {
@@ -474,29 +453,29 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
     }
   }
   const double share = fmax((double)a.uniforms[s * a.uniforms_stride_seq + a.drafts_n], 1e-130);  // 0: what is above NOTHING
-  if (threadIdx.x < 16) sixteenths[threadIdx.x] = exp2(threadIdx.x / 16.0);
+  if (threadIdx.x < 16) sixteenths[threadIdx.x] = STEPS.sixteenth[threadIdx.x];
   block8::wait_for_primary();
+#pragma unroll 1
   for (int j = warp; j <= count; j += DRAW_WARPS) {
     float top = -INFINITY, sum = 0.f, best_value = -INFINITY;
     int best = 0x7fffffff;
+#pragma unroll 1
     for (int i = lane; i < p.splits; i += 32) {
       const Partial x = p.partials[((int64_t)s * rows + j) * p.splits + i];
       better(best_value, best, x.top, x.best);
       join(top, sum, x.top, x.sum, c);
     }
+    float highest = top;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float t = __shfl_xor_sync(0xffffffffu, top, o), q = __shfl_xor_sync(0xffffffffu, sum, o);
-      const float v = __shfl_xor_sync(0xffffffffu, best_value, o);
-      const int i = __shfl_xor_sync(0xffffffffu, best, o);
-      better(best_value, best, v, i);
-      join(top, sum, t, q, c);
-    }
-    if (lane == 0) part[j] = {top, sum, best, 0};
+    for (int o = 16; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+    join(top, sum, highest, 0.f, c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    best = __reduce_min_sync(0xffffffffu, best_value == highest ? best : 0x7fffffff);
+    if (lane == 0) part[j] = {highest, sum, best, 0};
   }
   __syncthreads();
   // ---- the drafts
-  auto logprob_of = [&](int j, float x) { return ((double)x - (double)part[j].top) * inverse - log((double)part[j].sum); };
   if (warp == 0) {
     bool stays = false;
     if (lane < count && !outside) {
@@ -507,165 +486,161 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
     }
     const unsigned falls = ~__ballot_sync(0xffffffffu, stays);
     const int accepted = min(count, falls ? __ffs(falls) - 1 : 32);
+    if (lane == accepted) fallen_draft = lane < count && !outside ? (int)draft : -1;
     if (lane == 0) accepted_at = accepted;
   }
   __syncthreads();
-  if (rank == 0 && warp == 0) {
-    const int accepted = accepted_at;
-    if (lane < rows && lane != accepted) {
-      a.tokens[s * rows + lane] = lane < accepted ? (int)draft : -1;
-      a.logprobs[s * rows + lane] = lane < accepted ? (float)logprob_of(lane, draft_logit) : 0.f;
-    }
-    if (lane == 0) {
-      a.accepted[s] = accepted;
-      if (a.lengths) a.lengths[s] -= count - accepted;
-      if (a.counts && a.counts[s] != count) outside = true;
-    }
-    if (outside && lane <= accepted) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
-  }
-  const int j = accepted_at;
-  const float sum = part[j].sum;
+  const int j = accepted_at, fallen = fallen_draft;
+  const Partial here = part[j];
+  const bool none = !(here.sum > 0.f && here.sum < INFINITY);  // a NaN or an infinity among the logits, or nothing but -inf
+  Weights kind = none || greedy ? ANSWERED : fallen < 0 ? ALL : a.draft_probs ? LEFT : OTHERS;
   auto answer = [&](int token, float logit) {
     a.tokens[s * rows + j] = token;
-    a.logprobs[s * rows + j] = token < 0 ? __int_as_float(0x7fffffff) : (float)logprob_of(j, logit);
+    a.logprobs[s * rows + j] = token < 0 ? __int_as_float(0x7fffffff) : logprob_of(logit, here, inverse);
     if (token < 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
   };
-  const bool none = !(sum > 0.f && sum < INFINITY);  // a NaN or an infinity among the logits, or nothing but -inf
-  if (none || greedy) {
-    if (rank == 0 && threadIdx.x == 0) answer(none ? -1 : part[j].best, part[j].top);
-    return;
+  if (cta == 0 && warp == 0) {
+    if (lane < rows && lane != j) {
+      a.tokens[s * rows + lane] = lane < j ? (int)draft : -1;
+      a.logprobs[s * rows + lane] = lane < j ? logprob_of(draft_logit, part[lane], inverse) : 0.f;
+    }
+    if (lane == 0) {
+      a.accepted[s] = j;
+      if (a.lengths) a.lengths[s] -= count - j;
+      if (a.counts && a.counts[s] != count) outside = true;
+      if (kind == ANSWERED) answer(none ? -1 : here.best, here.top);
+    }
+    if (outside && lane <= j) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
   }
-  // ---- the draw, over the whole row in fp64: a warp has `each` adjacent vectors
+  if (kind == ANSWERED) return;
+
+  // ---- the sums of this warp's part
   const Row<T> row(logits, j * a.logits_stride_row, a.vocab);
   const Q* left = probs + j * a.probs_stride_row;
-  const int64_t draft_here = j < count ? draft_of(j) : -1;
-  const int fallen = draft_here >= 0 && draft_here < a.vocab ? (int)draft_here : -1;
-  Weights kind = fallen < 0 ? ALL : a.draft_probs ? LEFT : OTHERS;
-  const Exponential<T> exponential(part[j].top, (double)heat_of(temperature), sixteenths);
-  const int parts = ctas * DRAW_WARPS, mine = rank * DRAW_WARPS + warp;
-  const int each = (row.vectors + parts - 1) / parts;
-  auto begin_of = [&](int part) { return (int)min((int64_t)row.vectors, (int64_t)part * each); };
-  // What the draft leaves of p, max(e / Z - q, 0) with Z the sum of all e, would need a pass for Z first.  The pass takes the fp32
-  // sum instead, 1 / `unit`: as long as the same elements remain, the sums of what they leave and of their e give those for Z
-  // itself.  Elements that are so near to the border that they may change sides are summed too; where they could matter
-  // (they hardly ever do), the pass is made again with Z.
-  double unit = kind == LEFT ? 1.0 / (double)sum : 1.0;
-  for (int turn = 0;; turn ^= 1) {
-    Sums w = kind == LEFT ? sum_left<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, unit)
-                      : sum_others<T>(row, begin_of(mine), begin_of(mine + 1), exponential, kind == OTHERS ? fallen : -1);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      w.all += __shfl_xor_sync(0xffffffffu, w.all, o);
-      if (kind == LEFT) {
-        w.left += __shfl_xor_sync(0xffffffffu, w.left, o);
-        w.e_left += __shfl_xor_sync(0xffffffffu, w.e_left, o);
-        w.border += __shfl_xor_sync(0xffffffffu, w.border, o);
-      }
-    }
-    if (lane == 0) warp_sums[turn][warp] = w;
-    cluster.sync();
-    for (int i = threadIdx.x; i < parts; i += DRAW_THREADS)
-      all_sums[i] = *cluster.map_shared_rank(&warp_sums[turn][i % DRAW_WARPS], i / DRAW_WARPS);
+  const Exponential<T> exponential(here.top, heat, sixteenths);
+  const int parts = p.ctas * DRAW_WARPS, mine = cta * DRAW_WARPS + warp;
+  auto begin_of = [&](int part) { return (int)min((int64_t)row.vectors, (int64_t)part * p.part_vectors); };
+  double unit = 1.0 / (double)here.sum;
+  __shared__ Sums sums[MAX_PARTS];
+  __shared__ Verdict verdict;
+  {
+    const Sums w = sum_vectors<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, kind, unit, fallen);
+    if (lane == 0) p.sums[(int64_t)s * parts + mine] = w, __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) is_last = atomicAdd(&p.done[s], 1u) == p.ctas - 1;
+  __syncthreads();
+  if (!is_last) return;
+
+  // ---- the part that the next token lies in
+  __threadfence();
+  for (int i = threadIdx.x; i < 2 * parts; i += DRAW_THREADS)
+    reinterpret_cast<uint4*>(sums)[i] = __ldcg(reinterpret_cast<const uint4*>(p.sums + (int64_t)s * parts) + i);
+#pragma unroll 1
+  for (bool first_time = true;; first_time = false) {
     __syncthreads();
-    if (warp == 0) judge(all_sums, parts, kind, unit, share, turn == 0, verdict);
-    __syncthreads();
+    judge(sums, parts, kind, unit, share, first_time, verdict);
     kind = verdict.kind, unit = verdict.unit;
     if (!verdict.again) break;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = warp; i < parts; i += DRAW_WARPS) {
+      const Sums w = sum_vectors<T, Q>(row, left, begin_of(i), begin_of(i + 1), exponential, kind, unit, fallen);
+      if (lane == 0) sums[i] = w;
+    }
   }
   const double total = verdict.total;
-  cluster.barrier_arrive();  // this CTA has read the others' sums
   if (!(total > NOTHING && total < INFINITY)) {
-    if (rank == 0 && threadIdx.x == 0) answer(-1, 0.f);
-  } else if (verdict.owner / DRAW_WARPS == rank) {
-    // ---- the token, in the part that holds it: a warp for each 32 of its vectors.  Each time what is looked for is the first
-    // that reaches above the target, or where rounding leaves none, the last with a weight.
-    const double target = share * total;
-    const int begin = begin_of(verdict.owner), end = begin_of(verdict.owner + 1);
-    double before = verdict.before;
-    int last = -1;  // the last with a weight so far: every warp's the same
-    for (int base = begin; base < end; base += DRAW_THREADS) {
-      const int k = base + threadIdx.x;
-      double w[VEC], all = 0.0;
-      float x[VEC];
+    if (threadIdx.x == 0) answer(-1, 0.f);
+    return;
+  }
+  // ---- the token: a warp for each 32 vectors of the part.  Each time what is looked for is the first that reaches above the
+  // target, or where rounding leaves none, the last with a weight.
+  __shared__ double warp_weight[DRAW_WARPS];
+  __shared__ int firsts[DRAW_WARPS], lasts[DRAW_WARPS], fallback_token;
+  __shared__ float fallback_logit;
+  const double target = share * total;
+  const int begin = begin_of(verdict.owner), end = begin_of(verdict.owner + 1);
+  double before = verdict.before;
+  bool any = false;  // whether there is a fallback
+#pragma unroll 1
+  for (int base = begin; base < end; base += DRAW_THREADS) {
+    const int k = base + threadIdx.x;
+    double w[VEC], all = 0.0;
+    float x[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] = 0.0, x[i] = 0.f;
-      if (k < end) {
-        Probs<Q, VEC> q;
-        Row<T>::to_float(row.load(k), x);
-        if (kind == LEFT) q.load(left, row.first(k), a.vocab);
-        float prepared[VEC];
+    for (int i = 0; i < VEC; ++i) w[i] = 0.0, x[i] = 0.f;
+    if (k < end) {
+      Probs<Q, VEC> q;
+      Row<T>::to_float(row.load(k), x);
+      if (kind == LEFT) q.load(left, row.first(k), a.vocab);
+      float prepared[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) prepared[i] = x[i];
-        exponential.prepare(prepared);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          w[i] = exponential(prepared[i]);
-          if (kind == LEFT) {
-            const double rest = fma(w[i], unit, -(double)q[i]);
-            w[i] = remains(rest) ? rest : 0.0;
-          } else if (kind == OTHERS && row.first(k) + i == fallen) {
-            w[i] = 0.0;
-          }
-          if (w[i] < NOTHING) w[i] = 0.0;
-          all += w[i];
-        }
-      }
-      double upto = all;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-      }
-      __syncthreads();  // the last round's sums are read
-      if (lane == 31) all_sums[warp].all = upto;
-      __syncthreads();
-      double at = before;
-      for (int i = 0; i < DRAW_WARPS; ++i) {
-        if (i == warp) at = before;
-        before += all_sums[i].all;
-      }
-      double mine_at = __shfl_up_sync(0xffffffffu, upto, 1);
-      mine_at = at + (lane ? mine_at : 0.0);
-      // its tokens in order
-      int token = -1;
-      float logit = 0.f;
-      bool reached = false;
+      for (int i = 0; i < VEC; ++i) prepared[i] = x[i];
+      exponential.prepare(prepared);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        if (w[i] > 0.0 && !reached) {
-          token = row.first(k) + i, logit = x[i];
-          reached = mine_at + w[i] > target;
+        w[i] = exponential(prepared[i]);
+        if (kind == LEFT) {
+          const double rest = fma(w[i], unit, -(double)q[i]);
+          w[i] = remains(rest) ? rest : 0.0;
+        } else if (kind == OTHERS && row.first(k) + i == fallen) {
+          w[i] = 0.0;
         }
-        mine_at += w[i];
-      }
-      const unsigned reach = __ballot_sync(0xffffffffu, reached), some = __ballot_sync(0xffffffffu, token >= 0);
-      // the first warp that reaches it has the token; without one the last of the last warp with a weight stands
-      if (lane == 0) firsts[warp] = reach ? warp : DRAW_WARPS, lasts[warp] = some ? warp : -1;
-      __syncthreads();
-      int first = DRAW_WARPS, latest = -1;
-#pragma unroll
-      for (int i = 0; i < DRAW_WARPS; ++i) first = min(first, firsts[i]), latest = max(latest, lasts[i]);
-      if (first < DRAW_WARPS) {
-        if (warp == first && lane == __ffs(reach) - 1) answer(token, logit);
-        last = -1;
-        break;
-      }
-      if (latest >= 0) {
-        last = latest;
-        if (warp == latest && lane == 31 - __clz(some)) fallback_token = token, fallback_logit = logit;
+        if (w[i] < NOTHING) w[i] = 0.0;
+        all += w[i];
       }
     }
+    double upto = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    __syncthreads();  // the last round's weights are read
+    if (lane == 31) warp_weight[warp] = upto;
     __syncthreads();
-    if (last >= 0 && threadIdx.x == 0) answer(fallback_token, fallback_logit);
+    double at = before;
+#pragma unroll
+    for (int i = 0; i < DRAW_WARPS; ++i) {
+      if (i == warp) at = before;
+      before += warp_weight[i];
+    }
+    double mine_at = __shfl_up_sync(0xffffffffu, upto, 1);
+    mine_at = at + (lane ? mine_at : 0.0);
+    int token = -1;  // of this lane's
+    float logit = 0.f;
+    bool reached = false;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if (w[i] > 0.0 && !reached) {
+        token = row.first(k) + i, logit = x[i];
+        reached = mine_at + w[i] > target;
+      }
+      mine_at += w[i];
+    }
+    const unsigned reach = __ballot_sync(0xffffffffu, reached), some = __ballot_sync(0xffffffffu, token >= 0);
+    if (lane == 0) firsts[warp] = reach ? warp : DRAW_WARPS, lasts[warp] = some ? warp : -1;
+    __syncthreads();
+    int first = DRAW_WARPS, latest = -1;
+#pragma unroll
+    for (int i = 0; i < DRAW_WARPS; ++i) first = min(first, firsts[i]), latest = max(latest, lasts[i]);
+    if (first < DRAW_WARPS) {
+      if (warp == first && lane == __ffs(reach) - 1) answer(token, logit);
+      return;
+    }
+    if (latest >= 0) {
+      any = true;
+      if (warp == latest && lane == 31 - __clz(some)) fallback_token = token, fallback_logit = logit;
+    }
   }
-  cluster.barrier_wait();  // no CTA ends while others read its sums
+  __syncthreads();
+  if (threadIdx.x == 0) answer(any ? fallback_token : -1, any ? fallback_logit : 0.f);
 }
 
 template <typename T, typename Q> int launch_draw(const VerifyParams& p, cudaStream_t s) {
-  int ctas = DRAW_CLUSTER;
-  while (ctas > 1 && (int64_t)p.a.seqs * ctas > DRAW_CTAS * ucb_host::multiprocessors()) ctas /= 2;
-  return block8::launch(verify_draw_kernel<T, Q>, dim3((unsigned)p.a.seqs * ctas), dim3(DRAW_THREADS), 0, s, p,
-                        "verify_draw_kernel", ctas, true);
+  return block8::launch(verify_draw_kernel<T, Q>, dim3((unsigned)p.a.seqs * p.ctas), dim3(DRAW_THREADS), 0, s, p, "verify_draw_kernel", 1,
+                        true);
 }
 
 template <typename T> int launch_all(const VerifyParams& p, cudaStream_t s) {
@@ -678,11 +653,24 @@ template <typename T> int launch_all(const VerifyParams& p, cudaStream_t s) {
   }
 }
 
-// Parts of a row; one more vector than elements need where rows do not start on 16 bytes.
-int64_t splits_of(int vocab, int dtype) {
-  const int64_t vectors = vocab / (dtype == UCB_F32 ? 4 : 8) + 2;
-  return (vectors + ROW_VECTORS - 1) / ROW_VECTORS;
-}
+// How a call is cut up; false where the device cannot be asked.
+struct Layout {
+  int64_t splits, ctas, part_vectors, partials_bytes, sums_bytes, bytes;
+  bool make(int64_t seqs, int64_t rows, int64_t vocab, int dtype) {
+    const int sms = ucb_host::multiprocessors();
+    if (sms < 1) return false;
+    const int64_t vectors = vocab / (dtype == UCB_F32 ? 4 : 8) + 2;  // with those that rows not starting on 16 bytes add
+    splits = (vectors + ROW_VECTORS - 1) / ROW_VECTORS;
+    // the row that is drawn from: as many CTAs as are resident together
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(MAX_PARTS / DRAW_WARPS, (int64_t)sms * DRAW_CTAS / seqs));
+    part_vectors = (vectors + most * DRAW_THREADS - 1) / (most * DRAW_THREADS) * 32;
+    ctas = (vectors + part_vectors * DRAW_WARPS - 1) / (part_vectors * DRAW_WARPS);
+    partials_bytes = seqs * rows * splits * (int64_t)sizeof(Partial);
+    sums_bytes = seqs * ctas * DRAW_WARPS * (int64_t)sizeof(Sums);
+    bytes = partials_bytes + sums_bytes + seqs * (int64_t)sizeof(unsigned int);
+    return true;
+  }
+};
 
 }  // namespace
 }  // namespace verify
@@ -693,7 +681,8 @@ namespace uv = ucb::verify;
 
 extern "C" int64_t ucb_verify_drafts_workspace_bytes(int seqs, int drafts, int vocab, int dtype) {
   if (seqs < 1 || drafts < 0 || drafts >= uv::MAX_ROWS || vocab < 1) return -1;
-  return (int64_t)seqs * (drafts + 1) * uv::splits_of(vocab, dtype) * (int64_t)sizeof(uv::Partial);
+  uv::Layout layout;
+  return layout.make(seqs, drafts + 1, vocab, dtype) ? layout.bytes : -1;
 }
 
 extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
@@ -712,9 +701,15 @@ extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
     return set_error(UCB_ERR_UNSUPPORTED, "%s: unsupported dtype", what);
   unsigned int* err = ucb_host::device_error_word();
   if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
-  const int64_t splits = uv::splits_of(a->vocab, a->dtype);
-  if (splits * a->seqs * (a->drafts_n + 1) > 0x7fffffff) return set_error(UCB_ERR_UNSUPPORTED, "%s: too many rows or tokens", what);
-  const uv::VerifyParams p{*a, static_cast<uv::Partial*>(a->workspace), (int)splits, err};
+  uv::Layout layout;
+  if (!layout.make(a->seqs, a->drafts_n + 1, a->vocab, a->dtype))
+    return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
+  if (layout.splits * a->seqs * (a->drafts_n + 1) > 0x7fffffff || layout.ctas * a->seqs > 0x7fffffff || layout.part_vectors > 0x7fffffff)
+    return set_error(UCB_ERR_UNSUPPORTED, "%s: too many rows or tokens", what);
+  char* w = static_cast<char*>(a->workspace);
+  const uv::VerifyParams p{*a, reinterpret_cast<uv::Partial*>(w), reinterpret_cast<uv::Sums*>(w + layout.partials_bytes),
+                           reinterpret_cast<unsigned int*>(w + layout.partials_bytes + layout.sums_bytes), (int)layout.splits,
+                           (int)layout.ctas, (int)layout.part_vectors, err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case UCB_BF16: return uv::launch_all<__nv_bfloat16>(p, s);
