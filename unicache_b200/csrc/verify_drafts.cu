@@ -99,14 +99,22 @@ template <typename Q, int N> struct Probs {
     Q e[N];
   };
   __device__ __forceinline__ Probs() {}
-  __device__ __forceinline__ void load(const Q* q, int i, int vocab) {
-    if (i >= 0 && i + N <= vocab && reinterpret_cast<uintptr_t>(q + i) % ALIGN == 0) {
+  __device__ __forceinline__ void load(const Q* q) {  // all of them inside
+    if (reinterpret_cast<uintptr_t>(q) % ALIGN == 0) {
       if constexpr (BYTES >= 16) {
 #pragma unroll
-        for (int k = 0; k < BYTES / 16; ++k) w16[k] = reinterpret_cast<const uint4*>(q + i)[k];
+        for (int k = 0; k < BYTES / 16; ++k) w16[k] = reinterpret_cast<const uint4*>(q)[k];
       } else {
-        w8 = *reinterpret_cast<const uint2*>(q + i);
+        w8 = *reinterpret_cast<const uint2*>(q);
       }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) e[k] = q[k];
+    }
+  }
+  __device__ __forceinline__ void load(const Q* q, int i, int vocab) {
+    if (i >= 0 && i + N <= vocab) {
+      load(q + i);
     } else {
 #pragma unroll
       for (int k = 0; k < N; ++k) e[k] = i + k >= 0 && i + k < vocab ? q[i + k] : Dtype<Q>::from_f(0.f);
@@ -156,15 +164,18 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float low_of(uint64_t a) { return __uint_as_float((uint32_t)a); }
-__device__ __forceinline__ float high_of(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+__device__ __forceinline__ float2 halves_of(uint64_t a) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(a));
+  return v;
+}
 
 // One CTA a part of a row, all of it loaded at once: its maximum first, then the exponentials against that.
 template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC, WARPS = ROW_THREADS / 32;
   const ucb_verify_args& a = p.a;
   block8::launch_dependents();
-  const int rows = a.drafts_n + 1, split = blockIdx.x % p.splits, r = blockIdx.x / p.splits, s = r / rows, j = r % rows;
+  const int split = blockIdx.x, j = blockIdx.y, s = blockIdx.z;
   if (j > count_of(a, s)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (j == 0 && split == 0 && threadIdx.x == 0) p.done[s] = 0;  // for the next kernel
@@ -204,10 +215,12 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
 #pragma unroll
     for (int e = 0; e < VEC; e += 2) {
       const uint64_t y = mul_pair(add_pair(pair_of(x[e], x[e + 1]), from2), c2);
-      sum2 = add_pair(sum2, pair_of(fast_exp2(low_of(y)), fast_exp2(high_of(y))));
+      const float2 each = halves_of(y);
+      sum2 = add_pair(sum2, pair_of(fast_exp2(each.x), fast_exp2(each.y)));
     }
   }
-  float sum = low_of(sum2) + high_of(sum2);
+  const float2 sums = halves_of(sum2);
+  float sum = sums.x + sums.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   int best = 0x7fffffff;
@@ -227,7 +240,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
   if (threadIdx.x) return;
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) sum += warp_sum[w], best = min(best, warp_best[w]);
-  p.partials[blockIdx.x] = {top, sum, best, 0};
+  p.partials[((int64_t)s * gridDim.y + j) * gridDim.x + split] = {top, sum, best, 0};
 }
 
 // exp(d * T^-1) of the draw: 2^(k / 16) from a table, k the nearest whole number of the exponent in sixteenths, times a
@@ -283,44 +296,87 @@ template <typename T> struct Exponential {
 // Whether something remains: above 0, or no number.  By the bits, no compare on the fp64 pipe.
 __device__ __forceinline__ bool remains(double rest) { return ((uint32_t)__double2hiint(rest) ^ 0x80000000u) > 0x7ff00000u; }
 
+// Adds what remains of an element, predicated: a branch would cost more.
+__device__ __forceinline__ void add_remaining(Sums& s, double rest, double e) {
+  asm("{\n .reg .pred p;\n setp.gt.u32 p, %2, 0x7ff00000;\n @p add.f64 %0, %0, %3;\n @p add.f64 %1, %1, %4;\n}\n"
+      : "+d"(s.left), "+d"(s.e_left)
+      : "r"(__double2hiint(rest) ^ 0x80000000), "d"(rest), "d"(e));
+}
+
 // The sums of a warp's vectors [begin, end), the lanes side by side, the same in every lane.  One loop of little code: most calls go
 // through it once or a few times, and what costs most then is to fetch the instructions.
 template <typename T, typename Q> __device__ __forceinline__ Sums sum_vectors(const Row<T>& row, const Q* left, int begin, int end,
                                                                               const Exponential<T>& exponential, Weights kind,
                                                                               double unit, int fallen) {
   constexpr int VEC = Row<T>::VEC;
+  constexpr int NEAR = 20 << 20;  // an element is next to the border where its rest is below 2^-20 of q, by the numbers' upper words
+  const int lane = threadIdx.x & 31, first = max(begin, row.full_begin), last = min(end, row.full_end);
   const int but = kind == OTHERS ? fallen : -1;
   Sums s = {0.0, 0.0, 0.0, 0.0};
-  int k = begin + (threadIdx.x & 31);
+  // ---- the full vectors, the next one in flight
+  int i = row.first(first + lane), left_over = (last - first - lane + 31) >> 5;
+  const uint4* at = reinterpret_cast<const uint4*>(row.x + i);
   uint4 next_x = make_uint4(0, 0, 0, 0);
   Probs<Q, VEC> next_q;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) next_q.e[i] = Dtype<Q>::from_f(0.f);
-  auto fetch = [&]() {
-    next_x = row.load(k);
-    if (kind == LEFT) next_q.load(left, row.first(k), row.vocab);
-  };
-  if (k < end) fetch();
+  for (int e = 0; e < VEC; ++e) next_q.e[e] = Dtype<Q>::from_f(0.f);
+  if (left_over > 0) {
+    next_x = *at;
+    if (kind == LEFT) next_q.load(left + i);
+  }
 #pragma unroll 1
-  while (k < end) {
+  for (; left_over > 0; --left_over) {
     float x[VEC];
     Row<T>::to_float(next_x, x);
     exponential.prepare(x);
     const Probs<Q, VEC> now_q = next_q;
-    if ((unsigned)(but - row.first(k)) < VEC)
+    if ((unsigned)(but - i) < VEC)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (row.first(k) + i == but) x[i] = -INFINITY;
-    k += 32;
-    if (k < end) fetch();
+      for (int e = 0; e < VEC; ++e)
+        if (i + e == but) x[e] = -INFINITY;
+    at += 32, i += 32 * VEC;
+    if (left_over > 1) {
+      next_x = *at;
+      if (kind == LEFT) next_q.load(left + i);
+    }
+    double e[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const double e = exponential(x[i]);
+    for (int u = 0; u < VEC; ++u) e[u] = exponential(x[u]);
+    if (kind == LEFT) {
+      bool near = false;
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        const double q = (double)now_q[u], rest = fma(e[u], unit, -q);
+        add_remaining(s, rest, e[u]);
+        near |= (__double2hiint(rest) & 0x7fffffff) + NEAR < __double2hiint(q);
+      }
+      if (near)
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) {
+          const double q = (double)now_q[u], rest = fma(e[u], unit, -q);
+          if ((__double2hiint(rest) & 0x7fffffff) + NEAR < __double2hiint(q)) s.border += e[u];
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < VEC; o *= 2)
+#pragma unroll
+      for (int u = 0; u < VEC; u += 2 * o) e[u] += e[u + o];
+    s.all += e[0];
+  }
+  // ---- the row's ends, an element a lane: those in front of the first full vector, then those behind the last one
+  if (begin < end && (begin < row.full_begin || end > row.full_end)) {
+    const int front = begin < row.full_begin ? min(row.first(row.full_begin), row.vocab) : 0;
+    const int behind = end > row.full_end && row.full_end >= row.full_begin ? row.vocab - row.first(row.full_end) : 0;
+    const int at_end = lane < front ? lane : row.vocab - behind + lane - front;
+    if (lane < front + behind) {
+      float x[1] = {at_end == but ? -INFINITY : Dtype<T>::to_f(row.x[at_end])};
+      exponential.prepare(x);
+      const double e = exponential(x[0]);
       s.all += e;
       if (kind == LEFT) {
-        const double q = (double)now_q[i], rest = fma(e, unit, -q);
-        if (remains(rest)) s.left += rest, s.e_left += e;
-        if ((__double2hiint(rest) & 0x7ff00000) + (20 << 20) < (__double2hiint(q) & 0x7ff00000)) s.border += e;
+        const double q = (double)Dtype<Q>::to_f(left[at_end]), rest = fma(e, unit, -q);
+        add_remaining(s, rest, e);
+        if ((__double2hiint(rest) & 0x7fffffff) + NEAR < __double2hiint(q)) s.border += e;
       }
     }
   }
@@ -427,7 +483,7 @@ __device__ __forceinline__ float logprob_of(float logit, const Partial& row, dou
 template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS, DRAW_CTAS) verify_draw_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC;
   const ucb_verify_args& a = p.a;
-  const int s = blockIdx.x / p.ctas, cta = blockIdx.x % p.ctas;
+  const int s = blockIdx.y, cta = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = a.drafts_n + 1, count = count_of(a, s);
   __shared__ Partial part[MAX_ROWS];
   __shared__ int accepted_at, fallen_draft;
@@ -639,13 +695,13 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
 }
 
 template <typename T, typename Q> int launch_draw(const VerifyParams& p, cudaStream_t s) {
-  return block8::launch(verify_draw_kernel<T, Q>, dim3((unsigned)p.a.seqs * p.ctas), dim3(DRAW_THREADS), 0, s, p, "verify_draw_kernel", 1,
+  return block8::launch(verify_draw_kernel<T, Q>, dim3(p.ctas, p.a.seqs), dim3(DRAW_THREADS), 0, s, p, "verify_draw_kernel", 1,
                         true);
 }
 
 template <typename T> int launch_all(const VerifyParams& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)((int64_t)p.a.seqs * (p.a.drafts_n + 1) * p.splits);
-  if (int rc = block8::launch(verify_rows_kernel<T>, dim3(grid), dim3(ROW_THREADS), 0, s, p, "verify_rows_kernel")) return rc;
+  const dim3 grid(p.splits, p.a.drafts_n + 1, p.a.seqs);
+  if (int rc = block8::launch(verify_rows_kernel<T>, grid, dim3(ROW_THREADS), 0, s, p, "verify_rows_kernel")) return rc;
   switch (p.a.draft_probs ? p.a.probs_dtype : UCB_F32) {
     case UCB_BF16: return launch_draw<T, __nv_bfloat16>(p, s);
     case UCB_F16: return launch_draw<T, __half>(p, s);
@@ -690,8 +746,7 @@ extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
   if (!a) return set_error(UCB_ERR_INVALID, "%s: null pointer", what);
   if (a->seqs < 0 || a->drafts_n < 0 || a->vocab < 1) return set_error(UCB_ERR_INVALID, "%s: bad shape", what);
   if (a->drafts_n >= uv::MAX_ROWS) return set_error(UCB_ERR_UNSUPPORTED, "%s: at most %d drafts", what, uv::MAX_ROWS - 1);
-  if (a->vocab > 0x7fffff00 || (int64_t)a->seqs * (a->drafts_n + 1) > 0x1ffffff)
-    return set_error(UCB_ERR_UNSUPPORTED, "%s: too many rows or tokens", what);
+  if (a->vocab > 0x7fffff00 || a->seqs > 65535) return set_error(UCB_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
   if (!(a->temperature_all >= 0.f && a->temperature_all < 3.0e38f)) return set_error(UCB_ERR_INVALID, "%s: bad temperature", what);
   if (a->seqs == 0) return UCB_OK;
   if (!a->logits || (a->drafts_n && !a->drafts) || !a->uniforms || !a->tokens || !a->accepted || !a->logprobs || !a->workspace)
@@ -704,8 +759,6 @@ extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
   uv::Layout layout;
   if (!layout.make(a->seqs, a->drafts_n + 1, a->vocab, a->dtype))
     return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
-  if (layout.splits * a->seqs * (a->drafts_n + 1) > 0x7fffffff || layout.ctas * a->seqs > 0x7fffffff || layout.part_vectors > 0x7fffffff)
-    return set_error(UCB_ERR_UNSUPPORTED, "%s: too many rows or tokens", what);
   char* w = static_cast<char*>(a->workspace);
   const uv::VerifyParams p{*a, reinterpret_cast<uv::Partial*>(w), reinterpret_cast<uv::Sums*>(w + layout.partials_bytes),
                            reinterpret_cast<unsigned int*>(w + layout.partials_bytes + layout.sums_bytes), (int)layout.splits,
