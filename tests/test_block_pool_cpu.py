@@ -49,7 +49,7 @@ def test_bad_calls_are_refused():
             (lambda: lib.ucb_block_pool_fork(pool, None, one, 1, one, 1, 4, one, None), "null pointer"),
             (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, None, 1, 4, one, None), "no caches"),
             (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 0, 4, one, None), "no caches"),
-            (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 65536, 4, one, None), "65535"),
+            (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 32768, 4, one, None), "32767"),
             (lambda: lib.ucb_block_pool_fork(pool, one, one, 1, one, 1, 4, ctypes.c_void_p(4104), None), "aligned"),
             (lambda: lib.ucb_block_pool_compact(pool, one, 1, 4, None, one, None), "null pointer"),
             (lambda: lib.ucb_block_pool_compact(pool, None, 1, 4, one, one, None), "no caches"),

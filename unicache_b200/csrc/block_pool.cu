@@ -213,7 +213,7 @@ struct ForkParams {
   PoolParams p;
   const int32_t *parents, *children;
   int count;
-  int4* jobs;  // of each pair: source and target block of its incomplete block (-1: nothing to copy), parent, child
+  int4* jobs;  // of each pair: source and target block of its incomplete block (-1: nothing to copy), parent and above it rows, child
 };
 
 enum PairState : int { SKIPPED = -2, WHOLE = -1 };  // otherwise the rank of the block that the pair takes
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(const ForkParams q) 
       if (b >= 0 && b < pool.num_blocks) atomicAdd(&pool.references[b], 1); else bad = true;
     }
     if (lane == 0) {
-      int4 job = make_int4(-1, -1, from, to);
+      int4 job = make_int4(-1, -1, from | (length % bt) << 24, to);
       if (s >= 0 && fits) {
         const int b = source[shared], block = q.jobs[i].y;
         row[shared] = block;
@@ -327,54 +327,74 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(const ForkParams q) 
   if (bad) atomicOr(q.p.err, DEVERR_BAD_DESCRIPTOR);
 }
 
-// Copies of the bytes of one block, 16 at a time.
-__device__ __forceinline__ void copy16(void* to, const void* from, int64_t bytes, int thread, int threads) {
-  const uint4* src = static_cast<const uint4*>(from);
-  uint4* dst = static_cast<uint4*>(to);
-  const int64_t n = bytes / 16;
-  constexpr int AHEAD = 8;
-  for (int64_t i = thread; i < n; i += (int64_t)AHEAD * threads) {
-    uint4 x[AHEAD];
+// A piece of memory to be copied by a group of threads, 16 bytes at a time: loaded first, stored when other loads are on their way.
+template <int AHEAD> struct Piece {
+  uint4 x[AHEAD];
+  __device__ __forceinline__ void load(const void* from, int bytes, int thread, int threads) {
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (i + (int64_t)k * threads < n) x[k] = src[i + (int64_t)k * threads];
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (i + (int64_t)k * threads < n) dst[i + (int64_t)k * threads] = x[k];
+      if (thread + k * threads < bytes / 16) x[k] = static_cast<const uint4*>(from)[thread + k * threads];
   }
-}
+  __device__ __forceinline__ void store(void* to, int bytes, int thread, int threads) const {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (thread + k * threads < bytes / 16) static_cast<uint4*>(to)[thread + k * threads] = x[k];
+  }
+};
 
 struct ForkCopyParams {
   const int4* jobs;
-  const int32_t* lengths;
   const ucb_block8_cache* caches;
 };
 
-// Pair blockIdx.x, layer blockIdx.y; blockIdx.z is a head's keys or values: the rows that count, and the rows themselves
-// with the record of whose they are.
-__global__ void __launch_bounds__(256) fork_copy_kernel(const ForkCopyParams q) {
+constexpr int FORK_WARPS = 4;
+
+// Pair blockIdx.x, layer blockIdx.y; a warp copies a head's keys or values: the codes of the rows that count, the rows themselves, and
+// of the keys the record of whose rows they are and the bounds.  What a warp copies is a few KB and waits for the pair, then for
+// the data: 56 pairs x 28 layers x 4 heads x 128 (357 MB there and back) in 63 us; a CTA for each head's keys or values took 142.
+__global__ void __launch_bounds__(FORK_WARPS * 32) fork_copy_kernel(const ForkCopyParams q) {
   const ucb_block8_cache c = q.caches[blockIdx.y];
-  const int h = blockIdx.z >> 1, value = blockIdx.z & 1;
+  const int lane = threadIdx.x & 31, item = blockIdx.z * FORK_WARPS + (threadIdx.x >> 5), h = item >> 1, value = item & 1;
+  if (h >= c.kv_heads) return;
   wait_for_primary();
   const int4 job = q.jobs[blockIdx.x];
-  if (job.y < 0 || h >= c.kv_heads) return;
-  const int rows = q.lengths[job.z] % c.block_tokens;
+  if (job.y < 0) return;
+  const int rows = job.z >> 24, parent = job.z & 0xffffff, child = job.w;
   const int64_t block = (int64_t)c.block_tokens * c.head_dim;
   const int64_t from = (int64_t)job.x * c.kv_heads + h, to = (int64_t)job.y * c.kv_heads + h;
   int8_t* code = value ? c.value_code : c.key_code;
-  copy16(code + to * block, code + from * block, (int64_t)rows * c.head_dim, threadIdx.x, blockDim.x);
+  const int8_t* code_from = code + from * block;
+  int8_t* code_to = code + to * block;
   char* pending = static_cast<char*>(value ? c.pending_value : c.pending_key);
-  char* pending_to = pending + ((int64_t)job.w * c.kv_heads + h) * block * 2;
-  const char* pending_from = pending + ((int64_t)job.z * c.kv_heads + h) * block * 2;
-  copy16(pending_to, pending_from, (int64_t)rows * c.head_dim * 2, threadIdx.x, blockDim.x);
-  if (!value) {
-    const int64_t record = (int64_t)(c.block_tokens - 1) * c.head_dim * 2;
-    copy16(pending_to + record, pending_from + record, c.head_dim * 2, threadIdx.x, blockDim.x);
-    copy16(c.key_low + to * c.head_dim, c.key_low + from * c.head_dim, c.head_dim, threadIdx.x, blockDim.x);
-    copy16(c.key_high + to * c.head_dim, c.key_high + from * c.head_dim, c.head_dim, threadIdx.x, blockDim.x);
+  const char* pending_from = pending + ((int64_t)parent * c.kv_heads + h) * block * 2;
+  char* pending_to = pending + ((int64_t)child * c.kv_heads + h) * block * 2;
+  // the bounds and the record: of 16 bytes a lane, head_dim / 16 lanes each of the bounds, head_dim / 8 of the record
+  const int bound_lanes = value ? 0 : c.head_dim / 16, record_lanes = value ? 0 : c.head_dim / 8;
+  const int64_t record = (block - c.head_dim) * 2;
+  uint4 low, high, rec;
+  if (lane < bound_lanes) {
+    low = reinterpret_cast<const uint4*>(c.key_low + from * c.head_dim)[lane];
+    high = reinterpret_cast<const uint4*>(c.key_high + from * c.head_dim)[lane];
   }
+  if (lane < record_lanes) rec = reinterpret_cast<const uint4*>(pending_from + record)[lane];
   float* scale = value ? c.value_scale : c.key_scale;
-  if (threadIdx.x == 0) scale[to] = scale[from];
+  const float scale_from = scale[from];
+  constexpr int CODES = 4, ROWS = 8, STEP = CODES * 32 * 16;  // bytes of codes at a time, and twice as many of rows
+  const int bytes = rows * c.head_dim;
+  for (int at = 0; at < bytes; at += STEP) {
+    Piece<CODES> codes;
+    Piece<ROWS> held;
+    codes.load(code_from + at, bytes - at, lane, 32);
+    held.load(pending_from + 2 * at, 2 * (bytes - at), lane, 32);
+    codes.store(code_to + at, bytes - at, lane, 32);
+    held.store(pending_to + 2 * at, 2 * (bytes - at), lane, 32);
+  }
+  if (lane < bound_lanes) {
+    reinterpret_cast<uint4*>(c.key_low + to * c.head_dim)[lane] = low;
+    reinterpret_cast<uint4*>(c.key_high + to * c.head_dim)[lane] = high;
+  }
+  if (lane < record_lanes) reinterpret_cast<uint4*>(pending_to + record)[lane] = rec;
+  if (lane == 0) scale[to] = scale_from;
 }
 
 // ---------------------------------------------------------------- compact
@@ -425,29 +445,49 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_kernel(const CompactPara
   if (pass.rank == 0 && threadIdx.x == 0) *q.live = (int)live, *q.moves = (int)movers;
 }
 
-// The moved blocks of every layer, keys and values apart, and the table's entries.
-__global__ void __launch_bounds__(256) compact_copy_kernel(const CompactParams q) {
+constexpr int MOVE_THREADS = 256;
+
+// The moved blocks, and the table's entries.  blockIdx.y is a layer's keys or values, whose addresses a CTA looks up once; it
+// goes from move to move, the next one's blocks known before.
+__global__ void __launch_bounds__(MOVE_THREADS) compact_copy_kernel(const CompactParams q) {
   const ucb_block_pool& pool = q.p.pool;
+  const ucb_block8_cache& c = q.caches[blockIdx.y >> 1];
+  const int value = blockIdx.y & 1, heads = c.kv_heads, bound_bytes = heads * c.head_dim;
+  const int64_t block = (int64_t)bound_bytes * c.block_tokens;
+  int8_t* code = value ? c.value_code : c.key_code;
+  int8_t* bound = value ? c.key_high : c.key_low;
+  float* scale = value ? c.value_scale : c.key_scale;
   wait_for_primary();
   const int live = *q.live, moves = *q.moves;
   if (moves == 0) return;
-  const int64_t items = (int64_t)moves * q.layers * 2;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int value = item & 1;
-    const int64_t k = (item >> 1) / q.layers;
-    const ucb_block8_cache& c = q.caches[(item >> 1) % q.layers];
-    const int64_t from = q.movers[k], to = q.holes[k], heads = c.kv_heads, block = heads * c.block_tokens * c.head_dim;
-    int8_t* code = value ? c.value_code : c.key_code;
-    int8_t* bound = value ? c.key_high : c.key_low;
-    float* scale = value ? c.value_scale : c.key_scale;
-    copy16(code + to * block, code + from * block, block, threadIdx.x, blockDim.x);
-    copy16(bound + to * heads * c.head_dim, bound + from * heads * c.head_dim, heads * c.head_dim, threadIdx.x, blockDim.x);
-    for (int h = threadIdx.x; h < heads; h += blockDim.x) scale[to * heads + h] = scale[from * heads + h];
+  int k = blockIdx.x;
+  int64_t from = 0, to = 0;
+  if (k < moves) from = q.movers[k], to = q.holes[k];
+  while (k < moves) {
+    const int8_t* code_from = code + from * block;
+    int8_t* code_to = code + to * block;
+    const int8_t* bound_from = bound + from * bound_bytes;
+    int8_t* bound_to = bound + to * bound_bytes;
+    const float* scale_from = scale + from * heads;
+    float* scale_to = scale + to * heads;
+    k += gridDim.x;
+    if (k < moves) from = q.movers[k], to = q.holes[k];
+    for (int at = threadIdx.x * 16; at < bound_bytes; at += MOVE_THREADS * 16)
+      *reinterpret_cast<uint4*>(bound_to + at) = *reinterpret_cast<const uint4*>(bound_from + at);
+    for (int h = threadIdx.x; h < heads; h += MOVE_THREADS) scale_to[h] = scale_from[h];
+    constexpr int AHEAD = 8, STEP = AHEAD * MOVE_THREADS * 16;
+    for (int64_t at = 0; at < block; at += STEP) {
+      Piece<AHEAD> x;
+      const int bytes = (int)min((int64_t)STEP, block - at);
+      x.load(code_from + at, bytes, threadIdx.x, MOVE_THREADS);
+      x.store(code_to + at, bytes, threadIdx.x, MOVE_THREADS);
+    }
   }
-  for (int s = blockIdx.x; s < pool.num_seqs; s += gridDim.x) {
+  const int cta = blockIdx.y * gridDim.x + blockIdx.x, ctas = gridDim.x * gridDim.y;
+  for (int s = cta; s < pool.num_seqs; s += ctas) {
     int32_t* row = pool.block_table + (int64_t)s * pool.max_blocks;
     const int held = min(pool.held[s], pool.max_blocks);
-    for (int j = threadIdx.x; j < held; j += blockDim.x) {
+    for (int j = threadIdx.x; j < held; j += MOVE_THREADS) {
       const int b = row[j];
       if (b >= live && b < pool.num_blocks) row[j] = q.place[b];
     }
@@ -480,8 +520,8 @@ int plan_cluster(int64_t blocks) {
 
 int check_layers(const void* caches, int layers, int kv_heads, const char* what) {
   if (!caches || layers < 1 || kv_heads < 1) return ucb_host::set_error(UCB_ERR_INVALID, "%s: no caches", what);
-  if (layers > 65535 || kv_heads > 32767)
-    return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "%s: at most 65535 caches of 32767 KV heads", what);
+  if (layers > 32767 || kv_heads > 32767)
+    return ucb_host::set_error(UCB_ERR_UNSUPPORTED, "%s: at most 32767 caches of 32767 KV heads", what);
   if (reinterpret_cast<uintptr_t>(caches) & 7) return ucb_host::set_error(UCB_ERR_INVALID, "%s: caches must be 8-byte aligned", what);
   return UCB_OK;
 }
@@ -532,8 +572,9 @@ extern "C" int ucb_block_pool_fork(const ucb_block_pool* pool, const int32_t* pa
   const b8::ForkParams q{{*pool, err}, parents, children, count, static_cast<int4*>(workspace)};
   const int ctas = b8::plan_cluster(pool->num_blocks);
   if (int rc = b8::launch(b8::fork_kernel, dim3(ctas), dim3(b8::PLAN_THREADS), 0, s, q, "block pool fork_kernel", ctas)) return rc;
-  const b8::ForkCopyParams c{q.jobs, pool->lengths, caches};
-  return b8::launch(b8::fork_copy_kernel, dim3(count, layers, 2 * kv_heads), dim3(256), 0, s, c, "block pool fork_copy_kernel", 1, true);
+  const b8::ForkCopyParams c{q.jobs, caches};
+  return b8::launch(b8::fork_copy_kernel, dim3(count, layers, (2 * kv_heads + b8::FORK_WARPS - 1) / b8::FORK_WARPS),
+                    dim3(b8::FORK_WARPS * 32), 0, s, c, "block pool fork_copy_kernel", 1, true);
 }
 
 // The number of moves, then holes and movers (half of the pool at most each), then every block's place.
@@ -559,7 +600,8 @@ extern "C" int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_bloc
   if (int rc = b8::launch(b8::compact_kernel, dim3(ctas), dim3(b8::PLAN_THREADS), 0, s, q, "block pool compact_kernel", ctas)) return rc;
   const int sms = ucb_host::multiprocessors();
   if (sms < 1) return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
-  const int64_t items = std::max<int64_t>(half * layers * 2, pool->num_seqs);
-  const unsigned grid = (unsigned)std::min<int64_t>(items, (int64_t)sms * 8);
-  return b8::launch(b8::compact_copy_kernel, dim3(std::max(1u, grid)), dim3(256), 0, s, q, "block pool compact_copy_kernel", 1, true);
+  // a little more CTAs than are resident together, spread over the layers' keys and values
+  const int64_t across = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(half, 1), (int64_t)sms * 8 / (2 * layers)));
+  return b8::launch(b8::compact_copy_kernel, dim3((unsigned)across, 2 * layers), dim3(b8::MOVE_THREADS), 0, s, q,
+                    "block pool compact_copy_kernel", 1, true);
 }
