@@ -158,10 +158,10 @@ class BlockPool:
         blocks behind are then of no use, so that a pool can be cut or handed on."""
 
         self._need_caches()
-        workspace = self.lengths.new_empty(self._compact_bytes // 4 + 1)
+        workspace, live = self.lengths.new_empty(self._compact_bytes // 4), self.lengths.new_empty(1)
         kernels._call_on(self.index, "ucb_block_pool_compact", self.descriptor, self._layers_at, len(self.caches),
-                         self._kv_heads, workspace[-1:].data_ptr(), workspace.data_ptr(), kernels.stream_of(self.lengths))
-        return workspace[-1:]
+                         self._kv_heads, live.data_ptr(), workspace.data_ptr(), kernels.stream_of(self.lengths))
+        return live
 
     def free_blocks(self) -> int:
         """Blocks that no sequence names.  Waits for the device."""
