@@ -166,7 +166,6 @@ __global__ void __launch_bounds__(LANES_THREADS, 1)
     int of[4];
   };
   using Pos = std::conditional_t<AXES == NO_AXES, int64_t, std::conditional_t<AXES == ONE_AXIS, int, Rows>>;
-  const unsigned row_lanes = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1) << (threadIdx.x & 31 & ~(L - 1));
   auto row_of = [&](uint32_t t, int pair) {
     const int64_t pos = position_of(p, t + axis_of(p, pair) * p.axis_stride);
     return pos < 0 || pos >= p.table_rows ? -1 : (int)pos;
@@ -213,7 +212,6 @@ __global__ void __launch_bounds__(LANES_THREADS, 1)
         a.s = *reinterpret_cast<const float4*>(p.sin + at);
       }
     }
-    if (AXES != NO_AXES) a.bad = __any_sync(row_lanes, a.bad);  // of any of the row's lanes
     return a;
   };
   uint32_t t = t0;
@@ -227,20 +225,21 @@ __global__ void __launch_bounds__(LANES_THREADS, 1)
       next = fetch(t + token_step, pos);
       pos = position(t + 2 * token_step);
     }
-    if (now.bad && lane == 0 && rows > 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
+    if (now.bad && (AXES != NO_AXES || lane == 0) && rows > 0) atomicOr(p.err, DEVERR_BAD_DESCRIPTOR);
     const float c[4] = {now.c.x, now.c.y, now.c.z, now.c.w}, s[4] = {now.s.x, now.s.y, now.s.z, now.s.w};
     float wf[8];
     if (weight) w[0].to(wf), w[1].to(wf + 4);
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
-      float x[8], ss = 0.f;
+      // a position of any lane's that is outside the tables reaches the row's other lanes through the sum of squares
+      float x[8], ss = AXES != NO_AXES && now.bad ? __int_as_float(0x7fffffff) : 0.f;
       now.raw[i][0].to(x);
       now.raw[i][1].to(x + 4);
 #pragma unroll
       for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, L);
-      const float r = now.bad ? __int_as_float(0x7fffffff) : rsqrtf(ss * (1.f / (8 * L)) + p.eps);
+      const float r = AXES == NO_AXES && now.bad ? __int_as_float(0x7fffffff) : rsqrtf(ss * (1.f / (8 * L)) + p.eps);
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[k] = weight ? x[k] * r * wf[k] : x[k] * r;
       if (turned) {
