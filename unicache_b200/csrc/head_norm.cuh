@@ -136,7 +136,7 @@ template <typename T> __device__ __forceinline__ void store4(T* dst, const float
 // of angles a lane.
 enum Axes { NO_AXES, ONE_AXIS, ANY_AXIS };
 template <typename T, int L, int HEADS, bool PAIRS, bool STREAM, Axes AXES>
-__global__ void __launch_bounds__(LANES_THREADS, 1)
+__global__ void __launch_bounds__(LANES_THREADS, AXES == ANY_AXIS ? 4 : 1)
     head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units, uint32_t token_step) {
   const uint32_t group = (blockIdx.x * (uint32_t)LANES_THREADS + threadIdx.x) / L;
   const int lane = threadIdx.x % L;
