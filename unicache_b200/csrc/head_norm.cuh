@@ -128,15 +128,15 @@ template <typename T> __device__ __forceinline__ void store4(T* dst, const float
 // that the rotation needs no exchange and the lane four angles, which the HEADS rows
 // of one token that it has in flight share.  With STREAM a group of lanes goes from
 // token to token, the next one's rows and angles in flight.  Measured for
-// 16384 tokens x 32 heads x 128 (277 MB): 53 us (5.2 TB/s) with STREAM, one token
-// a group 57; 2 rows a lane 75, 1 row 85, 8 rows 84; blocks of 256 threads 59.  Neither memory nor issue slots (61%) are used
-// up there: 16 warps a multiprocessor, all that 128 registers leave, wait for their loads.  In fp32 (537 MB) 93 us, 5.8 TB/s.
+// 16384 tokens x 32 heads x 128 (277 MB): 47 us (5.9 TB/s) with STREAM; while positions were waited for where they are loaded 53, one
+// token a group 57, 2 rows a lane 75, 1 row 85, 8 rows 84, blocks of 256 threads 59.  Neither memory nor issue slots are used
+// up there: 16 warps a multiprocessor, all that 128 registers leave, wait for their loads.
 // AXES: each pair's angle is that of its own axis' position.  ONE_AXIS: a lane's four pairs share an axis, as sections
-// of whole fours have it, so that only the address of its position differs; ANY_AXIS: four positions and eight single loads
-// of angles a lane.
+// of whole fours have it, so that only the address of its position differs (47 us too); ANY_AXIS: four positions and eight single
+// loads of angles a lane (52; with the registers of three CTAs a multiprocessor 65).
 enum Axes { NO_AXES, ONE_AXIS, ANY_AXIS };
 template <typename T, int L, int HEADS, bool PAIRS, bool STREAM, Axes AXES>
-__global__ void __launch_bounds__(LANES_THREADS, AXES == ANY_AXIS ? 4 : 1)
+__global__ void __launch_bounds__(LANES_THREADS, AXES == ANY_AXIS && sizeof(T) == 2 ? 4 : 1)
     head_norm_lanes_kernel(const HeadNormParams p, uint32_t q_units, uint32_t units, uint32_t token_step) {
   const uint32_t group = (blockIdx.x * (uint32_t)LANES_THREADS + threadIdx.x) / L;
   const int lane = threadIdx.x % L;
@@ -161,18 +161,35 @@ __global__ void __launch_bounds__(LANES_THREADS, AXES == ANY_AXIS ? 4 : 1)
     float4 c, s;
     bool bad;
   };
-  // rows of the tables that a lane's pairs need of a token; with axes -1 for one outside
-  struct Rows {
+  // A token's positions as they are loaded, two tokens ahead: nothing may be computed from them before they are needed, or the
+  // lane waits for them there (32-bit positions that were extended at once cost 16384 tokens x 32 heads x 128 5 us).
+  struct Raw {
+    uint32_t low;
+    int32_t high;  // of 64 bits
+  };
+  struct Rows {  // with axes those of the lane's pairs; of 64 bits that are no row of the tables -1
     int of[4];
   };
-  using Pos = std::conditional_t<AXES == NO_AXES, int64_t, std::conditional_t<AXES == ONE_AXIS, int, Rows>>;
+  using Pos = std::conditional_t<AXES == NO_AXES, Raw, std::conditional_t<AXES == ONE_AXIS, int, Rows>>;
+  auto raw_of = [&](int64_t i) {
+    Raw r{0, 0};
+    if (p.pos64) {
+      const uint2 v = static_cast<const uint2*>(p.pos)[i];
+      r.low = v.x, r.high = (int32_t)v.y;
+    } else {
+      r.low = static_cast<const uint32_t*>(p.pos)[i];
+    }
+    return r;
+  };
   auto row_of = [&](uint32_t t, int pair) {
-    const int64_t pos = position_of(p, t + axis_of(p, pair) * p.axis_stride);
+    const int64_t i = t + axis_of(p, pair) * p.axis_stride;
+    if (!p.pos64) return static_cast<const int32_t*>(p.pos)[i];
+    const int64_t pos = static_cast<const int64_t*>(p.pos)[i];
     return pos < 0 || pos >= p.table_rows ? -1 : (int)pos;
   };
   auto position = [&](uint32_t t) {
     if constexpr (AXES == NO_AXES) {
-      return p.rot && t < p.tokens ? position_of(p, t) : 0;
+      return p.rot && t < p.tokens ? raw_of(t) : Raw{0, 0};
     } else if constexpr (AXES == ONE_AXIS) {
       return turned && t < p.tokens ? row_of(t, 4 * lane) : 0;
     } else {
@@ -194,20 +211,25 @@ __global__ void __launch_bounds__(LANES_THREADS, AXES == ANY_AXIS ? 4 : 1)
         a.raw[i][1].load(src + t * st + i * sh + d1);
       }
     if constexpr (AXES == ANY_AXIS) {
-      a.bad = min(min(pos.of[0], pos.of[1]), min(pos.of[2], pos.of[3])) < 0;
+      a.bad = false;
       if (turned) {
         float c[4], s[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int64_t at = (int64_t)max(pos.of[k], 0) * half + 4 * lane + k;
+          const bool inside = pos.of[k] >= 0 && pos.of[k] < p.table_rows;
+          const int64_t at = (int64_t)(inside ? pos.of[k] : 0) * half + 4 * lane + k;
+          a.bad |= !inside;
           c[k] = p.cos[at], s[k] = p.sin[at];
         }
         a.c = make_float4(c[0], c[1], c[2], c[3]), a.s = make_float4(s[0], s[1], s[2], s[3]);
       }
     } else {
-      a.bad = p.rot && (pos < 0 || pos >= p.table_rows);
+      int64_t row;
+      if constexpr (AXES == NO_AXES) row = p.pos64 ? (int64_t)pos.high << 32 | pos.low : (int64_t)(int32_t)pos.low;
+      else row = pos;
+      a.bad = p.rot && (row < 0 || row >= p.table_rows);
       if (turned) {
-        const int64_t at = (a.bad ? 0 : (int64_t)pos) * half + 4 * lane;
+        const int64_t at = (a.bad ? 0 : row) * half + 4 * lane;
         a.c = *reinterpret_cast<const float4*>(p.cos + at);
         a.s = *reinterpret_cast<const float4*>(p.sin + at);
       }
