@@ -366,7 +366,7 @@ constexpr int FORK_WARPS = 4;
 
 // Pair blockIdx.x, layer blockIdx.y; a warp copies a head's keys or values: the codes of the rows that count, the rows themselves, and
 // of the keys the record of whose rows they are and the bounds.  What a warp copies is a few KB and waits for the pair, then for
-// the data: 56 pairs x 28 layers x 4 heads x 128 (357 MB there and back) in 63 us; a CTA for each head's keys or values took 142.
+// the data: 56 pairs x 28 layers x 4 heads x 128 (203 MB, as seven children read the same parent) in 39 us; a CTA for each head took 142.
 __global__ void __launch_bounds__(FORK_WARPS * 32) fork_copy_kernel(const ForkCopyParams q) {
   const ucb_block8_cache c = q.caches[blockIdx.y];
   const int lane = threadIdx.x & 31, item = blockIdx.z * FORK_WARPS + (threadIdx.x >> 5), h = item >> 1, value = item & 1;
@@ -586,7 +586,8 @@ extern "C" int ucb_block_pool_fork(const ucb_block_pool* pool, const int32_t* pa
   if (!err) return set_error(UCB_ERR_CUDA, "%s: device error word unavailable", what);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const b8::ForkParams q{{*pool, err}, parents, children, count, static_cast<int4*>(workspace)};
-  const int ctas = b8::plan_cluster(pool->num_blocks);
+  // a warp a pair: many pairs have the widest cluster (56 pairs of 64 blocks 50.4 us against 51.8; 7 pairs 12.0 against 10.2)
+  const int ctas = count > b8::PLAN_THREADS / 32 ? b8::MAX_CLUSTER : b8::plan_cluster(pool->num_blocks);
   if (int rc = b8::launch(b8::fork_kernel, dim3(ctas), dim3(b8::PLAN_THREADS), 0, s, q, "block pool fork_kernel", ctas)) return rc;
   const b8::ForkCopyParams c{q.jobs, caches};
   return b8::launch(b8::fork_copy_kernel, dim3(count, layers, (2 * kv_heads + b8::FORK_WARPS - 1) / b8::FORK_WARPS),
@@ -616,8 +617,9 @@ extern "C" int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_bloc
   if (int rc = b8::launch(b8::compact_kernel, dim3(ctas), dim3(b8::PLAN_THREADS), 0, s, q, "block pool compact_kernel", ctas)) return rc;
   const int sms = ucb_host::multiprocessors();
   if (sms < 1) return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
-  // a little more CTAs than are resident together, spread over the layers' keys and values
-  const int64_t across = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(half, 1), (int64_t)sms * 8 / (2 * layers)));
+  // CTAs of a few moves each, spread over the layers' keys and values: 390 moves in 28 layers (917 MB there and back, with the
+  // admission around them) take 153 us with 64 a multiprocessor, of which three are resident; with 8 173, with 200 165
+  const int64_t across = std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(half, 1), (int64_t)sms * 64 / (2 * layers)));
   return b8::launch(b8::compact_copy_kernel, dim3((unsigned)across, 2 * layers), dim3(b8::MOVE_THREADS), 0, s, q,
                     "block pool compact_copy_kernel", 1, true);
 }
