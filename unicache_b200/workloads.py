@@ -23,6 +23,7 @@ import torch
 
 from . import kernels
 from .adapters.attention import int8_block_decode, long_query_attention_summary, sparse_int8_block_decode
+from .storage.block_pool import BlockPool
 from .storage.int8_block import Int8BlockCache
 from .storage.physical import GQAH2OCache, PackedKIVICache
 from .synthetic import make_kv, make_query
@@ -340,3 +341,149 @@ class Int8BlockDecode:
     def replay(self) -> torch.Tensor:
         self.graph.replay()
         return self.x
+
+
+# ---------------------------------------------------------------- drafted decode over a pool of blocks
+class DraftDecode:
+    """A small decoder that verifies drafted tokens over 8-bit caches of one block pool.
+
+    Every prompt starts with an image of ``image`` patches, whose keys turn by the time, row and column of the patch; text goes on behind
+    it on all axes.  A prompt is written once and continued in ``samples`` sequences (``BlockPool.fork``).  A step draws
+    ``drafts`` tokens a sequence from as many linear heads over the last hidden state, runs all of them through the
+    layers at once (``head_norm_rope`` by axes, ``Int8BlockCache.write``, ``int8_block_decode`` with several query tokens) and keeps what
+    ``verify_drafts`` leaves of them, which lowers the lengths that all layers share.  A draft that may be rejected in part
+    must not go past the end of its block, so a sequence near it drafts fewer.  Blocks, counts and lengths are on
+    the device: a step has no host state and is captured once as a CUDA graph.  Weights and prompts are seeded random.
+    """
+
+    def __init__(self, device, *, prompts: list[int], new_tokens: int, samples: int = 1, drafts: int = 3,
+                 image: tuple[int, int] = (4, 6), layers: int = 2, hidden: int = 512, q_heads: int = 8, kv_heads: int = 2,
+                 head_dim: int = 64, block_size: int = 64, vocab: int = 4096, temperature: float = 1.0, theta: float = 1.0e4,
+                 seed: int = 11):
+        self.device = torch.device(device)
+        self.hq, self.hkv, self.d, self.eps, self.n, self.vocab = q_heads, kv_heads, head_dim, 1.0e-6, drafts, vocab
+        patches, self.block = image[0] * image[1], block_size
+        if min(prompts) <= patches or not 0 <= drafts < min(16, block_size):
+            raise ValueError("prompts must be longer than the image, and drafts fewer than 16 and a block's tokens")
+        gen = torch.Generator(device=self.device).manual_seed(seed)
+
+        def normal(*shape, std=1.0, mean=0.0):
+            return (mean + std * torch.randn(*shape, generator=gen, device=self.device)).to(torch.bfloat16)
+
+        count, longest = len(prompts), max(prompts) + new_tokens + drafts + 1
+        seqs = count * samples
+        width = -(-longest // block_size)
+        self.pool = BlockPool.allocate(seqs, longest, sum(-(-n // block_size) for n in prompts) + seqs * (width - min(prompts) // block_size),
+                                       block_size=block_size, device=self.device)
+        self.cos, self.sin = kernels.rope_table(longest, head_dim, theta=theta, device=self.device)
+        half = head_dim // 2
+        sections = [half // 4 // 4 * 4, half // 8 * 3, half - half // 4 // 4 * 4 - half // 8 * 3]
+        self.axes = kernels.rope_axes(sections)
+        # positions of a prompt's tokens: patches by row and column, then text from the larger of the two on
+        i = torch.arange(longest, device=self.device, dtype=torch.int32)
+        text = i - patches + max(image)
+        self.where = torch.stack([torch.where(i < patches, x, text) for x in (i * 0, i // image[1], i % image[1])]).contiguous()
+        rows = torch.cat([torch.arange(n) for n in prompts]).to(self.device)
+        ends = torch.tensor([0, *prompts], dtype=torch.int32).cumsum(0, dtype=torch.int32)
+        starts = ends.tolist() + [ends[-1].item()] * (seqs - count)  # prompts in the first sequences
+        starts = torch.tensor(starts, dtype=torch.int32, device=self.device)
+        self.pool.advance(starts[1:] - starts[:-1])
+        self.w, self.caches = [], []
+        for _ in range(layers):
+            weights = {"norm": normal(hidden, std=0.1, mean=1.0),
+                       "qkv": normal(hidden, (q_heads + 2 * kv_heads) * head_dim, std=hidden ** -0.5),
+                       "q_norm": normal(head_dim, std=0.1, mean=1.0), "k_norm": normal(head_dim, std=0.1, mean=1.0),
+                       "o": normal(q_heads * head_dim, hidden, std=hidden ** -0.5)}
+            cache = self.pool.cache(num_kv_heads=kv_heads, head_dim=head_dim)
+            key, value = normal(sum(prompts), kv_heads, head_dim), normal(sum(prompts), kv_heads, head_dim)
+            _, key = kernels.head_norm_rope(None, key, None, weights["k_norm"], self.cos, self.sin,
+                                            self.where[:, rows].contiguous(), eps=self.eps, axes=self.axes)
+            cache.write(key, value, starts=starts)
+            self.w.append(weights)
+            self.caches.append(cache)
+        if samples > 1:
+            children = torch.arange(count, seqs, dtype=torch.int32, device=self.device)
+            self.pool.fork(children % count, children)
+        self.embed, self.final_norm = normal(vocab, hidden), normal(hidden, std=0.1, mean=1.0)
+        self.lm_head = normal(hidden, vocab, std=4.0 * hidden ** -0.5)
+        # heads near the model's own, so that some drafts stay
+        self.draft_heads = torch.cat([self.lm_head + normal(hidden, vocab, std=1.0 * hidden ** -0.5) for _ in range(drafts)], 1) \
+            if drafts else None
+        self.temperature = torch.full((seqs,), float(temperature), device=self.device)
+        self.last = torch.randint(0, vocab, (seqs,), generator=gen, device=self.device, dtype=torch.int32)
+        self.state = normal(seqs, hidden)  # of the token in front of the last one
+        self.uniforms = torch.rand(seqs, 2 * drafts + 1, generator=gen, device=self.device)  # the caller's to renew
+        self.graph = self.result = None
+
+    def propose(self):
+        """(drafts int32 [seqs, n], their distributions): one linear head each over the last hidden state."""
+
+        seqs, n = self.last.shape[0], self.n
+        if n == 0:
+            return self.last.new_empty((seqs, 0)), None
+        logits = (self.state @ self.draft_heads).view(seqs * n, 1, self.vocab)
+        heat = self.temperature.repeat_interleave(n)
+        # a draw without drafts to verify
+        tokens, _, _ = kernels.verify_drafts(logits, self.last.new_empty((seqs * n, 0)),
+                                             self.uniforms[:, :n].reshape(seqs * n, 1), temperature=heat)
+        probs = torch.softmax(logits.float() / torch.where(heat > 0, heat, 1.0)[:, None, None], -1)
+        return tokens.view(seqs, n), probs.view(seqs, n, self.vocab)
+
+    def step(self):
+        """One verified step of every sequence (device-only, capturable): (tokens [seqs, n + 1], accepted [seqs], logprobs)."""
+
+        hq, hkv, d, n = self.hq, self.hkv, self.d, self.n
+        lengths, seqs = self.pool.lengths, self.last.shape[0]
+        drafts, probs = self.propose()
+        held = lengths.clone()
+        counts = torch.clamp(self.block - 1 - held % self.block, max=n).to(torch.int32)  # up to the block's end
+        self.pool.advance(counts + 1)
+        # rows of the last token and its drafts; those that count, one behind the other, are the write's
+        i = torch.arange(n + 1, device=self.device)
+        meant = i[None] <= counts[:, None]
+        order = torch.sort((~meant).flatten().to(torch.uint8), stable=True).indices
+        starts = torch.zeros(seqs + 1, dtype=torch.int32, device=self.device)
+        torch.cumsum(counts + 1, 0, dtype=torch.int32, out=starts[1:])
+        positions = self.where[:, torch.clamp(held[:, None] + i, max=self.where.shape[1] - 1).flatten()]
+        # the attention takes a sequence's queries as its last tokens: rows that count to the end, and back
+        gap = (n - counts)[:, None]
+        to_end = (torch.clamp(i[None] - gap, min=0) + (n + 1) * torch.arange(seqs, device=self.device)[:, None]).flatten()
+        back = (torch.clamp(i[None] + gap, max=n) + (n + 1) * torch.arange(seqs, device=self.device)[:, None]).flatten()
+        x = self.embed[torch.cat((self.last[:, None], drafts), 1).flatten().long()]
+        for w, cache in zip(self.w, self.caches):
+            qkv = (kernels.rms_norm(x, w["norm"], self.eps) @ w["qkv"]).view(-1, hq + 2 * hkv, d)
+            query, key = kernels.head_norm_rope(qkv[:, :hq], qkv[:, hq:hq + hkv], w["q_norm"], w["k_norm"], self.cos,
+                                                self.sin, positions, eps=self.eps, axes=self.axes)
+            cache.write(key[order], qkv[:, hq + hkv:][order], starts=starts)
+            out, _ = int8_block_decode(query[to_end].view(seqs, n + 1, hq, d), cache)
+            x = torch.addmm(x, out.view(-1, hq * d)[back], w["o"])
+        x = kernels.rms_norm(x, self.final_norm, self.eps)
+        logits = (x @ self.lm_head).view(seqs, n + 1, self.vocab)
+        tokens, accepted, logprobs = kernels.verify_drafts(logits, drafts, self.uniforms[:, n:], draft_probs=probs,
+                                                           temperature=self.temperature, counts=counts, lengths=lengths)
+        at = accepted.long()[:, None]
+        self.last.copy_(tokens.gather(1, at)[:, 0])
+        self.state.copy_(x.view(seqs, n + 1, -1).gather(1, at[..., None].expand(-1, -1, x.shape[-1]))[:, 0])
+        self.result = {"logits": logits, "drafts": drafts, "probs": probs, "counts": counts}
+        return tokens, accepted, logprobs
+
+    def finish(self, sequences: torch.Tensor) -> None:
+        """Sequences (int32) that have ended: their blocks are free, and those still in use move together."""
+
+        self.pool.release(sequences)
+        self.pool.compact()
+
+    def capture(self) -> None:
+        """Capture one step as a CUDA graph, after a first eager one; ``replay`` then runs a step."""
+
+        stream = torch.cuda.Stream(device=self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream):
+            with torch.cuda.graph(self.graph, stream=stream):
+                self.captured = self.step()
+        torch.cuda.current_stream(self.device).wait_stream(stream)
+
+    def replay(self):
+        self.graph.replay()
+        return self.captured
