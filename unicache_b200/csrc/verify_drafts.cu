@@ -473,6 +473,12 @@ __device__ __forceinline__ void judge(const Sums* sums, int parts, Weights kind,
   __syncthreads();
 }
 
+__device__ __forceinline__ unsigned int count_release_acquire(unsigned int* n) {
+  unsigned int before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(n) : "memory");
+  return before;
+}
+
 // ln p of a token from its logit.
 __device__ __forceinline__ float logprob_of(float logit, const Partial& row, double inverse) {
   return (float)(((double)logit - (double)row.top) * inverse - (double)logf(row.sum));
@@ -581,15 +587,15 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   __shared__ Verdict verdict;
   {
     const Sums w = sum_vectors<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, kind, unit, fallen);
-    if (lane == 0) p.sums[(int64_t)s * parts + mine] = w, __threadfence();
+    if (lane == 0) p.sums[(int64_t)s * parts + mine] = w;
   }
   __syncthreads();
-  if (threadIdx.x == 0) is_last = atomicAdd(&p.done[s], 1u) == p.ctas - 1;
+  // the barrier orders the CTA's sums before the count, which releases them to whoever counts last
+  if (threadIdx.x == 0) is_last = count_release_acquire(&p.done[s]) == p.ctas - 1;
   __syncthreads();
   if (!is_last) return;
 
   // ---- the part that the next token lies in
-  __threadfence();
   for (int i = threadIdx.x; i < 2 * parts; i += DRAW_THREADS)
     reinterpret_cast<uint4*>(sums)[i] = __ldcg(reinterpret_cast<const uint4*>(p.sums + (int64_t)s * parts) + i);
 #pragma unroll 1
