@@ -784,7 +784,8 @@ UCB_API int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_block8_
  *
  * tokens [seqs, drafts_n + 1]: the drafts that stay, the next token, -1 behind; accepted [seqs]: how many stay;
  * logprobs fp32 [seqs, drafts_n + 1]: ln p of these tokens (at temperature 1 for temperature 0), 0 behind, NaN for a
- * next token of -1.  lengths (or NULL) [seqs] are lowered by the drafts that fell.  drafts_n <= 31.
+ * next token of -1.  lengths (or NULL) [seqs] are lowered by the drafts that fell.  drafts_n <= 31, seqs <= 65535,
+ * vocab <= 2^30.
  * workspace: ucb_verify_drafts_workspace_bytes bytes, 16-byte aligned. */
 typedef struct ucb_verify_args {
   const void* logits;

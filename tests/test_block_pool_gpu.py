@@ -314,6 +314,37 @@ def test_captured_calls_replay_on_the_state_of_their_time():
         same_contents(caches, before, oracle, forked=True, compacted=True)
 
 
+def test_a_captured_fork_outlives_a_later_attachment():
+    need_gpu()
+    pool, oracle = BlockPool.allocate(4, 64, 20, block_size=16), Pool(4, 4, 20, 16)
+    cache = pool.cache(num_kv_heads=2, head_dim=64)
+    fill(cache, 1)
+    kernels.device_status()
+    parents, children = ints([0]), ints([3])
+    pool.advance(21)
+    oracle.advance([21] * 4)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        pool.fork(parents, children)
+    torch.cuda.current_stream().wait_stream(stream)
+    later = pool.cache(num_kv_heads=4, head_dim=128)
+    assert [torch.full((112 * i,), 255, device="cuda", dtype=torch.uint8).sum() for i in range(1, 40)]  # reuse what is free
+    fill(later, 2)
+    before = snapshot([cache, later])
+    graph.replay()
+    oracle.fork([0], [3])
+    same_state(pool, oracle)
+    same_contents([cache], before[:1], oracle, forked=True)
+    oracle.copies = []
+    same_contents([later], before[1:], oracle, forked=True)  # not of its time
+    before = snapshot([cache, later])
+    pool.fork(parents, children)
+    oracle.fork([0], [3])
+    same_state(pool, oracle)
+    same_contents([cache, later], before, oracle, forked=True)
+
+
 def test_another_stream():
     need_gpu()
     pool, oracle = BlockPool.allocate(4, 64, 20, block_size=16), Pool(4, 4, 20, 16)

@@ -24,7 +24,7 @@ def test_packed_record_follows_the_header():
 @pytest.mark.parametrize("change,message", [
     ({0: 0}, "null pointer"), ({1: 0}, "null pointer"), ({3: 0}, "null pointer"), ({7: 0}, "null pointer"), ({10: 0}, "null pointer"),
     ({10: 4104}, "aligned"), ({17: -1}, "bad shape"), ({18: -1}, "bad shape"), ({18: 32}, "31 drafts"), ({19: 0}, "bad shape"),
-    ({17: 1 << 25}, "too many"), ({2: 4096, 21: 3}, "dtype"), ({24: -1.0}, "temperature"), ({24: float("nan")}, "temperature"),
+    ({17: 1 << 25}, "too many"), ({19: (1 << 30) + 1}, "too many"), ({2: 4096, 21: 3}, "dtype"), ({24: -1.0}, "temperature"), ({24: float("nan")}, "temperature"),
     ({24: float("inf")}, "temperature")])
 def test_bad_calls_are_refused(change, message):
     values = [4096, 4096, 0, 4096, 0, 0, 0, 4096, 4096, 4096, 4096, 300, 100, 200, 100, 2, 3, 5, 2, 100, 0, 0, 0, 0, 1.0]

@@ -742,7 +742,7 @@ using ucb_host::set_error;
 namespace uv = ucb::verify;
 
 extern "C" int64_t ucb_verify_drafts_workspace_bytes(int seqs, int drafts, int vocab, int dtype) {
-  if (seqs < 1 || drafts < 0 || drafts >= uv::MAX_ROWS || vocab < 1) return -1;
+  if (seqs < 1 || seqs > 65535 || drafts < 0 || drafts >= uv::MAX_ROWS || vocab < 1 || vocab > 1 << 30) return -1;
   uv::Layout layout;
   return layout.make(seqs, drafts + 1, vocab, dtype) ? layout.bytes : -1;
 }
@@ -752,7 +752,7 @@ extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
   if (!a) return set_error(UCB_ERR_INVALID, "%s: null pointer", what);
   if (a->seqs < 0 || a->drafts_n < 0 || a->vocab < 1) return set_error(UCB_ERR_INVALID, "%s: bad shape", what);
   if (a->drafts_n >= uv::MAX_ROWS) return set_error(UCB_ERR_UNSUPPORTED, "%s: at most %d drafts", what, uv::MAX_ROWS - 1);
-  if (a->vocab > 0x7fffff00 || a->seqs > 65535) return set_error(UCB_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
+  if (a->vocab > 1 << 30 || a->seqs > 65535) return set_error(UCB_ERR_UNSUPPORTED, "%s: too many sequences or tokens", what);
   if (!(a->temperature_all >= 0.f && a->temperature_all < 3.0e38f)) return set_error(UCB_ERR_INVALID, "%s: bad temperature", what);
   if (a->seqs == 0) return UCB_OK;
   if (!a->logits || (a->drafts_n && !a->drafts) || !a->uniforms || !a->tokens || !a->accepted || !a->logprobs || !a->workspace)

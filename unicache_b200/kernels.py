@@ -1452,7 +1452,7 @@ def _verify_patterns(index: int, seqs: int, drafts: int, vocab: int, dtype: int)
         with torch.cuda.device(index):  # the multiprocessors of the device that the launch will be on
             size = int(_capi.load().ucb_verify_drafts_workspace_bytes(seqs, drafts, vocab, dtype))
         if size < 0:
-            raise ValueError("verify_drafts takes at most 31 drafts and 65535 sequences")
+            raise ValueError("verify_drafts takes at most 31 drafts, 65535 sequences and 2^30 tokens")
     device = torch.device("cuda", index)
     return (torch.empty((seqs, drafts + 1), dtype=torch.int32, device=device), torch.empty((seqs, drafts + 1), device=device),
             torch.empty(seqs, dtype=torch.int32, device=device),

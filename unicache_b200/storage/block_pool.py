@@ -58,8 +58,8 @@ class BlockPool:
             block_tokens=block_size)
         self.descriptor = ctypes.addressof(self._struct)
         self.caches: list[Int8BlockCache] = []
-        self._layers = self._layers_at = None  # the caches' descriptors on the device
-        self._kv_heads = 0
+        self._layers: list[torch.Tensor] = []  # the caches' descriptors on the device
+        self._layers_at, self._kv_heads = None, 0
         self._compact_bytes = int(_capi.load().ucb_block_pool_compact_workspace_bytes(self.descriptor))
         if self._compact_bytes < 0:
             _capi.check(_capi.UCB_ERR_INVALID, "BlockPool")
@@ -90,7 +90,8 @@ class BlockPool:
         return cache
 
     def attach(self, caches: list) -> None:
-        """Caches whose blocks move with this pool's; they share its table and lengths.  Not while a graph is captured."""
+        """Caches whose blocks move with this pool's; they share its table and lengths.  Not while a graph is captured;
+        a graph that was captured before goes on with the caches of its time."""
 
         for cache in caches:
             if cache.block_table.data_ptr() != self.block_table.data_ptr() or cache.lengths.data_ptr() != self.lengths.data_ptr() \
@@ -104,9 +105,9 @@ class BlockPool:
         if not every:
             return
         raw = b"".join(ctypes.string_at(c.descriptor, ctypes.sizeof(_capi.UcbBlock8Cache)) for c in every)
-        # a new tensor: graphs that were captured with the old one keep its layers
-        self._layers = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(self.device)
-        self._layers_at, self._kv_heads, self.caches = self._layers.data_ptr(), max(c.num_kv_heads for c in every), every
+        # a new tensor beside the old ones, which graphs that were captured with them still read
+        self._layers.append(torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(self.device))
+        self._layers_at, self._kv_heads, self.caches = self._layers[-1].data_ptr(), max(c.num_kv_heads for c in every), every
 
     # ---------------------------------------------------------------- use
     def advance(self, tokens) -> None:
