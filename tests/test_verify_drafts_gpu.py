@@ -88,6 +88,30 @@ def test_vocabularies(vocab):
     check(*inputs(3, 3, vocab, seed=vocab + 1, dtype=torch.float32, probs=None))
 
 
+@pytest.mark.parametrize("vocab,dtype,probs", [(3_000_001, torch.float32, torch.bfloat16), (5_000_003, torch.bfloat16, torch.float32),
+                                               (2_100_000, torch.float16, None)])
+def test_the_largest_vocabularies(vocab, dtype, probs):
+    need_gpu()
+    for near in (0.0, 0.7):
+        check(*inputs(2, 1, vocab, seed=vocab, dtype=dtype, probs=probs, near=near))
+
+
+def test_the_most_sequences():
+    need_gpu()
+    seqs, vocab = 65535, 9
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    logits, uniforms = torch.randn(seqs, 1, vocab, generator=gen, device="cuda"), torch.rand(seqs, 1, generator=gen, device="cuda")
+    none = torch.empty(seqs, 0, device="cuda", dtype=torch.int32)
+    tokens, accepted, _ = verify_drafts(logits, none, uniforms)
+    p = torch.softmax(logits[:, 0].double(), -1).cumsum(-1)
+    target = uniforms.double() * p[:, -1:]
+    clear = ((p - target).abs() > 1e-12).all(-1)
+    assert torch.equal(tokens[clear, 0].long(), (p <= target).sum(-1)[clear]) and clear.sum() > seqs - 10 and (accepted == 0).all()
+    with pytest.raises(ValueError, match="65535 sequences"):
+        verify_drafts(torch.zeros(65536, 1, 8, device="cuda"), none.new_empty((65536, 0)), torch.zeros(65536, 1, device="cuda"))
+    check(*inputs(600, 1, 100, seed=5))  # one CTA a sequence
+
+
 @pytest.mark.parametrize("n", [0, 1, 15, 16, 31])
 @pytest.mark.parametrize("seqs", [1, 7])
 def test_numbers_of_drafts(n, seqs):
