@@ -74,6 +74,30 @@ template <typename T> struct Row {
     const uint32_t w = sizeof(T) == 4 ? 0xff800000u : Dtype<T>::code == UCB_BF16 ? 0xff80ff80u : 0xfc00fc00u;
     return make_uint4(w, w, w, w);
   }
+  // The largest of some vectors' elements that are numbers; two 16-bit ones at a time.
+  template <int N> static __device__ __forceinline__ float top_of(const uint4 (&w)[N]) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t top = nothing().x;
+#pragma unroll
+      for (int u = 0; u < N; ++u) top = larger(larger(top, larger(w[u].x, w[u].y)), larger(w[u].z, w[u].w));
+      return fmaxf(Dtype<T>::lo(top), Dtype<T>::hi(top));
+    } else {
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+        top = fmaxf(fmaxf(fmaxf(top, __uint_as_float(w[u].x)), __uint_as_float(w[u].y)), fmaxf(__uint_as_float(w[u].z), __uint_as_float(w[u].w)));
+      return top;
+    }
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {  // of two pairs, that of a number and a NaN the number
+    if constexpr (Dtype<T>::code == UCB_BF16) {
+      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+      const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
   // Any vector as bits, -inf outside the row.
   __device__ __forceinline__ uint4 load(int k) const {
     if (k >= full_begin && k < full_end) return raw(k);
@@ -189,14 +213,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
     else raw[u] = Row<T>::nothing();
   }
   const float temperature = temperature_of(a, s), c = LOG2E / heat_of(temperature);
-  float top = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < ROW_AHEAD; ++u) {
-    float x[VEC];
-    Row<T>::to_float(raw[u], x);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) top = fmaxf(top, x[e]);
-  }
+  float top = Row<T>::top_of(raw);
   __shared__ float warp_top[WARPS], warp_sum[WARPS];
   __shared__ int warp_best[WARPS];
 #pragma unroll
