@@ -277,6 +277,24 @@ def test_draft_distributions_that_are_the_target_but_for_a_few_tokens(vocab):
             assert left[token] > 0 and float(running[token]) >= u - 1e-6 and float(running[token] - left[token] / left.sum()) <= u + 1e-6
 
 
+@pytest.mark.parametrize("probs", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [3000, 151936])
+def test_draft_distributions_that_are_the_target_rounded(probs, vocab):
+    """Some elements are so near to p that they count for one side or the other by what Z is in its last bits."""
+
+    need_gpu()
+    seqs, n = 16, 1
+    logits, drafts, uniforms, _ = inputs(seqs, n, vocab, seed=vocab, dtype=torch.float32, probs=None)
+    heat = torch.linspace(0.4, 2.0, seqs, device="cuda")
+    q = torch.softmax(logits[:, :1].double() / heat.double()[:, None, None], -1).to(probs)
+    # of the drafts that are offered too often, the likeliest: with the largest random number it falls
+    over = q.double() - torch.softmax(logits[:, :1].double() / heat.double()[:, None, None], -1)
+    drafts[:] = over.argmax(-1)
+    uniforms[:, 0] = 1.0 - 2.0 ** -24
+    _, accepted, _ = check(logits, drafts, uniforms, q, heat, unclear=1)
+    assert int(accepted.sum()) == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_large_logits_and_temperatures(dtype):
     need_gpu()

@@ -33,16 +33,24 @@ struct Partial {
 
 enum Weights : int { ALL, LEFT, OTHERS, ANSWERED };  // p; what the draft's distribution leaves of it; p without the draft; no draw
 
-// Of some elements: the sum of their e; and for LEFT what remains of them, the e of those of which something does, and the e
-// of those next to the border.
+// Of some elements: the sum of their e; and for LEFT what remains of them, the e of those of which something does, and how many
+// of them are so near to the border that they may be on its other side (TOO_MANY: more than were kept).
 struct __align__(16) Sums {
-  double all, left, e_left, border;
+  double all, left, e_left, near;
 };
+struct __align__(16) NearElement {
+  double e;
+  float q;
+  float unused;
+};
+constexpr int NEAR_KEPT = 8;  // of a part
+constexpr double TOO_MANY = 1e9;
 
 struct VerifyParams {
   ucb_verify_args a;
   Partial* partials;  // [seqs * rows][splits]
   Sums* sums;         // [seqs][ctas * DRAW_WARPS]
+  NearElement* near;  // [seqs][ctas * DRAW_WARPS][NEAR_KEPT]
   unsigned int* done;  // [seqs]: CTAs whose sums are there
   int splits, ctas, part_vectors;
   unsigned int* err;
@@ -313,6 +321,9 @@ template <typename T> struct Exponential {
 // Whether something remains: above 0, or no number.  By the bits, no compare on the fp64 pipe.
 __device__ __forceinline__ bool remains(double rest) { return ((uint32_t)__double2hiint(rest) ^ 0x80000000u) > 0x7ff00000u; }
 
+// Whether an element's rest is below some 2^-19 of q, by the numbers' upper words.  Infinities and NaN count as near.
+__device__ __forceinline__ bool is_near(double rest, double q) { return (__double2hiint(rest) & 0x7fffffff) + (19 << 20) < __double2hiint(q); }
+
 // Adds what remains of an element, predicated: a branch would cost more.
 __device__ __forceinline__ void add_remaining(Sums& s, double rest, double e) {
   asm("{\n .reg .pred p;\n setp.gt.u32 p, %2, 0x7ff00000;\n @p add.f64 %0, %0, %3;\n @p add.f64 %1, %1, %4;\n}\n"
@@ -320,16 +331,26 @@ __device__ __forceinline__ void add_remaining(Sums& s, double rest, double e) {
       : "r"(__double2hiint(rest) ^ 0x80000000), "d"(rest), "d"(e));
 }
 
-// The sums of a warp's vectors [begin, end), the lanes side by side, the same in every lane.  One loop of little code: most calls go
+// The sums of a warp's vectors [begin, end), the lanes side by side, the same in every lane.  What the draft leaves of p,
+// max(e / Z - q, 0) with Z the sum of all e, would need a pass for Z first.  This one takes the fp32 sum instead, 1 / `unit`: as long as
+// the same elements remain, the sums of what they leave and of their e give those for Z itself.  Elements that are so near to the border
+// that they may change sides are kept, for the two sums to be put right; where they are too many (a draft's distribution that is
+// the target's but for its rounding), the pass is made again with Z.  One loop of little code: most calls go
 // through it once or a few times, and what costs most then is to fetch the instructions.
 template <typename T, typename Q> __device__ __forceinline__ Sums sum_vectors(const Row<T>& row, const Q* left, int begin, int end,
                                                                               const Exponential<T>& exponential, Weights kind,
-                                                                              double unit, int fallen) {
+                                                                              double unit, int fallen, NearElement* kept) {
   constexpr int VEC = Row<T>::VEC;
-  constexpr int NEAR = 20 << 20;  // an element is next to the border where its rest is below 2^-20 of q, by the numbers' upper words
   const int lane = threadIdx.x & 31, first = max(begin, row.full_begin), last = min(end, row.full_end);
   const int but = kind == OTHERS ? fallen : -1;
   Sums s = {0.0, 0.0, 0.0, 0.0};
+  int near_mine = 0;
+  NearElement near_first, near_second;
+  auto keep = [&](double e, double rest, double q) {
+    if (!is_near(rest, q)) return;
+    (near_mine ? near_second : near_first) = {e, (float)q, 0.f};
+    ++near_mine;
+  };
   // ---- the full vectors, the next one in flight
   int i = row.first(first + lane), left_over = (last - first - lane + 31) >> 5;
   const uint4* at = reinterpret_cast<const uint4*>(row.x + i);
@@ -365,13 +386,13 @@ template <typename T, typename Q> __device__ __forceinline__ Sums sum_vectors(co
       for (int u = 0; u < VEC; ++u) {
         const double q = (double)now_q[u], rest = fma(e[u], unit, -q);
         add_remaining(s, rest, e[u]);
-        near |= (__double2hiint(rest) & 0x7fffffff) + NEAR < __double2hiint(q);
+        near |= is_near(rest, q);
       }
       if (near)
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
           const double q = (double)now_q[u], rest = fma(e[u], unit, -q);
-          if ((__double2hiint(rest) & 0x7fffffff) + NEAR < __double2hiint(q)) s.border += e[u];
+          keep(e[u], rest, q);
         }
     }
 #pragma unroll
@@ -393,7 +414,7 @@ template <typename T, typename Q> __device__ __forceinline__ Sums sum_vectors(co
       if (kind == LEFT) {
         const double q = (double)Dtype<Q>::to_f(left[at_end]), rest = fma(e, unit, -q);
         add_remaining(s, rest, e);
-        if ((__double2hiint(rest) & 0x7fffffff) + NEAR < __double2hiint(q)) s.border += e;
+        keep(e, rest, q);
       }
     }
   }
@@ -403,7 +424,16 @@ template <typename T, typename Q> __device__ __forceinline__ Sums sum_vectors(co
     if (kind == LEFT) {
       s.left += __shfl_xor_sync(0xffffffffu, s.left, o);
       s.e_left += __shfl_xor_sync(0xffffffffu, s.e_left, o);
-      s.border += __shfl_xor_sync(0xffffffffu, s.border, o);
+    }
+  }
+  if (kind == LEFT && __any_sync(0xffffffffu, near_mine)) {
+    const unsigned one = __ballot_sync(0xffffffffu, near_mine >= 1), two = __ballot_sync(0xffffffffu, near_mine >= 2);
+    const int count = __popc(one) + __popc(two);
+    const unsigned before = (1u << lane) - 1;
+    s.near = __any_sync(0xffffffffu, near_mine > 2) || count > NEAR_KEPT ? TOO_MANY : count;
+    if (kept && s.near < TOO_MANY) {
+      if (near_mine >= 1) kept[__popc(one & before)] = near_first;
+      if (near_mine >= 2) kept[__popc(one) + __popc(two & before)] = near_second;
     }
   }
   return s;
@@ -423,41 +453,56 @@ struct Verdict {
 
 // The whole CTA: from the sums of all parts, the part with the drawn token, or that they have to be made again.  A thread has a few
 // adjacent parts.
-__device__ __forceinline__ void judge(const Sums* sums, int parts, Weights kind, double unit, double share, bool first_time,
-                                      Verdict& verdict) {
+__device__ __forceinline__ void judge(Sums* sums, const NearElement* kept, int parts, Weights kind, double unit, double share,
+                                      bool first_time, Verdict& verdict) {
   __shared__ Sums warp_sums[DRAW_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (parts + DRAW_THREADS - 1) / DRAW_THREADS;
   const int begin = min(parts, (int)threadIdx.x * each), end = min(parts, begin + each);
   if (threadIdx.x == 0) verdict.owner = -1, verdict.again = false;
-  Sums own = {0.0, 0.0, 0.0, 0.0};
-  for (int i = begin; i < end; ++i) own.all += sums[i].all, own.left += sums[i].left, own.e_left += sums[i].e_left, own.border += sums[i].border;
-  Sums upto = own;  // and the threads in front
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double all = __shfl_up_sync(0xffffffffu, upto.all, o), left = __shfl_up_sync(0xffffffffu, upto.left, o);
-    const double e_left = __shfl_up_sync(0xffffffffu, upto.e_left, o), border = __shfl_up_sync(0xffffffffu, upto.border, o);
-    if (lane >= o) upto.all += all, upto.left += left, upto.e_left += e_left, upto.border += border;
-  }
-  if (lane == 31) warp_sums[warp] = upto;
-  __syncthreads();
-  Sums whole = {0.0, 0.0, 0.0, 0.0}, front = whole;
-#pragma unroll
-  for (int i = 0; i < DRAW_WARPS; ++i) {
-    if (i == warp) front = whole;
-    const Sums x = warp_sums[i];
-    whole.all += x.all, whole.left += x.left, whole.e_left += x.e_left, whole.border += x.border;
-  }
+  Sums own, upto, whole, front;
   double right = unit;
-  if (kind == LEFT) {
-    right = 1.0 / whole.all;
-    // elements within 2^-20 of the border were summed apart: what they may be off by together has to be below 2^-35 of the
-    // whole, and the fp32 sum no further off than they were looked for
-    constexpr double NEAR = 1.0 / (1 << 20), TOLERATED = NEAR / (1 << 15);
-    const bool none = whole.left < NOTHING;
-    const double off = fabs(right - unit), remaining = none ? 0.0 : weight_of(whole, kind, right - unit);
-    const bool again = first_time && (off > NEAR * right || whole.border * off > TOLERATED * remaining);
-    if (again && threadIdx.x == 0) verdict.again = true;
-    if (none && !again) kind = ALL;  // nothing remains: from p itself, whose sums are here
+#pragma unroll 1
+  for (bool settled = !first_time || kind != LEFT;; settled = true) {
+    own = {0.0, 0.0, 0.0, 0.0};
+    for (int i = begin; i < end; ++i) own.all += sums[i].all, own.left += sums[i].left, own.e_left += sums[i].e_left, own.near += sums[i].near;
+    upto = own;  // and the threads in front
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double all = __shfl_up_sync(0xffffffffu, upto.all, o), left = __shfl_up_sync(0xffffffffu, upto.left, o);
+      const double e_left = __shfl_up_sync(0xffffffffu, upto.e_left, o), near = __shfl_up_sync(0xffffffffu, upto.near, o);
+      if (lane >= o) upto.all += all, upto.left += left, upto.e_left += e_left, upto.near += near;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    whole = front = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < DRAW_WARPS; ++i) {
+      if (i == warp) front = whole;
+      const Sums x = warp_sums[i];
+      whole.all += x.all, whole.left += x.left, whole.e_left += x.e_left, whole.near += x.near;
+    }
+    if (kind == LEFT) right = 1.0 / whole.all;
+    if (settled) break;
+    // Elements near the border of the unit that they were summed with may be on its other side for the right one: as long as the two
+    // are no further apart than they were looked for, those that were kept are all.
+    if (fabs(right - unit) * (1 << 20) > right || whole.near >= TOO_MANY) {
+      if (threadIdx.x == 0) verdict.again = true, verdict.unit = right, verdict.kind = kind;
+      __syncthreads();
+      return;
+    }
+    if (whole.near == 0.0) break;
+    for (int i = begin; i < end; ++i)
+      for (int k = 0; k < (int)sums[i].near; ++k) {
+        NearElement x;
+        *reinterpret_cast<uint4*>(&x) = __ldcg(reinterpret_cast<const uint4*>(kept + i * NEAR_KEPT + k));
+        const bool counted = remains(fma(x.e, unit, -(double)x.q));
+        const double rest = fma(x.e, right, -(double)x.q);
+        if (counted != remains(rest)) sums[i].left += counted ? -rest : rest;
+      }
+    __syncthreads();
+  }
+  if (kind == LEFT && whole.left < NOTHING) {
+    kind = ALL;  // nothing remains: from p itself, whose sums are here
   } else if (kind == OTHERS && whole.all < NOTHING) {
     kind = ALL;
     if (threadIdx.x == 0) verdict.again = true;
@@ -603,7 +648,8 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   __shared__ Sums sums[MAX_PARTS];
   __shared__ Verdict verdict;
   {
-    const Sums w = sum_vectors<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, kind, unit, fallen);
+    const Sums w = sum_vectors<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, kind, unit, fallen,
+                                             p.near + ((int64_t)s * parts + mine) * NEAR_KEPT);
     if (lane == 0) p.sums[(int64_t)s * parts + mine] = w;
   }
   __syncthreads();
@@ -618,13 +664,13 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
 #pragma unroll 1
   for (bool first_time = true;; first_time = false) {
     __syncthreads();
-    judge(sums, parts, kind, unit, share, first_time, verdict);
+    judge(sums, p.near + (int64_t)s * parts * NEAR_KEPT, parts, kind, unit, share, first_time, verdict);
     kind = verdict.kind, unit = verdict.unit;
     if (!verdict.again) break;
     __syncthreads();
 #pragma unroll 1
     for (int i = warp; i < parts; i += DRAW_WARPS) {
-      const Sums w = sum_vectors<T, Q>(row, left, begin_of(i), begin_of(i + 1), exponential, kind, unit, fallen);
+      const Sums w = sum_vectors<T, Q>(row, left, begin_of(i), begin_of(i + 1), exponential, kind, unit, fallen, nullptr);
       if (lane == 0) sums[i] = w;
     }
   }
@@ -734,7 +780,7 @@ template <typename T> int launch_all(const VerifyParams& p, cudaStream_t s) {
 
 // How a call is cut up; false where the device cannot be asked.
 struct Layout {
-  int64_t splits, ctas, part_vectors, partials_bytes, sums_bytes, bytes;
+  int64_t splits, ctas, part_vectors, partials_bytes, sums_bytes, near_bytes, bytes;
   bool make(int64_t seqs, int64_t rows, int64_t vocab, int dtype) {
     const int sms = ucb_host::multiprocessors();
     if (sms < 1) return false;
@@ -746,7 +792,8 @@ struct Layout {
     ctas = (vectors + part_vectors * DRAW_WARPS - 1) / (part_vectors * DRAW_WARPS);
     partials_bytes = seqs * rows * splits * (int64_t)sizeof(Partial);
     sums_bytes = seqs * ctas * DRAW_WARPS * (int64_t)sizeof(Sums);
-    bytes = partials_bytes + sums_bytes + seqs * (int64_t)sizeof(unsigned int);
+    near_bytes = seqs * ctas * DRAW_WARPS * NEAR_KEPT * (int64_t)sizeof(NearElement);
+    bytes = partials_bytes + sums_bytes + near_bytes + seqs * (int64_t)sizeof(unsigned int);
     return true;
   }
 };
@@ -784,8 +831,9 @@ extern "C" int ucb_verify_drafts(const ucb_verify_args* a, void* stream) {
     return set_error(UCB_ERR_CUDA, "%s: the device's multiprocessors are unknown", what);
   char* w = static_cast<char*>(a->workspace);
   const uv::VerifyParams p{*a, reinterpret_cast<uv::Partial*>(w), reinterpret_cast<uv::Sums*>(w + layout.partials_bytes),
-                           reinterpret_cast<unsigned int*>(w + layout.partials_bytes + layout.sums_bytes), (int)layout.splits,
-                           (int)layout.ctas, (int)layout.part_vectors, err};
+                           reinterpret_cast<uv::NearElement*>(w + layout.partials_bytes + layout.sums_bytes),
+                           reinterpret_cast<unsigned int*>(w + layout.partials_bytes + layout.sums_bytes + layout.near_bytes),
+                           (int)layout.splits, (int)layout.ctas, (int)layout.part_vectors, err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case UCB_BF16: return uv::launch_all<__nv_bfloat16>(p, s);
