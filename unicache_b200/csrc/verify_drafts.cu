@@ -3,12 +3,15 @@
 // at the first one that does not, a, the next token is drawn from max(p_a - q_a, 0), after all of
 // them from p_n: the first token whose running sum is above u_n times the sum.
 //
-// The first kernel reads every row once, many CTAs a row, with a running maximum and
-// sum in fp32: the tests compare numbers of relative error 1e-6 with a random one.  The
-// draw is another matter: in the long flat tail of a vocabulary a running
+// The first kernel reads every row once, many CTAs a row, maximum and sum in fp32: the tests compare numbers of
+// relative error 1e-6 with a random one.  The draw is another matter: in the long flat tail of a vocabulary a running
 // sum off by d names another token with a probability of up to d times the number of
 // tokens, which is percents for fp32.  So the one row of each sequence that is drawn from
-// is summed in fp64, exponentials included, by a cluster of CTAs.
+// is summed in fp64, exponentials included, by the second kernel.
+//
+// Measured on the device: 32 sequences of 4 drafts, 151936 tokens in bf16 with fp32 draft distributions (68 MB, 10.4 us of memory) take
+// 32.8 us: 13 for the rows, 19 for the draw, of which 7 are the sums and 8 the way from test to token.  64 sequences of 7
+// drafts in fp32 (331 MB, 50.6 us) take 72; one sequence of 4 drafts, 32000 tokens 10.7, of which 8 are that way.
 #include <algorithm>
 #include <type_traits>
 
@@ -202,7 +205,9 @@ __device__ __forceinline__ float2 halves_of(uint64_t a) {
   return v;
 }
 
-// One CTA a part of a row, all of it loaded at once: its maximum first, then the exponentials against that.
+// One CTA a part of a row, all of it loaded at once: its maximum first, then the exponentials against that.  512 rows of 151936 in
+// fp32 (311 MB) take 46 us (6.8 TB/s).  160 rows in bf16 (49 MB) take 13: four rounds of CTAs, each of which waits for its count and
+// then for its loads; twice the loads a thread 14.3, half of them 14.5, several parts a CTA with the next one in flight 13.8.
 template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC, WARPS = ROW_THREADS / 32;
   const ucb_verify_args& a = p.a;
@@ -548,6 +553,10 @@ __device__ __forceinline__ float logprob_of(float logit, const Partial& row, dou
 
 // Some CTAs a sequence, each with some parts of the row that the next token is drawn from, a part a warp.  Which row that is every
 // one of them finds by the tests; the first writes down what they say, and whichever is the last to have its sums finds the token.
+// 24 rows of 151936 take 19 us.  The sums, 47 instructions an element, issue at 41% of the slots with the 24 warps a multiprocessor
+// that 80 registers leave (fp64 pipe 23%; 64 registers spill and take 2 us more, 128 as long); the rest is a chain of
+// memory round trips: sums of the rows, tests, counting, all sums, the part, the token.  A cluster of CTAs a sequence in the place of
+// the count took 22 us, as some multiprocessors had two sequences' CTAs and others none.
 template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS, DRAW_CTAS) verify_draw_kernel(const VerifyParams p) {
   constexpr int VEC = Row<T>::VEC;
   const ucb_verify_args& a = p.a;
