@@ -771,7 +771,7 @@ UCB_API int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_block8_
  * are the target's at the drafted tokens and behind the last one; drafts [seqs, drafts_n]
  * int32, or int64 when drafts_64; draft_probs [seqs, drafts_n, vocab] (probs_dtype) the distributions that they were
  * drawn from, NULL for tokens that were not drawn; uniforms [seqs, drafts_n + 1] in [0, 1).
- * temperature [seqs] on the device, or NULL: temperature_all.  counts [seqs]: the first so many drafts of a
+ * temperature [seqs] on the device, or NULL: temperature_all (finite); outside 1e-30 .. 1e30 it counts as the nearer end.  counts [seqs]: the first so many drafts of a
  * sequence are meant (NULL: all; outside 0 .. drafts_n: limited, error bit).
  *
  * With p_j = softmax(logits_j / temperature), draft x_j stays while uniforms_j * q_j(x_j) < p_j(x_j) (q = 1 without

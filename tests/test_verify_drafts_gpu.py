@@ -320,6 +320,27 @@ def test_rows_of_the_lowest_value_are_uniform(dtype):
         assert (tokens[20:] < 10).all()
 
 
+def test_temperatures_at_their_ends():
+    need_gpu()
+    logits, drafts, uniforms, _ = inputs(8, 2, 900, seed=21, dtype=torch.float32, probs=None)
+    logits[:, :, 100:300] = -math.inf
+    heat = torch.tensor([1e-38, 1e-45, 1e30, 3e38, math.inf, 1e-30, -1.0, 1e-20], device="cuda")
+    tokens, _, _ = check(logits[:4], drafts[:4], uniforms[:4], None, heat[:4].clamp(1e-30, 1e30))
+    got = verify_drafts(logits, drafts, uniforms, temperature=heat)
+    assert torch.equal(got[0][:4], tokens)
+    masked = (got[0] >= 100) & (got[0] < 300)
+    assert not masked.any() and kernels.device_status() == 0
+    best = logits.argmax(-1)
+    for s in (0, 1, 5, 6, 7):  # as good as greedy: the next token is the arg max of what is left
+        at = int(got[1][s])
+        left = logits[s, at].clone()
+        if at < 2 and s != 6:
+            left[drafts[s, at]] = -math.inf
+        assert int(got[0][s, at]) == int(left.argmax()) and (at == 0 or int(got[0][s, 0]) == int(best[s, 0]))
+    got = verify_drafts(logits, drafts, uniforms, temperature=torch.full((8,), math.nan, device="cuda"))
+    assert (got[0][:, 0] == -1).all() and kernels.device_status() == BAD
+
+
 def test_strides_alignment_and_shared_rows():
     need_gpu()
     seqs, n, vocab = 5, 3, 1001

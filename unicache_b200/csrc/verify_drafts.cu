@@ -72,7 +72,6 @@ template <typename T> struct Row {
     full_end = (int)(((int64_t)vocab + shift) / VEC);
   }
   __device__ __forceinline__ int first(int k) const { return k * VEC - shift; }
-  __device__ __forceinline__ uint4 raw(int k) const { return *reinterpret_cast<const uint4*>(x + first(k)); }  // a full one
   static __device__ __forceinline__ void to_float(uint4 w, float (&v)[VEC]) {
     if constexpr (sizeof(T) == 2) {
       v[0] = Dtype<T>::lo(w.x), v[1] = Dtype<T>::hi(w.x), v[2] = Dtype<T>::lo(w.y), v[3] = Dtype<T>::hi(w.y);
@@ -111,7 +110,7 @@ template <typename T> struct Row {
   }
   // Any vector as bits, -inf outside the row.
   __device__ __forceinline__ uint4 load(int k) const {
-    if (k >= full_begin && k < full_end) return raw(k);
+    if (k >= full_begin && k < full_end) return *reinterpret_cast<const uint4*>(x + first(k));
     union {
       uint4 w;
       T e[VEC];
@@ -160,8 +159,11 @@ template <typename Q, int N> struct Probs {
 
 __device__ __forceinline__ float temperature_of(const ucb_verify_args& a, int s) { return a.temperature ? a.temperature[s] : a.temperature_all; }
 
-// What the exponent's differences are multiplied with: greedy sequences have their log-probabilities at temperature 1.
-__device__ __forceinline__ float heat_of(float temperature) { return temperature <= 0.f ? 1.f : temperature; }
+// The temperature that exponents are divided by: 1 for the log-probabilities of greedy sequences, else within 1e-30 to 1e30, where
+// neither the division nor a masked element's exponent leaves fp32's range.  NaN stays, and leaves no distribution.
+__device__ __forceinline__ float heat_of(float temperature) {
+  return temperature <= 0.f ? 1.f : temperature < 1e-30f ? 1e-30f : temperature > 1e30f ? 1e30f : temperature;
+}
 
 __device__ __forceinline__ int count_of(const ucb_verify_args& a, int s) {
   return a.counts ? max(0, min(a.counts[s], a.drafts_n)) : a.drafts_n;
@@ -222,8 +224,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
 #pragma unroll
   for (int u = 0; u < ROW_AHEAD; ++u) {
     const int k = begin + u * ROW_THREADS;
-    if (k < row.vectors) raw[u] = row.load(k);
-    else raw[u] = Row<T>::nothing();
+    raw[u] = k < row.vectors ? row.load(k) : Row<T>::nothing();
   }
   const float temperature = temperature_of(a, s), c = LOG2E / heat_of(temperature);
   float top = Row<T>::top_of(raw);
@@ -273,7 +274,8 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) verify_rows
   p.partials[((int64_t)s * gridDim.y + j) * gridDim.x + split] = {top, sum, best, 0};
 }
 
-// exp(d * T^-1) of the draw: 2^(k / 16) from a table, k the nearest whole number of the exponent in sixteenths, times a
+// exp(d * T^-1) of the draw, by a table as in Tang, "Table-Driven Implementation of the Exponential Function in IEEE Floating-Point
+// Arithmetic" (ACM TOMS 1989): 2^(k / 16), k the nearest whole number of the exponent in sixteenths, times a
 // polynomial in what is left of it (Taylor's to the fifth power, off by 1.4e-13 at most).  What is below e^-350 is taken as something
 // between e^-350 and e^-700: with masked elements it is below NOTHING wherever weights are compared.
 constexpr double NOTHING = 1e-145;
@@ -321,7 +323,6 @@ template <typename T> struct Exponential {
     return e * __hiloint2double(__double2hiint(step) + ((k & ~15) << 16), __double2loint(step));
   }
 };
-
 
 // Whether something remains: above 0, or no number.  By the bits, no compare on the fp64 pipe.
 __device__ __forceinline__ bool remains(double rest) { return ((uint32_t)__double2hiint(rest) ^ 0x80000000u) > 0x7ff00000u; }

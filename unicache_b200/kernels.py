@@ -1480,6 +1480,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Te
     takes the first token whose running sum exceeds ``uniforms[:, n]`` times the sum, in 64 bits.
 
     ``temperature``: a number or fp32 [S], default 1; 0 is greedy: a draft stays where it is the arg max (the lowest index of equals).
+    Below 1e-30 and above 1e30 it counts as those.
     ``counts`` int32 [S]: how many drafts a sequence has; what lies behind is not read.  ``tokens`` holds the drafts that stay, the next
     token and -1; ``accepted`` counts the drafts that stay; ``logprobs`` are ln p of these tokens (of temperature 1 for greedy
     sequences), 0 behind them.  ``lengths`` int32 [S] (``Int8BlockCache.lengths``, which count all drafts) are lowered
