@@ -158,7 +158,8 @@ class Int8BlockCache:
     # ---------------------------------------------------------------- use
     def advance(self, tokens) -> None:
         """Add ``tokens`` (a number or an int32 [num_seqs] tensor) to the lengths
-        before the write of that many rows: once for all caches that share them.
+        before the write of that many rows: once for all caches that share them.  Over a
+        ``BlockPool`` its ``advance`` takes the place of this one.
 
         Negative numbers withdraw the last rows, such as rejected drafts: as far as the start of
         the last block written, or back to the end of an earlier block.  From the middle
