@@ -450,7 +450,7 @@ __device__ __forceinline__ double weight_of(const Sums& s, Weights kind, double 
   return kind != LEFT ? s.all : fma(s.e_left, correction, s.left);
 }
 
-struct Verdict {
+struct Found {
   double unit, total, before;  // before: the weight in front of the owner's part
   int owner;                   // the part that holds the drawn token; -1: none
   Weights kind;
@@ -459,12 +459,12 @@ struct Verdict {
 
 // The whole CTA: from the sums of all parts, the part with the drawn token, or that they have to be made again.  A thread has a few
 // adjacent parts.
-__device__ __forceinline__ void judge(Sums* sums, const NearElement* kept, int parts, Weights kind, double unit, double share,
-                                      bool first_time, Verdict& verdict) {
+__device__ __forceinline__ void locate(Sums* sums, const NearElement* kept, int parts, Weights kind, double unit, double share,
+                                      bool first_time, Found& found_part) {
   __shared__ Sums warp_sums[DRAW_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (parts + DRAW_THREADS - 1) / DRAW_THREADS;
   const int begin = min(parts, (int)threadIdx.x * each), end = min(parts, begin + each);
-  if (threadIdx.x == 0) verdict.owner = -1, verdict.again = false;
+  if (threadIdx.x == 0) found_part.owner = -1, found_part.again = false;
   Sums own, upto, whole, front;
   double right = unit;
 #pragma unroll 1
@@ -492,7 +492,7 @@ __device__ __forceinline__ void judge(Sums* sums, const NearElement* kept, int p
     // Elements near the border of the unit that they were summed with may be on its other side for the right one: as long as the two
     // are no further apart than they were looked for, those that were kept are all.
     if (fabs(right - unit) * (1 << 20) > right || whole.near >= TOO_MANY) {
-      if (threadIdx.x == 0) verdict.again = true, verdict.unit = right, verdict.kind = kind;
+      if (threadIdx.x == 0) found_part.again = true, found_part.unit = right, found_part.kind = kind;
       __syncthreads();
       return;
     }
@@ -511,7 +511,7 @@ __device__ __forceinline__ void judge(Sums* sums, const NearElement* kept, int p
     kind = ALL;  // nothing remains: from p itself, whose sums are here
   } else if (kind == OTHERS && whole.all < NOTHING) {
     kind = ALL;
-    if (threadIdx.x == 0) verdict.again = true;
+    if (threadIdx.x == 0) found_part.again = true;
   }
   const double correction = right - unit, total = weight_of(whole, kind, correction), target = share * total;
   front.all += upto.all - own.all, front.left += upto.left - own.left, front.e_left += upto.e_left - own.e_left;
@@ -536,8 +536,8 @@ __device__ __forceinline__ void judge(Sums* sums, const NearElement* kept, int p
   for (int i = 0; i < DRAW_WARPS; ++i) which = min(which, firsts[i]), fallback = max(fallback, lasts[i]);
   const bool reached = which < parts;
   if (!reached) which = fallback;
-  if (threadIdx.x == 0) verdict.unit = right, verdict.total = total, verdict.kind = kind;
-  if (which >= begin && which < end) verdict.owner = which, verdict.before = reached ? found_at : last_at;
+  if (threadIdx.x == 0) found_part.unit = right, found_part.total = total, found_part.kind = kind;
+  if (which >= begin && which < end) found_part.owner = which, found_part.before = reached ? found_at : last_at;
   __syncthreads();
 }
 
@@ -656,7 +656,7 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   auto begin_of = [&](int part) { return (int)min((int64_t)row.vectors, (int64_t)part * p.part_vectors); };
   double unit = 1.0 / (double)here.sum;
   __shared__ Sums sums[MAX_PARTS];
-  __shared__ Verdict verdict;
+  __shared__ Found found_part;
   {
     const Sums w = sum_vectors<T, Q>(row, left, begin_of(mine), begin_of(mine + 1), exponential, kind, unit, fallen,
                                              p.near + ((int64_t)s * parts + mine) * NEAR_KEPT);
@@ -674,9 +674,9 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
 #pragma unroll 1
   for (bool first_time = true;; first_time = false) {
     __syncthreads();
-    judge(sums, p.near + (int64_t)s * parts * NEAR_KEPT, parts, kind, unit, share, first_time, verdict);
-    kind = verdict.kind, unit = verdict.unit;
-    if (!verdict.again) break;
+    locate(sums, p.near + (int64_t)s * parts * NEAR_KEPT, parts, kind, unit, share, first_time, found_part);
+    kind = found_part.kind, unit = found_part.unit;
+    if (!found_part.again) break;
     __syncthreads();
 #pragma unroll 1
     for (int i = warp; i < parts; i += DRAW_WARPS) {
@@ -684,7 +684,7 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
       if (lane == 0) sums[i] = w;
     }
   }
-  const double total = verdict.total;
+  const double total = found_part.total;
   if (!(total > NOTHING && total < INFINITY)) {
     if (threadIdx.x == 0) answer(-1, 0.f);
     return;
@@ -695,8 +695,8 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
   __shared__ int firsts[DRAW_WARPS], lasts[DRAW_WARPS], fallback_token;
   __shared__ float fallback_logit;
   const double target = share * total;
-  const int begin = begin_of(verdict.owner), end = begin_of(verdict.owner + 1);
-  double before = verdict.before;
+  const int begin = begin_of(found_part.owner), end = begin_of(found_part.owner + 1);
+  double before = found_part.before;
   bool any = false;  // whether there is a fallback
 #pragma unroll 1
   for (int base = begin; base < end; base += DRAW_THREADS) {
