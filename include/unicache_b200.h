@@ -740,7 +740,8 @@ typedef struct ucb_block_pool {
  * sequence), and blocks for what is longer than those that s holds.  Blocks behind
  * a shorter length stay held.  Where the pool runs out, the length counts all the
  * same, the entries stay -1 (writes to them are skipped) and the error bit is
- * set; so it is for a length below 0 (taken as 0) or past the table. */
+ * set; so it is for a length below 0 (taken as 0) or past the table, and for one taken back into a
+ * block that other entries name too: that length stays. */
 UCB_API int ucb_block_pool_advance(const ucb_block_pool* pool, const int32_t* tokens_dev, int each, void* stream);
 
 /* The sequences' entries become -1, their lengths 0; a block that no entry names any more is free.

@@ -28,8 +28,12 @@ class Pool:
         return deque(b for b, n in enumerate(self.references()) if n == 0)
 
     def advance(self, tokens: list[int]) -> None:
-        free = self.free()
+        free, references = self.free(), self.references()
         for s, t in enumerate(tokens):
+            j, inside = divmod(self.lengths[s] + t, self.block)
+            if t < 0 <= j < len(self.rows[s]) and inside and references[self.rows[s][j]] > 1:
+                self.refused = True  # back into a shared block: the length stays
+                continue
             self.refused |= not 0 <= self.lengths[s] + t <= self.width * self.block
             self.lengths[s] = max(0, self.lengths[s] + t)
             need = min(self.width, -(-self.lengths[s] // self.block))

@@ -192,6 +192,34 @@ def test_a_full_pool_leaves_entries_empty_and_recovers():
     assert cache.num_seqs == 3
 
 
+def test_no_length_goes_back_into_a_shared_block():
+    need_gpu()
+    pool, oracle = BlockPool.allocate(4, 64, 20, block_size=16), Pool(4, 4, 20, 16)
+    pool.cache(num_kv_heads=2, head_dim=64)
+    kernels.device_status()
+
+    def both(tokens):
+        pool.advance(ints(tokens))
+        oracle.advance(tokens)
+        same_state(pool, oracle)
+
+    both([32, 40, 32, 0])
+    pool.fork(ints([0, 1]), ints([3, 2]))  # at a block's end, and inside one
+    oracle.fork([0, 1], [3, 2])
+    both([-1, -1, -1, -1])  # 0 and 3 stay at 32, the others go back in blocks of their own
+    assert oracle.lengths == [32, 39, 39, 32]
+    both([-16, -9, 0, 5])  # to blocks' ends and further rows: 16 and 30 are refused or not by whom the block belongs to
+    assert oracle.lengths == [16, 39, 39, 37]
+    both([0, 0, 0, -3])
+    assert oracle.lengths[3] == 34
+    both([0, 0, 0, -4])  # 30: shared with sequence 0, which holds the block still
+    assert oracle.lengths[3] == 34
+    pool.release(ints([0, 2]))
+    oracle.release([0, 2])
+    both([0, -9, 0, -4])  # nobody shares them any more
+    assert oracle.lengths == [0, 30, 0, 30]
+
+
 def test_the_most_sequences():
     need_gpu()
     seqs, block = 4096, 16

@@ -166,8 +166,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     const int s = threadIdx.x * EACH + i;
     length[i] = held[i] = want[i] = 0;
     if (s >= seqs) continue;
-    const int64_t t = (int64_t)pool.lengths[s] + (q.tokens ? q.tokens[s] : q.each), most = (int64_t)pool.max_blocks * bt;
+    const int before = pool.lengths[s];
+    const int64_t most = (int64_t)pool.max_blocks * bt;
+    int64_t t = (int64_t)before + (q.tokens ? q.tokens[s] : q.each);
     bad |= t < 0 || t > most;
+    if (t < before && t > 0 && t % bt && t < most) {  // the next write would change the block that t lies in
+      const int b = pool.block_table[(int64_t)s * pool.max_blocks + t / bt];
+      if (b >= 0 && b < pool.num_blocks && pool.references[b] > 1) t = before, bad = true;
+    }
     length[i] = (int)max((int64_t)0, min(t, (int64_t)0x7fffffff));
     held[i] = pool.held[s];
     want[i] = max(0, (int)((min((int64_t)length[i], most) + bt - 1) / bt) - held[i]);
