@@ -738,9 +738,10 @@ typedef struct ucb_block_pool {
 
 /* lengths[s] += tokens[s] (int32 [num_seqs] on the device; NULL: `each` for every
  * sequence), and blocks for what is longer than those that s holds.  Blocks behind
- * a shorter length stay held.  Where the pool runs out, the length counts all the
- * same, the entries stay -1 (writes to them are skipped) and the error bit is
- * set; so it is for a length below 0 (taken as 0) or past the table, and for one taken back into a
+ * a shorter length stay held; where the length grows again from the start of one that other entries name too (by the
+ * references before the call), those from there on are given back first, for any sequence to take.  Where the pool runs
+ * out, the length counts all the same, the entries stay -1 (writes to them are skipped) and the error bit is
+ * set; so it is for a length below 0 (taken as 0) or past the table, and for one taken back into the middle of a
  * block that other entries name too: that length stays. */
 UCB_API int ucb_block_pool_advance(const ucb_block_pool* pool, const int32_t* tokens_dev, int each, void* stream);
 

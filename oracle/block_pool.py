@@ -28,20 +28,25 @@ class Pool:
         return deque(b for b, n in enumerate(self.references()) if n == 0)
 
     def advance(self, tokens: list[int]) -> None:
-        free, references = self.free(), self.references()
+        references = self.references()
         for s, t in enumerate(tokens):
+            row, (now, within) = self.rows[s], divmod(self.lengths[s], self.block)
             j, inside = divmod(self.lengths[s] + t, self.block)
-            if t < 0 <= j < len(self.rows[s]) and inside and references[self.rows[s][j]] > 1:
+            if t < 0 <= j < len(row) and inside and references[row[j]] > 1:
                 self.refused = True  # back into a shared block: the length stays
                 continue
+            if t > 0 and not within and now < len(row) and references[row[now]] > 1:
+                del row[now:]  # held from a longer length and shared: the next rows go into blocks of its own
             self.refused |= not 0 <= self.lengths[s] + t <= self.width * self.block
             self.lengths[s] = max(0, self.lengths[s] + t)
+        free = self.free()
+        for s, row in enumerate(self.rows):
             need = min(self.width, -(-self.lengths[s] // self.block))
-            while len(self.rows[s]) < need:
+            while len(row) < need:
                 if not free:
                     self.refused = True
                     break
-                self.rows[s].append(free.popleft())
+                row.append(free.popleft())
 
     def release(self, sequences: list[int]) -> None:
         for s in sequences:

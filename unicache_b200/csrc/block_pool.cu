@@ -148,6 +148,9 @@ struct AdvanceParams {
   int each;
 };
 
+// A sequence that grows from a block's start may hold that block from a longer length, and others may share it: its rows would
+// change theirs.  Then the entries from there on are given back, before blocks are taken (only leading blocks are
+// shared, so where that one is not, none behind it is).
 // Most steps of a decode want no block and end after the lengths: 3.7 us for 32 sequences, 4.8 for 2048, whatever the pool; with 8 prompts
 // of up to 256 blocks 6.5.
 __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvanceParams q) {
@@ -161,6 +164,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
   int length[EACH], held[EACH], want[EACH];
   int64_t mine = 0, wanted;
   bool bad = false;
+  unsigned given_back = 0;  // bit i: the thread's i-th sequence
+  auto shared = [&](int s, int64_t j) {
+    const int b = pool.block_table[(int64_t)s * pool.max_blocks + j];
+    return b >= 0 && b < pool.num_blocks && pool.references[b] > 1;
+  };
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int s = threadIdx.x * EACH + i;
@@ -169,13 +177,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     const int before = pool.lengths[s];
     const int64_t most = (int64_t)pool.max_blocks * bt;
     int64_t t = (int64_t)before + (q.tokens ? q.tokens[s] : q.each);
-    bad |= t < 0 || t > most;
-    if (t < before && t > 0 && t % bt && t < most) {  // the next write would change the block that t lies in
-      const int b = pool.block_table[(int64_t)s * pool.max_blocks + t / bt];
-      if (b >= 0 && b < pool.num_blocks && pool.references[b] > 1) t = before, bad = true;
-    }
-    length[i] = (int)max((int64_t)0, min(t, (int64_t)0x7fffffff));
     held[i] = pool.held[s];
+    bad |= t < 0 || t > most;
+    if (t < before && t > 0 && t % bt && t < most && shared(s, t / bt)) t = before, bad = true;  // the next write would change it
+    if (t > before && before >= 0 && before % bt == 0 && before / bt < min(held[i], pool.max_blocks) && shared(s, before / bt))
+      held[i] = before / bt, given_back |= 1u << i;
+    length[i] = (int)max((int64_t)0, min(t, (int64_t)0x7fffffff));
     want[i] = max(0, (int)((min((int64_t)length[i], most) + bt - 1) / bt) - held[i]);
     mine += want[i];
   }
@@ -189,7 +196,25 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     }
     at += want[i];
   }
-  __syncthreads();
+  if (__syncthreads_or(given_back)) {  // the same in every CTA
+    if (pass.ctas > 1) cg::this_cluster().sync();  // table, references and numbers of blocks are read
+    if (pass.rank == 0) {
+      const int lane = threadIdx.x & 31;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        for (unsigned lanes = __ballot_sync(0xffffffffu, given_back >> i & 1); lanes; lanes &= lanes - 1) {
+          const int owner = __ffs(lanes) - 1, s = ((threadIdx.x & ~31) + owner) * EACH + i;
+          const int from = __shfl_sync(0xffffffffu, held[i], owner), to = min(pool.held[s], pool.max_blocks);
+          int32_t* row = pool.block_table + (int64_t)s * pool.max_blocks;
+          for (int j = from + lane; j < to; j += 32) {
+            const int b = row[j];
+            row[j] = -1;
+            if (b >= 0 && b < pool.num_blocks) atomicSub(&pool.references[b], 1); else bad = true;
+          }
+        }
+    }
+    if (pass.ctas > 1) cg::this_cluster().sync(); else __syncthreads();
+  }
   int64_t found = 0;
   for (int round = 0; found < wanted && round * pass.round_blocks < pool.num_blocks; ++round) {
     const int64_t first = pass.first(round);
@@ -224,7 +249,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     if (s >= seqs) continue;
     pool.lengths[s] = length[i];
     const int64_t given = max((int64_t)0, min((int64_t)want[i], found - base[s]));
-    if (given) pool.held[s] = held[i] + (int)given;
+    if (given || (given_back >> i & 1)) pool.held[s] = held[i] + (int)given;
     bad |= given < want[i];
   }
   if (bad) atomicOr(q.p.err, DEVERR_BAD_DESCRIPTOR);

@@ -116,8 +116,9 @@ class BlockPool:
         numbers withdraw rows as there, and the blocks behind the new end stay the sequence's.
 
         Where the pool runs out the lengths count all the same, so that writes skip the missing blocks and ``advance`` of
-        the negative numbers takes the step back; a length below 0 becomes 0.  A length that would go back into a block
-        that other sequences share stays, as the next write would change their rows (device error bit 2)."""
+        the negative numbers takes the step back; a length below 0 becomes 0.  A length that would go back into the middle of a block
+        that other sequences share stays, as the next write would change their rows (device error bit 2).  It may go back to
+        such a block's start, or to nothing: when the sequence grows again it gives the shared blocks back and takes its own."""
 
         if isinstance(tokens, torch.Tensor):
             at, each = self._indices("tokens", tokens), 0
