@@ -85,6 +85,13 @@ struct Pass {
   __device__ int64_t first(int64_t round) const {
     return round * round_blocks + ((int64_t)rank * PLAN_THREADS + threadIdx.x) * per;
   }
+  // A barrier of the cluster in two halves, for what lies between not to wait: every CTA runs, and has passed arrive(), behind wait().
+  __device__ void arrive() const {
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  }
+  __device__ void wait() const {
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
 };
 
 struct RankSpace {
@@ -92,7 +99,8 @@ struct RankSpace {
   int cta_total[2][MAX_CLUSTER];  // every CTA's, by turns: the last round's may still be read
 };
 
-// How many of the round's marked blocks are in front of this thread's `mine`, and the round's in all, over the cluster.
+// How many of the round's marked blocks are in front of this thread's `mine`, and the round's in all, over the cluster.  It stores into
+// the other CTAs' shared memory: behind a barrier of the cluster, since a CTA's memory is there once it runs.
 __device__ __forceinline__ int rank_round(RankSpace& space, const Pass& pass, int mine, int turn, int& total) {
   int before = scan_block(mine, space.warp_sum, total);
   if (pass.ctas == 1) return before;
@@ -186,6 +194,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     want[i] = max(0, (int)((min((int64_t)length[i], most) + bt - 1) / bt) - held[i]);
     mine += want[i];
   }
+  pass.arrive();  // lengths, table, references and numbers of blocks are read
   int64_t at = scan_block(mine, wide_sum, wanted);
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -196,8 +205,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     }
     at += want[i];
   }
-  if (__syncthreads_or(given_back)) {  // the same in every CTA
-    if (pass.ctas > 1) cg::this_cluster().sync();  // table, references and numbers of blocks are read
+  const bool any_given_back = __syncthreads_or(given_back);  // the same in every CTA
+  pass.wait();
+  if (any_given_back) {
     if (pass.rank == 0) {
       const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -241,7 +251,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) advance_kernel(const AdvancePara
     }
     found += total;
   }
-  if (pass.ctas > 1) cg::this_cluster().sync(); else __syncthreads();  // lengths and numbers of blocks are read
   if (pass.rank) return;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -461,10 +470,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_kernel(const CompactPara
   __shared__ RankSpace space;
   const Pass pass(pool.num_blocks);
   launch_dependents();
+  pass.arrive();
   int64_t live = pool.num_blocks;
   int turn = 0, total;
   for (int round = 0; round * pass.round_blocks < pool.num_blocks; ++round) {
-    rank_round(space, pass, __popc(free_bits(pool.references, pool.num_blocks, pass.first(round), pass.per)), turn++, total);
+    const int free = __popc(free_bits(pool.references, pool.num_blocks, pass.first(round), pass.per));
+    if (round == 0) pass.wait();
+    rank_round(space, pass, free, turn++, total);
     live -= total;
   }
   // the i-th live block behind the live count goes to the i-th hole in front of it: as many are the ones as the others
