@@ -1454,7 +1454,8 @@ def _verify_patterns(index: int, seqs: int, drafts: int, vocab: int, dtype: int)
         if size < 0:
             raise ValueError("verify_drafts takes at most 31 drafts, 65535 sequences and 2^30 tokens")
     device = torch.device("cuda", index)
-    return (torch.empty((seqs, drafts + 1), dtype=torch.int32, device=device), torch.empty((seqs, drafts + 1), device=device),
+    return (torch.empty((seqs, drafts + 1), dtype=torch.int32, device=device),
+            torch.empty((seqs, drafts + 1), dtype=torch.float32, device=device),
             torch.empty(seqs, dtype=torch.int32, device=device),
             torch.empty(1, dtype=torch.uint8, device=device).expand(size))  # by one element: it may be megabytes
 
