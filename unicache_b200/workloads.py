@@ -368,7 +368,7 @@ class DraftDecode:
         gen = torch.Generator(device=self.device).manual_seed(seed)
 
         def normal(*shape, std=1.0, mean=0.0):
-            return (mean + std * torch.randn(*shape, generator=gen, device=self.device)).to(torch.bfloat16)
+            return (mean + std * torch.randn(*shape, generator=gen, device=self.device, dtype=torch.float32)).to(torch.bfloat16)
 
         count, longest = len(prompts), max(prompts) + new_tokens + drafts + 1
         seqs = count * samples
@@ -409,10 +409,10 @@ class DraftDecode:
         # heads near the model's own, so that some drafts stay
         self.draft_heads = torch.cat([self.lm_head + normal(hidden, vocab, std=1.0 * hidden ** -0.5) for _ in range(drafts)], 1) \
             if drafts else None
-        self.temperature = torch.full((seqs,), float(temperature), device=self.device)
+        self.temperature = torch.full((seqs,), float(temperature), device=self.device, dtype=torch.float32)
         self.last = torch.randint(0, vocab, (seqs,), generator=gen, device=self.device, dtype=torch.int32)
         self.state = normal(seqs, hidden)  # of the token in front of the last one
-        self.uniforms = torch.rand(seqs, 2 * drafts + 1, generator=gen, device=self.device)  # the caller's to renew
+        self.uniforms = torch.rand(seqs, 2 * drafts + 1, generator=gen, device=self.device, dtype=torch.float32)  # the caller's to renew
         self.graph = self.result = None
 
     def propose(self):
