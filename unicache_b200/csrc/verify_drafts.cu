@@ -615,7 +615,7 @@ template <typename T, typename Q> __global__ void __launch_bounds__(DRAW_THREADS
     if (lane < count && !outside) {
       const Partial& x = part[lane];
       // the sum is off by some 1e-7 in any case, and so may the exponential be
-      stays = greedy ? draft == x.best && x.sum < INFINITY
+      stays = greedy ? draft == x.best && x.sum > 0.f && x.sum < INFINITY  // a row of nothing but -inf has no best token
                      : (double)draft_uniform * draft_q * (double)x.sum < (double)fast_exp2((draft_logit - x.top) * c);
     }
     const unsigned falls = ~__ballot_sync(0xffffffffu, stays);
