@@ -41,6 +41,22 @@ __device__ __forceinline__ int held_tokens(const ucb_block8_cache& c, int s, uns
   return n < 0 ? 0 : (int)most;
 }
 
+// Whose rows the pending ones of a sequence and head are: the block's place in the sequence and how many of its rows were
+// written.  The record lies in their last row, which no held row needs (a block with that row is complete).  Anything else there
+// is no record: pending rows that ucb_block8_write did not write are taken as they are.
+constexpr uint32_t RECORD = 0x38424c4bu;
+__device__ __forceinline__ uint4 make_record(int j, int m) {
+  return make_uint4(RECORD, (uint32_t)j, (uint32_t)m, ~(RECORD ^ (uint32_t)j ^ (uint32_t)m << 16));
+}
+__device__ __forceinline__ bool is_record(uint4 r) { return r.x == RECORD && r.w == ~(RECORD ^ r.y ^ r.z << 16); }
+// Where it lies.
+__device__ __forceinline__ uint4* pending_record(const ucb_block8_cache& c, int s, int h) {
+  const int64_t rows = ((int64_t)s * c.kv_heads + h + 1) * c.block_tokens - 1;
+  return reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.pending_key) + rows * c.head_dim);
+}
+// The record of a sequence none of whose rows are pending: no block has this place.
+__device__ __forceinline__ uint4 record_of_nothing() { return make_record(-1, 0); }
+
 // Programmatic dependent launch: a kernel launched as `dependent` may become resident once every CTA of the kernel before
 // it in its stream has called launch_dependents (or ended).  It calls wait_for_primary before its first access to global
 // memory, which returns when that kernel is complete and its writes are visible.

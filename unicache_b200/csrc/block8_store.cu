@@ -115,15 +115,6 @@ template <bool BF> __device__ __forceinline__ uint32_t codes4(uint32_t w0, uint3
 // 1 / scale, 0 for a scale that is no number.
 __device__ __forceinline__ float inverse_of(float scale) { return scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f; }
 
-// Whose rows the pending ones of a sequence and head are: the block's place in the sequence and how many of its rows were
-// written.  The record lies in their last row, which no held row needs (a block with that row is complete).  Anything else there
-// is no record: pending rows that were not written by this kernel are taken as they are.
-constexpr uint32_t RECORD = 0x38424c4bu;
-__device__ __forceinline__ uint4 make_record(int j, int m) {
-  return make_uint4(RECORD, (uint32_t)j, (uint32_t)m, ~(RECORD ^ (uint32_t)j ^ (uint32_t)m << 16));
-}
-__device__ __forceinline__ bool is_record(uint4 r) { return r.x == RECORD && r.w == ~(RECORD ^ r.y ^ r.z << 16); }
-
 // Keys and values of block j of sequence s and one head: rows [0, held) are pending ones, rows [held, m) the call's.
 // The new rows decide whether the block's scale grows: where it does not, the codes
 // of the held rows stand (they depend on the scale alone, and the scale of a

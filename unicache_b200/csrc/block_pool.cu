@@ -269,10 +269,11 @@ struct ForkParams {
   PoolParams p;
   const int32_t *parents, *children;
   int count;
-  int4* jobs;  // of each pair: source and target block of its incomplete block (-1: nothing to copy), parent and above it rows, child
+  int4* jobs;  // of each pair: source and target block of its incomplete block (a JobKind: nothing to copy), parent and above it rows, child
 };
 
 enum PairState : int { SKIPPED = -2, WHOLE = -1 };  // otherwise the rank of the block that the pair takes
+enum JobKind : int { AT_A_BLOCKS_END = -2, NO_JOB = -1 };
 
 __global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(const ForkParams q) {
   const ucb_block_pool& pool = q.p.pool;
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(const ForkParams q) 
   for (int i = warp; i < q.count; i += warps) {
     const int s = state[i], from = q.parents[i], to = q.children[i];
     if (s == SKIPPED) {
-      if (lane == 0) q.jobs[i].y = -1;
+      if (lane == 0) q.jobs[i].y = NO_JOB;
       continue;
     }
     const int length = pool.lengths[from], shared = length / bt;
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(const ForkParams q) 
       if (b >= 0 && b < pool.num_blocks) atomicAdd(&pool.references[b], 1); else bad = true;
     }
     if (lane == 0) {
-      int4 job = make_int4(-1, -1, from | (length % bt) << 24, to);
+      int4 job = make_int4(-1, s == WHOLE ? AT_A_BLOCKS_END : NO_JOB, from | (length % bt) << 24, to);
       if (s >= 0 && fits) {
         const int b = source[shared], block = q.jobs[i].y;
         row[shared] = block;
@@ -414,8 +415,14 @@ __global__ void __launch_bounds__(FORK_WARPS * 32) fork_copy_kernel(const ForkCo
   if (h >= c.kv_heads) return;
   wait_for_primary();
   const int4 job = q.jobs[blockIdx.x];
-  if (job.y < 0) return;
   const int rows = job.z >> 24, parent = job.z & 0xffffff, child = job.w;
+  if (job.y == AT_A_BLOCKS_END && !value && lane == 0) {
+    // None of the child's rows are pending, and what it held before is another sequence's.  Rows without a record are their owner's affair: where
+    // neither sequence was ever written to they stay.
+    uint4* at = pending_record(c, child, h);
+    if (is_record(*at) || is_record(*pending_record(c, parent, h))) *at = record_of_nothing();
+  }
+  if (job.y < 0) return;
   const int64_t block = (int64_t)c.block_tokens * c.head_dim;
   const int64_t from = (int64_t)job.x * c.kv_heads + h, to = (int64_t)job.y * c.kv_heads + h;
   int8_t* code = value ? c.value_code : c.key_code;
