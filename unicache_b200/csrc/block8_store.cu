@@ -271,6 +271,12 @@ __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, 
   if (!FRESH && threadIdx.x == 0) *record_at = make_record(j, keep ? m : 0);
 }
 
+// Rows of block j from `held` on are skipped: rows in their places from before, withdrawn or an earlier sequence's, are not theirs.
+__device__ __forceinline__ void drop_record(uint4* at, int j, int held) {
+  const uint4 record = *at;
+  if (is_record(record) && record.y == (uint32_t)j && record.z > (uint32_t)held) *at = make_record(j, held);
+}
+
 // Work items of a head: item s < num_seqs is sequence s's first touched block
 // and then its last one (one CTA, since the first reads the pending rows that
 // the last overwrites); item num_seqs + i is the whole block in between that
@@ -309,7 +315,11 @@ __global__ void __launch_bounds__(THREADS, D * BT > 8192 ? 2 : 4) write_kernel(c
     const int64_t t0 = (int64_t)j * bt;
     const int m = (int)min((int64_t)bt, len - t0);
     const int held = (int)max((int64_t)0, min((int64_t)m, old - t0));
-    if (block >= 0) write_block<BF, D, BT, false>(p, s, h, block, j, m, held, a + t0 + held - old, j == last);
+    if (block >= 0) {
+      write_block<BF, D, BT, false>(p, s, h, block, j, m, held, a + t0 + held - old, j == last);
+    } else if (threadIdx.x == 0) {
+      drop_record(pending_record(c, s, h), j, held);
+    }
     if (j == last) break;
     j = last;
     __syncthreads();  // the pending rows of the first block are read
