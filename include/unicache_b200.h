@@ -619,7 +619,7 @@ UCB_API int ucb_head_norm_rope_axes(const ucb_head_norm_args* args, const ucb_ro
  * key_low / key_high hold the smallest and largest key code of each channel
  * over the block's tokens.  Token t of sequence s lies in row t % block_tokens
  * of block block_table[s][t / block_tokens].  pending_key / pending_value keep
- * the unquantised rows of the last block that a write touched, so a block that
+ * the unquantised rows of the last block that a write touched (of the first one where the table names no last), so a block that
  * grows row by row is after each write the quantisation of all its rows; their last row
  * holds the writer's record of whose rows they are and how many.  Several sequences may have a
  * complete block in common that none of them writes into; an incomplete one belongs to

@@ -97,3 +97,33 @@ def test_a_step_from_a_blocks_end_that_was_taken_back_is_made_again(block, dim, 
     rows = joined([x[:-3] for x in rows], layers.append(0, 3 + more, 4.0))
     layers.check(0, rows)
     assert kernels.device_status() == 0
+
+
+@pytest.mark.parametrize("block,dim,dtype", KINDS)
+@pytest.mark.parametrize("inside,more", [(1, 1), (4, 2), (9, 5), (4, 12)])
+def test_a_step_from_inside_a_block_that_was_taken_back_is_made_again(block, dim, dtype, inside, more):
+    """The step fills a block and needs another one that is not there."""
+
+    need_gpu()
+    layers = full(block, dim, dtype, inside)
+    rows = [x[:2 * block - inside] for x in layers.append(0, 2 * block - 1, 1.0)]
+    layers.back(0, inside - 1)
+    layers.append(2, 4 * block, 1.0)
+    assert kernels.device_status() == 0
+    layers.append(0, inside + more, 2.0)
+    assert kernels.device_status() & BAD
+    layers.back(0, inside + more)
+    layers.pool.release(ints([2]))
+    rows = joined(rows, layers.append(0, inside + more, 4.0))
+    layers.check(0, rows)
+    # a step over several blocks, of which the last is missing
+    layers.append(2, 2 * block, 1.0)
+    rows = joined(rows, layers.append(0, block - more - 1, 0.5))
+    assert kernels.device_status() == 0
+    layers.append(0, block + 3, 8.0)
+    assert kernels.device_status() & BAD and layers.pool.held.tolist() == [4, 0, 2]
+    layers.back(0, block + 3)
+    layers.pool.release(ints([2]))
+    rows = joined(rows, layers.append(0, block + 3, 0.7))
+    layers.check(0, rows)
+    assert kernels.device_status() == 0
