@@ -58,8 +58,10 @@ __device__ __forceinline__ uint4* pending_record(const ucb_block8_cache& c, int 
 __device__ __forceinline__ uint4 record_of_nothing() { return make_record(-1, 0); }
 
 // Programmatic dependent launch: a kernel launched as `dependent` may become resident once every CTA of the kernel before
-// it in its stream has called launch_dependents (or ended).  It calls wait_for_primary before its first access to global
-// memory, which returns when that kernel is complete and its writes are visible.
+// it in its stream, the primary, has called launch_dependents (or ended).  wait_for_primary returns when that kernel is complete and
+// its writes are visible.  In front of it a dependent kernel writes nothing and reads only what the primary does not write,
+// such as a call's inputs; and the primary is launched as an ordinary kernel, since otherwise kernels before that one might still be writing
+// these (verify_draw_kernel, fork_copy_kernel and compact_copy_kernel read so).
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
