@@ -751,8 +751,9 @@ UCB_API int ucb_block_pool_release(const ucb_block_pool* pool, const int32_t* se
 
 /* children[i] becomes a copy of parents[i] (int32 [count], count <= num_seqs): it is released,
  * shares the parent's complete blocks and gets a block of its own for the incomplete one,
- * whose rows, scales, bounds and pending rows are copied in every cache.  A child of a parent at a block's end has no
- * pending rows: a write into the middle of that block is refused.  caches_dev: `layers` descriptors in device
+ * whose rows, scales, bounds and pending rows are copied in every cache.  Of a parent at a block's end neither it nor the child
+ * has pending rows from then on: a write into the middle of that block is refused.  The rows that a parent's length counts are written
+ * before it is forked.  caches_dev: `layers` descriptors in device
  * memory that share the pool's table and lengths, kv_heads the largest number of their KV heads.  A pair of a sequence with
  * itself is nothing.  A pair is skipped (error bit) when it names a sequence outside, a child that an earlier
  * pair names, a parent that is a child of the call, or a parent whose length its blocks do not hold.  A child for whose block the

@@ -1,4 +1,4 @@
-"""A child forked at a block's end has none of its last block's unquantised rows: a write into the middle of that block is refused,
+"""A fork at a block's end leaves neither parent nor child the block's unquantised rows: a write into its middle is refused,
 whatever the child was before, and everything else is written."""
 
 from __future__ import annotations
@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from unicache_b200 import BlockPool, kernels
+from unicache_b200 import BlockPool, kernels, verify_drafts
 
 from .gpu_util import host, need_gpu
 from .test_block_pool_gpu import BAD, CONTENTS, ints, same_bits
@@ -92,16 +92,51 @@ def test_a_write_into_the_middle_of_the_childs_last_block_is_refused(block, dim,
     assert kernels.device_status() == 0
 
 
-def test_the_parent_keeps_its_rows():
-    """Once the child has ended the parent may go back inside its last block, as if it had never been forked."""
+@pytest.mark.parametrize("who", [0, 1, 2])
+@pytest.mark.parametrize("verified", [False, True])
+def test_nobody_writes_into_the_middle_of_a_block_shared_at_its_end(who, verified):
+    """Drafts up to a block's end, forked before they are verified: the lengths go back into the shared block without the pool."""
+
+    need_gpu()
+    layers = Layers(16, 64, torch.bfloat16, who)
+    rows = layers.append(0, 32, 1.0)
+    layers.pool.fork(ints([0, 0]), ints([1, 2]))
+    page = int(layers.pool.block_table[0, 1])
+    was = [{n: getattr(c, n)[page].clone() for n in CONTENTS} for c in layers.caches]
+    if verified:  # all greedy drafts fall
+        logits = torch.zeros(3, 4, 50, device="cuda")
+        logits[:, :, 7] = 1.0
+        _, accepted, _ = verify_drafts(logits, ints([[1, 2, 3]] * 3), torch.rand(3, 4, device="cuda"), temperature=0.0,
+                                       lengths=layers.pool.lengths)
+        assert accepted.tolist() == [0, 0, 0]
+    else:
+        layers.pool.lengths.sub_(3)
+    assert layers.pool.lengths.tolist() == [29] * 3 and kernels.device_status() == 0
+    layers.append(who, 1, 5.0)
+    assert kernels.device_status() & BAD
+    for cache, old in zip(layers.caches, was):
+        for name, x in old.items():
+            same_bits(getattr(cache, name)[page], x)
+    layers.back(who, 14)  # to the block's start
+    mine = joined([x[:16] for x in rows], layers.append(who, 20, 5.0))
+    assert layers.pool.held.tolist() == [2 + (s == who) for s in range(3)]
+    layers.check(who, mine)
+    for cache, old in zip(layers.caches, was):
+        for name, x in old.items():
+            same_bits(getattr(cache, name)[page], x)
+    assert kernels.device_status() == 0
+
+
+def test_a_parent_goes_on_behind_a_fork():
+    """Rows, drafts taken back and further ones, as if it had not been forked."""
 
     need_gpu()
     layers = Layers(16, 64, torch.bfloat16, 1)
     rows = layers.append(0, 32, 1.0)
     layers.pool.fork(ints([0]), ints([2]))
-    layers.pool.release(ints([2]))
-    layers.back(0, 5)
-    rows = joined([x[:27] for x in rows], layers.append(0, 9, 4.0))
+    rows = joined(rows, layers.append(0, 6, 1.0))
+    layers.back(0, 3)
+    rows = joined([x[:35] for x in rows], layers.append(0, 9, 4.0))
     layers.check(0, rows)
     assert kernels.device_status() == 0
 

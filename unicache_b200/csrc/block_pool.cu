@@ -417,10 +417,13 @@ __global__ void __launch_bounds__(FORK_WARPS * 32) fork_copy_kernel(const ForkCo
   const int4 job = q.jobs[blockIdx.x];
   const int rows = job.z >> 24, parent = job.z & 0xffffff, child = job.w;
   if (job.y == AT_A_BLOCKS_END && !value && lane == 0) {
-    // None of the child's rows are pending, and what it held before is another sequence's.  Rows without a record are their owner's affair: where
-    // neither sequence was ever written to they stay.
-    uint4* at = pending_record(c, child, h);
-    if (is_record(*at) || is_record(*pending_record(c, parent, h))) *at = record_of_nothing();
+    // The block is shared from now on, so neither may write into its middle, wherever their lengths are taken back to; and what the child's
+    // slot holds is another sequence's.  Rows without a record are their owner's affair: where neither was ever written to they stay.
+    // (Other pairs of the parent may do the same at once: either record of the parent's begins with RECORD.)
+    uint4 *of_child = pending_record(c, child, h), *of_parent = pending_record(c, parent, h);
+    const bool written = of_parent->x == RECORD;
+    if (written) *of_parent = record_of_nothing();
+    if (written || is_record(*of_child)) *of_child = record_of_nothing();
   }
   if (job.y < 0) return;
   const int64_t block = (int64_t)c.block_tokens * c.head_dim;

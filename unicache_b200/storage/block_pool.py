@@ -139,7 +139,9 @@ class BlockPool:
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         """Sequence ``children[i]`` becomes a copy of ``parents[i]`` (int32 [n] each): what it held is released, the parent's
-        complete blocks are shared and its incomplete block is copied in every attached cache.
+        complete blocks are shared and its incomplete block is copied in every attached cache.  The rows that the parent's length
+        counts are written, and its drafts verified, before: a write into the middle of a block that a fork at its end has shared is
+        refused (device error bit 2).
 
         No sequence may be a child twice, or parent and child in one call: such pairs are skipped.  A beam
         search lets a surviving beam stay where it is and forks only the further ones into
