@@ -779,7 +779,7 @@ UCB_API int ucb_block_pool_compact(const ucb_block_pool* pool, const ucb_block8_
  * sequence are meant (NULL: all; outside 0 .. drafts_n: limited, error bit).
  *
  * With p_j = softmax(logits_j / temperature), draft x_j stays while uniforms_j * q_j(x_j) < p_j(x_j) (q = 1 without
- * draft_probs).  At the first j that falls the next token comes from max(p_j - q_j, 0) (without draft_probs: p_j without
+ * draft_probs; in 32 bits, where p below 2^-126 of the row's largest is 0).  At the first j that falls the next token comes from max(p_j - q_j, 0) (without draft_probs: p_j without
  * x_j; where nothing is left, p_j), after all of them from the row behind: the first token whose
  * running sum is above uniforms[drafts_n] times the sum, in 64 bits.  Temperature 0 (or less): a draft stays where it
  * is the arg max, which is also the next token; the lowest index of equals.  A draft outside the vocabulary falls, the next token

@@ -3,7 +3,7 @@
 // Prompts move 2 bytes in and 1 out a value, and back: 45880
 // tokens x 4 heads x 128, keys and values, written in 27.5 us (5.1 TB/s, 75% of the issue slots busy) and
 // restored in 27.2 (waiting for table, scale and codes, one after the other).  One token of each of 32 sequences is a chain of round
-// trips: 3.7 us.  A CTA holds a whole block of one head in registers, so each row is
+// trips: 3.8 us.  A CTA holds a whole block of one head in registers, so each row is
 // read once; the block's largest magnitude and its channels' bounds are reduced
 // through one barrier.
 #include "block8.cuh"
@@ -120,7 +120,7 @@ __device__ __forceinline__ float inverse_of(float scale) { return scale < INFINI
 // of the held rows stand (they depend on the scale alone, and the scale of a
 // larger magnitude is never the smaller), and only the new rows are written.  Where rows
 // of the block were withdrawn since (the record counts more than `held`), scale and bounds
-// come from the held rows again (one token to each of 32 sequences, the one before it withdrawn: 3.9 us against 3.7).  Nothing is written where the held rows are not there any more, or never were.
+// come from the held rows again (one token to each of 32 sequences, the one before it withdrawn: 3.9 us against 3.8).  Nothing is written where the held rows are not there any more, or never were.
 // FRESH: a block without held rows.  KEEP: the last block that the call writes, whose rows stay pending.
 template <bool BF, int D, int BT, bool FRESH>
 __device__ __forceinline__ void write_block(const WriteParams& p, int s, int h, int64_t block, int j, int m, int held,

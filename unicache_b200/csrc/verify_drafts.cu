@@ -11,7 +11,7 @@
 //
 // Measured on the device: 32 sequences of 4 drafts, 151936 tokens in bf16 with fp32 draft distributions (68 MB, 10.4 us of memory) take
 // 32.8 us: 13 for the rows, 19 for the draw, of which 7 are the sums and 8 the way from test to token.  64 sequences of 7
-// drafts in fp32 (331 MB, 50.6 us) take 72; one sequence of 4 drafts, 32000 tokens 10.7, of which 8 are that way.
+// drafts in fp32 (331 MB, 50.6 us) take 73, 83 where most of the drafts fall; one sequence of 4 drafts, 32000 tokens 10.4, of which 8 are that way.
 #include <algorithm>
 #include <type_traits>
 
