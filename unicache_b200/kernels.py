@@ -1184,7 +1184,7 @@ def _packed_axes(axes: tuple, count: int, stride: int) -> bytes:
         raise ValueError("positions must be [axes, tokens] of 1 to 4 axes")
     words = [0] * 8
     for i, axis in enumerate(axes):
-        if not 0 <= axis < count:
+        if not 0 <= axis < count or axis != int(axis):
             raise ValueError("axes must name rows of positions")
         words[i // 16] |= int(axis) << 2 * (i % 16)
     return _capi.ROPE_AXES.pack(stride, *words, count, 0)
